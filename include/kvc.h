@@ -31,6 +31,10 @@
  *   kvc_deltanet_step           the Gated-DeltaNet layer step that mutates that
  *                               state (conv1d + delta rule + gated RMSNorm),
  *                               src/engine.cpp:3197-3327 and :2600-2716
+ *   kvc_kv_quantize             cold blocks into 8 bits, which kvc_decode_attn,
+ *                               kvc_prefill_attn and kvc_gather then read (new)
+ *   kvc_attn_weights, kvc_evict eviction from a sequence's cache by accumulated
+ *                               attention weight (new)
  *   kvc_snapshot_save/_restore  prefix-boundary copies of that state (new: the
  *                               reference can only extend one live sequence)
  *
@@ -131,7 +135,8 @@ typedef struct kvc_config {
     int32_t rope_dim;          /* rotated dims per head, pairs (p, p + rope_dim/2)
                                   (64, model_config.h:22); 0 or a power of two
                                   in [8, head_dim] */
-    int32_t reserved;          /* 0 */
+    int32_t q8_blocks;         /* 8-bit blocks per layer (kvc_kv_quantize); 0 = none.
+                                  A block of 32 tokens takes 32.1 KiB here, 64 in bf16 */
 } kvc_config;
 
 typedef struct kvc_stats {
@@ -146,6 +151,13 @@ typedef struct kvc_stats {
     int64_t prefix_hits;      /* tokens reused by kvc_prefix_match so far */
     int64_t evictions;        /* index blocks reclaimed under pressure */
 } kvc_stats;
+
+typedef struct kvc_seq_info {
+    int32_t len;        /* tokens in the cache (kvc_seq_len) */
+    int32_t pending;    /* reserved, not yet committed */
+    int32_t position;   /* text position of the next token: len + tokens evicted */
+    int32_t q8_tokens;  /* leading tokens held in 8 bits */
+} kvc_seq_info;
 
 typedef struct kvc_ctx kvc_ctx;
 
@@ -168,7 +180,8 @@ int kvc_seq_release(kvc_ctx* ctx, int32_t seq);
  * the fill: capture after it. */
 int kvc_seq_reset(kvc_ctx* ctx, int32_t seq);
 int kvc_seq_len(kvc_ctx* ctx, int32_t seq, int32_t* len);
-/* Drop tokens beyond len (rollback); len <= current length. */
+/* Drop tokens beyond len (rollback); len <= current length.  A len inside an
+ * 8-bit block that is no multiple of block_tokens is KVC_ERR_UNSUPPORTED. */
 int kvc_seq_truncate(kvc_ctx* ctx, int32_t seq, int32_t len);
 /* Make positions [len, len+n_tok) writable for every seq (allocates blocks and
  * publishes new block-table entries on `stream`).  Until commit, appends and
@@ -289,6 +302,71 @@ int kvc_prefill_step(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
 int kvc_gather(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
                int32_t n_seqs, int32_t tok0, const int32_t* n_tok,
                void* k_out, void* v_out, void* stream);
+
+/* ---- 8-bit blocks and eviction (no counterpart in the reference) ---------- */
+/* Moves blocks into 8 bits, K and V of every layer: of each seq, the full
+ * blocks that hold none of its last keep_tokens tokens (those that are in 8
+ * bits already stay as they are).  A unit (32 tokens of one kv head, K or V)
+ * becomes int8 values i and one fp32 scale s:
+ *   a = max |x|, s = max(a, 2^-100) / 127, i = rne(x * (127 / max(a, 2^-100)))
+ * and stands for i * s.  A unit that holds an infinity or a NaN gets s = NaN.
+ * dst NULL: in place; the bf16 blocks go back to the pool (or stay with the
+ * prefix index and other sequences that hold them).  Otherwise dst[i] is an
+ * empty sequence that becomes a copy of seqs[i] with those blocks in 8 bits
+ * and shares its others; seqs[i] stays as it is.  (Not with recurrent layers:
+ * KVC_ERR_UNSUPPORTED, since their state is not copied.)
+ * Sequences must have nothing pending.  The 8-bit pool has q8_blocks blocks;
+ * KVC_ERR_NOMEM, with no change, if they do not suffice.
+ * A sequence with 8-bit blocks is read by kvc_decode_attn (no weight is
+ * rounded to bf16), kvc_prefill_attn (weights as three bf16 parts when
+ * out_dtype is fp32, as one when it is bf16), kvc_gather (bf16, RNE of i * s),
+ * kvc_attn_weights and kvc_evict; kvc_append and kvc_qkv_append add to it.  It
+ * no longer feeds the prefix index and is refused (KVC_ERR_UNSUPPORTED) by
+ * kvc_decode_step, kvc_prefill_step, kvc_decode_attn_static, kvc_kv_checksum
+ * and by kvc_snapshot_save when the snapshot's segment is in 8 bits. */
+int kvc_kv_quantize(kvc_ctx* ctx, const int32_t* seqs, const int32_t* dst,
+                    int32_t n_seqs, int32_t keep_tokens, void* stream);
+/* The attention weight that each seq's last n_q tokens give its cached ones,
+ * added to an accumulator:
+ *   acc_out[s][h][j] = acc_in[s][h][j] + sum over the n_q rows i and the 4 q
+ *   heads of kv head h of softmax_j((q_i . k_j) * scale)
+ * for j < len + pending; row i sits at position len + pending - n_q + i and
+ * sees keys up to its own.  q: bf16 [n_seqs][n_q][Hq][D], n_q <= 256 and at
+ * most len + pending.  acc_in (NULL: zeros) and acc_out: device fp32
+ * [n_seqs][Hkv][acc_stride]; they may be the same array and must not overlap
+ * otherwise.  Entries from len + pending on are left as they are.  The scores
+ * go through the context's split-K workspace: 64 B per row and key of one seq
+ * must fit into its 138 MB (KVC_ERR_RANGE otherwise: fewer rows a call).
+ * fp32 throughout, without atomics: the same call gives the same bits. */
+int kvc_attn_weights(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
+                     int32_t n_seqs, int32_t n_q, const void* q, float scale,
+                     const void* acc_in, void* acc_out, int64_t acc_stride,
+                     void* stream);
+/* Cuts each seq to at most budget tokens.  In every layer and kv head the
+ * first n_sink and the last n_recent tokens stay, and of the others those of
+ * the greatest acc, budget - n_sink - n_recent of them (ties: the lower
+ * position; NaN counts as lowest), all in their order.  acc: device fp32
+ * [n_attn_layers][n_seqs][Hkv][acc_stride], acc_stride >= every length.
+ * kept: device int32 [n_attn_layers][n_seqs][Hkv][budget] receives the indices
+ * of the tokens that stay, -1 past a shorter seq's length.  acc_out (NULL, or
+ * shaped as acc and not overlapping it) receives their acc, then zeros up to
+ * the old length.  The kept rows are copied, bit for bit (8-bit ones as RNE
+ * bf16 of i * s), into fresh bf16 blocks, which must be free beforehand
+ * (KVC_ERR_NOMEM otherwise, with no change).
+ * dst as for kvc_kv_quantize; in place, a seq of at most budget tokens is left
+ * as it is.  len becomes the number of tokens kept, while positions go on:
+ * kvc_qkv_append rotates new tokens at kvc_seq_info.position (KVC_ERR_RANGE
+ * once that passes max_seq_len), rows of kvc_prefill_attn and kvc_attn_weights
+ * still see every cached token up to their own.  The seq no longer feeds the
+ * prefix index; kvc_decode_step, kvc_prefill_step and the snapshots refuse it
+ * (KVC_ERR_UNSUPPORTED) until it is reset. */
+int kvc_evict(kvc_ctx* ctx, const int32_t* seqs, const int32_t* dst,
+              int32_t n_seqs, int32_t budget, int32_t n_sink, int32_t n_recent,
+              const void* acc, void* acc_out, int64_t acc_stride,
+              int32_t* kept, void* stream);
+int kvc_seq_get_info(kvc_ctx* ctx, int32_t seq, kvc_seq_info* out);
+/* 8-bit blocks per layer, and how many of them are free. */
+int kvc_q8_stats(kvc_ctx* ctx, int64_t* blocks, int64_t* free_blocks);
 
 /* Integrity checksums of each seq's cached K/V in one layer, one per 16-KiB
  * (block, K|V, kv head) unit (no counterpart in the reference; a cheap check

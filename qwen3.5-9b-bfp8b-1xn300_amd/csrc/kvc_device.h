@@ -33,6 +33,17 @@ __device__ __forceinline__ uint32_t cvt_pk_bf16(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
+// 4 int8 -> 2 packed bf16 pairs, exact.
+__device__ __forceinline__ u32x2 i8x4_to_bf16(uint32_t w) {
+    const int x = (int)w;
+    const float f0 = (float)((x << 24) >> 24), f1 = (float)((x << 16) >> 24);
+    const float f2 = (float)((x << 8) >> 24), f3 = (float)(x >> 24);
+    u32x2 r;
+    r[0] = cvt_pk_bf16(f0, f1);
+    r[1] = cvt_pk_bf16(f2, f3);
+    return r;
+}
+
 // a.x*b.x + a.y*b.y + c on packed bf16 pairs (v_dot2_f32_bf16), fp32 result.
 __device__ __forceinline__ float dot2_bf16(uint32_t a, uint32_t b, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a),

@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "../../include/kvc.h"
+#include "kvc_decode_q8_split.h"
 #include "kvc_decode_split.h"
 #include "kvc_internal.h"
 #include "kvc_prefill_split.h"
@@ -92,6 +93,8 @@ struct Seq {
     // entries[i] stays a valid parent for block i + 1.
     std::vector<int32_t> pins;
     bool state_dirty = false;      // recurrent state must be zeroed before its next use
+    int32_t n8 = 0;       // leading blocks that are 8-bit ones (full and committed)
+    int32_t evicted = 0;  // tokens evicted: the next token's position is len + evicted
 };
 
 struct Entry {
@@ -130,6 +133,8 @@ struct kvc_ctx {
     int32_t* d_table = nullptr;
     uint8_t* d_state = nullptr;
     uint8_t* d_snap = nullptr;
+    uint8_t* d_q8 = nullptr;     // 8-bit blocks
+    float* d_scales = nullptr;   // their scales
     float* d_part = nullptr;
     int32_t* d_counters = nullptr;
     float* s_part = nullptr;        // this device's static decode workspace
@@ -138,6 +143,8 @@ struct kvc_ctx {
 
     std::vector<int32_t> refcnt;
     std::vector<int32_t> free_blocks;
+    std::vector<int32_t> refcnt8;  // of the 8-bit blocks, likewise
+    std::vector<int32_t> free_blocks8;
     std::vector<Seq> seqs;
     std::vector<int32_t> free_seqs;
 
@@ -204,6 +211,10 @@ bool evict_one(kvc_ctx* c) {
         }
     }
     return false;
+}
+
+void unref_block8(kvc_ctx* c, int32_t b) {
+    if (--c->refcnt8[b] == 0) c->free_blocks8.push_back(b);
 }
 
 int32_t alloc_block(kvc_ctx* c) {
@@ -347,9 +358,22 @@ void set_table(kvc_ctx* c, int32_t slot, int32_t idx, int32_t block) {
 void release_tail(kvc_ctx* c, int32_t slot, int32_t keep_blocks) {
     Seq& s = c->seqs[slot];
     while ((int32_t)s.blocks.size() > keep_blocks) {
-        unref_block(c, s.blocks.back());
+        if ((int32_t)s.blocks.size() <= s.n8)
+            unref_block8(c, s.blocks.back());
+        else
+            unref_block(c, s.blocks.back());
         s.blocks.pop_back();
     }
+    s.n8 = std::min(s.n8, keep_blocks);
+}
+
+// The sequence's K/V are no longer those of its token ids (some were rounded
+// to 8 bits, or evicted): it stops feeding the prefix index and the boundary
+// snapshots until a reset or a snapshot restore.
+void forget_tokens(kvc_ctx* c, Seq& s) {
+    s.tokens_known = false;
+    s.tokens.clear();
+    drop_entries(c, s, 0);
 }
 
 // A created or reset sequence's recurrent state reads as zero (reset_state()
@@ -467,6 +491,37 @@ int check_device(kvc_ctx* c) {
     return KVC_OK;
 }
 
+// A launch goes to the current device: for the calls that check it, the
+// context's own.
+int check_current(kvc_ctx* c) {
+    int dev = -1;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return hip_err(e, "hipGetDevice");
+    if (dev != c->cfg.device)
+        return set_err(KVC_ERR_INVALID, "the current device is %d, the context's is %d", dev, c->cfg.device);
+    return KVC_OK;
+}
+
+// For calls that do not read 8-bit blocks or that take a sequence's length for
+// its position.
+int refuse_mixed(kvc_ctx* c, const int32_t* seqs, int32_t n, const char* what, bool evicted_too) {
+    for (int32_t i = 0; i < n; i++) {
+        const Seq& s = c->seqs[seqs[i]];
+        if (s.n8 > 0)
+            return set_err(KVC_ERR_UNSUPPORTED, "sequence %d holds 8-bit blocks, which %s does not read", seqs[i], what);
+        if (evicted_too && s.evicted > 0)
+            return set_err(KVC_ERR_UNSUPPORTED, "sequence %d had tokens evicted, which %s does not support", seqs[i],
+                           what);
+    }
+    return KVC_OK;
+}
+
+bool any_q8(kvc_ctx* c, const int32_t* seqs, int32_t n) {
+    for (int32_t i = 0; i < n; i++)
+        if (c->seqs[seqs[i]].n8 > 0) return true;
+    return false;
+}
+
 int check_seqs(kvc_ctx* c, const int32_t* seqs, int32_t n) {
     if (!seqs || n <= 0) return set_err(KVC_ERR_INVALID, "empty sequence list");
     for (int32_t i = 0; i < n; i++) {
@@ -515,7 +570,7 @@ void kvc_config_default(kvc_config* cfg) {
     cfg->rms_norm_eps = 1e-6f;
     cfg->rope_freq_base = 1.0e7f;
     cfg->rope_dim = 64;
-    cfg->reserved = 0;
+    cfg->q8_blocks = 0;
 }
 
 static void free_device(kvc_ctx* c) {
@@ -524,6 +579,8 @@ static void free_device(kvc_ctx* c) {
     if (c->d_table) (void)hipFree(c->d_table);
     if (c->d_state) (void)hipFree(c->d_state);
     if (c->d_snap) (void)hipFree(c->d_snap);
+    if (c->d_q8) (void)hipFree(c->d_q8);
+    if (c->d_scales) (void)hipFree(c->d_scales);
     if (c->d_part) (void)hipFree(c->d_part);
     if (c->d_counters) (void)hipFree(c->d_counters);
     if (c->d_rope) (void)hipFree(c->d_rope);
@@ -578,6 +635,7 @@ int kvc_create(const kvc_config* cfg, kvc_ctx** out) {
         return set_err(KVC_ERR_INVALID, "layer/sequence counts must be positive");
     if (k.snapshot_interval < 0 || (k.snapshot_interval % k.block_tokens) != 0)
         return set_err(KVC_ERR_INVALID, "snapshot_interval must be a non-negative multiple of block_tokens");
+    if (k.q8_blocks < 0) return set_err(KVC_ERR_INVALID, "q8_blocks must be >= 0");
     if (k.snapshot_slots < 0) return set_err(KVC_ERR_INVALID, "snapshot_slots must be >= 0");
     if ((k.flags & KVC_FLAG_DECODE_SPLIT_D) && (k.flags & KVC_FLAG_DECODE_NO_SPLIT_D))
         return set_err(KVC_ERR_INVALID, "KVC_FLAG_DECODE_SPLIT_D and KVC_FLAG_DECODE_NO_SPLIT_D exclude each other");
@@ -620,14 +678,20 @@ int kvc_create(const kvc_config* cfg, kvc_ctx** out) {
             delete c;
             return hip_err(e, "hipSetDevice");
         }
-        const size_t table_bytes = (size_t)k.max_seqs * c->max_blocks * 4;
+        // kMaxBatch rows more than sequences: kvc_kv_quantize and kvc_evict
+        // stage the new block ids of sequences that they change in place
+        const size_t table_bytes = ((size_t)k.max_seqs + kMaxBatch) * c->max_blocks * 4;
         const size_t part_bytes = kPartBytes;
         const size_t ctr_bytes = kCounterBytes;
         if ((rc = dev_alloc(c, (void**)&c->d_table, table_bytes, "block table")) ||
             (rc = dev_alloc(c, (void**)&c->d_state, (size_t)c->state_bytes * k.max_seqs, "state pool")) ||
             (rc = dev_alloc(c, (void**)&c->d_snap, (size_t)c->snap_bytes * n_snap, "snapshot pool")) ||
             (rc = dev_alloc(c, (void**)&c->d_part, part_bytes, "split-K workspace")) ||
-            (rc = dev_alloc(c, (void**)&c->d_counters, ctr_bytes, "arrival counters"))) {
+            (rc = dev_alloc(c, (void**)&c->d_counters, ctr_bytes, "arrival counters")) ||
+            (rc = dev_alloc(c, (void**)&c->d_q8, (size_t)k.q8_blocks * kQ8BlockBytes * 2 * k.n_attn_layers,
+                            "8-bit K/V pools")) ||
+            (rc = dev_alloc(c, (void**)&c->d_scales, (size_t)k.q8_blocks * kKvHeads * 4 * 2 * k.n_attn_layers,
+                            "8-bit scales"))) {
             free_device(c);
             delete c;
             return rc;
@@ -697,6 +761,9 @@ int kvc_create(const kvc_config* cfg, kvc_ctx** out) {
             std::swap(c->free_blocks[i], c->free_blocks[r]);
         }
     }
+    c->refcnt8.assign(k.q8_blocks, 0);
+    c->free_blocks8.resize(k.q8_blocks);
+    for (int32_t i = 0; i < k.q8_blocks; i++) c->free_blocks8[i] = k.q8_blocks - 1 - i;
     c->seqs.resize(k.max_seqs);
     for (int32_t i = k.max_seqs - 1; i >= 0; i--) c->free_seqs.push_back(i);
     c->snaps.resize(n_snap);
@@ -750,7 +817,7 @@ int kvc_seq_reset(kvc_ctx* c, int32_t seq) {
     if (!seq_ok(c, seq)) return set_err(KVC_ERR_INVALID, "sequence %d is not live", seq);
     release_tail(c, seq, 0);
     Seq& s = c->seqs[seq];
-    s.len = s.pending = 0;
+    s.len = s.pending = s.evicted = 0;
     s.tokens.clear();
     drop_entries(c, s, 0);
     s.tokens_known = true;
@@ -779,7 +846,10 @@ int kvc_seq_truncate(kvc_ctx* c, int32_t seq, int32_t len) {
     Seq& s = c->seqs[seq];
     if (s.pending) return set_err(KVC_ERR_STATE, "sequence %d has %d uncommitted tokens", seq, s.pending);
     if (len < 0 || len > s.len) return set_err(KVC_ERR_RANGE, "truncate to %d outside [0, %d]", len, s.len);
+    if (len % kBlockTok && len / kBlockTok < s.n8)  // the cut block would be written to
+        return set_err(KVC_ERR_UNSUPPORTED, "truncate of sequence %d to %d ends inside an 8-bit block", seq, len);
     release_tail(c, seq, (len + kBlockTok - 1) / kBlockTok);
+    if (len == 0) s.evicted = 0;
     drop_entries(c, s, (size_t)(len / kBlockTok));
     if (c->cfg.n_ssm_layers > 0 && len < s.len) {
         // The recurrent state cannot be rolled back: it still holds the
@@ -1057,6 +1127,13 @@ int kvc_qkv_append(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_seq
                            c->seqs[seqs[i]].pending);
     if ((int64_t)std::min(kMaxBatch, n_seqs) * n_tok > INT32_MAX)
         return set_err(KVC_ERR_RANGE, "qkv append too large");
+    if (c->cfg.rope_dim > 0)
+        for (int32_t i = 0; i < n_seqs; i++) {
+            const Seq& s = c->seqs[seqs[i]];
+            if ((int64_t)s.len + s.pending + s.evicted > c->cfg.max_seq_len)
+                return set_err(KVC_ERR_RANGE, "sequence %d: position %lld (%d tokens evicted) is past max_seq_len %d",
+                               seqs[i], (long long)s.len + s.pending + s.evicted - 1, s.evicted, c->cfg.max_seq_len);
+        }
     const size_t esz = in_dtype == KVC_DTYPE_BF16 ? 2 : 4;
     const size_t qrow = (size_t)kQHeads * kHeadDim;
     for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
@@ -1082,6 +1159,7 @@ int kvc_qkv_append(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_seq
             const Seq& s = c->seqs[seqs[i0 + j]];
             a.slot[j] = seqs[i0 + j];
             a.pos0[j] = s.len + s.pending - n_tok;
+            a.rope0[j] = a.pos0[j] + s.evicted;
         }
         int e = launch_qkv_append(a, stream);
         if (e) return hip_err((hipError_t)e, "qkv append launch");
@@ -1185,6 +1263,55 @@ static int build_decode_args(kvc_ctx* c, int32_t layer, const int32_t* seqs, int
     return KVC_OK;
 }
 
+static MixedCache mixed_cache(kvc_ctx* c, int32_t layer) {
+    MixedCache m{};
+    const int64_t q8_kv = (int64_t)c->cfg.q8_blocks * (int64_t)kQ8BlockBytes, sc_kv = (int64_t)c->cfg.q8_blocks * kKvHeads;
+    m.kpool = reinterpret_cast<const uint16_t*>(c->d_pool + (int64_t)(layer * 2) * c->layer_kv_bytes);
+    m.vpool = reinterpret_cast<const uint16_t*>(c->d_pool + (int64_t)(layer * 2 + 1) * c->layer_kv_bytes);
+    m.k8 = c->d_q8 + (int64_t)(layer * 2) * q8_kv;
+    m.v8 = c->d_q8 + (int64_t)(layer * 2 + 1) * q8_kv;
+    m.ks = c->d_scales + (int64_t)(layer * 2) * sc_kv;
+    m.vs = c->d_scales + (int64_t)(layer * 2 + 1) * sc_kv;
+    m.table = c->d_table;
+    m.table_stride = c->max_blocks;
+    return m;
+}
+
+// The decode launch over seqs[i0, i0 + n) of which some hold 8-bit blocks.
+static int build_decode_q8_args(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t i0, int32_t n, const void* q,
+                                const void* k_new, const void* v_new, const void* gate, void* out, int32_t out_dtype,
+                                float scale, DecodeQ8Args& a) {
+    const size_t qrow = (size_t)kQHeads * kHeadDim, kvrow = (size_t)kKvHeads * kHeadDim;
+    memset(&a, 0, sizeof a);
+    int32_t nblk[kMaxBatch];
+    for (int32_t j = 0; j < n; j++) {
+        const Seq& s = c->seqs[seqs[i0 + j]];
+        const int32_t L = s.len + s.pending;
+        if (L <= 0) return set_err(KVC_ERR_STATE, "sequence %d has no keys to attend", seqs[i0 + j]);
+        if (k_new && s.pending < 1)
+            return set_err(KVC_ERR_STATE, "sequence %d: fused append needs a reserved token", seqs[i0 + j]);
+        a.slot[j] = seqs[i0 + j];
+        a.kv_len[j] = L;
+        a.n8[j] = s.n8;
+        nblk[j] = (L + kBlockTok - 1) / kBlockTok;
+    }
+    decode_q8_split(nblk, n, a);
+    a.c = mixed_cache(c, layer);
+    a.q = static_cast<const uint16_t*>(q) + (size_t)i0 * qrow;
+    a.k_new = k_new ? static_cast<const uint16_t*>(k_new) + (size_t)i0 * kvrow : nullptr;
+    a.v_new = v_new ? static_cast<const uint16_t*>(v_new) + (size_t)i0 * kvrow : nullptr;
+    a.gate = gate ? static_cast<const uint16_t*>(gate) + (size_t)i0 * qrow : nullptr;
+    a.out = static_cast<uint8_t*>(out) + (size_t)i0 * qrow * (out_dtype == KVC_DTYPE_BF16 ? 2 : 4);
+    a.part = c->d_part;
+    a.part_bytes = (uint32_t)kPartBytes;
+    a.counters = c->d_counters;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.out_bf16 = out_dtype == KVC_DTYPE_BF16;
+    a.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
+    a.n_seqs = n;
+    return KVC_OK;
+}
+
 // Decode over all seqs, 64 per launch; every launch is validated before the
 // first one is made.  Launches of one call run in stream order and share the
 // workspace.
@@ -1207,10 +1334,24 @@ static int decode_impl(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n
     if (out_dtype != KVC_DTYPE_F32 && out_dtype != KVC_DTYPE_BF16) return set_err(KVC_ERR_INVALID, "bad out_dtype");
     if (!std::isfinite(scale)) return set_err(KVC_ERR_INVALID, "scale must be finite");
     if (!part || !counters) return set_err(KVC_ERR_STATE, "no %s", workspace);
+    const bool q8 = any_q8(c, seqs, n_seqs);
+    if (prod.qkv && (rc = refuse_mixed(c, seqs, n_seqs, "kvc_decode_step", true))) return rc;
+    if (part != c->d_part && (rc = refuse_mixed(c, seqs, n_seqs, "kvc_decode_attn_static", false))) return rc;
+    if (q8 && (rc = check_current(c))) return rc;
     DecodeArgs a;
+    DecodeQ8Args a8;
     for (int pass = 0; pass < 2; pass++) {
         for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
             const int32_t n = std::min(kMaxBatch, n_seqs - i0);
+            if (q8 && any_q8(c, seqs + i0, n)) {
+                if ((rc = build_decode_q8_args(c, layer, seqs, i0, n, q, k_new, v_new, gate, out, out_dtype, scale, a8)))
+                    return rc;
+                if (pass == 1) {
+                    int e = launch_decode_q8(a8, stream);
+                    if (e) return hip_err((hipError_t)e, "decode launch (8-bit blocks)");
+                }
+                continue;
+            }
             if ((rc = build_decode_args(c, layer, seqs, i0, n, q, k_new, v_new, gate, prod, out, out_dtype, scale,
                                         part, part_bytes, counters, max_items, workspace, a)))
                 return rc;
@@ -1291,6 +1432,14 @@ static int prefill_launches(kvc_ctx* c, int32_t layer, const int32_t* seqs, int3
         a.n_seqs = n;
         a.n_q = n_q;
         a.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
+        if (any_q8(c, seqs + i0, n)) {
+            const MixedCache m = mixed_cache(c, layer);
+            a.k8 = m.k8;
+            a.v8 = m.v8;
+            a.ks = m.ks;
+            a.vs = m.vs;
+            for (int32_t j = 0; j < n; j++) a.n8[j] = c->seqs[seqs[i0 + j]].n8;
+        }
         a.n_groups = n * kKvHeads;
         for (int32_t j = 0; j < n; j++) a.seq_order[j] = j;
         std::stable_sort(a.seq_order, a.seq_order + n,
@@ -1335,6 +1484,7 @@ int kvc_prefill_attn(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
     if (!q) return set_err(KVC_ERR_INVALID, "prefill needs q, out and n_q > 0");
     int rc;
     if ((rc = check_prefill(c, layer, seqs, n_seqs, n_q, out, out_dtype, scale))) return rc;
+    if (any_q8(c, seqs, n_seqs) && (rc = check_current(c))) return rc;
     return prefill_launches(c, layer, seqs, n_seqs, n_q, q, gate, nullptr, KVC_DTYPE_BF16, nullptr, out, out_dtype,
                             scale, stream);
 }
@@ -1347,6 +1497,7 @@ int kvc_prefill_step(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
     if (in_dtype != KVC_DTYPE_F32 && in_dtype != KVC_DTYPE_BF16) return set_err(KVC_ERR_INVALID, "bad in_dtype");
     int rc;
     if ((rc = check_prefill(c, layer, seqs, n_seqs, n_q, out, out_dtype, scale))) return rc;
+    if ((rc = refuse_mixed(c, seqs, n_seqs, "kvc_prefill_step", true))) return rc;
     // the K/V side of the producer (kvc_qkv_append with no q / gate output),
     // then the attention with q and gate built from the rows
     if ((rc = kvc_qkv_append(c, layer, seqs, n_seqs, n_q, qkv, in_dtype, q_norm, k_norm, nullptr, nullptr, stream)))
@@ -1375,8 +1526,35 @@ int kvc_gather(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_seqs, i
     }
     const size_t row = (size_t)kKvHeads * kHeadDim;
     int64_t out_off = 0;
+    if (any_q8(c, seqs, n_seqs) && (rc = check_current(c))) return rc;
     for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
         const int32_t n = std::min(kMaxBatch, n_seqs - i0);
+        if (any_q8(c, seqs + i0, n)) {
+            GatherQ8Args g{};
+            int64_t tot = 0, items = 0;
+            for (int32_t j = 0; j < n; j++) {
+                const int32_t nt = n_tok[i0 + j];
+                g.slot[j] = seqs[i0 + j];
+                g.n8[j] = c->seqs[seqs[i0 + j]].n8;
+                g.out_begin[j] = (int32_t)tot;
+                g.item_begin[j] = (int32_t)items;
+                tot += nt;
+                if (nt > 0) items += (tok0 + nt - 1) / kBlockTok - tok0 / kBlockTok + 1;
+            }
+            g.out_begin[n] = (int32_t)tot;
+            g.item_begin[n] = g.n_items = (int32_t)items;
+            g.c = mixed_cache(c, layer);
+            g.k_out = static_cast<uint16_t*>(k_out) + (size_t)out_off * row;
+            g.v_out = static_cast<uint16_t*>(v_out) + (size_t)out_off * row;
+            g.n_seqs = n;
+            g.tok0 = tok0;
+            if (tot > 0) {
+                int e = launch_gather_q8(g, stream);
+                if (e) return hip_err((hipError_t)e, "gather launch (8-bit blocks)");
+            }
+            out_off += tot;
+            continue;
+        }
         GatherArgs a{};
         int64_t tot = 0, items = 0;
         for (int32_t j = 0; j < n; j++) {
@@ -1413,6 +1591,7 @@ int kvc_kv_checksum(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_se
     int rc;
     if ((rc = check_device(c)) || (rc = check_layer(c, layer)) || (rc = check_seqs(c, seqs, n_seqs))) return rc;
     if (!out) return set_err(KVC_ERR_INVALID, "checksum needs an output array");
+    if ((rc = refuse_mixed(c, seqs, n_seqs, "kvc_kv_checksum", false))) return rc;
     int64_t batch_units = 0;  // units of the current launch
     for (int32_t i = 0; i < n_seqs; i++) {
         const Seq& s = c->seqs[seqs[i]];
@@ -1447,6 +1626,313 @@ int kvc_kv_checksum(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_se
         }
         out_off += units;
     }
+    return KVC_OK;
+}
+
+// ---- 8-bit blocks, attention weights, eviction -------------------------------
+
+static MixedPools mixed_pools(kvc_ctx* c) {
+    MixedPools p{};
+    p.pool = c->d_pool;
+    p.q8 = c->d_q8;
+    p.scales = c->d_scales;
+    p.table = c->d_table;
+    p.layer_kv_bytes = c->layer_kv_bytes;
+    p.q8_kv_bytes = (int64_t)c->cfg.q8_blocks * (int64_t)kQ8BlockBytes;
+    p.scale_kv = (int64_t)c->cfg.q8_blocks * kKvHeads;
+    p.table_stride = c->max_blocks;
+    p.n_layers = c->cfg.n_attn_layers;
+    return p;
+}
+
+// The sequences that kvc_kv_quantize / kvc_evict read (and change, unless dst
+// names the empty sequences that receive the result).
+static int check_src_dst(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, const char* what) {
+    int rc;
+    if ((rc = check_seqs(c, seqs, n_seqs)) || (dst && (rc = check_seqs(c, dst, n_seqs)))) return rc;
+    for (int32_t i = 0; i < n_seqs; i++) {
+        if (c->seqs[seqs[i]].pending)
+            return set_err(KVC_ERR_STATE, "sequence %d has %d uncommitted tokens", seqs[i], c->seqs[seqs[i]].pending);
+        if (!dst) continue;
+        const Seq& d = c->seqs[dst[i]];
+        for (int32_t j = 0; j < n_seqs; j++)
+            if (seqs[j] == dst[i]) return set_err(KVC_ERR_INVALID, "sequence %d is both source and destination", dst[i]);
+        if (d.len || d.pending) return set_err(KVC_ERR_STATE, "destination %d is not empty", dst[i]);
+    }
+    if (dst && c->cfg.n_ssm_layers > 0)
+        return set_err(KVC_ERR_UNSUPPORTED, "%s into other sequences does not copy recurrent state", what);
+    return c->has_device ? check_current(c) : KVC_OK;
+}
+
+int kvc_kv_quantize(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, int32_t keep_tokens,
+                    void* stream) try {
+    if (!c) return set_err(KVC_ERR_INVALID, "null context");
+    int rc;
+    if (keep_tokens < 0) return set_err(KVC_ERR_INVALID, "keep_tokens must be >= 0");
+    if ((rc = check_src_dst(c, seqs, dst, n_seqs, "kvc_kv_quantize"))) return rc;
+    // blocks that become 8-bit ones: [n8, n8 + count)
+    std::vector<int32_t> count(n_seqs);
+    int64_t total = 0;
+    for (int32_t i = 0; i < n_seqs; i++) {
+        const Seq& s = c->seqs[seqs[i]];
+        count[i] = std::max(0, std::max(0, s.len - keep_tokens) / kBlockTok - s.n8);
+        total += count[i];
+    }
+    if (total > (int64_t)c->free_blocks8.size())
+        return set_err(KVC_ERR_NOMEM, "%lld 8-bit blocks needed, %zu of %d free", (long long)total,
+                       c->free_blocks8.size(), c->cfg.q8_blocks);
+    if (total * c->cfg.n_attn_layers * 2 * kKvHeads > INT32_MAX) return set_err(KVC_ERR_RANGE, "quantize too large");
+    for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
+        const int32_t n = std::min(kMaxBatch, n_seqs - i0);
+        QuantizeArgs a{};
+        a.p = mixed_pools(c);
+        a.n_seqs = n;
+        std::vector<std::vector<int32_t>> fresh(n);
+        for (int32_t j = 0; j < n; j++) {
+            const Seq& s = c->seqs[seqs[i0 + j]];
+            const int32_t row = dst ? dst[i0 + j] : c->cfg.max_seqs + j;
+            a.src[j] = seqs[i0 + j];
+            a.dst[j] = row;
+            a.first[j] = s.n8;
+            a.begin[j] = a.n_blocks;
+            a.n_blocks += count[i0 + j];
+            for (int32_t b = 0; b < count[i0 + j]; b++) {
+                const int32_t id = c->free_blocks8.back();
+                c->free_blocks8.pop_back();
+                c->refcnt8[id] = 1;
+                fresh[j].push_back(id);
+                set_table(c, row, s.n8 + b, id);
+            }
+            if (!dst) continue;
+            for (int32_t b = 0; b < (int32_t)s.blocks.size(); b++)  // shared with the source
+                if (b < s.n8 || b >= s.n8 + count[i0 + j]) set_table(c, row, b, s.blocks[b]);
+        }
+        a.begin[n] = a.n_blocks;
+        if ((rc = flush_table(c, stream))) return rc;
+        if (c->has_device && a.n_blocks > 0) {
+            int e = launch_quantize(a, stream);
+            if (e) return hip_err((hipError_t)e, "quantize launch");
+        }
+        for (int32_t j = 0; j < n; j++) {
+            Seq& s = c->seqs[seqs[i0 + j]];
+            const int32_t cnt = count[i0 + j], end = s.n8 + cnt;
+            if (dst) {
+                Seq& d = c->seqs[dst[i0 + j]];
+                for (int32_t b = 0; b < (int32_t)s.blocks.size(); b++) {
+                    const bool made = b >= s.n8 && b < end;
+                    if (!made) (b < s.n8 ? c->refcnt8 : c->refcnt)[s.blocks[b]]++;
+                    d.blocks.push_back(made ? fresh[j][b - s.n8] : s.blocks[b]);
+                }
+                d.len = s.len;
+                d.evicted = s.evicted;
+                d.n8 = end;
+                if (d.len > 0) forget_tokens(c, d);
+                continue;
+            }
+            if (cnt == 0) continue;
+            for (int32_t b = 0; b < cnt; b++) {
+                set_table(c, seqs[i0 + j], s.n8 + b, fresh[j][b]);
+                unref_block(c, s.blocks[s.n8 + b]);
+                s.blocks[s.n8 + b] = fresh[j][b];
+            }
+            s.n8 = end;
+            forget_tokens(c, s);
+        }
+        if (!dst && (rc = flush_table(c, stream))) return rc;
+    }
+    return KVC_OK;
+} catch (const std::bad_alloc&) {
+    return set_err(KVC_ERR_NOMEM, "host allocation failed");
+}
+
+int kvc_attn_weights(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_seqs, int32_t n_q, const void* q,
+                     float scale, const void* acc_in, void* acc_out, int64_t acc_stride, void* stream) {
+    if (!c) return set_err(KVC_ERR_INVALID, "null context");
+    int rc;
+    if ((rc = check_device(c)) || (rc = check_layer(c, layer)) || (rc = check_seqs(c, seqs, n_seqs))) return rc;
+    if (!q || !acc_out || n_q <= 0) return set_err(KVC_ERR_INVALID, "attention weights need q, acc_out and n_q > 0");
+    if (n_q > kWeightsMaxQ)
+        return set_err(KVC_ERR_RANGE, "attention weights of %d rows per sequence (at most %d)", n_q, kWeightsMaxQ);
+    if (!std::isfinite(scale)) return set_err(KVC_ERR_INVALID, "scale must be finite");
+    const int64_t rows = (int64_t)n_q * kGroup;
+    // workspace: scores of one block, statistics of one chunk
+    const auto bytes_of = [&](int64_t blocks, int64_t chunks) {
+        return kKvHeads * rows * (blocks * kBlockTok * 4 + chunks * 8);
+    };
+    const auto chunks_of = [](int64_t blocks) { return (blocks + kWeightsChunk - 1) / kWeightsChunk; };
+    for (int32_t i = 0; i < n_seqs; i++) {
+        const Seq& s = c->seqs[seqs[i]];
+        const int32_t L = s.len + s.pending;
+        if (L < n_q) return set_err(KVC_ERR_STATE, "sequence %d: %d rows but %d cached tokens", seqs[i], n_q, L);
+        if (acc_stride < L)
+            return set_err(KVC_ERR_RANGE, "sequence %d: %d cached tokens, acc_stride %lld", seqs[i], L,
+                           (long long)acc_stride);
+        const int64_t blocks = (L + kBlockTok - 1) / kBlockTok;
+        if (bytes_of(blocks, chunks_of(blocks)) > (int64_t)kPartBytes)
+            return set_err(KVC_ERR_RANGE, "sequence %d: the scores of %d rows over %d keys exceed the workspace", seqs[i],
+                           n_q, L);
+    }
+    if (acc_in && acc_in != acc_out) {
+        const size_t bytes = (size_t)n_seqs * kKvHeads * (size_t)acc_stride * 4;
+        const uint8_t *x = static_cast<const uint8_t*>(acc_in), *y = static_cast<const uint8_t*>(acc_out);
+        if (x < y + bytes && y < x + bytes)
+            return set_err(KVC_ERR_INVALID, "acc_in and acc_out overlap (they may be the same array)");
+    }
+    if ((rc = check_current(c))) return rc;
+    // as many sequences per launch as the workspace holds
+    for (int32_t i0 = 0; i0 < n_seqs;) {
+        WeightsArgs a{};
+        int64_t blocks = 0, chunks = 0, sums = 0;
+        int32_t n = 0;
+        for (; n < kMaxBatch && i0 + n < n_seqs; n++) {
+            const Seq& s = c->seqs[seqs[i0 + n]];
+            const int32_t L = s.len + s.pending;
+            const int64_t nb = (L + kBlockTok - 1) / kBlockTok;
+            if (n > 0 && bytes_of(blocks + nb, chunks + chunks_of(nb)) > (int64_t)kPartBytes) break;
+            a.slot[n] = seqs[i0 + n];
+            a.kv_len[n] = L;
+            a.n8[n] = s.n8;
+            a.block_begin[n] = (int32_t)blocks;
+            a.chunk_begin[n] = (int32_t)chunks;
+            a.sum_begin[n] = (int32_t)sums;
+            blocks += nb;
+            chunks += chunks_of(nb);
+            sums += (nb + kWsumBlocks - 1) / kWsumBlocks;
+        }
+        a.block_begin[n] = a.total_blocks = (int32_t)blocks;
+        a.chunk_begin[n] = a.total_chunks = (int32_t)chunks;
+        a.sum_begin[n] = a.sum_chunks = (int32_t)sums;
+        a.c = mixed_cache(c, layer);
+        a.q = static_cast<const uint16_t*>(q) + (size_t)i0 * n_q * kQHeads * kHeadDim;
+        const size_t off = (size_t)i0 * kKvHeads * (size_t)acc_stride;
+        a.acc_in = acc_in ? static_cast<const float*>(acc_in) + off : nullptr;
+        a.acc_out = static_cast<float*>(acc_out) + off;
+        a.stats = c->d_part;
+        a.scores = c->d_part + (size_t)kKvHeads * rows * 2 * (size_t)chunks;
+        a.stride = acc_stride;
+        a.scale_log2 = scale * 1.4426950408889634f;
+        a.n_seqs = n;
+        a.n_q = n_q;
+        int e = launch_weights(a, stream);
+        if (e) return hip_err((hipError_t)e, "attention weights launch");
+        i0 += n;
+    }
+    return KVC_OK;
+}
+
+int kvc_evict(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, int32_t budget, int32_t n_sink,
+              int32_t n_recent, const void* acc, void* acc_out, int64_t acc_stride, int32_t* kept, void* stream) try {
+    if (!c) return set_err(KVC_ERR_INVALID, "null context");
+    int rc;
+    if (budget <= 0 || n_sink < 0 || n_recent < 0 || (int64_t)n_sink + n_recent > budget)
+        return set_err(KVC_ERR_INVALID, "evict needs a positive budget that holds n_sink + n_recent tokens");
+    if (!acc || !kept) return set_err(KVC_ERR_INVALID, "evict needs acc and kept");
+    if ((rc = check_src_dst(c, seqs, dst, n_seqs, "kvc_evict"))) return rc;
+    for (int32_t i = 0; i < n_seqs; i++)
+        if (acc_stride < c->seqs[seqs[i]].len)
+            return set_err(KVC_ERR_RANGE, "sequence %d: %d cached tokens, acc_stride %lld", seqs[i],
+                           c->seqs[seqs[i]].len, (long long)acc_stride);
+    if (acc_out) {
+        const size_t bytes = (size_t)c->cfg.n_attn_layers * n_seqs * kKvHeads * (size_t)acc_stride * 4;
+        const uint8_t *x = static_cast<const uint8_t*>(acc), *y = static_cast<const uint8_t*>(acc_out);
+        if (x < y + bytes && y < x + bytes) return set_err(KVC_ERR_INVALID, "acc and acc_out overlap");
+    }
+    // fresh blocks for every sequence that changes, before anything is moved
+    std::vector<std::vector<int32_t>> fresh(n_seqs);
+    int64_t total = 0;
+    bool fail = false;
+    for (int32_t i = 0; i < n_seqs && !fail; i++) {
+        const Seq& s = c->seqs[seqs[i]];
+        if (!dst && s.len <= budget) continue;  // keeps all of its tokens, where they are
+        const int32_t need = (std::min(s.len, budget) + kBlockTok - 1) / kBlockTok;
+        for (int32_t b = 0; b < need; b++) {
+            const int32_t id = alloc_block(c);
+            if (id < 0) { fail = true; break; }
+            fresh[i].push_back(id);
+        }
+        total += need;
+    }
+    if (fail || total * c->cfg.n_attn_layers * 2 * kKvHeads > INT32_MAX) {
+        for (const auto& f : fresh)
+            for (int32_t id : f) unref_block(c, id);
+        if (!fail) return set_err(KVC_ERR_RANGE, "evict too large");
+        return set_err(KVC_ERR_NOMEM, "block pool exhausted: eviction writes the kept tokens to fresh blocks");
+    }
+    for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
+        const int32_t n = std::min(kMaxBatch, n_seqs - i0);
+        EvictSelectArgs sel{};
+        EvictCopyArgs cp{};
+        sel.acc = static_cast<const float*>(acc);
+        sel.acc_out = static_cast<float*>(acc_out);
+        sel.kept = kept;
+        cp.kept = kept;
+        sel.stride = acc_stride;
+        sel.call_seqs = cp.call_seqs = n_seqs;
+        sel.seq0 = cp.seq0 = i0;
+        sel.n_seqs = cp.n_seqs = n;
+        sel.n_layers = c->cfg.n_attn_layers;
+        sel.budget = cp.budget = budget;
+        sel.n_sink = n_sink;
+        sel.n_recent = n_recent;
+        cp.p = mixed_pools(c);
+        for (int32_t j = 0; j < n; j++) {
+            const Seq& s = c->seqs[seqs[i0 + j]];
+            const int32_t row = dst ? dst[i0 + j] : c->cfg.max_seqs + j;
+            sel.len[j] = s.len;
+            cp.src[j] = seqs[i0 + j];
+            cp.dst[j] = row;
+            cp.n8[j] = s.n8;
+            cp.new_len[j] = std::min(s.len, budget);
+            cp.begin[j] = cp.n_blocks;
+            cp.n_blocks += (int32_t)fresh[i0 + j].size();
+            for (int32_t b = 0; b < (int32_t)fresh[i0 + j].size(); b++) set_table(c, row, b, fresh[i0 + j][b]);
+        }
+        cp.begin[n] = cp.n_blocks;
+        if ((rc = flush_table(c, stream))) return rc;
+        if (c->has_device) {
+            int e = launch_evict_select(sel, stream);
+            if (e) return hip_err((hipError_t)e, "evict selection launch");
+            if (cp.n_blocks > 0 && (e = launch_evict_copy(cp, stream)))
+                return hip_err((hipError_t)e, "evict copy launch");
+        }
+        for (int32_t j = 0; j < n; j++) {
+            Seq& s = c->seqs[seqs[i0 + j]];
+            const std::vector<int32_t>& f = fresh[i0 + j];
+            const int32_t gone = std::max(0, s.len - budget);
+            if (!dst && f.empty()) continue;
+            Seq& d = dst ? c->seqs[dst[i0 + j]] : s;
+            const int32_t new_len = s.len - gone, evicted = s.evicted + gone;
+            if (!dst) {
+                release_tail(c, seqs[i0 + j], 0);
+                for (int32_t b = 0; b < (int32_t)f.size(); b++) set_table(c, seqs[i0 + j], b, f[b]);
+            }
+            d.blocks = f;
+            d.len = new_len;
+            d.evicted = evicted;
+            if (d.len > 0) forget_tokens(c, d);
+        }
+        if (!dst && (rc = flush_table(c, stream))) return rc;
+    }
+    return KVC_OK;
+} catch (const std::bad_alloc&) {
+    return set_err(KVC_ERR_NOMEM, "host allocation failed");
+}
+
+int kvc_seq_get_info(kvc_ctx* c, int32_t seq, kvc_seq_info* out) {
+    if (!c || !out) return set_err(KVC_ERR_INVALID, "null argument");
+    if (!seq_ok(c, seq)) return set_err(KVC_ERR_INVALID, "sequence %d is not live", seq);
+    const Seq& s = c->seqs[seq];
+    out->len = s.len;
+    out->pending = s.pending;
+    out->position = s.len + s.evicted;
+    out->q8_tokens = s.n8 * kBlockTok;
+    return KVC_OK;
+}
+
+int kvc_q8_stats(kvc_ctx* c, int64_t* blocks, int64_t* free_blocks) {
+    if (!c || !blocks || !free_blocks) return set_err(KVC_ERR_INVALID, "null argument");
+    *blocks = c->cfg.q8_blocks;
+    *free_blocks = (int64_t)c->free_blocks8.size();
     return KVC_OK;
 }
 
@@ -1554,6 +2040,9 @@ int kvc_snapshot_save(kvc_ctx* c, const int32_t* seqs, int32_t n_seqs, int32_t* 
         if (s.pending) return set_err(KVC_ERR_STATE, "sequence %d has uncommitted tokens", seqs[i]);
         if (s.len <= 0 || s.len % iv)
             return set_err(KVC_ERR_STATE, "sequence %d length %d is not a positive multiple of %d", seqs[i], s.len, iv);
+        if (s.evicted > 0 || s.n8 > (s.len - iv) / kBlockTok)
+            return set_err(KVC_ERR_UNSUPPORTED, "sequence %d: a snapshot holds whole segments in bf16 (8-bit blocks or "
+                           "evicted tokens)", seqs[i]);
     }
     // Count the slots first (free, or held by an unpinned snapshot that may
     // be evicted), so that a save that cannot fit fails with no side effect.
@@ -1593,6 +2082,8 @@ int kvc_snapshot_restore(kvc_ctx* c, const int32_t* seqs, const int32_t* snap_id
         if (s.len < c->snaps[id].boundary - iv)
             return set_err(KVC_ERR_STATE, "sequence %d holds %d tokens; snapshot at %d needs %d", seqs[i], s.len,
                            c->snaps[id].boundary, c->snaps[id].boundary - iv);
+        if (s.evicted > 0)
+            return set_err(KVC_ERR_UNSUPPORTED, "sequence %d had tokens evicted: reset it before a restore", seqs[i]);
     }
     // allocate fresh segment blocks for every pair first
     std::vector<int32_t> granted;

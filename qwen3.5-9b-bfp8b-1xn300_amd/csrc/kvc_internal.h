@@ -9,6 +9,17 @@
 // every layer's pool.  The reference keeps one contiguous fp32 array per layer
 // instead (src/engine.cpp:81-84, index pos*kv_dim + kv_h*D + d at :3539).
 //
+// 8-bit blocks live in pools of their own (kvc_config.q8_blocks), ids shared by
+// all layers too; a sequence's leading blocks may be 8-bit ones, and its table
+// entries for those name blocks of
+//   q8[layer][kv][block][kv_head][8 KiB]   int8, one unit = 32 tokens x 256 dims
+//   scale[layer][kv][block][kv_head]       fp32
+// A unit holds its 16-byte pieces in the order in which a wave's lanes read
+// them as matrix operands (lane = 16 g + c):
+//   K piece (t, s, lane): token 16 t + c, dims 64 s + 16 g .. + 15
+//   V piece (p, lane):    dim 32 p + c, then dim 32 p + 16 + c, of the tokens
+//                         4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3
+//
 // Recurrent state of a sequence slot (one contiguous region per slot):
 //   [ssm_layer][ rec fp32 [v_heads][v_dim][k_dim] | conv fp32 [rows][channels] ]
 // matching g_ssm_state / g_conv_state (src/engine.cpp:86-94, :3840-3843).
@@ -30,6 +41,9 @@ constexpr int kQHeads = kKvHeads * kGroup;
 constexpr int kBlockTok = 32;
 constexpr size_t kUnitBytes = (size_t)kBlockTok * kHeadDim * 2;  // 16 KiB
 constexpr size_t kBlockBytes = kUnitBytes * kKvHeads;            // 64 KiB
+
+constexpr size_t kQ8UnitBytes = (size_t)kBlockTok * kHeadDim;   // 8 KiB
+constexpr size_t kQ8BlockBytes = kQ8UnitBytes * kKvHeads;        // 32 KiB
 
 constexpr int kMaxBatch = 64;        // seqs per kernel launch (argument block)
 constexpr int kMaxChunks = 8192;     // split-K work chunks per decode launch
@@ -153,7 +167,8 @@ struct QkvArgs {
     int32_t n_tok;
     int32_t pad;
     int32_t slot[kMaxBatch];
-    int32_t pos0[kMaxBatch];  // first position written
+    int32_t pos0[kMaxBatch];   // first cache position written
+    int32_t rope0[kMaxBatch];  // its position in the text (RoPE): pos0 + evicted tokens
 };
 
 // Gated-DeltaNet shapes the step kernel is built for (model_config.h:25-31)
@@ -273,6 +288,159 @@ struct PrefillArgs {
     int32_t q_pos0[kMaxBatch];  // position of query row 0
     int32_t seq_order[kMaxBatch];  // batch indices, most keys first
     int32_t unit_begin[kMaxBatch + 1];  // first unit of each sequence, in seq_order
+    // sequences with leading 8-bit blocks (k8 not null): this layer's 8-bit
+    // pools and scales, and the 8-bit blocks of each sequence
+    int32_t pad3;
+    const uint8_t* k8;
+    const uint8_t* v8;
+    const float* ks;
+    const float* vs;
+    int32_t n8[kMaxBatch];
+};
+
+// ---- 8-bit blocks and eviction -------------------------------------------
+
+// One layer's K and V, in bf16 and in 8 bits.
+struct MixedCache {
+    const uint16_t* kpool;
+    const uint16_t* vpool;
+    const uint8_t* k8;
+    const uint8_t* v8;
+    const float* ks;
+    const float* vs;
+    const int32_t* table;
+    int32_t table_stride;
+    int32_t pad;
+};
+
+// Decode over sequences that start with 8-bit blocks.  Chunks of a sequence:
+// those of its 8-bit blocks (cb8 blocks each), then those of its bf16 blocks
+// (cbf each).
+struct DecodeQ8Args {
+    MixedCache c;
+    const uint16_t* q;      // as DecodeArgs
+    const uint16_t* k_new;
+    const uint16_t* v_new;
+    const uint16_t* gate;
+    void* out;
+    float* part;
+    int32_t* counters;
+    uint32_t part_bytes;
+    float scale_log2;
+    int32_t out_bf16;
+    int32_t gate_ref;
+    int32_t n_seqs;
+    int32_t cb8;
+    int32_t cbf;
+    int32_t total_chunks;
+    int32_t n_items;
+    int32_t per_xcd;
+    int32_t slot[kMaxBatch];
+    int32_t kv_len[kMaxBatch];
+    int32_t n8[kMaxBatch];
+    int32_t chunk_begin[kMaxBatch + 1];
+};
+
+// All layers of the K/V pools and of the 8-bit pools.
+struct MixedPools {
+    uint8_t* pool;
+    uint8_t* q8;
+    float* scales;
+    const int32_t* table;
+    int64_t layer_kv_bytes;   // of one (layer, kv) bf16 pool
+    int64_t q8_kv_bytes;      // of one (layer, kv) 8-bit pool
+    int64_t scale_kv;         // scales of one (layer, kv)
+    int32_t table_stride;
+    int32_t n_layers;
+};
+
+// bf16 blocks [first, first + count) of table row src into the 8-bit blocks
+// that table row dst names at the same indices, K and V of every layer.
+struct QuantizeArgs {
+    MixedPools p;
+    int32_t n_seqs;
+    int32_t n_blocks;                 // sum of counts
+    int32_t src[kMaxBatch];
+    int32_t dst[kMaxBatch];
+    int32_t first[kMaxBatch];
+    int32_t begin[kMaxBatch + 1];     // first block of each sequence in the launch
+};
+
+// Gather over sequences with 8-bit blocks: one work item = one cache block.
+struct GatherQ8Args {
+    MixedCache c;
+    uint16_t* k_out;
+    uint16_t* v_out;
+    int32_t n_seqs;
+    int32_t tok0;
+    int32_t n_items;
+    int32_t pad;
+    int32_t slot[kMaxBatch];
+    int32_t n8[kMaxBatch];
+    int32_t out_begin[kMaxBatch + 1];
+    int32_t item_begin[kMaxBatch + 1];
+};
+
+// Attention weights: the scores of every (kv head, block, row, key) and per
+// chunk the rows' (max, sum) go through the workspace.  Rows of a kv head:
+// query i, q head g of the group -> row 4 i + g.
+struct WeightsArgs {
+    MixedCache c;
+    const uint16_t* q;        // [n_seqs][n_q][Hq][D]
+    const float* acc_in;      // [n_seqs][Hkv][stride] or null (zeros)
+    float* acc_out;
+    float* scores;            // [sequence's block][row][32] per kv head
+    float* stats;             // [chunk of all][row][max, sum]
+    int64_t stride;
+    float scale_log2;
+    int32_t n_seqs;
+    int32_t n_q;
+    int32_t total_chunks;     // of kWeightsChunk blocks, per kv head
+    int32_t total_blocks;
+    int32_t sum_chunks;       // of kWsumBlocks blocks each
+    int32_t slot[kMaxBatch];
+    int32_t kv_len[kMaxBatch];
+    int32_t n8[kMaxBatch];
+    int32_t block_begin[kMaxBatch + 1];
+    int32_t chunk_begin[kMaxBatch + 1];
+    int32_t sum_begin[kMaxBatch + 1];
+};
+constexpr int kWeightsChunk = 4;   // blocks per workgroup of the scoring launch
+constexpr int kWsumBlocks = 8;     // blocks per workgroup of the summing launch
+constexpr int kWeightsMaxQ = 256;  // query rows per sequence
+
+// Which tokens stay: one row per (layer, sequence, kv head).
+struct EvictSelectArgs {
+    const float* acc;         // [layers][call's seqs][Hkv][stride]
+    float* acc_out;           // likewise or null
+    int32_t* kept;            // [layers][call's seqs][Hkv][budget]
+    int64_t stride;
+    int32_t call_seqs;        // sequences of the call
+    int32_t seq0;             // of them, the first of this launch
+    int32_t n_seqs;
+    int32_t n_layers;
+    int32_t budget;
+    int32_t n_sink;
+    int32_t n_recent;
+    int32_t pad;
+    int32_t len[kMaxBatch];
+};
+
+// Moves the kept rows into fresh bf16 blocks.
+struct EvictCopyArgs {
+    MixedPools p;
+    const int32_t* kept;
+    int32_t call_seqs;
+    int32_t seq0;
+    int32_t n_seqs;
+    int32_t budget;
+    int32_t n_blocks;                 // new blocks of the launch
+    int32_t pad;
+    int32_t src[kMaxBatch];           // table rows
+    int32_t dst[kMaxBatch];
+    int32_t n8[kMaxBatch];            // of the source
+    int32_t new_len[kMaxBatch];
+    int32_t begin[kMaxBatch + 1];
 };
 
 // Snapshot copy: per pair, state bytes then the K/V segment.
@@ -307,6 +475,10 @@ struct BlockCopyArgs {
     int32_t dst[kMaxBatch];
 };
 
+static_assert(sizeof(DecodeQ8Args) < 4096 && sizeof(QuantizeArgs) < 4096 && sizeof(GatherQ8Args) < 4096 &&
+                  sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillArgs) < 4096,
+              "argument blocks are passed by value");
+
 // ---- launchers (kvc_kernels.hip); return hipError_t as int ---------------
 // Device address of this GPU's static decode workspace (split-K partials,
 // then the arrival counters), looked up once per device with
@@ -325,6 +497,12 @@ int launch_checksum(const ChecksumArgs& a, void* stream);
 int launch_prefill(const PrefillArgs& a, void* stream);
 int launch_snapshot(const SnapshotArgs& a, void* stream);
 int launch_block_copy(const BlockCopyArgs& a, void* stream);
+int launch_decode_q8(const DecodeQ8Args& a, void* stream);
+int launch_quantize(const QuantizeArgs& a, void* stream);
+int launch_gather_q8(const GatherQ8Args& a, void* stream);
+int launch_weights(const WeightsArgs& a, void* stream);
+int launch_evict_select(const EvictSelectArgs& a, void* stream);
+int launch_evict_copy(const EvictCopyArgs& a, void* stream);
 int launch_fill_normal(uint16_t* dst, int64_t n, uint64_t seed, float scale,
                        void* stream);
 

@@ -46,7 +46,8 @@ EXPORTS = [
     "kvc_seq_commit", "kvc_prefix_match", "kvc_append", "kvc_qkv_append", "kvc_decode_attn",
     "kvc_decode_attn_static", "kvc_decode_step", "kvc_prefill_attn", "kvc_prefill_step", "kvc_gather", "kvc_kv_checksum", "kvc_state_ptrs", "kvc_deltanet_step", "kvc_snapshot_save",
     "kvc_snapshot_restore", "kvc_snapshot_release", "kvc_pool_fill_normal",
-    "kvc_fill_normal_bf16", "kvc_sync",
+    "kvc_fill_normal_bf16", "kvc_sync", "kvc_kv_quantize", "kvc_attn_weights", "kvc_evict", "kvc_seq_get_info",
+    "kvc_q8_stats",
 ]
 
 
@@ -70,7 +71,7 @@ class Config(ctypes.Structure):
         ("device", ctypes.c_int32), ("flags", ctypes.c_uint32),
         ("alloc_seed", ctypes.c_uint64),
         ("rms_norm_eps", ctypes.c_float), ("rope_freq_base", ctypes.c_float),
-        ("rope_dim", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("rope_dim", ctypes.c_int32), ("q8_blocks", ctypes.c_int32),
     ]
 
 
@@ -79,6 +80,10 @@ class Stats(ctypes.Structure):
         "pool_blocks", "free_blocks", "cached_blocks", "indexed_blocks",
         "snapshots", "snapshot_slots", "hbm_bytes", "block_bytes",
         "prefix_hits", "evictions")]
+
+
+class SeqInfo(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("len", "pending", "position", "q8_tokens")]
 
 
 _lib = None
@@ -128,6 +133,11 @@ def lib() -> ctypes.CDLL:
             "kvc_pool_fill_normal": (ctypes.c_int, [P, U64, P]),
             "kvc_fill_normal_bf16": (ctypes.c_int, [P, P, I64, U64, F32, P]),
             "kvc_sync": (ctypes.c_int, [P, P]),
+            "kvc_kv_quantize": (ctypes.c_int, [P, pI32, pI32, I32, I32, P]),
+            "kvc_attn_weights": (ctypes.c_int, [P, I32, pI32, I32, I32, P, F32, P, P, I64, P]),
+            "kvc_evict": (ctypes.c_int, [P, pI32, pI32, I32, I32, I32, I32, P, P, I64, P, P]),
+            "kvc_seq_get_info": (ctypes.c_int, [P, I32, ctypes.POINTER(SeqInfo)]),
+            "kvc_q8_stats": (ctypes.c_int, [P, ctypes.POINTER(I64), ctypes.POINTER(I64)]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -138,6 +148,8 @@ def lib() -> ctypes.CDLL:
 
 
 def _i32(seq):
+    if isinstance(seq, ctypes.Array) and seq._type_ is ctypes.c_int32:  # made before, to be passed many times
+        return seq
     arr = (ctypes.c_int32 * len(seq))(*[int(x) for x in seq])
     return arr
 
@@ -412,6 +424,38 @@ class Context:
     def gather(self, layer, seqs, tok0, n_tok, k_out, v_out, stream=None):
         _check(self.L.kvc_gather(self.ptr, layer, _i32(seqs), len(seqs), tok0, _i32(n_tok),
                                  self._p(k_out), self._p(v_out), stream))
+
+    def kv_quantize(self, seqs, keep_tokens=0, dst=None, stream=None):
+        """full blocks before the last keep_tokens tokens into 8 bits, in place or as copies in dst"""
+        _check(self.L.kvc_kv_quantize(self.ptr, _i32(seqs), None if dst is None else self._pair(seqs, dst), len(seqs),
+                                      keep_tokens, stream))
+
+    def attn_weights(self, layer, seqs, n_q, q, acc_out, acc_stride, acc_in=None, scale=1.0 / 16, stream=None):
+        """acc_out = acc_in + the weight that the last n_q tokens' queries give every cached token"""
+        _check(self.L.kvc_attn_weights(self.ptr, layer, _i32(seqs), len(seqs), n_q, self._p(q), ctypes.c_float(scale),
+                                       self._p(acc_in), self._p(acc_out), acc_stride, stream))
+
+    def evict(self, seqs, budget, acc, acc_stride, kept, n_sink=0, n_recent=0, dst=None, acc_out=None, stream=None):
+        """cut to the budget tokens of greatest acc per layer and kv head, in place or as copies in dst"""
+        _check(self.L.kvc_evict(self.ptr, _i32(seqs), None if dst is None else self._pair(seqs, dst), len(seqs), budget,
+                                n_sink, n_recent, self._p(acc), self._p(acc_out), acc_stride, self._p(kept), stream))
+
+    @staticmethod
+    def _pair(seqs, dst):
+        if len(dst) != len(seqs):
+            raise ValueError(f"{len(seqs)} sequences, {len(dst)} destinations")
+        return _i32(dst)
+
+    def seq_info(self, s) -> SeqInfo:
+        i = SeqInfo()
+        _check(self.L.kvc_seq_get_info(self.ptr, s, ctypes.byref(i)))
+        return i
+
+    def q8_stats(self):
+        """(8-bit blocks per layer, of them free)"""
+        n, f = ctypes.c_int64(), ctypes.c_int64()
+        _check(self.L.kvc_q8_stats(self.ptr, ctypes.byref(n), ctypes.byref(f)))
+        return n.value, f.value
 
     def kv_checksum(self, layer, seqs, out, stream=None):
         """out (device uint64) = per-unit checksums of each seq's K/V in `layer`"""

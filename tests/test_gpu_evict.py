@@ -1,0 +1,367 @@
+"""GPU tests of attention weights and eviction against 64-bit results, alone and
+in the run they are made for: attend, accumulate, evict, park in 8 bits, go on.
+
+Tolerance of the accumulated weights (derived): a weight's score is within
+2^-22 B of the exact one in the log2 domain (B as in test_gpu_q8.py), the
+exponential, the row's sum and the division add 2^-21, and the sum over the
+rows of a token loses at most 2^-24 of the result per row."""
+import numpy as np
+import pytest
+
+import _oracle as O
+import kvc
+import q8_ref as Q
+from gpu_util import D, NKV, NQ, say
+
+pytestmark = pytest.mark.gpu
+SCALE = 1.0 / 16
+
+
+def weights_case(lens, n_q, keep, scale=SCALE, seed=90, acc="own", pending=0, stride_more=3):
+    with Q.Filled(lens, seed=seed, extra=pending) as f:
+        f.ctx.kv_quantize(f.seqs, keep)
+        if pending:
+            f.add(f.seqs, pending, commit=False)
+        n = len(lens)
+        total = [x + pending for x in lens]
+        stride = max(total) + stride_more
+        q = O.normal_bf16(n * n_q * NQ * D, seed + 1).reshape(n, n_q, NQ, D)
+        start = np.random.default_rng(seed).random((n, NKV, stride)).astype(np.float32)
+        qb, ab, ob = kvc.to_device(q), kvc.to_device(start), kvc.to_device(np.full_like(start, 7.0))
+        src = {"own": ab, "none": None, "same": ob}[acc]
+        if acc == "same":
+            ob.upload(start)
+        f.ctx.attn_weights(0, f.seqs, n_q, qb, ob, stride, acc_in=src, scale=scale)
+        f.ctx.sync()
+        got = ob.download(np.float32, start.shape)
+        if acc != "same":  # the same call, the same bits
+            f.ctx.attn_weights(0, f.seqs, n_q, qb, ob, stride, acc_in=src, scale=scale)
+            f.ctx.sync()
+            assert np.array_equal(ob.download(np.uint32, start.shape), got.view(np.uint32))
+            assert np.array_equal(ab.download(np.uint32, start.shape), start.view(np.uint32))
+        for x in (qb, ab, ob):
+            x.free()
+        for i, s in enumerate(f.seqs):
+            n8 = max(0, lens[i] - keep) // 32 * 32
+            k = Q.values(f.rows[0, s][0], n8)
+            w = Q.weights(Q.f64(q[i]), k, scale, total[i] - n_q)
+            _, _, big = Q.attend(Q.f64(q[i]), k, k, scale, first=total[i] - n_q)
+            base = start[i].astype(np.float64) if acc != "none" else np.zeros((NKV, stride))
+            want = base[:, :total[i]] + w
+            rows = 4 * n_q
+            tol = w * (2.0 ** -22 * big + 2.0 ** -21) + want * 2.0 ** -24 * (rows + 1)
+            off = np.abs(got[i, :, :total[i]] - want) / np.maximum(tol, 1e-30)
+            assert off.max() <= 1.0, (i, lens[i], float(off.max()))
+            say(f"  {n_q} rows over {total[i]} ({n8} in 8 bits): {off.max():.3f} of the tolerance")
+            rest = start[i, :, total[i]:] if acc == "same" else np.float32(7.0)
+            assert (got[i, :, total[i]:] == rest).all()
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 127, 128, 129, 300, 1000, 4100])
+@pytest.mark.parametrize("keep", [0, 10 ** 6])
+def test_weights_of_one_token(n, keep):
+    say(f"weights {n} keep {keep}")
+    weights_case([n], 1, keep, seed=91 + n)
+
+
+@pytest.mark.parametrize("n,n_q", [(2, 2), (33, 33), (40, 3), (64, 16), (300, 5), (300, 32), (511, 100), (700, 256)])
+def test_weights_of_several_rows(n, n_q):
+    """rows that end inside 8-bit blocks too: the last of them are committed"""
+    say(f"weights {n_q} rows of {n}")
+    weights_case([n], n_q, 0, seed=92 + n)
+
+
+@pytest.mark.parametrize("acc", ["own", "none", "same"])
+def test_weights_of_a_ragged_batch(acc):
+    say(f"weights ragged acc {acc}")
+    weights_case([7, 32, 64, 100, 1500, 333, 96, 12], 7, 50, seed=93, acc=acc)
+
+
+def test_weights_with_pending_rows():
+    say("weights pending")
+    weights_case([100, 64, 31], 4, 0, seed=94, pending=4, stride_more=0)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.25])
+def test_weights_scales(scale):
+    say(f"weights scale {scale}")
+    weights_case([200], 3, 40, scale=scale, seed=95)
+
+
+def test_weights_in_several_launches():
+    """70 sequences, and scores that fill the workspace more than once: 40
+    sequences of 2000 keys, 128 rows each"""
+    say("weights 70 sequences")
+    weights_case([int(x) for x in np.random.default_rng(1).integers(5, 200, 70)], 3, 20, seed=96)
+    say("weights 128 rows")
+    weights_case([2000] * 12, 128, 0, seed=97)
+
+
+def test_weights_refusals():
+    say("weights refusals")
+    with Q.Filled([100, 40], seed=98) as f:
+        c, (a, b) = f.ctx, f.seqs
+        buf = kvc.hip().malloc(1 << 20).zero()
+        P = buf.ptr
+        for code, args in [
+            (kvc.KVC_ERR_INVALID, dict(seqs=[a], n_q=0, q=P, acc_out=P, acc_stride=100)),
+            (kvc.KVC_ERR_INVALID, dict(seqs=[a], n_q=1, q=None, acc_out=P, acc_stride=100)),
+            (kvc.KVC_ERR_INVALID, dict(seqs=[a], n_q=1, q=P, acc_out=None, acc_stride=100)),
+            (kvc.KVC_ERR_INVALID, dict(seqs=[a], n_q=1, q=P, acc_out=P, acc_stride=100, scale=float("nan"))),
+            (kvc.KVC_ERR_INVALID, dict(seqs=[a, a], n_q=1, q=P, acc_out=P, acc_stride=100)),
+            (kvc.KVC_ERR_INVALID, dict(seqs=[a], n_q=1, q=P, acc_out=P, acc_in=P + 400, acc_stride=100)),
+            (kvc.KVC_ERR_RANGE, dict(seqs=[b], n_q=257, q=P, acc_out=P, acc_stride=100)),
+            (kvc.KVC_ERR_RANGE, dict(seqs=[a], n_q=1, q=P, acc_out=P, acc_stride=99)),
+            (kvc.KVC_ERR_STATE, dict(seqs=[a, b], n_q=41, q=P, acc_out=P, acc_stride=100)),
+        ]:
+            with pytest.raises(kvc.KvcError) as e:
+                c.attn_weights(0, **args)
+            assert e.value.code == code, args
+        with pytest.raises(kvc.KvcError) as e:
+            c.attn_weights(1, [a], 1, P, P, 100)
+        assert e.value.code == kvc.KVC_ERR_RANGE
+        c.sync()
+        assert not buf.download(np.uint8, (1 << 20,)).any()
+        buf.free()
+
+
+# ---- eviction -------------------------------------------------------------------
+
+
+def accumulated(kind, shape, rng):
+    a = rng.random(shape).astype(np.float32) ** 6
+    if kind == "ties":
+        a = np.floor(a * 8).astype(np.float32) / 8
+    elif kind == "equal":
+        a[:] = 0.25
+    elif kind == "special":
+        a = rng.normal(size=shape).astype(np.float32)  # negative ones too
+        flat = a.reshape(-1)
+        pick = rng.permutation(flat.size)
+        m = max(1, flat.size // 12)
+        for j, x in enumerate((np.nan, np.inf, -np.inf, 0.0, -0.0, 1e-42)):
+            flat[pick[j * m:(j + 1) * m]] = x
+    return a
+
+
+def evict_case(lens, budget, sink, recent, kind, copy, keep=10 ** 6, seed=100, layers=2, with_acc_out=True):
+    with Q.Filled(lens, layers=layers, seed=seed) as f:
+        f.ctx.kv_quantize(f.seqs, keep)
+        n, stride = len(lens), max(lens) + 5
+        acc = accumulated(kind, (layers, n, NKV, stride), np.random.default_rng(seed))
+        ab = kvc.to_device(acc)
+        kb = kvc.hip().malloc(layers * n * NKV * budget * 4)
+        kb.upload(np.full((layers, n, NKV, budget), -9, np.int32))
+        ob = kvc.to_device(np.full_like(acc, 7.0)) if with_acc_out else None
+        dst = [f.ctx.seq_create() for _ in lens] if copy else None
+        f.ctx.evict(f.seqs, budget, ab, stride, kb, n_sink=sink, n_recent=recent, dst=dst, acc_out=ob)
+        f.ctx.sync()
+        kept = kb.download(np.int32, (layers, n, NKV, budget))
+        out = ob.download(np.float32, acc.shape) if with_acc_out else None
+        assert np.array_equal(ab.download(np.uint32, acc.shape), acc.view(np.uint32))
+        for i, L in enumerate(lens):
+            new = min(L, budget)
+            s = dst[i] if copy else f.seqs[i]
+            assert f.ctx.seq_len(s) == new and f.ctx.seq_info(s).position == L
+            n8 = max(0, L - keep) // 32 * 32
+            for layer in range(layers):
+                rows = [Q.readback(x, n8) for x in f.rows[layer, f.seqs[i]]]
+                got = f.gather(layer, s, new)
+                for h in range(NKV):
+                    want = Q.keep(acc[layer, i, h, :L], budget, sink, recent)
+                    assert np.array_equal(kept[layer, i, h, :new], want), (L, layer, h)
+                    assert (kept[layer, i, h, new:] == -1).all()
+                    if out is not None:
+                        assert np.array_equal(out[layer, i, h, :new].view(np.uint32),
+                                              acc[layer, i, h][want].view(np.uint32))
+                        assert (out[layer, i, h, new:L] == 0).all() and (out[layer, i, h, L:] == 7).all()
+                    for j in range(2):
+                        Q.same_bits(got[j][:, h], rows[j][want, h])
+                if copy:
+                    for j in range(2):
+                        Q.same_bits(f.gather(layer, f.seqs[i], L)[j], rows[j])
+        for b in (ab, kb, ob):
+            if b is not None:
+                b.free()
+
+
+@pytest.mark.parametrize("kind", ["plain", "ties", "equal", "special"])
+@pytest.mark.parametrize("copy", [False, True])
+def test_evict_choices(kind, copy):
+    say(f"evict {kind} copy {copy}")
+    evict_case([300, 64, 65, 1, 1100, 200], 64, 3, 20, kind, copy, seed=101)
+
+
+@pytest.mark.parametrize("budget,sink,recent", [(1, 0, 0), (1, 1, 0), (1, 0, 1), (50, 50, 0), (50, 0, 50), (33, 16, 17),
+                                                (199, 0, 0), (200, 4, 4), (500, 1, 1)])
+def test_evict_budgets(budget, sink, recent):
+    say(f"evict {budget} {sink} {recent}")
+    evict_case([200, 33], budget, sink, recent, "ties", False, seed=102, with_acc_out=budget % 2 == 0)
+
+
+def test_evict_long_rows():
+    """rows longer than a workgroup, with ties across its passes"""
+    say("evict 5000")
+    evict_case([5000, 2048, 1025], 1001, 2, 100, "ties", True, seed=103, layers=1)
+
+
+@pytest.mark.parametrize("keep", [0, 100])
+def test_evict_8_bit_sources(keep):
+    say(f"evict 8-bit keep {keep}")
+    evict_case([300, 128, 97], 90, 1, 7, "plain", keep == 0, keep=keep, seed=104)
+
+
+def test_evict_70_sequences():
+    say("evict 70")
+    evict_case([int(x) for x in np.random.default_rng(9).integers(1, 150, 70)], 40, 2, 5, "plain", False, seed=105, layers=1)
+
+
+def test_positions_go_on_after_eviction():
+    """kvc_qkv_append rotates a new token at its position in the text: the rows
+    equal those of a sequence that kept everything; the one-launch steps and the
+    snapshots refuse the cut sequence."""
+    say("evict positions")
+    rng = np.random.default_rng(6)
+    with Q.Filled([150, 150, 90], seed=106, extra=4, rope_dim=64, snapshot_slots=2, snapshot_interval=32,
+                  max_seq_len=160) as f:
+        c, (a, b, d) = f.ctx, f.seqs
+        acc = kvc.to_device(rng.random((1, 1, NKV, 150)).astype(np.float32))
+        kept = kvc.hip().malloc(NKV * 64 * 4)
+        c.evict([a], 64, acc, 150, kept)
+        row = NQ * 2 * D + 2 * NKV * D
+        qkv = kvc.to_device(O.normal_bf16(3 * row, 5))
+        w = kvc.to_device((rng.random(D) + 0.5).astype(np.float32))
+        for s, n in ((a, 64), (b, 150)):
+            c.reserve([s], 3)
+            qo = kvc.hip().malloc(3 * NQ * D * 2)
+            c.qkv_append(0, [s], 3, qkv, w, w, q_out=qo)
+            c.commit([s], 3)
+            c.sync()
+            got = f.gather(0, s, 3, n) + [qo.download(np.uint16, (3, NQ, D))]
+            if s == a:
+                want = got
+            for x, y in zip(got, want):
+                assert np.array_equal(x, y)
+        assert c.seq_info(a).position == 153 and c.seq_len(a) == 67
+        # a batch of sequences with different shifts
+        c.reserve([a, d], 1)
+        c.qkv_append(0, [d, a], 1, qkv, w, w)
+        un = kvc.KVC_ERR_UNSUPPORTED
+        for call in (lambda: c.decode_step(0, [a], qkv, w, w, qo), lambda: c.prefill_step(0, [a], 1, qkv, w, w, qo)):
+            with pytest.raises(kvc.KvcError) as e:
+                call()
+            assert e.value.code == un
+        c.commit([a, d], 1)
+        c.seq_truncate(a, 64)
+        for call in (lambda: c.snapshot_save([a]),):
+            with pytest.raises(kvc.KvcError) as e:
+                call()
+            assert e.value.code == un
+        c.reserve([a], 11)  # position 150 + 11 is past max_seq_len 160
+        with pytest.raises(kvc.KvcError) as e:
+            c.qkv_append(0, [a], 11, qkv, w, w)
+        assert e.value.code == kvc.KVC_ERR_RANGE
+
+
+def test_the_run_they_are_made_for():
+    """Two sessions: a prompt, its window's weights, a cut, the rest in 8 bits,
+    then decode steps that go on accumulating, another cut and a new chunk."""
+    say("evict + 8 bits run")
+    n_q, budget, layers = 16, 96, 2
+    rng = np.random.default_rng(8)
+    with Q.Filled([400, 250], layers=layers, seed=107, extra=400) as f:
+        c, seqs = f.ctx, f.seqs
+        stride = 512
+        acc = [kvc.hip().malloc(layers * 2 * NKV * stride * 4).zero() for _ in range(2)]
+        per = 2 * NKV * stride * 4
+        model = {}  # (layer, i) -> [k, v] values, and accumulated weights
+        for layer in range(layers):
+            for i, s in enumerate(seqs):
+                model[layer, i] = [[Q.f64(x) for x in f.rows[layer, s]], np.zeros((NKV, len(f.rows[layer, s][0])))]
+
+        def accumulate(n_q):
+            for layer in range(layers):
+                q = O.normal_bf16(2 * n_q * NQ * D, int(rng.integers(1 << 30))).reshape(2, n_q, NQ, D)
+                qb = kvc.to_device(q)
+                at = acc[0].ptr + layer * per
+                c.attn_weights(layer, seqs, n_q, qb, at, stride, acc_in=at)
+                c.sync()
+                qb.free()
+                for i in range(2):
+                    (k, _), w = model[layer, i]
+                    w += Q.weights(Q.f64(q[i]), k, SCALE, len(k) - n_q)
+            got = acc[0].download(np.float32, (layers, 2, NKV, stride))
+            for layer in range(layers):
+                for i in range(2):
+                    w = model[layer, i][1]
+                    assert np.abs(got[layer, i, :, :w.shape[1]] - w).max() <= 2.0 ** -16 * max(1.0, w.max())
+
+        def cut():
+            kept = kvc.hip().malloc(layers * 2 * NKV * budget * 4)
+            c.evict(seqs, budget, acc[0], stride, kept, n_sink=2, n_recent=12, acc_out=acc[1])
+            c.sync()
+            acc.reverse()
+            got = kept.download(np.int32, (layers, 2, NKV, budget))
+            kept.free()
+            for layer in range(layers):
+                for i in range(2):
+                    kv, w = model[layer, i]
+                    idx = got[layer, i]
+                    # the choice is the one of the device's own sums: held to
+                    # the model's where no two of its values are near
+                    for h in range(NKV):
+                        want = Q.keep(w[h], budget, 2, 12)
+                        assert len(np.setdiff1d(want, idx[h])) <= 1
+                    model[layer, i] = [[np.stack([x[idx[h], h] for h in range(NKV)], 1) for x in kv],
+                                       np.stack([w[h][idx[h]] for h in range(NKV)])]
+
+        def park(keep):
+            c.kv_quantize(seqs, keep)
+            for layer in range(layers):
+                for i in range(2):
+                    kv, _ = model[layer, i]
+                    n8 = c.seq_info(seqs[i]).q8_tokens
+                    model[layer, i][0] = [np.concatenate([Q.values(Q.bf16_bits(x[:n8]), n8), x[n8:]]) for x in kv]
+
+        def step():
+            c.reserve(seqs, 1)
+            for layer in range(layers):
+                q, k, v = (O.normal_bf16(2 * w * D, int(rng.integers(1 << 30))).reshape(2, w, D) for w in (NQ, NKV, NKV))
+                got = f.run(lambda a, b, d, o: c.decode_attn(layer, seqs, a, o, k_new=b, v_new=d), (2, NQ, D), np.float32,
+                            q, k, v)
+                for i in range(2):
+                    kv, w = model[layer, i]
+                    kv = [np.concatenate([x, Q.f64(y[i])[None]]) for x, y in zip(kv, (k, v))]
+                    model[layer, i] = [kv, np.concatenate([w, np.zeros((NKV, 1))], 1)]
+                    want, mag, big, dig = Q.attend(Q.f64(q[i])[None], *kv, SCALE, digits=True)
+                    tol = mag * 2.0 ** -22 * (big + 2) + np.abs(want) * 2.0 ** -22 + 2.0 ** -30 * dig
+                    assert (np.abs(got[i] - want[0]) <= tol[0]).all()
+            c.commit(seqs, 1)
+
+        accumulate(n_q)
+        cut()
+        park(20)
+        assert c.seq_info(seqs[0]).q8_tokens == 64
+        for _ in range(5):
+            step()
+        # weights over the mixed cache, then a cut that reads 8-bit rows
+        for layer in range(layers):
+            q = O.normal_bf16(2 * NQ * D, 77 + layer).reshape(2, 1, NQ, D)
+            qb = kvc.to_device(q)
+            at = acc[0].ptr + layer * per
+            c.attn_weights(layer, seqs, 1, qb, at, stride, acc_in=at)
+            c.sync()
+            qb.free()
+            for i in range(2):
+                (k, _), w = model[layer, i]
+                w += Q.weights(Q.f64(q[i]), k, SCALE, len(k) - 1)
+        cut()
+        for layer in range(layers):
+            for i in range(2):
+                n = len(model[layer, i][0][0])
+                for got, x in zip(f.gather(layer, seqs[i], n), model[layer, i][0]):
+                    Q.same_bits(got, Q.bf16_bits(x))
+                model[layer, i][0] = [Q.f64(Q.bf16_bits(x)) for x in model[layer, i][0]]
+        park(20)
+        step()
+        assert c.seq_info(seqs[0]).position == 400 + 6 and c.seq_len(seqs[0]) == budget + 1
