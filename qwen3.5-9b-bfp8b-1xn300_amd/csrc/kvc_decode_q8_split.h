@@ -12,12 +12,13 @@ namespace kvc {
 
 // Chunk lengths (a.cb8 8-bit blocks, a.cbf bf16 blocks), the sequences' first
 // chunks and the launch's items, from the block counts nb[n] and a.n8.
-inline void decode_q8_split(const int32_t* nb, int32_t n, DecodeQ8Args& a) {
+// chunk_blocks: the caller's choice for both (kvc_config), 0 = automatic.
+inline void decode_q8_split(const int32_t* nb, int32_t n, int32_t chunk_blocks, DecodeQ8Args& a) {
     int64_t total = 0;  // in 8-bit blocks; a bf16 block has the bytes of two
     for (int32_t j = 0; j < n; j++) total += a.n8[j] + 2 * (nb[j] - a.n8[j]);
-    int32_t cb8 = std::max(4, (int32_t)std::lround(0.25 * std::sqrt((double)total)));
+    int32_t cb8 = chunk_blocks > 0 ? chunk_blocks : std::max(4, (int32_t)std::lround(0.25 * std::sqrt((double)total)));
     for (;; cb8 *= 2) {
-        const int32_t cbf = std::max(2, cb8 / 2);
+        const int32_t cbf = chunk_blocks > 0 ? cb8 : std::max(2, cb8 / 2);
         int64_t chunks = 0;
         for (int32_t j = 0; j < n; j++) {
             a.chunk_begin[j] = (int32_t)chunks;

@@ -1295,7 +1295,7 @@ static int build_decode_q8_args(kvc_ctx* c, int32_t layer, const int32_t* seqs, 
         a.n8[j] = s.n8;
         nblk[j] = (L + kBlockTok - 1) / kBlockTok;
     }
-    decode_q8_split(nblk, n, a);
+    decode_q8_split(nblk, n, c->cfg.decode_chunk_blocks, a);
     a.c = mixed_cache(c, layer);
     a.q = static_cast<const uint16_t*>(q) + (size_t)i0 * qrow;
     a.k_new = k_new ? static_cast<const uint16_t*>(k_new) + (size_t)i0 * kvrow : nullptr;
@@ -1393,6 +1393,39 @@ int kvc_decode_attn_static(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
                        kStaticItems, "static decode workspace");
 }
 
+// One prefill launch over sequences of which some hold 8-bit blocks (at most 64).
+static int prefill_q8_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n, int32_t n_q, const void* q,
+                             const void* gate, void* out, int32_t out_dtype, float scale, void* stream) {
+    PrefillQ8Args a{};
+    int64_t total = 0;
+    for (int32_t j = 0; j < n; j++) {
+        const Seq& s = c->seqs[seqs[j]];
+        a.slot[j] = seqs[j];
+        a.q_pos0[j] = s.len + s.pending - n_q;
+        a.n8[j] = s.n8;
+        a.begin[j] = (int32_t)total;
+        for (int64_t r = 0; r < n_q; r += kP8Rows)
+            total += (a.q_pos0[j] + std::min<int64_t>(r + kP8Rows, n_q) + kBlockTok - 1) / kBlockTok * kKvHeads;
+    }
+    if (total > INT32_MAX / 2) return set_err(KVC_ERR_RANGE, "prefill too large");
+    a.begin[n] = a.total = (int32_t)total;
+    a.c = mixed_cache(c, layer);
+    a.q = static_cast<const uint16_t*>(q);
+    a.gate = static_cast<const uint16_t*>(gate);
+    a.out = out;
+    a.part = c->d_part;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.out_bf16 = out_dtype == KVC_DTYPE_BF16;
+    a.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
+    a.n_seqs = n;
+    a.n_q = n_q;
+    a.per_wg = (int32_t)std::max<int64_t>(kP8MinBlocks, (total + kP8MaxWgs - 1) / kP8MaxWgs);
+    a.n_wgs = (int32_t)((total + a.per_wg - 1) / a.per_wg);
+    a.per_xcd = (a.n_wgs + 7) / 8;
+    int e = launch_prefill_q8(a, stream);
+    return e ? hip_err((hipError_t)e, "prefill launch (8-bit blocks)") : KVC_OK;
+}
+
 // Prefill launches over all seqs, 64 per launch (arguments checked by the
 // caller).  With qkv (the prefill step), q and gate come from the projection
 // rows instead of q / gate.
@@ -1404,6 +1437,14 @@ static int prefill_launches(kvc_ctx* c, int32_t layer, const int32_t* seqs, int3
     const size_t isz = in_dtype == KVC_DTYPE_F32 ? 4 : 2;
     for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
         const int32_t n = std::min(kMaxBatch, n_seqs - i0);
+        if (any_q8(c, seqs + i0, n)) {  // (never with qkv: kvc_prefill_step refuses them)
+            const size_t off = (size_t)i0 * qrow;
+            int rc = prefill_q8_launch(c, layer, seqs + i0, n, n_q, static_cast<const uint16_t*>(q) + off,
+                                       gate ? static_cast<const uint16_t*>(gate) + off : nullptr,
+                                       static_cast<uint8_t*>(out) + off * osz, out_dtype, scale, stream);
+            if (rc) return rc;
+            continue;
+        }
         PrefillArgs a{};
         for (int32_t j = 0; j < n; j++) {
             const Seq& s = c->seqs[seqs[i0 + j]];
@@ -1432,14 +1473,6 @@ static int prefill_launches(kvc_ctx* c, int32_t layer, const int32_t* seqs, int3
         a.n_seqs = n;
         a.n_q = n_q;
         a.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
-        if (any_q8(c, seqs + i0, n)) {
-            const MixedCache m = mixed_cache(c, layer);
-            a.k8 = m.k8;
-            a.v8 = m.v8;
-            a.ks = m.ks;
-            a.vs = m.vs;
-            for (int32_t j = 0; j < n; j++) a.n8[j] = c->seqs[seqs[i0 + j]].n8;
-        }
         a.n_groups = n * kKvHeads;
         for (int32_t j = 0; j < n; j++) a.seq_order[j] = j;
         std::stable_sort(a.seq_order, a.seq_order + n,

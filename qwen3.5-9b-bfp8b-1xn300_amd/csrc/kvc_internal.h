@@ -18,7 +18,7 @@
 // them as matrix operands (lane = 16 g + c):
 //   K piece (t, s, lane): token 16 t + c, dims 64 s + 16 g .. + 15
 //   V piece (p, lane):    dim 32 p + c, then dim 32 p + 16 + c, of the tokens
-//                         4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3
+//                         t0 .. t0 + 3, t0 + 8 .. t0 + 11, t0 = 16 (g / 2) + 4 (g % 2)
 //
 // Recurrent state of a sequence slot (one contiguous region per slot):
 //   [ssm_layer][ rec fp32 [v_heads][v_dim][k_dim] | conv fp32 [rows][channels] ]
@@ -288,14 +288,6 @@ struct PrefillArgs {
     int32_t q_pos0[kMaxBatch];  // position of query row 0
     int32_t seq_order[kMaxBatch];  // batch indices, most keys first
     int32_t unit_begin[kMaxBatch + 1];  // first unit of each sequence, in seq_order
-    // sequences with leading 8-bit blocks (k8 not null): this layer's 8-bit
-    // pools and scales, and the 8-bit blocks of each sequence
-    int32_t pad3;
-    const uint8_t* k8;
-    const uint8_t* v8;
-    const float* ks;
-    const float* vs;
-    int32_t n8[kMaxBatch];
 };
 
 // ---- 8-bit blocks and eviction -------------------------------------------
@@ -340,6 +332,39 @@ struct DecodeQ8Args {
     int32_t n8[kMaxBatch];
     int32_t chunk_begin[kMaxBatch + 1];
 };
+
+// Prefill over such sequences.  An item is 64 query rows of one (sequence, kv
+// head); the items' key blocks stand in one line, in the order sequence, kv
+// head, rows, and workgroup w takes units [w per_wg, (w + 1) per_wg) of it.
+struct PrefillQ8Args {
+    MixedCache c;
+    const uint16_t* q;     // [n_seqs][n_q][Hq][D]
+    const uint16_t* gate;  // same or null
+    void* out;
+    float* part;           // 2 partials per workgroup
+    float scale_log2;
+    int32_t out_bf16;
+    int32_t gate_ref;
+    int32_t n_seqs;
+    int32_t n_q;
+    int32_t total;         // units
+    int32_t per_wg;
+    int32_t n_wgs;
+    int32_t per_xcd;       // ceil(n_wgs / 8)
+    int32_t pad;
+    int32_t slot[kMaxBatch];
+    int32_t q_pos0[kMaxBatch];
+    int32_t n8[kMaxBatch];
+    int32_t begin[kMaxBatch + 1];  // first unit of each sequence
+};
+// one partial: unnormalised output [q head, 32 rows][8 dim tiles][4][64
+// lanes][4], then (max, sum) per row [q head, 32 rows][32]
+constexpr int kP8PartAcc = 8 * 8 * 4 * 64 * 4;
+constexpr int kP8PartFloats = kP8PartAcc + 8 * 32 * 2;
+constexpr int kP8MaxWgs = 256;
+constexpr int kP8MinBlocks = 4;  // blocks per workgroup at least
+constexpr int kP8Rows = 64;
+static_assert((size_t)2 * kP8MaxWgs * kP8PartFloats * 4 <= kPartBytes, "partials live in the split-K workspace");
 
 // All layers of the K/V pools and of the 8-bit pools.
 struct MixedPools {
@@ -476,7 +501,7 @@ struct BlockCopyArgs {
 };
 
 static_assert(sizeof(DecodeQ8Args) < 4096 && sizeof(QuantizeArgs) < 4096 && sizeof(GatherQ8Args) < 4096 &&
-                  sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillArgs) < 4096,
+                  sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillQ8Args) < 4096,
               "argument blocks are passed by value");
 
 // ---- launchers (kvc_kernels.hip); return hipError_t as int ---------------
@@ -498,6 +523,7 @@ int launch_prefill(const PrefillArgs& a, void* stream);
 int launch_snapshot(const SnapshotArgs& a, void* stream);
 int launch_block_copy(const BlockCopyArgs& a, void* stream);
 int launch_decode_q8(const DecodeQ8Args& a, void* stream);
+int launch_prefill_q8(const PrefillQ8Args& a, void* stream);
 int launch_quantize(const QuantizeArgs& a, void* stream);
 int launch_gather_q8(const GatherQ8Args& a, void* stream);
 int launch_weights(const WeightsArgs& a, void* stream);

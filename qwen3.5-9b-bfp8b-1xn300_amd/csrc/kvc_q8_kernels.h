@@ -24,7 +24,7 @@ __device__ __forceinline__ int q8_k_off(int tok, int d) {
     return (((tok >> 4) * 4 + (d >> 6)) * 64 + ((d >> 4) & 3) * 16 + (tok & 15)) * 16 + (d & 15);
 }
 __device__ __forceinline__ int q8_v_off(int tok, int d) {
-    const int g = (tok >> 2) & 3, e = (tok & 3) + 4 * (tok >> 4);
+    const int g = ((tok >> 2) & 1) + 2 * (tok >> 4), e = (tok & 3) + 4 * ((tok >> 3) & 1);
     return ((d >> 5) * 64 + g * 16 + (d & 15)) * 16 + ((d >> 4) & 1) * 8 + e;
 }
 
@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a) {
         } else {
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const uint16_t* col = tile + (4 * g + 16 * (k & 1)) * kHeadDim + 32 * e + 16 * (k >> 1) + c;
+                const uint16_t* col =
+                    tile + (16 * (g >> 1) + 4 * (g & 1) + 8 * (k & 1)) * kHeadDim + 32 * e + 16 * (k >> 1) + c;
                 o[k] = q1(col[0]) | q1(col[kHeadDim]) << 8 | q1(col[2 * kHeadDim]) << 16 | q1(col[3 * kHeadDim]) << 24;
             }
         }
@@ -144,7 +145,8 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(GatherQ8Args a) {
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; k++) {  // tokens (2k, 2k + 1) % 4 of their groups
-                    const int tok = 4 * g + 16 * ((k >> 1) & 1) + 2 * (k & 1), d = 32 * e + 16 * (k >> 2) + c;
+                    const int tok = 16 * (g >> 1) + 4 * (g & 1) + 8 * ((k >> 1) & 1) + 2 * (k & 1);
+                    const int d = 32 * e + 16 * (k >> 2) + c;
                     tile[tok * kRow + d] = (uint16_t)w[k];
                     tile[(tok + 1) * kRow + d] = (uint16_t)(w[k] >> 16);
                 }
@@ -318,7 +320,8 @@ __device__ __forceinline__ void q8_block(const Q8Block& b, Q8Wave& w, uint32_t* 
         }
     }
     // digits of p to LDS at [head][position of the key in V's token order]
-    const int pos = 8 * (c >> 2) + (c & 3) + 4 * (g & 1), h0 = 2 * (g >> 1);
+    // (token 16 (g & 1) + c: group 2 (g & 1) + (c / 4) % 2, element c % 4 + 4 (c / 8))
+    const int pos = 16 * (g & 1) + 8 * ((c >> 2) & 1) + (c & 3) + 4 * (c >> 3), h0 = 2 * (g >> 1);
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         f[j] = fast_exp2(f[j] - w.m[j]);
