@@ -27,6 +27,7 @@
 #include "kvc_decode_q8_split.h"
 #include "kvc_decode_split.h"
 #include "kvc_internal.h"
+#include "kvc_prefill_q8_split.h"
 #include "kvc_prefill_split.h"
 
 using namespace kvc;
@@ -1397,18 +1398,15 @@ int kvc_decode_attn_static(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
 static int prefill_q8_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n, int32_t n_q, const void* q,
                              const void* gate, void* out, int32_t out_dtype, float scale, void* stream) {
     PrefillQ8Args a{};
-    int64_t total = 0;
     for (int32_t j = 0; j < n; j++) {
         const Seq& s = c->seqs[seqs[j]];
         a.slot[j] = seqs[j];
         a.q_pos0[j] = s.len + s.pending - n_q;
         a.n8[j] = s.n8;
-        a.begin[j] = (int32_t)total;
-        for (int64_t r = 0; r < n_q; r += kP8Rows)
-            total += (a.q_pos0[j] + std::min<int64_t>(r + kP8Rows, n_q) + kBlockTok - 1) / kBlockTok * kKvHeads;
     }
-    if (total > INT32_MAX / 2) return set_err(KVC_ERR_RANGE, "prefill too large");
-    a.begin[n] = a.total = (int32_t)total;
+    a.n_seqs = n;
+    a.n_q = n_q;
+    if (!prefill_q8_split(a)) return set_err(KVC_ERR_RANGE, "prefill too large");
     a.c = mixed_cache(c, layer);
     a.q = static_cast<const uint16_t*>(q);
     a.gate = static_cast<const uint16_t*>(gate);
@@ -1417,11 +1415,6 @@ static int prefill_q8_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int
     a.scale_log2 = scale * 1.4426950408889634f;
     a.out_bf16 = out_dtype == KVC_DTYPE_BF16;
     a.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
-    a.n_seqs = n;
-    a.n_q = n_q;
-    a.per_wg = (int32_t)std::max<int64_t>(kP8MinBlocks, (total + kP8MaxWgs - 1) / kP8MaxWgs);
-    a.n_wgs = (int32_t)((total + a.per_wg - 1) / a.per_wg);
-    a.per_xcd = (a.n_wgs + 7) / 8;
     int e = launch_prefill_q8(a, stream);
     return e ? hip_err((hipError_t)e, "prefill launch (8-bit blocks)") : KVC_OK;
 }

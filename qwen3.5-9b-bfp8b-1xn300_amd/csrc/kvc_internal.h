@@ -333,9 +333,11 @@ struct DecodeQ8Args {
     int32_t chunk_begin[kMaxBatch + 1];
 };
 
+constexpr int kP8MaxWgs = 256;
+constexpr int kP8Rows = 64;
 // Prefill over such sequences.  An item is 64 query rows of one (sequence, kv
 // head); the items' key blocks stand in one line, in the order sequence, kv
-// head, rows, and workgroup w takes units [w per_wg, (w + 1) per_wg) of it.
+// head, rows, and workgroup w takes units [cut[w], cut[w + 1]) of it.
 struct PrefillQ8Args {
     MixedCache c;
     const uint16_t* q;     // [n_seqs][n_q][Hq][D]
@@ -347,23 +349,21 @@ struct PrefillQ8Args {
     int32_t gate_ref;
     int32_t n_seqs;
     int32_t n_q;
-    int32_t total;         // units
-    int32_t per_wg;
     int32_t n_wgs;
     int32_t per_xcd;       // ceil(n_wgs / 8)
+    int32_t fold;          // workgroups per cut of the combining launch
     int32_t pad;
     int32_t slot[kMaxBatch];
     int32_t q_pos0[kMaxBatch];
     int32_t n8[kMaxBatch];
     int32_t begin[kMaxBatch + 1];  // first unit of each sequence
+    int32_t cut[kP8MaxWgs + 1];
+    uint8_t seq_at[kP8MaxWgs];     // sequence of unit cut[w]
 };
 // one partial: unnormalised output [q head, 32 rows][8 dim tiles][4][64
 // lanes][4], then (max, sum) per row [q head, 32 rows][32]
 constexpr int kP8PartAcc = 8 * 8 * 4 * 64 * 4;
 constexpr int kP8PartFloats = kP8PartAcc + 8 * 32 * 2;
-constexpr int kP8MaxWgs = 256;
-constexpr int kP8MinBlocks = 4;  // blocks per workgroup at least
-constexpr int kP8Rows = 64;
 static_assert((size_t)2 * kP8MaxWgs * kP8PartFloats * 4 <= kPartBytes, "partials live in the split-K workspace");
 
 // All layers of the K/V pools and of the 8-bit pools.

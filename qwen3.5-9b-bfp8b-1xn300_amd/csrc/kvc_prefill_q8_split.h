@@ -1,0 +1,80 @@
+// kvc_prefill_q8_split.h -- the rule for the work split of a prefill launch over
+// sequences with 8-bit blocks (host code without HIP, so that a test can
+// compile it alone).
+#pragma once
+
+#include <algorithm>
+
+#include "kvc_internal.h"
+
+namespace kvc {
+
+// Fills begin, cut, seq_at, n_wgs and per_xcd from n_seqs, n_q and q_pos0;
+// false if the line is too long.  A workgroup pays kP8Item blocks' time for
+// each item that it takes up (its query rows, first copies and result) and a
+// block's for each block; a cut inside an item costs two partials and their
+// fold.  So runs are filled in order up to a common bound, an item that fits
+// is not cut, and one that does not is cut only into parts of a fifth of the
+// bound and more; the bound is raised until the runs are few enough.
+inline bool prefill_q8_split(PrefillQ8Args& a) {
+    constexpr int64_t kP8Item = 7, kP8MinPart = 4;
+    const auto blocks = [&](int32_t j, int64_t rb) {
+        return (a.q_pos0[j] + std::min<int64_t>((rb + 1) * kP8Rows, a.n_q) + kBlockTok - 1) / kBlockTok;
+    };
+    const int64_t n_rb = (a.n_q + kP8Rows - 1) / kP8Rows;
+    int64_t total = 0, longest = 0;
+    for (int32_t j = 0; j < a.n_seqs; j++) {
+        a.begin[j] = (int32_t)total;
+        for (int64_t rb = 0; rb < n_rb; rb++) total += kKvHeads * blocks(j, rb);
+        longest = std::max(longest, blocks(j, n_rb - 1));
+        if (total > INT32_MAX / 2) return false;
+    }
+    a.begin[a.n_seqs] = (int32_t)total;
+    const int64_t items = a.n_seqs * n_rb * kKvHeads;
+    const auto fill = [&](int64_t bound) -> bool {
+        const int64_t part = std::max(kP8MinPart, bound / 5);
+        int32_t w = 0;
+        int64_t load = 0, at = 0;
+        const auto next = [&](int32_t j) {
+            load = 0;
+            if (++w >= kP8MaxWgs) return false;
+            a.cut[w] = (int32_t)at;
+            a.seq_at[w] = (uint8_t)j;
+            return true;
+        };
+        a.cut[0] = 0;
+        a.seq_at[0] = 0;
+        for (int32_t j = 0; j < a.n_seqs; j++)
+            for (int32_t h = 0; h < kKvHeads; h++)
+                for (int64_t rb = 0; rb < n_rb; rb++) {
+                    int64_t left = blocks(j, rb);
+                    if (load && load + kP8Item + std::min(left, part) > bound && !next(j)) return false;
+                    while (left > 0) {
+                        const int64_t room = bound - load - kP8Item;
+                        int64_t take = left;
+                        if (left > room) {
+                            take = std::max(room, part);
+                            if (left - take < part) take = left >= 2 * part ? left - part : left;
+                            if (load && take >= left) {  // too short to be cut here
+                                if (!next(j)) return false;
+                                continue;
+                            }
+                        }
+                        load += kP8Item + take;
+                        at += take;
+                        left -= take;
+                        if (left > 0 && !next(j)) return false;
+                    }
+                }
+        a.n_wgs = w + 1;
+        a.cut[w + 1] = (int32_t)at;
+        return true;
+    };
+    int64_t bound = std::max<int64_t>(kP8Item + kP8MinPart, (total + kP8Item * items + kP8MaxWgs - 1) / kP8MaxWgs);
+    while (!fill(bound)) bound += std::max<int64_t>(1, bound / 24);
+    a.per_xcd = (a.n_wgs + 7) / 8;
+    a.fold = 16;
+    return true;
+}
+
+}  // namespace kvc
