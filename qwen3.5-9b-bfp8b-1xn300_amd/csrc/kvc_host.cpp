@@ -1430,19 +1430,22 @@ static int prefill_launches(kvc_ctx* c, int32_t layer, const int32_t* seqs, int3
     const size_t isz = in_dtype == KVC_DTYPE_F32 ? 4 : 2;
     for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
         const int32_t n = std::min(kMaxBatch, n_seqs - i0);
-        if (any_q8(c, seqs + i0, n)) {  // (never with qkv: kvc_prefill_step refuses them)
+        PrefillArgs a{};
+        for (int32_t j = 0; j < n; j++) {
+            const Seq& s = c->seqs[seqs[i0 + j]];
+            a.slot[j] = seqs[i0 + j];
+            a.q_pos0[j] = s.len + s.pending - n_q;
+        }
+        a.n_seqs = n;
+        a.n_q = n_q;
+        const bool q8 = any_q8(c, seqs + i0, n);  // (never with qkv: kvc_prefill_step refuses them)
+        if (q8 && !prefill_q8_few(a)) {
             const size_t off = (size_t)i0 * qrow;
             int rc = prefill_q8_launch(c, layer, seqs + i0, n, n_q, static_cast<const uint16_t*>(q) + off,
                                        gate ? static_cast<const uint16_t*>(gate) + off : nullptr,
                                        static_cast<uint8_t*>(out) + off * osz, out_dtype, scale, stream);
             if (rc) return rc;
             continue;
-        }
-        PrefillArgs a{};
-        for (int32_t j = 0; j < n; j++) {
-            const Seq& s = c->seqs[seqs[i0 + j]];
-            a.slot[j] = seqs[i0 + j];
-            a.q_pos0[j] = s.len + s.pending - n_q;
         }
         a.kpool = reinterpret_cast<const uint16_t*>(c->d_pool + (int64_t)(layer * 2) * c->layer_kv_bytes);
         a.vpool = reinterpret_cast<const uint16_t*>(c->d_pool + (int64_t)(layer * 2 + 1) * c->layer_kv_bytes);
@@ -1463,14 +1466,20 @@ static int prefill_launches(kvc_ctx* c, int32_t layer, const int32_t* seqs, int3
         a.scale_log2 = scale * 1.4426950408889634f;
         a.out_bf16 = out_dtype == KVC_DTYPE_BF16;
         a.table_stride = c->max_blocks;
-        a.n_seqs = n;
-        a.n_q = n_q;
         a.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
+        if (q8) {
+            const MixedCache m = mixed_cache(c, layer);
+            a.k8 = m.k8;
+            a.v8 = m.v8;
+            a.ks = m.ks;
+            a.vs = m.vs;
+            for (int32_t j = 0; j < n; j++) a.n8[j] = c->seqs[seqs[i0 + j]].n8;
+        }
         a.n_groups = n * kKvHeads;
         for (int32_t j = 0; j < n; j++) a.seq_order[j] = j;
         std::stable_sort(a.seq_order, a.seq_order + n,
                          [&](int32_t x, int32_t y) { return a.q_pos0[x] > a.q_pos0[y]; });
-        prefill_split(a);
+        prefill_split(a, q8 ? 32 : 16);
         int32_t units = a.n_groups;
         if (a.piece_tiles > 0) {
             a.part = c->d_part;

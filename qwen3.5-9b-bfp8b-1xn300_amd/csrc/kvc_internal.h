@@ -288,6 +288,14 @@ struct PrefillArgs {
     int32_t q_pos0[kMaxBatch];  // position of query row 0
     int32_t seq_order[kMaxBatch];  // batch indices, most keys first
     int32_t unit_begin[kMaxBatch + 1];  // first unit of each sequence, in seq_order
+    // sequences with leading 8-bit blocks (k8 not null): this layer's 8-bit
+    // pools and scales, and the 8-bit blocks of each sequence
+    int32_t pad3;
+    const uint8_t* k8;
+    const uint8_t* v8;
+    const float* ks;
+    const float* vs;
+    int32_t n8[kMaxBatch];
 };
 
 // ---- 8-bit blocks and eviction -------------------------------------------
@@ -501,7 +509,7 @@ struct BlockCopyArgs {
 };
 
 static_assert(sizeof(DecodeQ8Args) < 4096 && sizeof(QuantizeArgs) < 4096 && sizeof(GatherQ8Args) < 4096 &&
-                  sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillQ8Args) < 4096,
+                  sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillQ8Args) < 4096 && sizeof(PrefillArgs) < 4096,
               "argument blocks are passed by value");
 
 // ---- launchers (kvc_kernels.hip); return hipError_t as int ---------------

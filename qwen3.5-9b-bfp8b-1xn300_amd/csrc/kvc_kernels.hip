@@ -1482,7 +1482,18 @@ __device__ __forceinline__ void prefill_q_row(const void* qkv, size_t row, const
 // workspace for prefill_combine_kernel; a block that one piece covers is
 // finished here.  Chosen by the host for launches that would leave most CUs
 // idle (prefill_split).
-template <int ROWS, int PROD, bool SPLIT>
+// Q8 != 0: few rows over sequences that start with 8-bit blocks
+// (kvc_q8_kernels.h; more rows run prefill_q8_kernel), in a launch with bf16 ones.  A wave's part of a tile lies in one block.  If that is
+// an 8-bit one the wave fetches its pieces into registers when tile t + 1's
+// copies are issued and, after tile t's products, writes them to LDS as bf16
+// integers (exact): K rows in the layout of the copies, V as the P.V products'
+// fragments in order (V pieces hold a lane's 8 tokens), which are then read
+// back whole instead of through the transposing read.  Key scales multiply the
+// scores, value scales the weights before their rounding; the denominator is
+// summed from the weights in fp32.  Q8 = 2 (fp32 output): weights in three
+// bf16 parts (24 bits), three times the P.V products, for results as exact as
+// fp32 sums instead of 2e-3 off.
+template <int ROWS, int PROD, bool SPLIT, int Q8 = 0>
 // (launch bounds of 512 threads in either size: told of 256, the compiler
 // plans for one wave per SIMD and keeps the accumulators in AGPRs, which cost
 // the softmax and epilogue a copy each; 500 rows of one sequence 28.7 -> 26.7
@@ -1493,6 +1504,7 @@ void prefill_mfma_kernel(PrefillArgs a) {
     constexpr bool F32IN = PROD == 2;
     constexpr int kWavesPf = ROWS / 4;
     constexpr int kLoadRows = kPfKeys / kWavesPf;  // tile rows each wave loads
+    constexpr int kPieces = Q8 ? 16 / kWavesPf : 1;  // 64-piece groups of an 8-bit K or V unit each wave loads
     __shared__ PrefillSmem sm;
     // Workgroup b runs on XCD b % 8.  The n_pb query blocks of one (sequence,
     // kv head) group share its K/V, so they go to one XCD (one L2), in
@@ -1578,6 +1590,70 @@ void prefill_mfma_kernel(PrefillArgs a) {
             lds_dma16s(base, off, lds_tile + r0 * kHeadDim * 2);
         }
     };
+    // 8-bit blocks: the wave's pieces of tile t, and the scales of its two blocks
+    const int n8 = Q8 ? a.n8[s] : 0;
+    const int e0 = (wave % (kWavesPf / 2)) * kPieces;
+    u32x4 k8[kPieces], v8[kPieces];
+    float ksc[2] = {1.f, 1.f}, vsc[2] = {1.f, 1.f}, ksn[2], vsn[2];  // this tile's, the next one's
+    auto load_q8 = [&](int t) {
+        const int id = __builtin_amdgcn_readlane(idv, 2 * t + half - idw0);
+        const size_t unit = (size_t)id * kKvHeads + h;
+        const u32x4* k = reinterpret_cast<const u32x4*>(a.k8 + unit * kQ8UnitBytes) + e0 * 64 + lane;
+        const u32x4* v = reinterpret_cast<const u32x4*>(a.v8 + unit * kQ8UnitBytes) + e0 * 64 + lane;
+#pragma unroll
+        for (int j = 0; j < kPieces; j++) {
+            k8[j] = k[64 * j];
+            v8[j] = v[64 * j];
+        }
+    };
+    auto load_scales = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            ksn[i] = vsn[i] = 1.f;
+            if (2 * t + i < n8) {
+                const size_t unit = (size_t)__builtin_amdgcn_readlane(idv, 2 * t + i - idw0) * kKvHeads + h;
+                ksn[i] = a.ks[unit];
+                vsn[i] = a.vs[unit];
+            }
+        }
+    };
+    auto store_q8 = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < kPieces; j++) {
+            const int e = e0 + j;
+            const int kr = 32 * half + 16 * (e >> 2) + r16, ch = 8 * (e & 3) + 2 * q4;  // K row, first 16-B chunk
+            u32x4 x0, x1;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const u32x2 lo = i8x4_to_bf16(k8[j][i]), hi = i8x4_to_bf16(k8[j][2 + i]);
+                x0[2 * i] = lo[0];
+                x0[2 * i + 1] = lo[1];
+                x1[2 * i] = hi[0];
+                x1[2 * i + 1] = hi[1];
+            }
+            u32x4* kd = reinterpret_cast<u32x4*>(&sm.k[buf][kr * kHeadDim]);
+            kd[ch ^ kswz(kr)] = x0;
+            kd[(ch + 1) ^ kswz(kr)] = x1;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const u32x2 lo = i8x4_to_bf16(v8[j][i]), hi = i8x4_to_bf16(v8[j][2 + i]);
+                x0[2 * i] = lo[0];
+                x0[2 * i + 1] = lo[1];
+                x1[2 * i] = hi[0];
+                x1[2 * i + 1] = hi[1];
+            }
+            // a piece's tokens are two of the 8 groups of 4 in a block, tg and tg + 2;
+            // group 4 hi + q is half hi of lane q's 8 in a fragment
+            const int tg = 4 * (q4 >> 1) + (q4 & 1);
+            u32x2* vd = reinterpret_cast<u32x2*>(&sm.v[buf][32 * half * kHeadDim]) + (tg >> 2);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {  // dims 32 e + r16, then 32 e + 16 + r16
+                const u32x4 x = i ? x1 : x0;
+                vd[((2 * e + i) * 64 + 16 * (tg & 3) + r16) * 2] = u32x2{x[0], x[1]};
+                vd[((2 * e + i) * 64 + 16 * ((tg + 2) & 3) + r16) * 2] = u32x2{x[2], x[3]};
+            }
+        }
+    };
     auto issue_k = [&](int t, int buf) { issue_rows(a.kpool, cbk, 5, lds_addr(&sm.k[buf][0]), t); };
     auto issue_v = [&](int t, int buf) { issue_rows(a.vpool, cbv, 6, lds_addr(&sm.v[buf][0]), t); };
 
@@ -1585,6 +1661,19 @@ void prefill_mfma_kernel(PrefillArgs a) {
     // The first tile's copies are issued right after the q loads and before the
     // q arithmetic of the prefill step.
     auto issue_first = [&] {
+        if constexpr (Q8 != 0) {
+            load_scales(t_begin);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                ksc[i] = ksn[i];
+                vsc[i] = vsn[i];
+            }
+            if (2 * t_begin + half < n8) {
+                load_q8(t_begin);
+                store_q8(0);
+                return;
+            }
+        }
         issue_k(t_begin, 0);
         issue_v(t_begin, 0);
     };
@@ -1608,7 +1697,7 @@ void prefill_mfma_kernel(PrefillArgs a) {
     }
     if constexpr (!PRODUCE) issue_first();
 
-    f32x4 o[16], ol;  // ol: the all-ones row block (softmax denominator)
+    f32x4 o[16], ol;  // ol: the all-ones row block (softmax denominator; Q8: ol[0] is the lane's part)
     float m_run = kNegBig;
 #pragma unroll
     for (int dt = 0; dt < 16; dt++) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1673,8 +1762,13 @@ void prefill_mfma_kernel(PrefillArgs a) {
                 idw0 = 2 * (t + 1);
                 idv = idw0 + lane < n_blocks ? trow[idw0 + lane] : 0;
             }
-            issue_k(t + 1, B ^ 1);
-            issue_v(t + 1, B ^ 1);
+            if constexpr (Q8 != 0) load_scales(t + 1);
+            if (Q8 != 0 && 2 * (t + 1) + half < n8) {
+                load_q8(t + 1);
+            } else {
+                issue_k(t + 1, B ^ 1);
+                issue_v(t + 1, B ^ 1);
+            }
         }
         f32x4 st[4];
         // the MFMA runs (S here, P.V below) issue at raised wave priority, so
@@ -1691,6 +1785,12 @@ void prefill_mfma_kernel(PrefillArgs a) {
         }
         __builtin_amdgcn_s_setprio(0);
 
+        if constexpr (Q8 != 0) {
+            if (2 * t < n8) {
+#pragma unroll
+                for (int kt = 0; kt < 4; kt++) st[kt] *= ksc[kt >> 1];
+            }
+        }
         // Tile max in the log2 domain.  A full tile (all keys exist and
         // precede the wave's first row) keeps raw scores: the max is scaled
         // once (c >= 0 keeps the order).  A tile that reaches the diagonal or
@@ -1731,24 +1831,93 @@ void prefill_mfma_kernel(PrefillArgs a) {
 #pragma unroll
             for (int dt = 0; dt < 16; dt++)
                 o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(z8, z8, o[dt] * cr, 0, 0, 0);
-            ol = __builtin_amdgcn_mfma_f32_16x16x32_bf16(z8, z8, ol * cr, 0, 0, 0);
+            if constexpr (Q8 != 0)
+                ol[0] *= cr;
+            else
+                ol = __builtin_amdgcn_mfma_f32_16x16x32_bf16(z8, z8, ol * cr, 0, 0, 0);
         }
         // P^T as the B operand (bf16), k-slot order (4q4 + i, 16 + 4q4 + i);
         // p = 2^(s * cs - m) with one rounding before the exponential
-        bf16x8_t pb_[2];
+        bf16x8_t pb_[2], pl_[2], pt_[2];  // pl_, pt_: second and third parts (Q8 = 2)
         const float nm = -m_run;
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
-            u32x4 w;
+            u32x4 w, wl = {}, wt = {};
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {
                 const f32x4 sv = st[2 * kk + hf];
+                if constexpr (Q8 != 0) {
+                    float p[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        p[i] = fast_exp2(fmaf(sv[i], cs, nm));
+                        ol[0] += p[i];
+                        p[i] *= vsc[kk];
+                    }
+                    w[2 * hf] = cvt_pk_bf16(p[0], p[1]);
+                    w[2 * hf + 1] = cvt_pk_bf16(p[2], p[3]);
+                    if constexpr (Q8 == 2) {
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {  // each difference is exact
+                            const float x = p[2 * i] - bf16lo(w[2 * hf + i]), y = p[2 * i + 1] - bf16hi(w[2 * hf + i]);
+                            const uint32_t l = cvt_pk_bf16(x, y);
+                            wl[2 * hf + i] = l;
+                            wt[2 * hf + i] = cvt_pk_bf16(x - bf16lo(l), y - bf16hi(l));
+                        }
+                    }
+                    continue;
+                }
                 w[2 * hf] = cvt_pk_bf16(fast_exp2(fmaf(sv[0], cs, nm)), fast_exp2(fmaf(sv[1], cs, nm)));
                 w[2 * hf + 1] = cvt_pk_bf16(fast_exp2(fmaf(sv[2], cs, nm)), fast_exp2(fmaf(sv[3], cs, nm)));
             }
             pb_[kk] = as_bf16x8(w);
+            pl_[kk] = as_bf16x8(wl);
+            pt_[kk] = as_bf16x8(wt);
         }
 
+        if constexpr (Q8 != 0) {
+            // each half of the tile is one block: whole fragments of an 8-bit
+            // block, transposed pieces of a bf16 one
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                bf16x8_t vf[kPfAhead];
+                const auto products = [&](auto&& read) {
+#pragma unroll
+                    for (int i = 0; i < kPfAhead; i++) vf[i] = read(i);
+#pragma unroll
+                    for (int dt = 0; dt < 16; dt++) {
+                        const bf16x8_t va = vf[dt % kPfAhead];
+                        if (dt + kPfAhead < 16) vf[dt % kPfAhead] = read(dt + kPfAhead);
+                        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb_[kk], o[dt], 0, 0, 0);
+                        if constexpr (Q8 == 2) {
+                            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pl_[kk], o[dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pt_[kk], o[dt], 0, 0, 0);
+                        }
+                    }
+                };
+                if (2 * t + kk < n8) {
+                    const uint32_t base = v0 + kVOff + 16384 * kk + lane * 16;
+                    products([&](int dt) { return as_bf16x8(lds_load16(base, 1024 * dt)); });
+                } else {
+                    products([&](int dt) {
+                        const u32x2 lo = lds_load_tr16(vaddr[dt], kVOff + 16384 * kk);
+                        const u32x2 hi = lds_load_tr16(vaddr[dt], kVOff + 16384 * kk + 8192);
+                        return as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
+                    });
+                }
+            }
+            __builtin_amdgcn_s_setprio(0);
+            if (t + 1 < t_end) {
+                if (2 * (t + 1) + half < n8) store_q8(B ^ 1);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    ksc[i] = ksn[i];
+                    vsc[i] = vsn[i];
+                }
+            }
+            return;
+        }
         // O^T += V^T . P^T; the V^T operand of lane (q4, r16) is V[keys
         // 32kk + 4q4 + e (+16)][16dt + r16]: lane J of the group addresses
         // row 32kk + 4q4 + J/4 (+16), dims 16dt + 4(J%4) .. +3
@@ -1791,6 +1960,7 @@ void prefill_mfma_kernel(PrefillArgs a) {
         step(PfBuf<0>{}, t);
         if (t + 1 < t_end) step(PfBuf<1>{}, t + 1);
     }
+    if constexpr (Q8 != 0) ol[0] = sum_xor32(sum_xor16(ol[0]));
     if constexpr (SPLIT) {
         if (n_tiles > a.piece_tiles) {
             // 1-KiB stores: lane (q4, r16) holds dims 16dt + 4q4 .. +3 of row
@@ -4183,7 +4353,12 @@ template <int ROWS, bool SPLIT>
 static void launch_prefill_t(const PrefillArgs& a, hipStream_t st) {
     const int n = SPLIT ? a.n_units : a.n_groups, n_pb = (a.n_q + ROWS - 1) / ROWS;
     const int grid = 8 * ((n * a.pb_div + 7) / 8) * ((n_pb + a.pb_div - 1) / a.pb_div);
-    if (a.qkv && a.qkv_f32)
+    if (a.k8) {  // (32 rows always: prefill_split)
+        if (a.out_bf16)
+            hipLaunchKernelGGL((prefill_mfma_kernel<32, 0, SPLIT, 1>), dim3(grid), dim3(32 * 16), 0, st, a);
+        else
+            hipLaunchKernelGGL((prefill_mfma_kernel<32, 0, SPLIT, 2>), dim3(grid), dim3(32 * 16), 0, st, a);
+    } else if (a.qkv && a.qkv_f32)
         hipLaunchKernelGGL((prefill_mfma_kernel<ROWS, 2, SPLIT>), dim3(grid), dim3(ROWS * 16), 0, st, a);
     else if (a.qkv)
         hipLaunchKernelGGL((prefill_mfma_kernel<ROWS, 1, SPLIT>), dim3(grid), dim3(ROWS * 16), 0, st, a);

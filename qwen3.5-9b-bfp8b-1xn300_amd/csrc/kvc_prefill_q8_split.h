@@ -9,6 +9,24 @@
 
 namespace kvc {
 
+// Whether a launch runs as the bf16 prefill's variant instead, whose workgroups
+// take 32 query rows: prefill_q8_kernel pads to 64, and its runs begin and end
+// more slowly (8 us a run, 15-20 us for the fold of the cut items).  us, that
+// variant / prefill_q8_kernel, bf16 out: 1 sequence over 4001 keys, 64 rows 30 /
+// 45, 128 rows 34 / 57, 200 rows 51 / 53, 512 rows 76 / 73; 4 over 1000-4000, 64
+// rows 37 / 51, 128 rows 60 / 58, 400 rows 167 / 113; 16 over 256-6000, 32 rows
+// 63 / 78, 64 rows 101 / 94, 128 rows 228 / 165; 64 over 100-3000, 32 rows 143 /
+// 158; 8 over 8000-16000, 32 rows 98 / 127, 128 rows 354 / 232.
+inline bool prefill_q8_few(const PrefillArgs& a) {
+    constexpr int64_t kMost = 2000;  // blocks of 64 rows and 32 keys
+    if (a.n_q <= 32) return true;
+    int64_t blocks = 0;
+    for (int32_t j = 0; j < a.n_seqs; j++)
+        for (int64_t r = 0; r < a.n_q && blocks <= kMost; r += kP8Rows)
+            blocks += (a.q_pos0[j] + std::min<int64_t>(r + kP8Rows, a.n_q) + kBlockTok - 1) / kBlockTok * kKvHeads;
+    return blocks <= kMost;
+}
+
 // Fills begin, cut, seq_at, n_wgs and per_xcd from n_seqs, n_q and q_pos0;
 // false if the line is too long.  A workgroup pays kP8Item blocks' time for
 // each item that it takes up (its query rows, first copies and result) and a

@@ -35,7 +35,12 @@ namespace kvc {
 // keys 489 -> 59; 128 rows over 1000 keys 47.2 -> 25.8; 500 rows over none 33.6
 // -> 26.7 (16 rows, unsplit); 40 sequences of 16 rows over 100-12000 keys 368 ->
 // 237.  Launches of 512 and more 32-row workgroups have no idle CU to fill.
-inline void prefill_split(PrefillArgs& a) {
+// least_rows: 32 keeps to 32-row workgroups.  Launches over 8-bit blocks do,
+// whose widening 8 waves share there and 4 in a 16-row one.  us, 16 / 32 rows: 1
+// sequence of 16 rows over 4001 keys 24.3 / 21.8, of 32 rows 32.2 / 25.3; 4 of 16
+// over 1000-4000 33.9 / 25.1; 16 of 16 over 256-6000 93 / 57; 64 of 4 over
+// 100-3000 236 / 134.
+inline void prefill_split(PrefillArgs& a, int least_rows = 16) {
     constexpr double kCus = 256, kTail = 0.3, kFold = 6.0, kPartBytesPerUs = 6e6, kMargin = 1.15;
     const auto blocks_of = [&](int rows) { return (a.n_q + rows - 1) / (int64_t)rows; };
     a.rows = 32;
@@ -48,7 +53,7 @@ inline void prefill_split(PrefillArgs& a) {
         a.rows = rows;
         a.piece_tiles = (int32_t)piece_tiles;
     };
-    for (int rows = 16; rows <= 32; rows += 16) {
+    for (int rows = least_rows; rows <= 32; rows += 16) {
         const int64_t n_pb = blocks_of(rows);
         const auto tiles_of = [&](int32_t j, int64_t b) {
             return (a.q_pos0[j] + std::min<int64_t>((b + 1) * rows, a.n_q) + kPfKeys - 1) / kPfKeys;
