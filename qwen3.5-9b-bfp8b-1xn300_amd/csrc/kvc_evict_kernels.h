@@ -6,14 +6,16 @@
 namespace kvc {
 
 // ---------------------------------------------------------------------------
-// Attention weights, first launch: scores of all rows of a kv head (row 4 i +
-// g = query i, q head g of the group) against the keys of a chunk of
-// kWeightsChunk blocks, one block per wave.  The block's K sits in registers
-// as A operand (keys x dims; 8-bit blocks as exact bf16 integers, scaled
-// after the product) and the rows pass by in tiles of 16 (B operand).  Scores
-// go to the workspace in the log2 domain, -infinity where the row does not see
-// the key, with the chunk's (max, sum 2^(s - max)) per row; the second launch
-// needs every chunk's before it can normalise any weight.
+// Attention weights: acc[key] += sum over rows of 2^(s - m_row) / l_row, with
+// s the row's score in the log2 domain, m_row and l_row its maximum and sum
+// over every key.  No weight is known before the last key's score is, so the
+// keys are passed twice, in two launches.
+//
+// A wave takes one block of one kv head.  The block's K sits in registers as A
+// operand (keys x dims; 8-bit blocks as exact bf16 integers, scaled after the
+// product), and the rows (row 4 i + g = query i, q head g of the group) pass
+// by in tiles of 16 as B operand, 128 rows at a time out of LDS, where they lie
+// in operand order for all 8 waves.  A lane then has 8 keys of one row.
 __device__ __forceinline__ void weights_load_k(u32x4 (&kf)[2][8], const MixedCache& c, int id, int h, bool q8, int lane) {
     const int r16 = lane & 15, g = lane >> 4;
     const size_t unit = (size_t)id * kKvHeads + h;
@@ -41,130 +43,249 @@ __device__ __forceinline__ void weights_load_k(u32x4 (&kf)[2][8], const MixedCac
     }
 }
 
-__global__ __launch_bounds__(256) void weights_score_kernel(WeightsArgs a) {
-    // (max, sum) of each wave's block and row
-    __shared__ float2 ml[kWeightsChunk][kWeightsMaxQ * kGroup];
+// Bytes from the sequence's first query to the lane's piece of B operand slice
+// ks (dims 32 ks + 8 (lane / 16) ..) of row r0 + lane % 16; rows past the last
+// repeat it.
+__device__ __forceinline__ uint32_t weights_q(const WeightsArgs& a, int h, int r0, int ks, int lane) {
+    const int rc = min(r0 + (lane & 15), a.n_q * kGroup - 1);
+    return (((rc >> 2) * kQHeads + h * kGroup + (rc & 3)) * kHeadDim + 32 * ks + 8 * (lane >> 4)) * 2;
+}
+
+// Rows g0 .. end - 1 into LDS as [tile][ks][lane], the waves in turn a slice.
+__device__ __forceinline__ void weights_stage_q(uint32_t lds, const WeightsArgs& a, const uint16_t* q, int h, int g0, int end,
+                                                int wave, int waves, int lane) {
+    for (int i = wave; i < ((end - g0 + 15) >> 4) * 8; i += waves)
+        lds_dma16s(q, weights_q(a, h, g0 + 16 * (i >> 3), i & 7, lane), lds + i * 1024);
+}
+
+// Raw products of the lane's keys 16 t + 4 (lane / 16) + i with one row.
+__device__ __forceinline__ void weights_product(f32x4 (&st)[2], const u32x4 (&kf)[2][8], const u32x4 (&qf)[8]) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+            st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[t][ks]), as_bf16x8(qf[ks]), st[t], 0, 0, 0);
+}
+
+// -infinity for the keys from key0 on that row r0 + lane % 16 does not see.
+__device__ __forceinline__ void weights_mask(f32x4 (&st)[2], const WeightsArgs& a, int L, int key0, int r0, int lane) {
+    const int last = L - a.n_q + (min(r0 + (lane & 15), a.n_q * kGroup - 1) >> 2) - key0;  // last one it sees
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (16 * t + 4 * (lane >> 4) + i > last) st[t][i] = -__builtin_inff();
+}
+
+// First launch: (max, sum 2^(s - max)) of every row over a chunk of one block
+// per wave.  STORE: one tile of rows, whose scores go to the workspace.
+template <bool STORE>
+__global__ __launch_bounds__(64 * weights_chunk(STORE), 4) void weights_score_kernel(WeightsArgs a) {
+    constexpr int W = weights_chunk(STORE), ROWS = STORE ? 16 : kWeightsRows;
+    __shared__ float2 ml[W][ROWS];
+    __shared__ u32x4 qs[STORE ? 1 : ROWS * kHeadDim / 8];
     const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int chunk = blockIdx.x >> 2, h = blockIdx.x & 3;
     const int s = find_seq(a.chunk_begin, a.n_seqs, chunk);
     const int L = a.kv_len[s], R = a.n_q * kGroup;
     const int nb = (L + kBlockTok - 1) / kBlockTok;
-    const int b = (chunk - a.chunk_begin[s]) * kWeightsChunk + wave;
-    const float none = -__builtin_inff();
+    const int b = (chunk - a.chunk_begin[s]) * W + wave;
+    const bool masked = (b + 1) * kBlockTok > L - a.n_q + 1;  // a key that some row does not see
+    const uint16_t* q = a.q + (size_t)s * a.n_q * kQHeads * kHeadDim;
+    u32x4 kf[2][8];
+    float scale = a.scale_log2;
+    if (!STORE) weights_stage_q(lds_addr(qs), a, q, h, 0, min(ROWS, R), wave, W, lane);
     if (b < nb) {
         const int id = a.c.table[(size_t)a.slot[s] * a.c.table_stride + b];
         const bool q8 = b < a.n8[s];
-        u32x4 kf[2][8];
         weights_load_k(kf, a.c, id, h, q8, lane);
-        const float scale = q8 ? a.scale_log2 * a.c.ks[(size_t)id * kKvHeads + h] : a.scale_log2;
-        float* out = a.scores + ((size_t)h * a.total_blocks + a.block_begin[s] + b) * R * kBlockTok;
-        for (int r0 = 0; r0 < R; r0 += 16) {
-            const int row = r0 + r16;
-            const int rc = min(row, R - 1);
-            const uint16_t* q = a.q + (((size_t)s * a.n_q + (rc >> 2)) * kQHeads + h * kGroup + (rc & 3)) * kHeadDim + 8 * g;
-            u32x4 qf[8];
-#pragma unroll
-            for (int ks = 0; ks < 8; ks++) qf[ks] = *reinterpret_cast<const u32x4*>(q + 32 * ks);
-            f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int ks = 0; ks < 8; ks++)
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[t][ks]), as_bf16x8(qf[ks]), st[t], 0, 0, 0);
-            // lane: keys 16 t + 4 g + i of row `row`
-            const int last = L - a.n_q + (rc >> 2);  // last key the row sees
-            float mx = none;
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    st[t][i] = b * kBlockTok + 16 * t + 4 * g + i <= last ? st[t][i] * scale : none;
-                    mx = fmaxf(mx, st[t][i]);
-                }
-            mx = max_xor16(mx);
-            mx = max_xor32(mx);
-            float l = 0.f;
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) l += fast_exp2(st[t][i] - fmaxf(mx, kNegBig));  // 0 for -infinity
-            l = sum_xor16(l);
-            l = sum_xor32(l);
-            if (row < R) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-                    *reinterpret_cast<f32x4*>(out + (size_t)row * kBlockTok + 16 * t + 4 * g) = st[t];
-                if (g == 0) ml[wave][row] = make_float2(fmaxf(mx, kNegBig), l);
-            }
-        }
-    } else {
-        for (int r = lane; r < R; r += 64) ml[wave][r] = make_float2(kNegBig, 0.f);
+        if (q8) scale *= a.c.ks[(size_t)id * kKvHeads + h];
     }
-    __syncthreads();
     float2* stats = reinterpret_cast<float2*>(a.stats) + ((size_t)h * a.total_chunks + chunk) * R;
-    for (int r = threadIdx.x; r < R; r += 256) {
-        float m = kNegBig, l = 0.f;
+    for (int g0 = 0; g0 < R; g0 += ROWS) {
+        const int end = min(g0 + ROWS, R);
+        if (!STORE) {
+            if (g0) weights_stage_q(lds_addr(qs), a, q, h, g0, end, wave, W, lane);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+        if (b < nb) {
+            for (int r0 = g0; r0 < end; r0 += 16) {
+                u32x4 qf[8];
 #pragma unroll
-        for (int w = 0; w < kWeightsChunk; w++) m = fmaxf(m, ml[w][r].x);
+                for (int ks = 0; ks < 8; ks++)
+                    qf[ks] = STORE ? *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(q) + weights_q(a, h, r0, ks, lane))
+                                   : qs[((r0 - g0) / 2 + ks) * 64 + lane];
+                f32x4 st[2];
+                weights_product(st, kf, qf);
 #pragma unroll
-        for (int w = 0; w < kWeightsChunk; w++) l = fmaf(fast_exp2(ml[w][r].x - m), ml[w][r].y, l);
-        stats[r] = make_float2(m, l);
+                for (int t = 0; t < 2; t++) st[t] *= scale;
+                if (masked) weights_mask(st, a, L, b * kBlockTok, r0, lane);
+                float mx = kNegBig;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, st[t][i]);
+                mx = max_xor16(mx);
+                mx = max_xor32(mx);
+                float l = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) l += fast_exp2(st[t][i] - mx);  // 0 for -infinity
+                l = sum_xor16(l);
+                l = sum_xor32(l);
+                if (STORE && r16 < R) {
+                    float* out = a.scores + (((size_t)h * a.total_blocks + a.block_begin[s] + b) * R + r16) * kBlockTok;
+#pragma unroll
+                    for (int t = 0; t < 2; t++) *reinterpret_cast<f32x4*>(out + 16 * t + 4 * g) = st[t];
+                }
+                if (g == 0) ml[wave][r0 - g0 + r16] = make_float2(mx, l);
+            }
+        } else {
+            for (int r = lane; r < ROWS; r += 64) ml[wave][r] = make_float2(kNegBig, 0.f);
+        }
+        __syncthreads();
+        for (int r = threadIdx.x; r < end - g0; r += 64 * W) {
+            float m = kNegBig, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; w++) m = fmaxf(m, ml[w][r].x);
+#pragma unroll
+            for (int w = 0; w < W; w++) l = fmaf(fast_exp2(ml[w][r].x - m), ml[w][r].y, l);
+            stats[g0 + r] = make_float2(m, l);
+        }
+        __syncthreads();
     }
 }
 
-// Second launch: one workgroup = kWsumBlocks blocks of one kv head.  It folds
-// the chunks' row statistics (each thread takes every 256 / R'th chunk of a
-// row), then thread (key, block) sums its key's weights over the rows in
-// order and adds them to the accumulator: no atomics, the same bits each time.
+// Folds (max, sum) of two parts of a row.
+__device__ __forceinline__ float2 weights_fold(float2 x, float2 y) {
+    const float m = fmaxf(x.x, y.x);
+    return make_float2(m, fmaf(x.y, fast_exp2(x.x - m), y.y * fast_exp2(y.x - m)));
+}
+
+// (max, 1 / sum) of rows g0 .. g0 + n - 1 (n <= THREADS) over the nc chunks of
+// a sequence: LANES neighbouring threads share a row and take every LANES'th
+// chunk of it.
+template <int THREADS>
+__device__ __forceinline__ void weights_rows(float2* row_ml, const float2* stats, int R, int g0, int n, int nc, int t) {
+    int lanes = 64;
+    while (lanes > 1 && lanes * n > THREADS) lanes >>= 1;
+    const int r = t / lanes;
+    float2 x = make_float2(kNegBig, 0.f);
+    if (r < n)
+#pragma unroll 4
+        for (int k = t % lanes; k < nc; k += lanes) x = weights_fold(x, stats[(size_t)k * R + g0 + r]);
+    for (int d = lanes >> 1; d > 0; d >>= 1) x = weights_fold(x, make_float2(__shfl_xor(x.x, d), __shfl_xor(x.y, d)));
+    if (t % lanes == 0 && r < n) row_ml[r] = make_float2(x.x, 1.0f / x.y);
+}
+
+// Second launch after stored scores: one workgroup = kWsumBlocks blocks of one
+// kv head; thread (key, block) sums its key's weights over the rows in order
+// and adds them to the accumulator: no atomics, the same bits each time.
 __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsArgs a) {
-    __shared__ float2 row_ml[kWeightsMaxQ * kGroup];
-    __shared__ float2 part[256];
+    __shared__ float2 row_ml[16];
     const int t = threadIdx.x;
     const int item = blockIdx.x >> 2, h = blockIdx.x & 3;
     const int s = find_seq(a.sum_begin, a.n_seqs, item);
     const int L = a.kv_len[s], R = a.n_q * kGroup;
     const int nb = (L + kBlockTok - 1) / kBlockTok;
-    const int nc = a.chunk_begin[s + 1] - a.chunk_begin[s];
-    const float2* stats = reinterpret_cast<const float2*>(a.stats) + ((size_t)h * a.total_chunks + a.chunk_begin[s]) * R;
-    int lanes = 256;  // threads per row: a power of two
-    while (lanes > 1 && lanes * R > 256) lanes >>= 1;
-    const int rows = 256 / lanes;
-    for (int r0 = 0; r0 < R; r0 += rows) {
-        const int r = r0 + t / lanes;
-        float m = kNegBig, l = 0.f;
-        if (r < R)
-            for (int k = t % lanes; k < nc; k += lanes) {
-                const float2 x = stats[(size_t)k * R + r];
-                const float mn = fmaxf(m, x.x);
-                l = fmaf(l, fast_exp2(m - mn), x.y * fast_exp2(x.x - mn));
-                m = mn;
-            }
-        part[t] = make_float2(m, l);
-        __syncthreads();
-        for (int d = lanes >> 1; d > 0; d >>= 1) {
-            if (t % lanes < d) {
-                const float2 x = part[t], y = part[t + d];
-                const float mn = fmaxf(x.x, y.x);
-                part[t] = make_float2(mn, fmaf(x.y, fast_exp2(x.x - mn), y.y * fast_exp2(y.x - mn)));
-            }
-            __syncthreads();
-        }
-        if (t % lanes == 0 && r < R) row_ml[r] = make_float2(part[t].x, 1.0f / part[t].y);
-        __syncthreads();
-    }
     const int b = (item - a.sum_begin[s]) * kWsumBlocks + (t >> 5), key = t & 31;
     const int pos = b * kBlockTok + key;
-    if (b >= nb || pos >= L) return;
-    const float* sc = a.scores + ((size_t)h * a.total_blocks + a.block_begin[s] + b) * R * kBlockTok + key;
-    float w = 0.f;
-#pragma unroll 8
-    for (int r = 0; r < R; r++) {
-        const float2 x = row_ml[r];
-        w = fmaf(fast_exp2(sc[(size_t)r * kBlockTok] - x.x), x.y, w);
-    }
+    const bool in = b < nb && pos < L;
     const size_t o = ((size_t)s * kKvHeads + h) * (size_t)a.stride + pos;
-    a.acc_out[o] = (a.acc_in ? a.acc_in[o] : 0.f) + w;
+    const float* sc = a.scores + ((size_t)h * a.total_blocks + a.block_begin[s] + b) * R * kBlockTok + key;
+    // asked for before the statistics are folded
+    const float before = in && a.acc_in ? a.acc_in[o] : 0.f;
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; r++) x[r] = in && r < R ? sc[(size_t)r * kBlockTok] : 0.f;
+    weights_rows<256>(row_ml, reinterpret_cast<const float2*>(a.stats) + ((size_t)h * a.total_chunks + a.chunk_begin[s]) * R,
+                      R, 0, R, a.chunk_begin[s + 1] - a.chunk_begin[s], t);
+    __syncthreads();
+    if (!in) return;
+    float w = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+        if (r < R) w = fmaf(fast_exp2(x[r] - row_ml[r].x), row_ml[r].y, w);
+    a.acc_out[o] = before + w;
+}
+
+// Second launch without stored scores: the same waves compute them again.  A
+// lane sums its 8 keys' weights over the tiles in order, the 16 lanes of a key
+// are added at the end: the same bits each time.
+__global__ __launch_bounds__(64 * weights_chunk(false), 4) void weights_again_kernel(WeightsArgs a) {
+    constexpr int W = weights_chunk(false), ROWS = kWeightsRows;
+    __shared__ float2 row_ml[ROWS];
+    __shared__ u32x4 qs[ROWS * kHeadDim / 8];
+    const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int chunk = blockIdx.x >> 2, h = blockIdx.x & 3;
+    const int s = find_seq(a.chunk_begin, a.n_seqs, chunk);
+    const int L = a.kv_len[s], R = a.n_q * kGroup;
+    const int nb = (L + kBlockTok - 1) / kBlockTok;
+    const int b = (chunk - a.chunk_begin[s]) * W + wave;
+    const bool masked = (b + 1) * kBlockTok > L - a.n_q + 1;
+    const uint16_t* q = a.q + (size_t)s * a.n_q * kQHeads * kHeadDim;
+    u32x4 kf[2][8];
+    float scale = a.scale_log2;
+    weights_stage_q(lds_addr(qs), a, q, h, 0, min(ROWS, R), wave, W, lane);
+    if (b < nb) {
+        const int id = a.c.table[(size_t)a.slot[s] * a.c.table_stride + b];
+        const bool q8 = b < a.n8[s];
+        weights_load_k(kf, a.c, id, h, q8, lane);
+        if (q8) scale *= a.c.ks[(size_t)id * kKvHeads + h];
+    }
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + ((size_t)h * a.total_chunks + a.chunk_begin[s]) * R;
+    const int nc = a.chunk_begin[s + 1] - a.chunk_begin[s];
+    f32x4 w[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    for (int g0 = 0; g0 < R; g0 += ROWS) {
+        const int end = min(g0 + ROWS, R);
+        if (g0) {
+            __syncthreads();
+            weights_stage_q(lds_addr(qs), a, q, h, g0, end, wave, W, lane);
+        }
+        // a row past the last counts for nothing: 2^(s - inf)
+        for (int r = R - g0 + threadIdx.x; r < ROWS; r += 64 * W) row_ml[r] = make_float2(__builtin_inff(), 0.f);
+        weights_rows<64 * W>(row_ml, stats, R, g0, end - g0, nc, threadIdx.x);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (b >= nb) continue;
+        for (int r0 = g0; r0 < end; r0 += 16) {
+            u32x4 qf[8];
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++) qf[ks] = qs[((r0 - g0) / 2 + ks) * 64 + lane];
+            const float2 x = row_ml[r0 - g0 + r16];
+            f32x4 st[2];
+            weights_product(st, kf, qf);
+#pragma unroll
+            for (int t = 0; t < 2; t++) st[t] *= scale;
+            if (masked) weights_mask(st, a, L, b * kBlockTok, r0, lane);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[t][i] = fmaf(fast_exp2(st[t][i] - x.x), x.y, w[t][i]);
+        }
+    }
+    if (b >= nb) return;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) w[t][i] += __shfl_xor(w[t][i], d);
+    // lane r16 = 4 t + i of a group writes key 16 t + 4 g + i
+    if (r16 < 8) {
+        float mine = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) mine = r16 == i ? w[i >> 2][i & 3] : mine;
+        const int pos = b * kBlockTok + 16 * (r16 >> 2) + 4 * g + (r16 & 3);
+        const size_t o = ((size_t)s * kKvHeads + h) * (size_t)a.stride + pos;
+        if (pos < L) a.acc_out[o] = (a.acc_in ? a.acc_in[o] : 0.f) + mine;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -331,8 +452,14 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(EvictCopyArgs a) {
 
 int launch_weights(const WeightsArgs& a, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(weights_score_kernel, dim3(a.total_chunks * kKvHeads), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(weights_sum_kernel, dim3(a.sum_chunks * kKvHeads), dim3(256), 0, st, a);
+    const dim3 grid(a.total_chunks * kKvHeads);
+    if (weights_store(a.n_q)) {
+        hipLaunchKernelGGL(weights_score_kernel<true>, grid, dim3(64 * weights_chunk(true)), 0, st, a);
+        hipLaunchKernelGGL(weights_sum_kernel, dim3(a.sum_chunks * kKvHeads), dim3(256), 0, st, a);
+    } else {
+        hipLaunchKernelGGL(weights_score_kernel<false>, grid, dim3(64 * weights_chunk(false)), 0, st, a);
+        hipLaunchKernelGGL(weights_again_kernel, grid, dim3(64 * weights_chunk(false)), 0, st, a);
+    }
     return (int)hipGetLastError();
 }
 

@@ -1790,11 +1790,12 @@ int kvc_attn_weights(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
         return set_err(KVC_ERR_RANGE, "attention weights of %d rows per sequence (at most %d)", n_q, kWeightsMaxQ);
     if (!std::isfinite(scale)) return set_err(KVC_ERR_INVALID, "scale must be finite");
     const int64_t rows = (int64_t)n_q * kGroup;
+    const bool store = weights_store(n_q);
     // workspace: scores of one block, statistics of one chunk
     const auto bytes_of = [&](int64_t blocks, int64_t chunks) {
-        return kKvHeads * rows * (blocks * kBlockTok * 4 + chunks * 8);
+        return kKvHeads * rows * ((store ? blocks * kBlockTok * 4 : 0) + chunks * 8);
     };
-    const auto chunks_of = [](int64_t blocks) { return (blocks + kWeightsChunk - 1) / kWeightsChunk; };
+    const auto chunks_of = [&](int64_t blocks) { return (blocks + weights_chunk(store) - 1) / weights_chunk(store); };
     for (int32_t i = 0; i < n_seqs; i++) {
         const Seq& s = c->seqs[seqs[i]];
         const int32_t L = s.len + s.pending;

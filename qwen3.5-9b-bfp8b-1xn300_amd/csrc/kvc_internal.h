@@ -422,13 +422,13 @@ struct WeightsArgs {
     const uint16_t* q;        // [n_seqs][n_q][Hq][D]
     const float* acc_in;      // [n_seqs][Hkv][stride] or null (zeros)
     float* acc_out;
-    float* scores;            // [sequence's block][row][32] per kv head
+    float* scores;            // [sequence's block][row][32] per kv head, where stored
     float* stats;             // [chunk of all][row][max, sum]
     int64_t stride;
     float scale_log2;
     int32_t n_seqs;
     int32_t n_q;
-    int32_t total_chunks;     // of kWeightsChunk blocks, per kv head
+    int32_t total_chunks;     // of weights_chunk blocks, per kv head
     int32_t total_blocks;
     int32_t sum_chunks;       // of kWsumBlocks blocks each
     int32_t slot[kMaxBatch];
@@ -438,7 +438,11 @@ struct WeightsArgs {
     int32_t chunk_begin[kMaxBatch + 1];
     int32_t sum_begin[kMaxBatch + 1];
 };
-constexpr int kWeightsChunk = 4;   // blocks per workgroup of the scoring launch
+// Up to one tile of rows the scores are stored between the two launches, above
+// they are computed again.
+constexpr bool weights_store(int n_q) { return n_q * kGroup <= 16; }
+constexpr int weights_chunk(bool store) { return store ? 4 : 8; }  // blocks (waves) per workgroup
+constexpr int kWeightsRows = 128;  // rows whose statistics a workgroup holds at once
 constexpr int kWsumBlocks = 8;     // blocks per workgroup of the summing launch
 constexpr int kWeightsMaxQ = 256;  // query rows per sequence
 
