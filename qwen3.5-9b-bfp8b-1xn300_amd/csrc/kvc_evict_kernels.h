@@ -290,12 +290,14 @@ __global__ __launch_bounds__(64 * weights_chunk(false), 4) void weights_again_ke
 
 // ---------------------------------------------------------------------------
 // Which tokens stay: one workgroup per (layer, sequence, kv head).  Accumulated
-// weights are ordered as unsigned integers (evict_key); the value of the last
-// one that stays comes from 4 passes over the row, 8 bits of the key each
-// (histogram in LDS), and the row is then walked once more in order: a token
-// stays if its key is greater, or equal and among the first of the equal ones
-// that still fit.  Sinks and recent tokens have no part in the choice.
-constexpr int kSelThreads = 1024;
+// weights are ordered as unsigned integers (evict_key); the key of the last one
+// that stays comes from 3 passes over the row, 11, 11 and 10 of the key's bits
+// each (histogram in LDS; integer atomics: any order, the same counts).  A
+// token stays if its key is greater, or equal and among the first of the equal
+// ones that still fit.  Sinks and recent tokens have no part in the choice.
+// Wave w takes the w'th sixteenth of the row; REGS keys per thread stay in
+// registers over the passes, 0: rows too long for that are read again.
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelRegs = 8, kSelBins = 2048;
 
 // Greater weight -> greater key; NaN lowest; -0 as +0.
 __device__ __forceinline__ uint32_t evict_key(float x) {
@@ -304,11 +306,12 @@ __device__ __forceinline__ uint32_t evict_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+template <int REGS>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictSelectArgs a) {
-    __shared__ uint32_t hist[256];
+    __shared__ uint32_t hist[kSelBins];
     __shared__ uint32_t sh_key, sh_need;
-    __shared__ int wsum[2][kSelThreads / 64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    __shared__ uint32_t wsum[2][kSelWaves];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int h = blockIdx.x % kKvHeads, j = blockIdx.x / kKvHeads % a.n_seqs, layer = blockIdx.x / kKvHeads / a.n_seqs;
     const size_t row = ((size_t)layer * a.call_seqs + a.seq0 + j) * kKvHeads + h;
     const float* acc = a.acc + row * (size_t)a.stride;
@@ -318,86 +321,109 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictSelectAr
     const int n_keep = min(L, a.budget);
     const int lo = min(a.n_sink, L), hi = max(lo, L - a.n_recent);  // the choice: [lo, hi)
     const int n_pick = L <= a.budget ? hi - lo : a.budget - a.n_sink - a.n_recent;
+    const int steps = (L + kSelThreads - 1) / kSelThreads;  // tokens per thread
+    const int first = wave * steps * 64 + lane;             // the thread's: first + 64 k
+    float x[REGS > 0 ? REGS : 1];
+    if constexpr (REGS > 0) {
+#pragma unroll
+        for (int k = 0; k < REGS; k++) x[k] = k < steps && first + 64 * k < L ? acc[first + 64 * k] : 0.f;
+    }
+    // f(token, weight) for the thread's tokens in order, all lanes at once (the
+    // token may be L or more)
+    const auto walk = [&](auto f) {
+        if constexpr (REGS > 0) {
+#pragma unroll
+            for (int k = 0; k < REGS; k++)
+                if (k < steps) f(first + 64 * k, x[k]);
+        } else {
+            for (int k = 0; k < steps; k += 4) {
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = k + i < steps && first + 64 * (k + i) < L ? acc[first + 64 * (k + i)] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (k + i < steps) f(first + 64 * (k + i), y[i]);
+            }
+        }
+    };
     uint32_t key = 0, need = 0;  // keys > key stay, and the first `need` equal ones
     if (n_pick < hi - lo) {
         if (n_pick == 0) {
             key = 0xFFFFFFFFu;
         } else {
-            uint32_t left = (uint32_t)n_pick;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int i = t; i < 256; i += kSelThreads) hist[i] = 0;
+            need = (uint32_t)n_pick;
+#pragma unroll
+            for (int pass = 0; pass < 3; pass++) {
+                constexpr int kShift[3] = {21, 10, 0};
+                const int shift = kShift[pass];
+                const uint32_t digits = pass < 2 ? 2048 : 1024;
+                for (int i = t; i < kSelBins; i += kSelThreads) hist[i] = 0;
                 __syncthreads();
-                for (int i = lo + t; i < hi; i += kSelThreads) {
-                    const uint32_t k = evict_key(acc[i]);
-                    if (shift == 24 || (k >> (shift + 8)) == (key >> (shift + 8)))
-                        __hip_atomic_fetch_add(&hist[(k >> shift) & 255], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                walk([&](int i, float w) {
+                    const uint32_t k = evict_key(w);
+                    if (i >= lo && i < hi && (pass == 0 || (k ^ key) >> (pass == 1 ? 21 : 10) == 0))
+                        __hip_atomic_fetch_add(&hist[(k >> shift) & (digits - 1)], 1u, __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_WORKGROUP);
+                });
+                __syncthreads();
+                // thread t holds digits 2047 - 2 t and 2046 - 2 t, greatest first
+                const uint32_t c0 = hist[kSelBins - 1 - 2 * t], c1 = hist[kSelBins - 2 - 2 * t];
+                uint32_t before = c0 + c1;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint32_t o = __shfl_up(before, d);
+                    if (lane >= d) before += o;
                 }
+                if (lane == 63) wsum[0][wave] = before;
                 __syncthreads();
-                if (wave == 0) {
-                    // lane holds digits 255 - 4 lane .. 252 - 4 lane, greatest first
-                    uint32_t c[4], sum = 0;
+                before -= c0 + c1;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        c[i] = hist[255 - 4 * lane - i];
-                        sum += c[i];
-                    }
-                    uint32_t before = sum;  // inclusive prefix over the lanes
-                    for (int d = 1; d < 64; d <<= 1) {
-                        const uint32_t o = __shfl_up(before, d);
-                        if (lane >= d) before += o;
-                    }
-                    before -= sum;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (before < left && left <= before + c[i]) {
-                            sh_key = key | (uint32_t)(255 - 4 * lane - i) << shift;
-                            sh_need = left - before;
-                        }
-                        before += c[i];
-                    }
+                for (int w = 0; w < kSelWaves; w++) before += w < wave ? wsum[0][w] : 0;
+                if (before < need && need <= before + c0) {
+                    sh_key = key | (uint32_t)(kSelBins - 1 - 2 * t) << shift;
+                    sh_need = need - before;
+                }
+                before += c0;
+                if (before < need && need <= before + c1) {
+                    sh_key = key | (uint32_t)(kSelBins - 2 - 2 * t) << shift;
+                    sh_need = need - before;
                 }
                 __syncthreads();
                 key = sh_key;
-                left = sh_need;
-                __syncthreads();
+                need = sh_need;
             }
-            need = left;
         }
     }
     const bool all = n_pick >= hi - lo;
-    int n_out = 0;
-    uint32_t n_equal = 0;
-    for (int i0 = 0; i0 < L; i0 += kSelThreads) {
-        const int i = i0 + t;
-        const float x = i < L ? acc[i] : 0.f;
-        const bool forced = i < L && (i < lo || i >= hi || all);
-        const uint32_t k = evict_key(x);
-        const bool pick = i < L && !forced;
-        const bool equal = pick && k == key && need > 0;
-        const uint64_t eq = __builtin_amdgcn_ballot_w64(equal);
-        const uint64_t below = (1ull << lane) - 1ull;
-        if (lane == 0) wsum[0][wave] = __popcll(eq);
-        __syncthreads();
-        uint32_t rank = n_equal + __popcll(eq & below);
-        for (int w = 0; w < kSelThreads / 64; w++) {
-            if (w < wave) rank += wsum[0][w];
-            n_equal += wsum[0][w];
-        }
-        const bool stay = forced || (pick && k > key) || (equal && rank < need);
-        const uint64_t st = __builtin_amdgcn_ballot_w64(stay);
-        if (lane == 0) wsum[1][wave] = __popcll(st);
-        __syncthreads();
-        int at = n_out + __popcll(st & below);
-        for (int w = 0; w < kSelThreads / 64; w++) {
-            if (w < wave) at += wsum[1][w];
-            n_out += wsum[1][w];
-        }
-        if (stay) {
-            kept[at] = i;
-            if (acc_out) acc_out[at] = x;
-        }
-        __syncthreads();
+    const auto above = [&](int i, float w) { return i < L && (i < lo || i >= hi || all || evict_key(w) > key); };
+    const auto equal = [&](int i, float w) { return i >= lo && i < hi && !all && evict_key(w) == key; };
+    uint32_t n_above = 0, n_equal = 0;  // of the wave's tokens, then of all before the one at hand
+    walk([&](int i, float w) {
+        n_above += __popcll(__builtin_amdgcn_ballot_w64(above(i, w)));
+        n_equal += __popcll(__builtin_amdgcn_ballot_w64(equal(i, w)));
+    });
+    __syncthreads();
+    if (lane == 0) wsum[0][wave] = n_above, wsum[1][wave] = n_equal;
+    __syncthreads();
+    n_above = n_equal = 0;
+#pragma unroll
+    for (int w = 0; w < kSelWaves; w++) {
+        n_above += w < wave ? wsum[0][w] : 0;
+        n_equal += w < wave ? wsum[1][w] : 0;
     }
+    const uint64_t below = (1ull << lane) - 1ull;
+    walk([&](int i, float w) {
+        const bool ab = above(i, w), eq = equal(i, w);
+        const uint64_t ab_m = __builtin_amdgcn_ballot_w64(ab), eq_m = __builtin_amdgcn_ballot_w64(eq);
+        const uint32_t rank = n_equal + __popcll(eq_m & below);
+        const uint32_t at = n_above + __popcll(ab_m & below) + min(rank, need);
+        if (ab || (eq && rank < need)) {
+            kept[at] = i;
+            if (acc_out) acc_out[at] = w;
+        }
+        n_above += __popcll(ab_m);
+        n_equal += __popcll(eq_m);
+    });
     for (int i = n_keep + t; i < a.budget; i += kSelThreads) kept[i] = -1;
     if (acc_out)
         for (int i = n_keep + t; i < L; i += kSelThreads) acc_out[i] = 0.f;
@@ -464,8 +490,13 @@ int launch_weights(const WeightsArgs& a, void* stream) {
 }
 
 int launch_evict_select(const EvictSelectArgs& a, void* stream) {
-    hipLaunchKernelGGL(evict_select_kernel, dim3(a.n_layers * a.n_seqs * kKvHeads), dim3(kSelThreads), 0,
-                       (hipStream_t)stream, a);
+    const dim3 grid(a.n_layers * a.n_seqs * kKvHeads), block(kSelThreads);
+    int32_t longest = 0;
+    for (int32_t j = 0; j < a.n_seqs; j++) longest = std::max(longest, a.len[j]);
+    if (longest <= kSelRegs * kSelThreads)
+        hipLaunchKernelGGL(evict_select_kernel<kSelRegs>, grid, block, 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, (hipStream_t)stream, a);
     return (int)hipGetLastError();
 }
 

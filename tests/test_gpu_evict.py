@@ -97,6 +97,17 @@ def test_weights_in_several_launches():
     weights_case([2000] * 12, 128, 0, seed=97)
 
 
+@pytest.mark.parametrize("lens,n_q", [([200, 31, 900], 4), ([200, 31, 900], 5), ([257, 600], 33)])
+def test_weights_around_a_tile_of_rows(lens, n_q):
+    """16 rows per kv head are the last whose scores are stored, 128 the last
+    that are staged at once; the rows end inside a tile and inside blocks"""
+    if min(lens) < n_q:
+        lens = [max(x, n_q) for x in lens]
+    for keep in (0, 40):
+        say(f"weights {lens} {n_q} rows keep {keep}")
+        weights_case(lens, n_q, keep, seed=109 + n_q)
+
+
 def test_weights_refusals():
     say("weights refusals")
     with Q.Filled([100, 40], seed=98) as f:
@@ -203,6 +214,14 @@ def test_evict_long_rows():
     """rows longer than a workgroup, with ties across its passes"""
     say("evict 5000")
     evict_case([5000, 2048, 1025], 1001, 2, 100, "ties", True, seed=103, layers=1)
+
+
+@pytest.mark.parametrize("lens", [[8192, 1], [8193, 70, 2049]])
+@pytest.mark.parametrize("kind", ["ties", "special"])
+def test_evict_longest_rows(lens, kind):
+    """the longest rows whose keys stay in registers, and longer ones"""
+    say(f"evict {lens} {kind}")
+    evict_case(lens, 2500, 3, 77, kind, True, seed=108, layers=1)
 
 
 @pytest.mark.parametrize("keep", [0, 100])
