@@ -5,19 +5,25 @@
 namespace kvc {
 
 // ---------------------------------------------------------------------------
-// One workgroup holds 64 query rows of one kv head: 4 waves, wave g those of q
-// head g, in two halves of 32 rows.  Keys pass by one 32-token block a step:
+// One workgroup holds 64 query rows of one kv head: 8 waves, wave g + 4 rg the
+// 32 rows of half rg of q head g.  Keys pass by one 32-token block a step:
 //   S^T[32 keys x 32 rows] = K . Q^T          (A = K rows from LDS, B = Q)
 //   P^T = 2^(c ks S^T - m) vs                 (bf16; fp32 sums of 2^(..) beside)
 //   O^T[256 dims x 32 rows] += V^T . P^T      (A = V^T from LDS)
-// with v_mfma_f32_32x32x16_bf16.  A wave alone on its SIMD has 512 registers: O
-// (256), Q (128), S and P of 64 rows.  An operand fragment read from LDS
-// serves 64 (K) or 32 (V^T) rows, so the LDS pipe is busy 1536 cycles a step
-// beside 2048 of the matrix pipe, and the first half's P.V products cover the
-// second half's softmax.  A lane works on one row (l % 32) of a half and 16 of
-// the block's keys, in an order in which P^T leaves the S^T accumulator as B
-// operand: lane half f, product j takes keys 16 j + 4 f + {0..3, 8..11}, the
+// with v_mfma_f32_32x32x16_bf16; c is the softmax scale times log2(e), ks and vs
+// the block's 8-bit scales (1 for a bf16 block).  The row maximum m moves only
+// when a block exceeds it by more than kRescaleSlack.  bf16 output rounds P
+// once (2^-8 of each weight, as the output is); fp32 output (FINE) takes P as
+// three bf16 parts, 2^-26, in three products.  O (128) and Q (64 registers) stay
+// in registers: at 2 waves per SIMD a lane has 256.  A lane works on one row and
+// 16 of the block's keys, in an order in which P^T leaves the S^T accumulator as
+// B operand: lane half f, product j takes keys 16 j + 4 f + {0..3, 8..11}, the
 // order in which V pieces hold their tokens.
+//
+// Bounds: a step is 1024 cycles of products per SIMD (2 waves x 32 x 16) and 256
+// KB out of LDS per CU, 2048 cycles at 128 B each; softmax and widening fill
+// what is left.  16 sequences of 128 rows over 256..6000 keys: 150 us, 650
+// TFLOP/s, against 1260 of a large matrix product; the fold 20 us.
 //
 // 8-bit blocks: pieces go from memory straight to LDS as they are
 // (global_load_lds, 3 steps ahead of their use, no registers); during step b
@@ -194,12 +200,10 @@ void prefill_q8_kernel(PrefillQ8Args a) {
         }
 
         {
-            constexpr int H = 1;
-            f32x16 o[H][8];
-            float m_run[H], l_run[H];
-            bf16x8_t qb[H][16];
-#pragma unroll
-            for (int x = 0; x < H; x++) {
+            f32x16 o[8];
+            float m_run = kNegBig, l_run = 0.f;
+            bf16x8_t qb[16];
+            {
                 const int r = row0 + min(32 * rg + r32, rows - 1);
                 const uint16_t* q = a.q + (((size_t)s * a.n_q + r) * kQHeads + h * kGroup + g) * kHeadDim + 8 * hf;
 #pragma unroll
@@ -207,14 +211,12 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                     u32x4 w = *reinterpret_cast<const u32x4*>(q + 16 * ks);
 #pragma unroll
                     for (int i = 0; i < 4; i++) w[i] ^= qflip;
-                    qb[x][ks] = as_bf16x8(w);
+                    qb[ks] = as_bf16x8(w);
                 }
 #pragma unroll
                 for (int dt = 0; dt < 8; dt++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[x][dt][i] = 0.f;
-                m_run[x] = kNegBig;
-                l_run[x] = 0.f;
+                    for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
             }
             if (b0 < n_raw) {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -276,7 +278,7 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                 const int r32 = ln & 31, hf = ln >> 5;
                 // K fragment ks: row r32, chunk 2 ks + hf, its low 4 bits swizzled
                 const uint32_t krow = k0 + r32 * 512 + 16 * (hf ^ p8_kswz(r32));
-                f32x16 st[H];
+                f32x16 st;
                 {
                     bf16x8_t kf[4];
                     const auto read = [&](int ks) { return as_bf16x8(lds_load16(krow ^ (32 * (ks & 7)), 256 * (ks >> 3))); };
@@ -287,7 +289,7 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                     for (int ks = 0; ks < 16; ks++) {
                         const bf16x8_t ka = kf[ks & 3];
                         if (ks + 4 < 16) kf[ks & 3] = read(ks + 4);
-                        st[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qb[0][ks], ks ? st[0] : zero, 0, 0, 0);
+                        st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qb[ks], ks ? st : zero, 0, 0, 0);
                     }
                     __builtin_amdgcn_sched_group_barrier(kSgDsRead, 4, 0);
 #pragma unroll
@@ -304,41 +306,41 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                 for (int i = 0; i + 1 < kP8Raw; i++) id[i] = id[i + 1];
                 id[kP8Raw - 1] = trow[min(b + kP8Raw, b1 - 1)];
                 const float cq = c * kscale;  // >= 0 (or NaN)
-                bf16x8_t pb[H][2], pl[H][2], pt[H][2];
-                // lane: keys 8 (i / 4) + 4 hf + i % 4 of row r32 of half x.  A block
+                bf16x8_t pb[2], pl[2], pt[2];
+                // lane: keys 8 (i / 4) + 4 hf + i % 4 of row r32.  A block
                 // that the half's rows see whole keeps raw scores: the maximum is
                 // scaled once and the scale enters the exponent through an FMA
-                const auto softmax = [&](int x) {
+                const auto softmax = [&] {
                     const bool full = b * kBlockTok + kBlockTok - 1 <= pos0 + row0 + 32 * rg && (b + 1) * kBlockTok <= kmax;
                     if (!full) {
                         asm volatile("");
                         const int qpos = min(pos0 + row0 + 32 * rg + r32, kmax - 1);
 #pragma unroll
                         for (int i = 0; i < 16; i++)
-                            st[x][i] = b * kBlockTok + 8 * (i >> 2) + 4 * hf + (i & 3) <= qpos ? st[x][i] * cq : kNegBig;
+                            st[i] = b * kBlockTok + 8 * (i >> 2) + 4 * hf + (i & 3) <= qpos ? st[i] * cq : kNegBig;
                     }
                     const float cs = full ? cq : 1.f;
-                    float mx = st[x][0];
+                    float mx = st[0];
 #pragma unroll
-                    for (int i = 1; i < 16; i++) mx = fmaxf(mx, st[x][i]);
+                    for (int i = 1; i < 16; i++) mx = fmaxf(mx, st[i]);
                     mx = max_xor32(mx);
                     mx = full ? mx * cq : mx;
-                    if (__builtin_amdgcn_ballot_w64(mx > m_run[x] + kRescaleSlack) != 0) {
-                        const bool up = mx > m_run[x] + kRescaleSlack;
-                        const float cr = up ? fast_exp2(m_run[x] - mx) : 1.f;
-                        m_run[x] = up ? mx : m_run[x];
-                        l_run[x] *= cr;
+                    if (__builtin_amdgcn_ballot_w64(mx > m_run + kRescaleSlack) != 0) {
+                        const bool up = mx > m_run + kRescaleSlack;
+                        const float cr = up ? fast_exp2(m_run - mx) : 1.f;
+                        m_run = up ? mx : m_run;
+                        l_run *= cr;
 #pragma unroll
-                        for (int dt = 0; dt < 8; dt++) o[x][dt] *= cr;
+                        for (int dt = 0; dt < 8; dt++) o[dt] *= cr;
                     }
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         u32x4 w, wl = {}, wt = {};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            float y = fast_exp2(fmaf(st[x][8 * j + 2 * i], cs, -m_run[x]));
-                            float z = fast_exp2(fmaf(st[x][8 * j + 2 * i + 1], cs, -m_run[x]));
-                            l_run[x] += y + z;
+                            float y = fast_exp2(fmaf(st[8 * j + 2 * i], cs, -m_run));
+                            float z = fast_exp2(fmaf(st[8 * j + 2 * i + 1], cs, -m_run));
+                            l_run += y + z;
                             y *= vscale;
                             z *= vscale;
                             w[i] = cvt_pk_bf16(y, z);
@@ -349,12 +351,12 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                                 wt[i] = cvt_pk_bf16(y - bf16lo(wl[i]), z - bf16hi(wl[i]));
                             }
                         }
-                        pb[x][j] = as_bf16x8(w);
-                        pl[x][j] = as_bf16x8(wl);
-                        pt[x][j] = as_bf16x8(wt);
+                        pb[j] = as_bf16x8(w);
+                        pl[j] = as_bf16x8(wl);
+                        pt[j] = as_bf16x8(wt);
                     }
                 };
-                const auto products = [&](int x, auto&& read) {
+                const auto products = [&](auto&& read) {
                     bf16x8_t vf[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) vf[i] = read(i);
@@ -363,10 +365,10 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                         const int dt = i & 7, j = i >> 3;  // products in a row are independent
                         const bf16x8_t va = vf[i & 3];
                         if (i + 4 < 16) vf[i & 3] = read(i + 4);
-                        o[x][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[x][j], o[x][dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[j], o[dt], 0, 0, 0);
                         if constexpr (FINE) {
-                            o[x][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pl[x][j], o[x][dt], 0, 0, 0);
-                            o[x][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pt[x][j], o[x][dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pl[j], o[dt], 0, 0, 0);
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pt[j], o[dt], 0, 0, 0);
                         }
                     }
                     constexpr int kReads = q8 ? 1 : 2, kProducts = FINE ? 3 : 1;
@@ -377,17 +379,17 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                         __builtin_amdgcn_sched_group_barrier(kSgMfma, kProducts, 1);
                     }
                 };
-                const auto pv = [&](int x) {
+                const auto pv = [&] {
                     if constexpr (q8) {
                         const uint32_t base = v0 + ln * 16;
-                        products(x, [&](int i) { return as_bf16x8(lds_load16(base, 2048 * (i & 7) + 1024 * (i >> 3))); });
+                        products([&](int i) { return as_bf16x8(lds_load16(base, 2048 * (i & 7) + 1024 * (i >> 3))); });
                     } else {
                         // V^T through the transposing read: 16-lane group G takes dims
                         // 32 dt + 16 (G & 1) .. + 15 of rows 16 j + 4 hf + 0..3 (+ 8); its
                         // lane J addresses row J / 4, dims 4 (J % 4)
                         const int J = ln & 15, vr = 4 * hf + (J >> 2);
                         const uint32_t vtr = v0 + vr * 512 + 32 * ((ln >> 4) & 1) + 8 * (J & 3);
-                        products(x, [&](int i) {
+                        products([&](int i) {
                             // 64-B piece dt of rows vr (+ 8, + 16 j), all of one r & 7
                             const uint32_t y = vtr + (((i & 7) ^ (vr & 7)) << 6);
                             const u32x2 lo = lds_load_tr16(y, 8192 * (i >> 3)), hi = lds_load_tr16(y, 8192 * (i >> 3) + 4096);
@@ -395,10 +397,8 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                         });
                     }
                 };
-                softmax(0);
-                if constexpr (H == 2) softmax(1);
-                pv(0);
-                if constexpr (H == 2) pv(1);
+                softmax();
+                pv();
                 if (late == 0) next_tile();
             };
             int b = b0;
@@ -406,9 +406,8 @@ void prefill_q8_kernel(PrefillQ8Args a) {
             for (; b < b1; b++) step(PfBuf<0>{}, b);
             const bool whole = b0 == 0 && b1 == it.n;
             const int part_slot = 2 * wg + (at > u_begin);
-#pragma unroll
-            for (int x = 0; x < H; x++) {
-                l_run[x] = sum_xor32(l_run[x]);
+            {
+                l_run = sum_xor32(l_run);
                 if (32 * rg >= rows) {  // no rows
                 } else if (!whole) {  // a part of the item's keys
                     float* part = a.part + (size_t)part_slot * kP8PartFloats;
@@ -418,16 +417,16 @@ void prefill_q8_kernel(PrefillQ8Args a) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
                             *reinterpret_cast<f32x4*>(acc + (dt * 4 + q) * 256) =
-                                f32x4{o[x][dt][4 * q], o[x][dt][4 * q + 1], o[x][dt][4 * q + 2], o[x][dt][4 * q + 3]};
+                                f32x4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
                     if (hf == 0)
                         *reinterpret_cast<float2*>(part + kP8PartAcc + ((2 * g + rg) * 32 + r32) * 2) =
-                            make_float2(m_run[x], l_run[x]);
+                            make_float2(m_run, l_run);
                 } else if (32 * rg + r32 < rows) {
                     const size_t orow =
                         (((size_t)s * a.n_q + row0 + 32 * rg + r32) * kQHeads + h * kGroup + g) * kHeadDim + 4 * hf;
                     // (one copy per kind of gate, with nothing decided inside: the code
                     // runs once, and its fetch is what it costs)
-                    const float inv = __builtin_amdgcn_rcpf(l_run[x]);
+                    const float inv = __builtin_amdgcn_rcpf(l_run);
                     const auto finish = [&](auto kind_) {
                         constexpr int kind = decltype(kind_)::value;  // 0: no gate, 1: exact, 2: the reference's
                         // gate words 8 pieces ahead: the stores keep loads behind them
@@ -443,7 +442,7 @@ void prefill_q8_kernel(PrefillQ8Args a) {
                         for (int i = 0; i < 32; i++) {
                             if constexpr (kind != 0)
                                 if (i % 8 == 0 && i < 24) ask(i + 8);
-                            const f32x16 y = o[x][i >> 2];
+                            const f32x16 y = o[i >> 2];
                             float f[4];
 #pragma unroll
                             for (int k = 0; k < 4; k++) f[k] = y[4 * (i & 3) + k] * inv;

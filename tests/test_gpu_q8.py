@@ -307,6 +307,126 @@ def test_prefill_unsplit_large_launch():
     prefill_case([64 * (i % 5) + 33 * (i % 2) + 32 for i in range(24)], 700, 0, False, True, seed=74, check_seqs=[0, 11, 23])
 
 
+@pytest.mark.parametrize("gated,bf16_out", [(True, False), (False, False), (True, True), (False, True)])
+def test_prefill_ragged_runs(gated, bf16_out):
+    """enough rows and keys for prefill_q8_kernel: sequences of no 8-bit block,
+    of one, of an odd and an even number; row blocks of 64, 64 and 2 rows"""
+    say(f"prefill8 ragged runs gated {gated} bf16 {bf16_out}")
+    prefill_case([0, 5, 32, 64, 95, 200, 1111, 640, 31, 800, 96, 2500], 130, 40, gated, bf16_out, seed=76)
+
+
+@pytest.mark.parametrize("n,keep", [(8100, 0), (8100, 300), (8100, 7000)])
+@pytest.mark.parametrize("bf16_out", [False, True])
+def test_prefill_items_cut_into_many_runs(n, keep, bf16_out):
+    """few items, each over tens of workgroups, with tails of 4, 13 and 222 bf16
+    blocks, and a short sequence beside them"""
+    say(f"prefill8 cut items {n} keep {keep}")
+    prefill_case([n, 64], 100, keep, True, bf16_out, seed=77 + keep % 7, check_seqs=[0, 1])
+
+
+def test_prefill_70_sequences():
+    """two launches, the second one small"""
+    say("prefill8 70 sequences")
+    lens = [int(x) for x in np.random.default_rng(12).integers(60, 400, 70)]
+    prefill_case(lens, 65, 33, False, False, seed=79, check_seqs=[0, 1, 31, 63, 64, 69])
+
+
+def test_prefill_many_short_sequences_of_few_blocks():
+    """the 32-row variant, not split"""
+    say("prefill8 64 x 40 rows")
+    lens = [int(x) for x in np.random.default_rng(13).integers(20, 130, 64)]
+    prefill_case(lens, 40, 0, True, True, seed=80, check_seqs=[0, 7, 40, 63])
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0 / 16])
+def test_prefill_scales_of_a_large_launch(scale):
+    say(f"prefill8 scale {scale}, large")
+    prefill_case([4500], 129, 64, False, False, scale=scale, seed=81)
+
+
+@pytest.mark.parametrize("n_q", [3, 130])
+def test_prefill_in_a_graph(n_q):
+    """either prefill, weights and decode captured as one run, replayed between
+    eager calls of them"""
+    say(f"prefill8 graph {n_q}")
+    h = kvc.hip()
+    lens = [3000, 70, 1201]
+    with Q.Filled(lens, seed=82, extra=n_q) as f:
+        f.ctx.kv_quantize(f.seqs, 16)
+        f.add(f.seqs, n_q, commit=False)
+        st = h.stream()
+        q = kvc.to_device(O.normal_bf16(3 * n_q * NQ * D, 60))
+        shape, ashape = (3, n_q, NQ, D), (3, NKV, 3200)
+        bufs = [[h.malloc(int(np.prod(shape)) * 4), h.malloc(int(np.prod(ashape)) * 4), h.malloc(3 * NQ * D * 4)]
+                for _ in range(2)]
+
+        def call(b):
+            f.ctx.prefill_attn(0, f.seqs, n_q, q, b[0], stream=st)
+            f.ctx.attn_weights(0, f.seqs, n_q, q, b[1], 3200, stream=st)
+            f.ctx.decode_attn(0, f.seqs, q, b[2], stream=st)
+
+        def read(b):
+            return [b[0].download(np.uint32, shape), b[1].download(np.uint32, ashape), b[2].download(np.uint32, (3, NQ, D))]
+
+        for b in bufs:
+            for x in b:
+                x.zero()
+        h.sync()
+        call(bufs[0])
+        h.stream_sync(st)
+        want = read(bufs[0])
+        assert all(w.any() for w in want)
+        g = h.capture(st, lambda: call(bufs[1]))
+        for i in range(4):
+            for x in bufs[1]:
+                x.zero()
+            h.sync()
+            h.graph_launch(g, st)
+            h.stream_sync(st)
+            assert all(np.array_equal(a, b) for a, b in zip(read(bufs[1]), want)), i
+            call(bufs[0])
+            h.stream_sync(st)
+            assert all(np.array_equal(a, b) for a, b in zip(read(bufs[0]), want)), i
+        h.graph_destroy(g)
+
+
+@pytest.mark.parametrize("n_q,lens", [(5, [75, 200, 33]), (130, [2500, 75, 200, 33, 1500, 1000])])
+def test_rows_behind_the_last_token_hold_nan(n_q, lens):
+    """Blocks that another sequence filled with NaN, taken again: slots past a
+    sequence's end take part in nothing, and stay as they are."""
+    say(f"stale NaN rows, {n_q} queries over {lens}")
+    blocks = sum((x + n_q) // 32 + 1 for x in lens) + len(lens)
+    bad = [np.full((blocks * 32, NKV, D), 0x7FC0, np.uint16)] * 2
+    with Q.Filled([0], seed=83, extra=blocks * 32, pool_blocks=blocks, q8_blocks=blocks, max_seqs=len(lens) + 1) as f:
+        c, p = f.ctx, f.seqs[0]
+        f.add([p], blocks * 32, rows=bad)
+        c.seq_reset(p)
+        del f.rows[0, p]
+        seqs = [c.seq_create() for _ in lens]
+        for s, x in zip(seqs, lens):
+            f.add([s], x)
+        c.kv_quantize(seqs, 20)
+        f.add(seqs, n_q, commit=False)
+        n = len(lens)
+        q = O.normal_bf16(n * n_q * NQ * D, 84).reshape(n, n_q, NQ, D)
+        stride = max(lens) + n_q
+        got = [f.run(lambda qb, ob: c.prefill_attn(0, seqs, n_q, qb, ob, scale=SCALE), q.shape, np.float32, q),
+               f.run(lambda qb, ob: c.prefill_attn(0, seqs, n_q, qb, ob, scale=SCALE, out_dtype=kvc.DTYPE_BF16), q.shape,
+                     np.uint16, q),
+               f.run(lambda qb, ob: c.decode_attn(0, seqs, qb, ob, scale=SCALE), (n, NQ, D), np.float32, q[:, -1].copy()),
+               f.run(lambda qb, ob: c.attn_weights(0, seqs, n_q, qb, ob, stride, scale=SCALE), (n, NKV, stride), np.float32,
+                     q, fill=0)]
+        for i, s in enumerate(seqs):
+            n8 = max(0, lens[i] - 20) // 32 * 32
+            k, v = (Q.values(f.rows[0, s][j], n8) for j in range(2))
+            want, mag, big, dig = Q.attend(Q.f64(q[i]), k, v, SCALE, first=lens[i], digits=True)
+            check(got[0][i].astype(np.float64), want, mag, big, False, False, f"fp32, {lens[i]}", dig)
+            check(load_out(got[1][i], True), want, mag, big, True, True, f"bf16, {lens[i]}", dig)
+            check(got[2][i].astype(np.float64), want[-1], mag[-1], big, False, False, f"decode, {lens[i]}", dig[-1])
+            w = Q.weights(Q.f64(q[i]), k, SCALE, lens[i])
+            assert np.abs(got[3][i, :, :lens[i] + n_q] - w).max() <= 2.0 ** -16 * max(1.0, w.max())
+
+
 @pytest.mark.parametrize("scale", [0.0, -1.0 / 16])
 def test_prefill_scales(scale):
     say(f"prefill8 scale {scale}")
