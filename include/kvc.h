@@ -320,7 +320,9 @@ int kvc_gather(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * A sequence with 8-bit blocks is read by kvc_decode_attn (no weight is
  * rounded to bf16), kvc_prefill_attn (weights as three bf16 parts when
  * out_dtype is fp32, as one when it is bf16), kvc_gather (bf16, RNE of i * s),
- * kvc_attn_weights and kvc_evict; kvc_append and kvc_qkv_append add to it.  It
+ * kvc_attn_weights and kvc_evict; kvc_append and kvc_qkv_append add to it.
+ * Sequences without such blocks in the same call are computed likewise (64 seqs
+ * at a time), so their last bits can differ from a call without the others.  It
  * no longer feeds the prefix index and is refused (KVC_ERR_UNSUPPORTED) by
  * kvc_decode_step, kvc_prefill_step, kvc_decode_attn_static, kvc_kv_checksum
  * and by kvc_snapshot_save when the snapshot's segment is in 8 bits. */
@@ -334,9 +336,10 @@ int kvc_kv_quantize(kvc_ctx* ctx, const int32_t* seqs, const int32_t* dst,
  * sees keys up to its own.  q: bf16 [n_seqs][n_q][Hq][D], n_q <= 256 and at
  * most len + pending.  acc_in (NULL: zeros) and acc_out: device fp32
  * [n_seqs][Hkv][acc_stride]; they may be the same array and must not overlap
- * otherwise.  Entries from len + pending on are left as they are.  The scores
- * go through the context's split-K workspace: 64 B per row and key of one seq
- * must fit into its 138 MB (KVC_ERR_RANGE otherwise: fewer rows a call).
+ * otherwise.  Entries from len + pending on are left as they are.  Partial
+ * results go through the context's split-K workspace: n_q times 65 B (n_q <= 4)
+ * or 0.5 B per key of one seq must fit into its 138 MB (KVC_ERR_RANGE
+ * otherwise: fewer rows a call).
  * fp32 throughout, without atomics: the same call gives the same bits. */
 int kvc_attn_weights(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
                      int32_t n_seqs, int32_t n_q, const void* q, float scale,
@@ -346,17 +349,18 @@ int kvc_attn_weights(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * first n_sink and the last n_recent tokens stay, and of the others those of
  * the greatest acc, budget - n_sink - n_recent of them (ties: the lower
  * position; NaN counts as lowest), all in their order.  acc: device fp32
- * [n_attn_layers][n_seqs][Hkv][acc_stride], acc_stride >= every length.
+ * [n_attn_layers][n_seqs][Hkv][acc_stride], acc_stride >= every length.  acc,
+ * acc_out and kept must not overlap.
  * kept: device int32 [n_attn_layers][n_seqs][Hkv][budget] receives the indices
  * of the tokens that stay, -1 past a shorter seq's length.  acc_out (NULL, or
- * shaped as acc and not overlapping it) receives their acc, then zeros up to
+ * shaped as acc) receives their acc, then zeros up to
  * the old length.  The kept rows are copied, bit for bit (8-bit ones as RNE
  * bf16 of i * s), into fresh bf16 blocks, which must be free beforehand
  * (KVC_ERR_NOMEM otherwise, with no change).
  * dst as for kvc_kv_quantize; in place, a seq of at most budget tokens is left
  * as it is.  len becomes the number of tokens kept, while positions go on:
  * kvc_qkv_append rotates new tokens at kvc_seq_info.position (KVC_ERR_RANGE
- * once that passes max_seq_len), rows of kvc_prefill_attn and kvc_attn_weights
+ * once that passes max_seq_len; kvc_evict itself once it nears 2^31), rows of kvc_prefill_attn and kvc_attn_weights
  * still see every cached token up to their own.  The seq no longer feeds the
  * prefix index; kvc_decode_step, kvc_prefill_step and the snapshots refuse it
  * (KVC_ERR_UNSUPPORTED) until it is reset. */

@@ -424,7 +424,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictSelectAr
         n_above += __popcll(ab_m);
         n_equal += __popcll(eq_m);
     });
-    for (int i = n_keep + t; i < a.budget; i += kSelThreads) kept[i] = -1;
+    for (uint32_t i = n_keep + t; i < (uint32_t)a.budget; i += kSelThreads) kept[i] = -1;  // (a budget near 2^31)
     if (acc_out)
         for (int i = n_keep + t; i < L; i += kSelThreads) acc_out[i] = 0.f;
 }

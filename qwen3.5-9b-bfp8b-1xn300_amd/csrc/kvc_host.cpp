@@ -1868,11 +1868,21 @@ int kvc_evict(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seq
         if (acc_stride < c->seqs[seqs[i]].len)
             return set_err(KVC_ERR_RANGE, "sequence %d: %d cached tokens, acc_stride %lld", seqs[i],
                            c->seqs[seqs[i]].len, (long long)acc_stride);
-    if (acc_out) {
-        const size_t bytes = (size_t)c->cfg.n_attn_layers * n_seqs * kKvHeads * (size_t)acc_stride * 4;
-        const uint8_t *x = static_cast<const uint8_t*>(acc), *y = static_cast<const uint8_t*>(acc_out);
-        if (x < y + bytes && y < x + bytes) return set_err(KVC_ERR_INVALID, "acc and acc_out overlap");
+    for (int32_t i = 0; i < n_seqs; i++) {
+        const Seq& s = c->seqs[seqs[i]];
+        if ((int64_t)s.evicted + s.len > INT32_MAX - c->cfg.max_seq_len)
+            return set_err(KVC_ERR_RANGE, "sequence %d: position %lld, the next tokens' would pass 32 bits", seqs[i],
+                           (long long)s.evicted + s.len);
     }
+    // (kept is read back as positions: what another array writes there must not be)
+    const size_t rows = (size_t)c->cfg.n_attn_layers * n_seqs * kKvHeads;
+    const size_t acc_bytes = rows * (size_t)acc_stride * 4, kept_bytes = rows * (size_t)budget * 4;
+    const auto overlap = [](const void* x, size_t nx, const void* y, size_t ny) {
+        return (uintptr_t)x < (uintptr_t)y + ny && (uintptr_t)y < (uintptr_t)x + nx;
+    };
+    if (overlap(acc, acc_bytes, kept, kept_bytes) ||
+        (acc_out && (overlap(acc, acc_bytes, acc_out, acc_bytes) || overlap(acc_out, acc_bytes, kept, kept_bytes))))
+        return set_err(KVC_ERR_INVALID, "acc, acc_out and kept must not overlap");
     // fresh blocks for every sequence that changes, before anything is moved
     std::vector<std::vector<int32_t>> fresh(n_seqs);
     int64_t total = 0;

@@ -384,3 +384,101 @@ def test_the_run_they_are_made_for():
         park(20)
         step()
         assert c.seq_info(seqs[0]).position == 400 + 6 and c.seq_len(seqs[0]) == budget + 1
+
+
+def test_calls_in_a_row_on_a_stream():
+    """weights, a cut, 8 bits, a chunk's rows, its attention and a decode step,
+    queued on a stream of their own with nothing waited for: the bits of the
+    same calls made one after the other"""
+    say("a run on a stream")
+    h = kvc.hip()
+    layers, n_q, budget, stride = 2, 16, 700, 1500
+    rng = np.random.default_rng(14)
+    rows = [O.normal_bf16(3 * n_q * NKV * D, 140 + i).reshape(3, n_q, NKV, D) for i in range(2)]
+    q = O.normal_bf16(3 * n_q * NQ * D, 142)
+    start = rng.random((layers, 3, NKV, stride)).astype(np.float32)
+
+    def run(stream, sync):
+        with Q.Filled([1400, 333, 900], layers=layers, seed=143, extra=n_q) as f:
+            c, seqs = f.ctx, f.seqs
+            qb, kb, vb = kvc.to_device(q), kvc.to_device(rows[0]), kvc.to_device(rows[1])
+            acc = kvc.to_device(start)
+            acc2 = kvc.to_device(np.full_like(start, 7.0))
+            kept = h.malloc(layers * 3 * NKV * budget * 4)
+            outs = [h.malloc(3 * n_q * NQ * D * 4) for _ in range(layers)] + [h.malloc(3 * NQ * D * 4) for _ in range(layers)]
+            h.sync()
+            per = 3 * NKV * stride * 4
+            steps = [lambda l=l: c.attn_weights(l, seqs, n_q, qb, acc.ptr + l * per, stride, acc_in=acc.ptr + l * per,
+                                                stream=stream) for l in range(layers)]
+            steps += [lambda: c.evict(seqs, budget, acc, stride, kept, n_sink=4, n_recent=64, acc_out=acc2, stream=stream),
+                      lambda: c.kv_quantize(seqs, 30, stream=stream), lambda: c.reserve(seqs, n_q, stream=stream)]
+            for l in range(layers):
+                steps += [lambda l=l: c.append(l, seqs, n_q, kb, vb, stream=stream),
+                          lambda l=l: c.prefill_attn(l, seqs, n_q, qb, outs[l], stream=stream)]
+            steps += [lambda: c.commit(seqs, n_q, stream=stream)]
+            steps += [lambda l=l: c.decode_attn(l, seqs, qb, outs[layers + l], stream=stream) for l in range(layers)]
+            for s in steps:
+                s()
+                if sync:
+                    h.sync()
+            h.sync()
+            assert [c.seq_info(s).position for s in seqs] == [1416, 349, 916]
+            assert [c.seq_len(s) for s in seqs] == [716, 349, 716]
+            got = [acc.download(np.uint32, start.shape), acc2.download(np.uint32, start.shape),
+                   kept.download(np.int32, (layers, 3, NKV, budget))]
+            return got + [o.download(np.uint32, (3, (n_q if i < layers else 1) * NQ * D)) for i, o in enumerate(outs)]
+
+    st = h.stream()
+    for a, b in zip(run(None, True), run(st, False)):
+        assert np.array_equal(a, b)
+
+
+def test_blocks_past_4_gib():
+    """pools of which a layer's K or V is over 4 GiB, bf16 and 8-bit: block ids
+    on either side"""
+    say("blocks past 4 GiB")
+    big = 66000  # blocks; 32 KiB each in 8 bits, 64 KiB in bf16
+    with Q.Filled([0], seed=150, max_seqs=4, max_seq_len=big * 32, pool_blocks=2 * big + 2000, q8_blocks=2 * big + 100) as f:
+        c = f.ctx
+        c.pool_fill_normal(3)
+        fill = [f.seqs[0], c.seq_create()]
+        for s in fill:  # the 8-bit ids below 4 GiB
+            c.reserve([s], big * 32)
+            c.commit([s], big * 32)
+            c.kv_quantize([s])
+            assert c.seq_info(s).q8_tokens == big * 32
+        c.sync()
+        a = c.seq_create()
+        n = 2000
+        f.add([a], n)
+        c.kv_quantize([a], 900)  # 34 8-bit blocks, 29 bf16 ones spread over their pool
+        rows = f.rows[0, a]
+        for got, x in zip(f.gather(0, a, n), rows):
+            Q.same_bits(got, Q.readback(x, 1088))
+        for n_q in (1, 8, 600):  # decode, and either prefill
+            if n_q > 1:
+                f.add([a], n_q, commit=False)
+                n += n_q
+            k, v = (Q.values(x, 1088) for x in f.rows[0, a])
+            q = O.normal_bf16(n_q * NQ * D, 151 + n_q).reshape(1, n_q, NQ, D)
+            if n_q == 1:
+                got = f.run(lambda x, o: c.decode_attn(0, [a], x, o, scale=SCALE), (1, NQ, D), np.float32, q)
+            else:
+                got = f.run(lambda x, o: c.prefill_attn(0, [a], n_q, x, o, scale=SCALE), (n_q, NQ, D), np.float32, q)
+            want, mag, big_qk, dig = Q.attend(Q.f64(q[0]), k, v, SCALE, first=n - n_q, digits=True)
+            tol = mag * 2.0 ** -22 * (big_qk + 2) + np.abs(want) * 2.0 ** -22 + 2.0 ** -30 * dig
+            assert (np.abs(got - want) <= tol).all(), n_q
+            if n_q <= 8:
+                w = f.run(lambda x, o: c.attn_weights(0, [a], n_q, x, o, n, scale=SCALE), (1, NKV, n), np.float32, q)
+                assert np.abs(w[0] - Q.weights(Q.f64(q[0]), k, SCALE, n - n_q)).max() <= 2.0 ** -16
+            if n_q > 1:
+                c.commit([a], n_q)
+        acc = np.random.default_rng(152).random((1, 1, NKV, n)).astype(np.float32)
+        ab, kept = kvc.to_device(acc), kvc.hip().malloc(NKV * 500 * 4)
+        c.evict([a], 500, ab, n, kept, n_sink=2, n_recent=9)
+        back = [Q.readback(x, 1088) for x in f.rows[0, a]]
+        got = f.gather(0, a, 500)
+        for h in range(NKV):
+            want = Q.keep(acc[0, 0, h], 500, 2, 9)
+            for j in range(2):
+                Q.same_bits(got[j][:, h], back[j][want, h])

@@ -281,3 +281,45 @@ def test_random_calls_keep_the_books():
         for x in list(live):
             c.seq_release(x)
         assert c.q8_stats()[1] == 40 and c.stats().free_blocks == 80
+
+
+def test_evict_refuses_arrays_that_overlap():
+    """kept is read back as positions"""
+    with ctx(n_attn_layers=2) as c:
+        s = fill(c, 100)
+        acc_bytes, kept_bytes = 2 * 4 * 128 * 4, 2 * 4 * 10 * 4
+        far = FAKE + (1 << 30)
+
+        def call(acc, kept, acc_out=None):
+            c.evict([s], 10, acc, 128, kept, acc_out=acc_out)
+
+        for args in ((FAKE, FAKE), (FAKE, FAKE + acc_bytes - 4), (FAKE, FAKE - kept_bytes + 4), (FAKE, far, FAKE),
+                     (FAKE, far, FAKE + acc_bytes - 4), (FAKE, far, far), (FAKE, far, far - acc_bytes + 4),
+                     (FAKE, far, far + kept_bytes - 4)):
+            assert code(call, *args) == kvc.KVC_ERR_INVALID, args
+        assert c.seq_info(s).len == 100
+        call(FAKE, FAKE + acc_bytes, FAKE + acc_bytes + kept_bytes)  # back to back
+        assert c.seq_info(s).len == 10
+
+
+def test_positions_end_below_31_bits():
+    """a sequence that is cut again and again: its positions go on, up to where
+    those of the next tokens could pass a 32-bit integer"""
+    n = 1 << 23
+    with ctx(max_seq_len=n, pool_blocks=n // 32 + 8, max_seqs=1, n_attn_layers=1, q8_blocks=0) as c:
+        s = fill(c, n)
+        rounds = 0
+        while True:
+            try:
+                c.evict([s], 1, FAKE, n, FAKE + (1 << 40))
+            except kvc.KvcError as e:
+                assert e.code == kvc.KVC_ERR_RANGE
+                break
+            rounds += 1
+            assert c.seq_info(s).position == n + (rounds - 1) * (n - 1)
+            c.reserve([s], n - 1)
+            c.commit([s], n - 1)
+        i = c.seq_info(s)
+        assert i.len == n and 2 ** 31 - 1 - n < i.position <= 2 ** 31 - 1
+        c.seq_reset(s)
+        assert c.seq_info(s).position == 0
