@@ -79,11 +79,13 @@ __device__ __forceinline__ void weights_mask(f32x4 (&st)[2], const WeightsArgs& 
             if (16 * t + 4 * (lane >> 4) + i > last) st[t][i] = -__builtin_inff();
 }
 
-// First launch: (max, sum 2^(s - max)) of every row over a chunk of one block
-// per wave.  STORE: one tile of rows, whose scores go to the workspace.
+// First launch: (max, sum 2^(s - max)) of every row over a chunk of a.chunk
+// blocks.  STORE: one tile of rows, whose scores go to the workspace, one block
+// per wave; otherwise the waves share the chunk's blocks, and those of a block
+// its tiles.
 template <bool STORE>
-__global__ __launch_bounds__(64 * weights_chunk(STORE), 4) void weights_score_kernel(WeightsArgs a) {
-    constexpr int W = weights_chunk(STORE), ROWS = STORE ? 16 : kWeightsRows;
+__global__ __launch_bounds__(64 * weights_waves(STORE), 4) void weights_score_kernel(WeightsArgs a) {
+    constexpr int W = weights_waves(STORE), ROWS = STORE ? 16 : kWeightsRows;
     __shared__ float2 ml[W][ROWS];
     __shared__ u32x4 qs[STORE ? 1 : ROWS * kHeadDim / 8];
     const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
@@ -92,7 +94,9 @@ __global__ __launch_bounds__(64 * weights_chunk(STORE), 4) void weights_score_ke
     const int s = find_seq(a.chunk_begin, a.n_seqs, chunk);
     const int L = a.kv_len[s], R = a.n_q * kGroup;
     const int nb = (L + kBlockTok - 1) / kBlockTok;
-    const int b = (chunk - a.chunk_begin[s]) * W + wave;
+    const int bw = STORE ? wave : wave & (a.chunk - 1);  // its block of the chunk
+    const int b = (chunk - a.chunk_begin[s]) * a.chunk + bw;
+    const int tile0 = STORE ? 0 : 16 * wave / a.chunk & ~15, tiles = STORE ? 16 : 16 * W / a.chunk;
     const bool masked = (b + 1) * kBlockTok > L - a.n_q + 1;  // a key that some row does not see
     const uint16_t* q = a.q + (size_t)s * a.n_q * kQHeads * kHeadDim;
     u32x4 kf[2][8];
@@ -113,7 +117,7 @@ __global__ __launch_bounds__(64 * weights_chunk(STORE), 4) void weights_score_ke
             __syncthreads();
         }
         if (b < nb) {
-            for (int r0 = g0; r0 < end; r0 += 16) {
+            for (int r0 = g0 + tile0; r0 < end; r0 += tiles) {
                 u32x4 qf[8];
 #pragma unroll
                 for (int ks = 0; ks < 8; ks++)
@@ -143,18 +147,16 @@ __global__ __launch_bounds__(64 * weights_chunk(STORE), 4) void weights_score_ke
 #pragma unroll
                     for (int t = 0; t < 2; t++) *reinterpret_cast<f32x4*>(out + 16 * t + 4 * g) = st[t];
                 }
-                if (g == 0) ml[wave][r0 - g0 + r16] = make_float2(mx, l);
+                if (g == 0) ml[bw][r0 - g0 + r16] = make_float2(mx, l);
             }
         } else {
-            for (int r = lane; r < ROWS; r += 64) ml[wave][r] = make_float2(kNegBig, 0.f);
+            for (int r = lane; r < ROWS; r += 64) ml[bw][r] = make_float2(kNegBig, 0.f);
         }
         __syncthreads();
         for (int r = threadIdx.x; r < end - g0; r += 64 * W) {
             float m = kNegBig, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; w++) m = fmaxf(m, ml[w][r].x);
-#pragma unroll
-            for (int w = 0; w < W; w++) l = fmaf(fast_exp2(ml[w][r].x - m), ml[w][r].y, l);
+            for (int w = 0; w < a.chunk; w++) m = fmaxf(m, ml[w][r].x);
+            for (int w = 0; w < a.chunk; w++) l = fmaf(fast_exp2(ml[w][r].x - m), ml[w][r].y, l);
             stats[g0 + r] = make_float2(m, l);
         }
         __syncthreads();
@@ -167,20 +169,38 @@ __device__ __forceinline__ float2 weights_fold(float2 x, float2 y) {
     return make_float2(m, fmaf(x.y, fast_exp2(x.x - m), y.y * fast_exp2(y.x - m)));
 }
 
-// (max, 1 / sum) of rows g0 .. g0 + n - 1 (n <= THREADS) over the nc chunks of
-// a sequence: LANES neighbouring threads share a row and take every LANES'th
-// chunk of it.
-template <int THREADS>
-__device__ __forceinline__ void weights_rows(float2* row_ml, const float2* stats, int R, int g0, int n, int nc, int t) {
+// (max, 1 / sum) of the R <= 16 rows over the nc chunks of a sequence: LANES
+// neighbouring threads of 256 share a row and take every LANES'th chunk of it.
+__device__ __forceinline__ void weights_few_rows(float2* row_ml, const float2* stats, int R, int nc, int t) {
     int lanes = 64;
-    while (lanes > 1 && lanes * n > THREADS) lanes >>= 1;
+    while (lanes * R > 256) lanes >>= 1;
     const int r = t / lanes;
+    float2 x = make_float2(kNegBig, 0.f);
+    if (r < R)
+#pragma unroll 4
+        for (int k = t % lanes; k < nc; k += lanes) x = weights_fold(x, stats[(size_t)k * R + r]);
+    for (int d = lanes >> 1; d > 0; d >>= 1) x = weights_fold(x, make_float2(__shfl_xor(x.x, d), __shfl_xor(x.y, d)));
+    if (t % lanes == 0 && r < R) row_ml[r] = make_float2(x.x, 1.0f / x.y);
+}
+
+// The same of n <= kWeightsRows rows from g0 on: neighbouring threads take
+// neighbouring rows, each of the PARTS groups of threads every PARTS'th chunk.
+// Rows from n on count for nothing: 2^(s - inf).
+template <int THREADS>
+__device__ __forceinline__ void weights_rows(float2* row_ml, float2* part, const float2* stats, int R, int g0, int n, int nc, int t) {
+    const int wide = n > 64 ? 128 : n > 32 ? 64 : 32, parts = THREADS / wide;
+    const int r = t % wide;
     float2 x = make_float2(kNegBig, 0.f);
     if (r < n)
 #pragma unroll 4
-        for (int k = t % lanes; k < nc; k += lanes) x = weights_fold(x, stats[(size_t)k * R + g0 + r]);
-    for (int d = lanes >> 1; d > 0; d >>= 1) x = weights_fold(x, make_float2(__shfl_xor(x.x, d), __shfl_xor(x.y, d)));
-    if (t % lanes == 0 && r < n) row_ml[r] = make_float2(x.x, 1.0f / x.y);
+        for (int k = t / wide; k < nc; k += parts) x = weights_fold(x, stats[(size_t)k * R + g0 + r]);
+    part[t] = x;
+    __syncthreads();
+    if (t < kWeightsRows) {
+        if (t < n)
+            for (int k = 1; k < parts; k++) x = weights_fold(x, part[k * wide + t]);
+        row_ml[t] = t < n ? make_float2(x.x, 1.0f / x.y) : make_float2(__builtin_inff(), 0.f);
+    }
 }
 
 // Second launch after stored scores: one workgroup = kWsumBlocks blocks of one
@@ -203,8 +223,8 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsArgs a) {
     float x[16];
 #pragma unroll
     for (int r = 0; r < 16; r++) x[r] = in && r < R ? sc[(size_t)r * kBlockTok] : 0.f;
-    weights_rows<256>(row_ml, reinterpret_cast<const float2*>(a.stats) + ((size_t)h * a.total_chunks + a.chunk_begin[s]) * R,
-                      R, 0, R, a.chunk_begin[s + 1] - a.chunk_begin[s], t);
+    weights_few_rows(row_ml, reinterpret_cast<const float2*>(a.stats) + ((size_t)h * a.total_chunks + a.chunk_begin[s]) * R,
+                     R, a.chunk_begin[s + 1] - a.chunk_begin[s], t);
     __syncthreads();
     if (!in) return;
     float w = 0.f;
@@ -215,11 +235,13 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightsArgs a) {
 }
 
 // Second launch without stored scores: the same waves compute them again.  A
-// lane sums its 8 keys' weights over the tiles in order, the 16 lanes of a key
-// are added at the end: the same bits each time.
-__global__ __launch_bounds__(64 * weights_chunk(false), 4) void weights_again_kernel(WeightsArgs a) {
-    constexpr int W = weights_chunk(false), ROWS = kWeightsRows;
+// lane sums its 8 keys' weights over the tiles in order; the 16 lanes of a key
+// and then the waves of a block are added at the end: the same bits each time.
+__global__ __launch_bounds__(64 * weights_waves(false), 4) void weights_again_kernel(WeightsArgs a) {
+    constexpr int W = weights_waves(false), ROWS = kWeightsRows;
     __shared__ float2 row_ml[ROWS];
+    __shared__ float2 part[64 * W];
+    __shared__ float sums[W][kBlockTok];
     __shared__ u32x4 qs[ROWS * kHeadDim / 8];
     const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -227,7 +249,8 @@ __global__ __launch_bounds__(64 * weights_chunk(false), 4) void weights_again_ke
     const int s = find_seq(a.chunk_begin, a.n_seqs, chunk);
     const int L = a.kv_len[s], R = a.n_q * kGroup;
     const int nb = (L + kBlockTok - 1) / kBlockTok;
-    const int b = (chunk - a.chunk_begin[s]) * W + wave;
+    const int b = (chunk - a.chunk_begin[s]) * a.chunk + (wave & (a.chunk - 1));
+    const int tile0 = 16 * wave / a.chunk & ~15, tiles = 16 * W / a.chunk;
     const bool masked = (b + 1) * kBlockTok > L - a.n_q + 1;
     const uint16_t* q = a.q + (size_t)s * a.n_q * kQHeads * kHeadDim;
     u32x4 kf[2][8];
@@ -248,13 +271,11 @@ __global__ __launch_bounds__(64 * weights_chunk(false), 4) void weights_again_ke
             __syncthreads();
             weights_stage_q(lds_addr(qs), a, q, h, g0, end, wave, W, lane);
         }
-        // a row past the last counts for nothing: 2^(s - inf)
-        for (int r = R - g0 + threadIdx.x; r < ROWS; r += 64 * W) row_ml[r] = make_float2(__builtin_inff(), 0.f);
-        weights_rows<64 * W>(row_ml, stats, R, g0, end - g0, nc, threadIdx.x);
+        weights_rows<64 * W>(row_ml, part, stats, R, g0, end - g0, nc, threadIdx.x);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (b >= nb) continue;
-        for (int r0 = g0; r0 < end; r0 += 16) {
+        for (int r0 = g0 + tile0; r0 < end; r0 += tiles) {
             u32x4 qf[8];
 #pragma unroll
             for (int ks = 0; ks < 8; ks++) qf[ks] = qs[((r0 - g0) / 2 + ks) * 64 + lane];
@@ -270,7 +291,6 @@ __global__ __launch_bounds__(64 * weights_chunk(false), 4) void weights_again_ke
                 for (int i = 0; i < 4; i++) w[t][i] = fmaf(fast_exp2(st[t][i] - x.x), x.y, w[t][i]);
         }
     }
-    if (b >= nb) return;
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -282,9 +302,15 @@ __global__ __launch_bounds__(64 * weights_chunk(false), 4) void weights_again_ke
         float mine = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) mine = r16 == i ? w[i >> 2][i & 3] : mine;
-        const int pos = b * kBlockTok + 16 * (r16 >> 2) + 4 * g + (r16 & 3);
+        sums[wave][16 * (r16 >> 2) + 4 * g + (r16 & 3)] = mine;
+    }
+    __syncthreads();
+    const int pos = (chunk - a.chunk_begin[s]) * a.chunk * kBlockTok + threadIdx.x;
+    if ((int)threadIdx.x < a.chunk * kBlockTok && pos < L) {
+        float sum = 0.f;
+        for (int v = threadIdx.x >> 5; v < W; v += a.chunk) sum += sums[v][threadIdx.x & 31];
         const size_t o = ((size_t)s * kKvHeads + h) * (size_t)a.stride + pos;
-        if (pos < L) a.acc_out[o] = (a.acc_in ? a.acc_in[o] : 0.f) + mine;
+        a.acc_out[o] = (a.acc_in ? a.acc_in[o] : 0.f) + sum;
     }
 }
 
@@ -480,11 +506,11 @@ int launch_weights(const WeightsArgs& a, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
     const dim3 grid(a.total_chunks * kKvHeads);
     if (weights_store(a.n_q)) {
-        hipLaunchKernelGGL(weights_score_kernel<true>, grid, dim3(64 * weights_chunk(true)), 0, st, a);
+        hipLaunchKernelGGL(weights_score_kernel<true>, grid, dim3(64 * weights_waves(true)), 0, st, a);
         hipLaunchKernelGGL(weights_sum_kernel, dim3(a.sum_chunks * kKvHeads), dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL(weights_score_kernel<false>, grid, dim3(64 * weights_chunk(false)), 0, st, a);
-        hipLaunchKernelGGL(weights_again_kernel, grid, dim3(64 * weights_chunk(false)), 0, st, a);
+        hipLaunchKernelGGL(weights_score_kernel<false>, grid, dim3(64 * weights_waves(false)), 0, st, a);
+        hipLaunchKernelGGL(weights_again_kernel, grid, dim3(64 * weights_waves(false)), 0, st, a);
     }
     return (int)hipGetLastError();
 }

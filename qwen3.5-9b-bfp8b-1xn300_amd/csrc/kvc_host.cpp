@@ -1795,7 +1795,11 @@ int kvc_attn_weights(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
     const auto bytes_of = [&](int64_t blocks, int64_t chunks) {
         return kKvHeads * rows * ((store ? blocks * kBlockTok * 4 : 0) + chunks * 8);
     };
-    const auto chunks_of = [&](int64_t blocks) { return (blocks + weights_chunk(store) - 1) / weights_chunk(store); };
+    int64_t all_blocks = 0;
+    for (int32_t i = 0; i < n_seqs; i++)
+        all_blocks += (c->seqs[seqs[i]].len + (int64_t)c->seqs[seqs[i]].pending + kBlockTok - 1) / kBlockTok;
+    const int32_t chunk = weights_chunk(n_q, all_blocks);
+    const auto chunks_of = [&](int64_t blocks) { return (blocks + chunk - 1) / chunk; };
     for (int32_t i = 0; i < n_seqs; i++) {
         const Seq& s = c->seqs[seqs[i]];
         const int32_t L = s.len + s.pending;
@@ -1849,6 +1853,7 @@ int kvc_attn_weights(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
         a.scale_log2 = scale * 1.4426950408889634f;
         a.n_seqs = n;
         a.n_q = n_q;
+        a.chunk = chunk;
         int e = launch_weights(a, stream);
         if (e) return hip_err((hipError_t)e, "attention weights launch");
         i0 += n;

@@ -428,7 +428,8 @@ struct WeightsArgs {
     float scale_log2;
     int32_t n_seqs;
     int32_t n_q;
-    int32_t total_chunks;     // of weights_chunk blocks, per kv head
+    int32_t chunk;            // blocks per workgroup of the first launch
+    int32_t total_chunks;     // per kv head
     int32_t total_blocks;
     int32_t sum_chunks;       // of kWsumBlocks blocks each
     int32_t slot[kMaxBatch];
@@ -438,10 +439,26 @@ struct WeightsArgs {
     int32_t chunk_begin[kMaxBatch + 1];
     int32_t sum_begin[kMaxBatch + 1];
 };
-// Up to one tile of rows the scores are stored between the two launches, above
-// they are computed again.
+// Up to one tile of rows the scores are stored between the two launches (R x 32
+// floats a block, beside 8 or 16 KB of keys), above they are computed again.  us
+// per layer, stored / again: 1 sequence of 4096 tokens, 1 query 8.9 / 14.0; 16
+// of 500-6000, 1 query 18.9 / 27.5; 64 of 500-8000, 1 query 99 / 150, 4 queries
+// 116 / 155; 16 x 32 queries over 500-6000 (stored: by a kernel without LDS) 98 /
+// 47.
 constexpr bool weights_store(int n_q) { return n_q * kGroup <= 16; }
-constexpr int weights_chunk(bool store) { return store ? 4 : 8; }  // blocks (waves) per workgroup
+constexpr int weights_waves(bool store) { return store ? 4 : 8; }  // per workgroup
+// Blocks per workgroup: one per wave; fewer, and several waves to a block, in
+// launches of few blocks while each wave has a tile of rows.  (Every workgroup
+// stages all rows.)  us per layer, this rule / one per wave: 1 sequence of 64
+// tokens, 64 queries 21.9 / 29.4; 8 of 64-100, 60 queries 23.2 / 29.4; 1 of 300,
+// 30 queries 17.1 / 19.0.  1 of 4000, 64 queries (one per wave), at 2 to a
+// workgroup: 32.5, 38.3.
+inline int weights_chunk(int n_q, int64_t blocks) {
+    const bool store = weights_store(n_q);
+    int chunk = weights_waves(store);
+    while (!store && chunk > 1 && blocks * kKvHeads < 32 * chunk && 16 * 8 / (chunk / 2) <= n_q * kGroup + 15) chunk /= 2;
+    return chunk;
+}
 constexpr int kWeightsRows = 128;  // rows whose statistics a workgroup holds at once
 constexpr int kWsumBlocks = 8;     // blocks per workgroup of the summing launch
 constexpr int kWeightsMaxQ = 256;  // query rows per sequence
