@@ -317,9 +317,11 @@ int kvc_gather(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * KVC_ERR_UNSUPPORTED, since their state is not copied.)
  * Sequences must have nothing pending.  The 8-bit pool has q8_blocks blocks;
  * KVC_ERR_NOMEM, with no change, if they do not suffice.
+ * Neither this call nor kvc_evict can be captured into a graph (KVC_ERR_STATE).
  * A sequence with 8-bit blocks is read by kvc_decode_attn (no weight is
  * rounded to bf16), kvc_prefill_attn (weights as three bf16 parts when
- * out_dtype is fp32, as one when it is bf16), kvc_gather (bf16, RNE of i * s),
+ * out_dtype is fp32, as one when it is bf16; a NaN or infinity in a value row of
+ * the chunk itself may also reach up to 63 rows before it), kvc_gather (bf16, RNE of i * s),
  * kvc_attn_weights and kvc_evict; kvc_append and kvc_qkv_append add to it.
  * Sequences without such blocks in the same call are computed likewise (64 seqs
  * at a time), so their last bits can differ from a call without the others.  It

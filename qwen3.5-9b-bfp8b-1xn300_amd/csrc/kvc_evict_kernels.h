@@ -15,7 +15,14 @@ namespace kvc {
 // operand (keys x dims; 8-bit blocks as exact bf16 integers, scaled after the
 // product), and the rows (row 4 i + g = query i, q head g of the group) pass
 // by in tiles of 16 as B operand, 128 rows at a time out of LDS, where they lie
-// in operand order for all 8 waves.  A lane then has 8 keys of one row.
+// in operand order for all 8 waves.  (Read from memory by every wave, 64 KB of
+// rows beside 8 of keys, they took the L1 path 3 times as long: 16 sequences x
+// 32 queries 119 us, with LDS 51.)  A lane then has 8 keys of one row.
+//
+// Few rows are bound by memory, or by two launches' latency: 64 sequences of
+// 500..8000 tokens, 1 query, bf16 144 us, 3.9 TB/s, 8-bit 99 us; 1 x 4096 10 us
+// (6 and 4).  Many rows by the exponentials and the row sums: 16 x 32 queries
+// over 500..6000 8-bit tokens 25 and 27 us, twice 13.6 GFLOP and 53 MB.
 __device__ __forceinline__ void weights_load_k(u32x4 (&kf)[2][8], const MixedCache& c, int id, int h, bool q8, int lane) {
     const int r16 = lane & 15, g = lane >> 4;
     const size_t unit = (size_t)id * kKvHeads + h;
@@ -323,6 +330,9 @@ __global__ __launch_bounds__(64 * weights_waves(false), 4) void weights_again_ke
 // ones that still fit.  Sinks and recent tokens have no part in the choice.
 // Wave w takes the w'th sixteenth of the row; REGS keys per thread stay in
 // registers over the passes, 0: rows too long for that are read again.
+// Bound by latency (one memory access, 14 barriers of 16 waves, the atomics of
+// equal digits): 8 layers of 4096 tokens 11-12 us, 16 sequences of 5000 12 us
+// (four passes of 8 bits over memory 13.2 and 14.2).
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelRegs = 8, kSelBins = 2048;
 
 // Greater weight -> greater key; NaN lowest; -0 as +0.
@@ -457,7 +467,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictSelectAr
 
 // Moves the kept rows: one workgroup = one (layer, K|V, kv head) unit of a new
 // block.  Rows of 8-bit blocks become bf16(i s).  Slots past the new length
-// are left as they were.
+// are left as they were.  Bound by memory, 512 B at a time from anywhere: 1501
+// of 5000 tokens of 16 sequences 34 us, 5.8 TB/s read and written.
 __global__ __launch_bounds__(256) void evict_copy_kernel(EvictCopyArgs a) {
     const int per = a.p.n_layers * 2 * kKvHeads;
     const int i = blockIdx.x / per, u = blockIdx.x % per;

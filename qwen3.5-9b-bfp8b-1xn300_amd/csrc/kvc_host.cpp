@@ -1681,8 +1681,10 @@ static MixedPools mixed_pools(kvc_ctx* c) {
 }
 
 // The sequences that kvc_kv_quantize / kvc_evict read (and change, unless dst
-// names the empty sequences that receive the result).
-static int check_src_dst(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, const char* what) {
+// names the empty sequences that receive the result).  A graph would replay the
+// blocks of the capture, which others hold by then.
+static int check_src_dst(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, const char* what,
+                         void* stream) {
     int rc;
     if ((rc = check_seqs(c, seqs, n_seqs)) || (dst && (rc = check_seqs(c, dst, n_seqs)))) return rc;
     for (int32_t i = 0; i < n_seqs; i++) {
@@ -1696,7 +1698,15 @@ static int check_src_dst(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, in
     }
     if (dst && c->cfg.n_ssm_layers > 0)
         return set_err(KVC_ERR_UNSUPPORTED, "%s into other sequences does not copy recurrent state", what);
-    return c->has_device ? check_current(c) : KVC_OK;
+    if (!c->has_device) return KVC_OK;
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (stream) {  // (the null stream is never captured)
+        hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &capture);
+        if (e != hipSuccess) return hip_err(e, "hipStreamIsCapturing");
+    }
+    if (capture != hipStreamCaptureStatusNone)
+        return set_err(KVC_ERR_STATE, "%s changes block tables and cannot be captured into a graph", what);
+    return check_current(c);
 }
 
 int kvc_kv_quantize(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, int32_t keep_tokens,
@@ -1704,7 +1714,7 @@ int kvc_kv_quantize(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t
     if (!c) return set_err(KVC_ERR_INVALID, "null context");
     int rc;
     if (keep_tokens < 0) return set_err(KVC_ERR_INVALID, "keep_tokens must be >= 0");
-    if ((rc = check_src_dst(c, seqs, dst, n_seqs, "kvc_kv_quantize"))) return rc;
+    if ((rc = check_src_dst(c, seqs, dst, n_seqs, "kvc_kv_quantize", stream))) return rc;
     // blocks that become 8-bit ones: [n8, n8 + count)
     std::vector<int32_t> count(n_seqs);
     int64_t total = 0;
@@ -1868,7 +1878,7 @@ int kvc_evict(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seq
     if (budget <= 0 || n_sink < 0 || n_recent < 0 || (int64_t)n_sink + n_recent > budget)
         return set_err(KVC_ERR_INVALID, "evict needs a positive budget that holds n_sink + n_recent tokens");
     if (!acc || !kept) return set_err(KVC_ERR_INVALID, "evict needs acc and kept");
-    if ((rc = check_src_dst(c, seqs, dst, n_seqs, "kvc_evict"))) return rc;
+    if ((rc = check_src_dst(c, seqs, dst, n_seqs, "kvc_evict", stream))) return rc;
     for (int32_t i = 0; i < n_seqs; i++)
         if (acc_stride < c->seqs[seqs[i]].len)
             return set_err(KVC_ERR_RANGE, "sequence %d: %d cached tokens, acc_stride %lld", seqs[i],

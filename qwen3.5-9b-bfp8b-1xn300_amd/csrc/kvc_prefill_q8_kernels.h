@@ -20,10 +20,13 @@ namespace kvc {
 // B operand: lane half f, product j takes keys 16 j + 4 f + {0..3, 8..11}, the
 // order in which V pieces hold their tokens.
 //
-// Bounds: a step is 1024 cycles of products per SIMD (2 waves x 32 x 16) and 256
-// KB out of LDS per CU, 2048 cycles at 128 B each; softmax and widening fill
-// what is left.  16 sequences of 128 rows over 256..6000 keys: 150 us, 650
-// TFLOP/s, against 1260 of a large matrix product; the fold 20 us.
+// Bounds: a step is 2048 cycles of products per SIMD (2 waves x 32 x 32) and 304
+// KB through the LDS port per CU, about as long; softmax and widening another
+// 1500 of VALU issue.  Measured, 16 sequences of 128 rows over 256..6000 keys:
+// 150 us, 650 TFLOP/s, against 1260 of a large matrix product (the clock is near
+// 1.7 GHz); the matrix pipe is busy 37 % of the cycles, VALU 27 %, LDS 24 %, and
+// the two waves per SIMD spend 35 % of their time at waits and barriers.  The
+// fold takes another 21 us.
 //
 // 8-bit blocks: pieces go from memory straight to LDS as they are
 // (global_load_lds, 3 steps ahead of their use, no registers); during step b
@@ -477,6 +480,8 @@ void prefill_q8_kernel(PrefillQ8Args a) {
 // sum(w_p acc_p) / sum(w_p l_p), w_p = 2^(m_p - max m).  a.fold workgroups per
 // cut (those of a cut that is not its item's first have nothing to do); a wave
 // takes 32 rows of a q head x 32 dims at a time, as the parts stored them.
+// Bound by the partials' bytes (262 KB each): 21 us after 16 sequences of 128
+// rows over 256..6000 keys.
 constexpr int kP8Fold = 3;  // parts requested at once
 __global__ __launch_bounds__(256) void prefill_q8_combine_kernel(PrefillQ8Args a) {
     const int cut = blockIdx.x / a.fold + 1;  // between workgroups cut - 1 and cut

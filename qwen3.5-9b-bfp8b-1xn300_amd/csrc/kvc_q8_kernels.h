@@ -35,7 +35,10 @@ __device__ __forceinline__ int q8_v_off(int tok, int d) {
 // floor under a keeps the reciprocal finite: a unit of smaller values reads as
 // (nearly) zeros.  A unit with an infinity or a NaN gets s = NaN, so that
 // everything computed from it is NaN, as it would be from the bf16 rows.
-// V pieces hold 8 tokens of a dim, so the unit is turned through LDS.
+// V pieces hold 8 tokens of a dim, so the unit is turned through LDS.  Bound by
+// memory: each byte is read once and the unit sits in registers between the
+// maximum and the rounding.  8 layers of 4096 tokens (134 MB read, 67 written)
+// 36 us, 5.6 TB/s; 2 layers of 16 x 992 tokens 32 us, 6.1 TB/s.
 __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a) {
     __shared__ __align__(16) uint16_t tile[kBlockTok * kHeadDim];
     __shared__ uint32_t wmax[4];
@@ -105,7 +108,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a) {
 // Gather over sequences with 8-bit blocks: one workgroup = one unit of a cache
 // block that the range [tok0, tok0 + n) of its sequence touches.  8-bit units
 // become bf16(i s) rows in LDS first, so that the output rows (512 B a token
-// and head) are written whole.
+// and head) are written whole.  One layer of 16 x 1000 tokens 20 us, 4.9 TB/s;
+// of 4096 tokens 6.5 us, of which most is the launch and one memory latency.
 __global__ __launch_bounds__(256) void gather_q8_kernel(GatherQ8Args a) {
     // rows 16 B apart from a multiple of 128 B: 16 lanes that write one dim
     // range of 16 tokens fall on different banks
@@ -180,6 +184,10 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(GatherQ8Args a) {
 // than 2^-30 of it per weight, whatever other blocks hold.  The matrix pipe
 // has rows to spare (4 heads of 16 rows), so the digits are free; the block's
 // 16 KiB cost about 220 VALU instructions and 24 MFMAs.
+// Bound by memory from some tens of sequences on: 64 sequences of 512..16384
+// tokens 178 us, 1037 MB at 5.8 TB/s; 8 of 777..6001 20.5 us a layer, 3.5 TB/s
+// (the run-up of 2 workgroups a CU); below that by latency: 1 x 4096 8.8 us, 1 x
+// 300 6.6 us a layer.
 //
 // digits: bytes 0..3 of dig30(x) are x's signed base-256 digits
 __device__ __forceinline__ uint32_t dig30(int n) { return ((uint32_t)n + 0x00808080u) ^ 0x00808080u; }

@@ -482,3 +482,35 @@ def test_blocks_past_4_gib():
             want = Q.keep(acc[0, 0, h], 500, 2, 9)
             for j in range(2):
                 Q.same_bits(got[j][:, h], back[j][want, h])
+
+
+def test_calls_that_change_tables_are_not_captured():
+    say("quantize and evict refuse capture")
+    h = kvc.hip()
+    with Q.Filled([200, 100], seed=160) as f:
+        c, seqs = f.ctx, f.seqs
+        st = h.stream()
+        acc, kept = h.malloc(2 * NKV * 200 * 4).zero(), h.malloc(2 * NKV * 50 * 4).zero()
+        out = h.malloc(2 * NKV * 200 * 4).zero()
+        q = kvc.to_device(O.normal_bf16(2 * NQ * D, 161))
+        h.sync()
+        codes = []
+
+        def body():
+            for call in (lambda: c.kv_quantize(seqs, stream=st), lambda: c.evict(seqs, 50, acc, 200, kept, stream=st)):
+                try:
+                    call()
+                    codes.append(0)
+                except kvc.KvcError as e:
+                    codes.append(e.code)
+            c.attn_weights(0, seqs, 1, q, out, 200, stream=st)
+
+        g = h.capture(st, body)
+        assert codes == [kvc.KVC_ERR_STATE] * 2
+        h.graph_launch(g, st)
+        h.stream_sync(st)
+        assert [c.seq_len(s) for s in seqs] == [200, 100] and c.seq_info(seqs[0]).q8_tokens == 0
+        assert not kept.download(np.uint32, (2 * NKV * 50,)).any()
+        got = out.download(np.float32, (2, NKV, 200))
+        assert np.abs(got[0].sum(1) - 4).max() < 1e-4 and np.abs(got[1].sum(1) - 4).max() < 1e-4
+        h.graph_destroy(g)
