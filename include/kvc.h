@@ -335,8 +335,8 @@ int kvc_kv_quantize(kvc_ctx* ctx, const int32_t* seqs, const int32_t* dst,
  *   acc_out[s][h][j] = acc_in[s][h][j] + sum over the n_q rows i and the 4 q
  *   heads of kv head h of softmax_j((q_i . k_j) * scale)
  * for j < len + pending; row i sits at position len + pending - n_q + i and
- * sees keys up to its own.  q: bf16 [n_seqs][n_q][Hq][D], n_q <= 256 and at
- * most len + pending.  acc_in (NULL: zeros) and acc_out: device fp32
+ * sees keys up to its own.  q: bf16 [n_seqs][n_q][Hq][D], aligned to 16 bytes,
+ * n_q <= 256 and at most len + pending.  acc_in (NULL: zeros) and acc_out: device fp32
  * [n_seqs][Hkv][acc_stride]; they may be the same array and must not overlap
  * otherwise.  Entries from len + pending on are left as they are.  Partial
  * results go through the context's split-K workspace: n_q times 65 B (n_q <= 4)

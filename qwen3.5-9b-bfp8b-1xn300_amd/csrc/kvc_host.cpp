@@ -1406,7 +1406,7 @@ static int prefill_q8_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int
     }
     a.n_seqs = n;
     a.n_q = n_q;
-    if (!prefill_q8_split(a)) return set_err(KVC_ERR_RANGE, "prefill too large");
+    prefill_q8_split(a);
     a.c = mixed_cache(c, layer);
     a.q = static_cast<const uint16_t*>(q);
     a.gate = static_cast<const uint16_t*>(gate);
@@ -1520,6 +1520,15 @@ int kvc_prefill_attn(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
     int rc;
     if ((rc = check_prefill(c, layer, seqs, n_seqs, n_q, out, out_dtype, scale))) return rc;
     if (any_q8(c, seqs, n_seqs) && (rc = check_current(c))) return rc;
+    for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
+        PrefillArgs a;
+        a.n_seqs = std::min(kMaxBatch, n_seqs - i0);
+        a.n_q = n_q;
+        if (!any_q8(c, seqs + i0, a.n_seqs)) continue;
+        for (int32_t j = 0; j < a.n_seqs; j++)
+            a.q_pos0[j] = c->seqs[seqs[i0 + j]].len + c->seqs[seqs[i0 + j]].pending - n_q;
+        if (!prefill_q8_fits(a)) return set_err(KVC_ERR_RANGE, "prefill of %d rows too large", n_q);
+    }
     return prefill_launches(c, layer, seqs, n_seqs, n_q, q, gate, nullptr, KVC_DTYPE_BF16, nullptr, out, out_dtype,
                             scale, stream);
 }
@@ -1796,6 +1805,8 @@ int kvc_attn_weights(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
     int rc;
     if ((rc = check_device(c)) || (rc = check_layer(c, layer)) || (rc = check_seqs(c, seqs, n_seqs))) return rc;
     if (!q || !acc_out || n_q <= 0) return set_err(KVC_ERR_INVALID, "attention weights need q, acc_out and n_q > 0");
+    if (((uintptr_t)q & 15) || (((uintptr_t)acc_in | (uintptr_t)acc_out) & 3))
+        return set_err(KVC_ERR_INVALID, "attention weights need q aligned to 16 bytes, the accumulators to 4");
     if (n_q > kWeightsMaxQ)
         return set_err(KVC_ERR_RANGE, "attention weights of %d rows per sequence (at most %d)", n_q, kWeightsMaxQ);
     if (!std::isfinite(scale)) return set_err(KVC_ERR_INVALID, "scale must be finite");
@@ -1878,6 +1889,8 @@ int kvc_evict(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seq
     if (budget <= 0 || n_sink < 0 || n_recent < 0 || (int64_t)n_sink + n_recent > budget)
         return set_err(KVC_ERR_INVALID, "evict needs a positive budget that holds n_sink + n_recent tokens");
     if (!acc || !kept) return set_err(KVC_ERR_INVALID, "evict needs acc and kept");
+    if (((uintptr_t)acc | (uintptr_t)acc_out | (uintptr_t)kept) & 3)
+        return set_err(KVC_ERR_INVALID, "evict needs acc, acc_out and kept aligned to 4 bytes");
     if ((rc = check_src_dst(c, seqs, dst, n_seqs, "kvc_evict", stream))) return rc;
     for (int32_t i = 0; i < n_seqs; i++)
         if (acc_stride < c->seqs[seqs[i]].len)

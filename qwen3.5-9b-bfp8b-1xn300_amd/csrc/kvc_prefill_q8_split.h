@@ -27,14 +27,25 @@ inline bool prefill_q8_few(const PrefillArgs& a) {
     return blocks <= kMost;
 }
 
-// Fills begin, cut, seq_at, n_wgs and per_xcd from n_seqs, n_q and q_pos0;
-// false if the line is too long.  A workgroup pays kP8Item blocks' time for
+// Whether the line of a launch's key blocks has 32-bit indices with room to
+// spare (every item counted as its sequence's longest): checked for a call's
+// launches before the first one is made.
+inline bool prefill_q8_fits(const PrefillArgs& a) {
+    const int64_t n_rb = ((int64_t)a.n_q + kP8Rows - 1) / kP8Rows;
+    int64_t total = 0;
+    for (int32_t j = 0; j < a.n_seqs; j++)
+        total += kKvHeads * n_rb * (((int64_t)a.q_pos0[j] + a.n_q + kBlockTok - 1) / kBlockTok);
+    return total <= INT32_MAX / 2;
+}
+
+// Fills begin, cut, seq_at, n_wgs and per_xcd from n_seqs, n_q and q_pos0, for
+// launches that fit.  A workgroup pays kP8Item blocks' time for
 // each item that it takes up (its query rows, first copies and result) and a
 // block's for each block; a cut inside an item costs two partials and their
 // fold.  So runs are filled in order up to a common bound, an item that fits
 // is not cut, and one that does not is cut only into parts of a fifth of the
 // bound and more; the bound is raised until the runs are few enough.
-inline bool prefill_q8_split(PrefillQ8Args& a) {
+inline void prefill_q8_split(PrefillQ8Args& a) {
     constexpr int64_t kP8Item = 7, kP8MinPart = 4;
     const auto blocks = [&](int32_t j, int64_t rb) {
         return (a.q_pos0[j] + std::min<int64_t>((rb + 1) * kP8Rows, a.n_q) + kBlockTok - 1) / kBlockTok;
@@ -45,7 +56,6 @@ inline bool prefill_q8_split(PrefillQ8Args& a) {
         a.begin[j] = (int32_t)total;
         for (int64_t rb = 0; rb < n_rb; rb++) total += kKvHeads * blocks(j, rb);
         longest = std::max(longest, blocks(j, n_rb - 1));
-        if (total > INT32_MAX / 2) return false;
     }
     a.begin[a.n_seqs] = (int32_t)total;
     const int64_t items = a.n_seqs * n_rb * kKvHeads;
@@ -92,7 +102,6 @@ inline bool prefill_q8_split(PrefillQ8Args& a) {
     while (!fill(bound)) bound += std::max<int64_t>(1, bound / 24);
     a.per_xcd = (a.n_wgs + 7) / 8;
     a.fold = 16;
-    return true;
 }
 
 }  // namespace kvc

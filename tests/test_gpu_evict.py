@@ -97,6 +97,23 @@ def test_weights_in_several_launches():
     weights_case([2000] * 12, 128, 0, seed=97)
 
 
+def test_alignment_refusals():
+    say("weights and evict alignment")
+    with Q.Filled([100], seed=98) as f:
+        c, (a,) = f.ctx, f.seqs
+        buf = kvc.hip().malloc(1 << 20).zero()
+        P, F = buf.ptr, buf.ptr + (1 << 19)
+        for call in (lambda: c.attn_weights(0, [a], 1, P + 8, F, 100), lambda: c.attn_weights(0, [a], 1, P, F + 2, 100),
+                     lambda: c.attn_weights(0, [a], 1, P, F, 100, acc_in=F + 4001), lambda: c.evict([a], 50, P + 1, 100, F),
+                     lambda: c.evict([a], 50, P, 100, F + 2), lambda: c.evict([a], 50, P, 100, F, acc_out=F + 8003)):
+            with pytest.raises(kvc.KvcError) as e:
+                call()
+            assert e.value.code == kvc.KVC_ERR_INVALID
+        c.sync()
+        assert not buf.download(np.uint8, (1 << 20,)).any() and c.seq_len(a) == 100
+        buf.free()
+
+
 @pytest.mark.parametrize("lens,n_q", [([200, 31, 900], 4), ([200, 31, 900], 5), ([257, 600], 33)])
 def test_weights_around_a_tile_of_rows(lens, n_q):
     """16 rows per kv head are the last whose scores are stored, 128 the last

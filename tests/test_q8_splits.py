@@ -44,7 +44,8 @@ int main() {
             in >> a->n_q;
             few.n_q = a->n_q;
             for (int p; in >> p;) few.q_pos0[few.n_seqs++] = a->q_pos0[a->n_seqs++] = p;
-            const bool ok = prefill_q8_split(*a);
+            const bool ok = prefill_q8_fits(few);
+            if (ok) prefill_q8_split(*a);
             std::printf("%d %d %d %d", (int)prefill_q8_few(few), (int)ok, a->n_wgs, a->per_xcd);
             for (int j = 0; ok && j <= a->n_seqs; j++) std::printf(" %d", a->begin[j]);
             for (int w = 0; ok && w <= a->n_wgs; w++) std::printf(" %d", a->cut[w]);
@@ -140,5 +141,6 @@ def test_prefill_runs_cover_every_block(split):
 
 
 def test_prefill_too_large_is_refused(split):
-    (few, ok, *_), = split([("p", 1 << 20, 1 << 20)])
-    assert not few and not ok
+    for n_q, prefix in ((1 << 20, [1 << 20]), (1 << 15, [1 << 20] * 64), (2 ** 31 - 64, [0])):
+        (few, ok, *_), = split([("p", n_q, *prefix)])
+        assert not few and not ok
