@@ -89,12 +89,39 @@ def test_weights_scales(scale):
 
 
 def test_weights_in_several_launches():
-    """70 sequences, and scores that fill the workspace more than once: 40
-    sequences of 2000 keys, 128 rows each"""
+    """70 sequences, and 12 of 2000 keys with 128 rows each"""
     say("weights 70 sequences")
     weights_case([int(x) for x in np.random.default_rng(1).integers(5, 200, 70)], 3, 20, seed=96)
     say("weights 128 rows")
     weights_case([2000] * 12, 128, 0, seed=97)
+
+
+@pytest.mark.parametrize("n,n_q", [(20, 4), (40, 256)])
+def test_weights_that_fill_the_workspace(n, n_q):
+    """stored scores (20 sequences of 30000 keys: 156 MB) and row statistics (40:
+    154 MB) take two launches: the bits of calls of one sequence each"""
+    say(f"weights, workspace filled by {n_q} queries")
+    L = 30000
+    with Q.Filled([0], seed=110, max_seqs=n + 1, max_seq_len=L, pool_blocks=n * (L // 32 + 1), q8_blocks=8) as f:
+        c, h = f.ctx, f.h
+        c.pool_fill_normal(5)
+        seqs = [f.seqs[0]] + [c.seq_create() for _ in range(n - 1)]
+        c.reserve(seqs, L)
+        c.commit(seqs, L)
+        q = kvc.to_device(O.normal_bf16(n * n_q * NQ * D, 111))
+        per = NKV * L * 4
+        a, b = h.malloc(n * per).zero(), h.malloc(n * per).zero()
+        h.sync()
+        c.attn_weights(0, seqs, n_q, q, a, L)
+        for i, s in enumerate(seqs):
+            c.attn_weights(0, [s], n_q, q.ptr + i * n_q * NQ * D * 2, b.ptr + i * per, L)
+        c.sync()
+        x, y = (z.download(np.float32, (n, NKV, L)) for z in (a, b))
+        assert np.array_equal(x, y)
+        # a row's weights sum to 1 within the scores' 2^-22 sum |q k| scale log2(e), below 64 here
+        assert np.abs(x.sum(2, dtype=np.float64) - 4 * n_q).max() <= 4 * n_q * 2.0 ** -16
+        for z in (q, a, b):
+            z.free()
 
 
 def test_alignment_refusals():
