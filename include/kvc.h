@@ -241,7 +241,8 @@ int kvc_decode_attn(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
 /* No counterpart in the reference.  kvc_decode_attn for callers that cannot
  * allocate device memory (code under HIP graph capture, tight serving loops,
  * harnesses that forbid hipMalloc): same arguments, semantics and results
- * (bit for bit: same work split and kernels), but the split-K partials and
+ * (bit for bit: same work split and kernels, unless out is fp32 and q8_blocks >
+ * 0: kvc_kv_quantize), but the split-K partials and
  * arrival counters live in the library's static per-GPU workspace -- a
  * file-scope __device__ array of 4096 split-K items plus counters, 17.6 MB,
  * held by each GPU the library runs on until the process ends -- instead of
@@ -265,7 +266,8 @@ int kvc_decode_attn_static(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * in_dtype; q_norm, k_norm: device fp32 [D]; out: [n_seqs][Hq][D] in
  * out_dtype.  Same bits as kvc_qkv_append (same rows, one token) followed by
  * kvc_decode_attn with the produced q and gate and with the appended k / v
- * rows passed as k_new / v_new.  Uses the context's split-K workspace. */
+ * rows passed as k_new / v_new (unless out is fp32 and q8_blocks > 0:
+ * kvc_kv_quantize).  Uses the context's split-K workspace. */
 int kvc_decode_step(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
                     int32_t n_seqs, const void* qkv, int32_t in_dtype,
                     const void* q_norm, const void* k_norm, void* out,
@@ -290,7 +292,8 @@ int kvc_prefill_attn(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * qkv: [n_seqs][n_q][Hq*2*D + 2*Hkv*D] in kvc_qkv_append's layout, fp32 or
  * bf16 by in_dtype; q_norm, k_norm: device fp32 [D]; out: [n_seqs][n_q][Hq][D]
  * in out_dtype.  Same bits (output and cache) as kvc_qkv_append with q_out and
- * gate_out followed by kvc_prefill_attn on them.  Two launches, three when the
+ * gate_out followed by kvc_prefill_attn on them (unless out is fp32 and
+ * q8_blocks > 0: kvc_kv_quantize).  Two launches, three when the
  * keys are split (kvc_prefill_attn). */
 int kvc_prefill_step(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
                      int32_t n_seqs, int32_t n_q, const void* qkv,
@@ -323,8 +326,12 @@ int kvc_gather(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * out_dtype is fp32, as one when it is bf16; a NaN or infinity in a value row of
  * the chunk itself may also reach up to 63 rows before it), kvc_gather (bf16, RNE of i * s),
  * kvc_attn_weights and kvc_evict; kvc_append and kvc_qkv_append add to it.
- * Sequences without such blocks in the same call are computed likewise (64 seqs
- * at a time), so their last bits can differ from a call without the others.  It
+ * In a context with q8_blocks > 0, kvc_decode_attn and kvc_prefill_attn with
+ * fp32 output compute every sequence likewise, whether it or another one of the
+ * call holds 8-bit blocks.  With bf16 output they do so for the sequences that
+ * share 64 of a call with one that holds some; the last bits can differ from a
+ * call without it.  (kvc_decode_step, kvc_prefill_step and
+ * kvc_decode_attn_static round weights to bf16 in every context.)  The sequence
  * no longer feeds the prefix index and is refused (KVC_ERR_UNSUPPORTED) by
  * kvc_decode_step, kvc_prefill_step, kvc_decode_attn_static, kvc_kv_checksum
  * and by kvc_snapshot_save when the snapshot's segment is in 8 bits. */

@@ -523,6 +523,14 @@ bool any_q8(kvc_ctx* c, const int32_t* seqs, int32_t n) {
     return false;
 }
 
+// Whether an attention launch runs the kernels that read 8-bit blocks.  They
+// hold weights in more than bf16, so with fp32 output a context that has such
+// blocks runs them in every launch: else a sequence would be 1e-3 off or not by
+// whether another one of the launch holds an 8-bit block.
+bool mixed_launch(kvc_ctx* c, const int32_t* seqs, int32_t n, int32_t out_dtype) {
+    return any_q8(c, seqs, n) || (c->cfg.q8_blocks > 0 && out_dtype == KVC_DTYPE_F32);
+}
+
 int check_seqs(kvc_ctx* c, const int32_t* seqs, int32_t n) {
     if (!seqs || n <= 0) return set_err(KVC_ERR_INVALID, "empty sequence list");
     for (int32_t i = 0; i < n; i++) {
@@ -1278,7 +1286,7 @@ static MixedCache mixed_cache(kvc_ctx* c, int32_t layer) {
     return m;
 }
 
-// The decode launch over seqs[i0, i0 + n) of which some hold 8-bit blocks.
+// The decode launch over seqs[i0, i0 + n) of which some may hold 8-bit blocks.
 static int build_decode_q8_args(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t i0, int32_t n, const void* q,
                                 const void* k_new, const void* v_new, const void* gate, void* out, int32_t out_dtype,
                                 float scale, DecodeQ8Args& a) {
@@ -1335,7 +1343,8 @@ static int decode_impl(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n
     if (out_dtype != KVC_DTYPE_F32 && out_dtype != KVC_DTYPE_BF16) return set_err(KVC_ERR_INVALID, "bad out_dtype");
     if (!std::isfinite(scale)) return set_err(KVC_ERR_INVALID, "scale must be finite");
     if (!part || !counters) return set_err(KVC_ERR_STATE, "no %s", workspace);
-    const bool q8 = any_q8(c, seqs, n_seqs);
+    // (kvc_decode_attn alone has both kinds of launch)
+    const bool q8 = !prod.qkv && part == c->d_part && mixed_launch(c, seqs, n_seqs, out_dtype);
     if (prod.qkv && (rc = refuse_mixed(c, seqs, n_seqs, "kvc_decode_step", true))) return rc;
     if (part != c->d_part && (rc = refuse_mixed(c, seqs, n_seqs, "kvc_decode_attn_static", false))) return rc;
     if (q8 && (rc = check_current(c))) return rc;
@@ -1344,7 +1353,7 @@ static int decode_impl(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n
     for (int pass = 0; pass < 2; pass++) {
         for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
             const int32_t n = std::min(kMaxBatch, n_seqs - i0);
-            if (q8 && any_q8(c, seqs + i0, n)) {
+            if (q8 && mixed_launch(c, seqs + i0, n, out_dtype)) {
                 if ((rc = build_decode_q8_args(c, layer, seqs, i0, n, q, k_new, v_new, gate, out, out_dtype, scale, a8)))
                     return rc;
                 if (pass == 1) {
@@ -1394,7 +1403,7 @@ int kvc_decode_attn_static(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
                        kStaticItems, "static decode workspace");
 }
 
-// One prefill launch over sequences of which some hold 8-bit blocks (at most 64).
+// One prefill launch over sequences of which some may hold 8-bit blocks (at most 64).
 static int prefill_q8_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n, int32_t n_q, const void* q,
                              const void* gate, void* out, int32_t out_dtype, float scale, void* stream) {
     PrefillQ8Args a{};
@@ -1438,7 +1447,7 @@ static int prefill_launches(kvc_ctx* c, int32_t layer, const int32_t* seqs, int3
         }
         a.n_seqs = n;
         a.n_q = n_q;
-        const bool q8 = any_q8(c, seqs + i0, n);  // (never with qkv: kvc_prefill_step refuses them)
+        const bool q8 = !qkv && mixed_launch(c, seqs + i0, n, out_dtype);  // (kvc_prefill_step refuses 8-bit blocks)
         if (q8 && !prefill_q8_few(a)) {
             const size_t off = (size_t)i0 * qrow;
             int rc = prefill_q8_launch(c, layer, seqs + i0, n, n_q, static_cast<const uint16_t*>(q) + off,
@@ -1519,12 +1528,12 @@ int kvc_prefill_attn(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_s
     if (!q) return set_err(KVC_ERR_INVALID, "prefill needs q, out and n_q > 0");
     int rc;
     if ((rc = check_prefill(c, layer, seqs, n_seqs, n_q, out, out_dtype, scale))) return rc;
-    if (any_q8(c, seqs, n_seqs) && (rc = check_current(c))) return rc;
+    if (mixed_launch(c, seqs, n_seqs, out_dtype) && (rc = check_current(c))) return rc;
     for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
         PrefillArgs a;
         a.n_seqs = std::min(kMaxBatch, n_seqs - i0);
         a.n_q = n_q;
-        if (!any_q8(c, seqs + i0, a.n_seqs)) continue;
+        if (!mixed_launch(c, seqs + i0, a.n_seqs, out_dtype)) continue;
         for (int32_t j = 0; j < a.n_seqs; j++)
             a.q_pos0[j] = c->seqs[seqs[i0 + j]].len + c->seqs[seqs[i0 + j]].pending - n_q;
         if (!prefill_q8_fits(a)) return set_err(KVC_ERR_RANGE, "prefill of %d rows too large", n_q);
