@@ -173,10 +173,14 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(GatherQ8Args a) {
 // Decode over 8-bit blocks.  A wave takes whole blocks of its chunk (one kv
 // head), straight from memory into matrix operands, and works in int8
 // products with int32 sums, which are exact:
-//   q of a head = amax 2^-30 (sum over k of 256^k Q_k), Q_k signed base-256
-//     digits (30 bits of the row's largest value); the 4 digit planes of the
-//     4 heads are the 16 rows of the A operand, K's tokens the columns
-//   s = amax 2^-30 scale ks (sum over k of 256^k Q_k . K)
+//   q of a head = 2^(e - 29) (sum over k of 256^k Q_k), 2^e the power of two at
+//     or below the row's largest value, Q_k signed base-256 digits; the 4 digit
+//     planes of the 4 heads are the 16 rows of the A operand, K's tokens the
+//     columns.  bf16 values from 2^(e - 22) on are exact in them.  If the wave
+//     has smaller ones that are not, what is left of them, in 30 more bits, takes
+//     4 more planes and a second set of products (they decide the scores where
+//     K is near 0 in the large channels)
+//   s = 2^(e - 29) scale ks (sum over k of 256^k Q_k . K)
 //   p = 2^(s - m), m = the block's largest score of the head, in 30-bit digits
 //     likewise; o += 2^(m - M) vs 2^-30 (sum over k of 256^k P_k . V)
 // with fp32 running M (the offset, raised when a block exceeds it by the
@@ -194,7 +198,8 @@ __device__ __forceinline__ uint32_t dig30(int n) { return ((uint32_t)n + 0x00808
 
 struct Q8Wave {
     i32x4_t q[4];      // A operand: row (plane k = c / 4, head c % 4), dims 64 s + 16 g .. +15
-    float qs[2];       // amax 2^-30 scale log2(e) of heads 2 (g / 2), + 1
+    bool low;          // the planes of what q leaves are in use (LDS, laid out as q's)
+    float qs[2];       // 2^(e - 29) scale log2(e) of heads 2 (g / 2), + 1
     float acc[16][4];  // dims 16 t + c of head r, plane g's share
     float m[2], l[2];  // of heads 2 (g / 2), + 1: offset (uniform over the heads' lanes), lane's part of the sum
 };
@@ -240,31 +245,49 @@ __device__ __forceinline__ void q8_load_q(Q8Wave& w, const uint16_t* qhead0, flo
     mf = max_xor16(mf);
     mf = max_xor32(mf);
     mx = (uint32_t)mf;
-    const float amax = fmaxf(__uint_as_float(mx << 16), 0x1p-90f);
+    // 2^e, at least 2^-90
+    const uint32_t e = max(mx >> 7, 127u - 90u) << 23;
     const bool bad = mx >= 0x7F80u;
-    const float up = 0x1p30f / amax;
+    const float up = bad ? 0.f : __uint_as_float(((2 * 127 + 29) << 23) - e);  // 2^(29 - e)
     uint32_t dg[16];
+    const auto planes = [&] {
 #pragma unroll
-    for (int i = 0; i < 16; i++) dg[i] = dig30((int)(bad ? 0.f : f[i] * up));
+        for (int k = 0; k < 4; k++) {  // plane k: byte k of each digit word
+            u32x4 o;
+            const uint32_t sel = (uint32_t)k | (uint32_t)(k + 4) << 8 | 0x0C0C0000u;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {  // plane k: byte k of each digit word
-        u32x4 o;
-        const uint32_t sel = (uint32_t)k | (uint32_t)(k + 4) << 8 | 0x0C0C0000u;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t lo = __builtin_amdgcn_perm(dg[4 * i + 1], dg[4 * i], sel);
-            const uint32_t hi = __builtin_amdgcn_perm(dg[4 * i + 3], dg[4 * i + 2], sel);
-            o[i] = lo | hi << 16;
+            for (int i = 0; i < 4; i++) {
+                const uint32_t lo = __builtin_amdgcn_perm(dg[4 * i + 1], dg[4 * i], sel);
+                const uint32_t hi = __builtin_amdgcn_perm(dg[4 * i + 3], dg[4 * i + 2], sel);
+                o[i] = lo | hi << 16;
+            }
+            lds[((k * 4 + head) * 4 + sp) * 4 + g] = o;
         }
-        lds[((k * 4 + head) * 4 + sp) * 4 + g] = o;
+        wave_lds_sync();
+    };
+    bool low = false;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        f[i] = bad ? 0.f : f[i] * up;  // exact
+        const float y = rintf(f[i]);
+        dg[i] = dig30((int)y);
+        f[i] -= y;  // exact, at most 1/2
+        low |= f[i] != 0.f;
     }
-    wave_lds_sync();
+    planes();
 #pragma unroll
     for (int s = 0; s < 4; s++) {
         const u32x4 o = lds[(c * 4 + s) * 4 + g];
         w.q[s] = __builtin_bit_cast(i32x4_t, o);
     }
-    const float mine = bad ? nan_f() : amax * 0x1p-30f * scale_log2;
+    w.low = __builtin_amdgcn_ballot_w64(low) != 0;
+    if (w.low) {
+        wave_lds_sync();
+#pragma unroll
+        for (int i = 0; i < 16; i++) dg[i] = dig30((int)rintf(f[i] * 0x1p30f));
+        planes();
+    }
+    const float mine = bad ? nan_f() : __uint_as_float(e) * 0x1p-29f * scale_log2;
     const float h0 = readlane(mine, 0), h1 = readlane(mine, 1), h2 = readlane(mine, 2), h3 = readlane(mine, 3);
     w.qs[0] = g < 2 ? h0 : h2;
     w.qs[1] = g < 2 ? h1 : h3;
@@ -280,7 +303,7 @@ __device__ __forceinline__ float swap32_add(float a, float b) {  // lower half: 
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-__device__ __forceinline__ void q8_block(const Q8Block& b, Q8Wave& w, uint32_t* pl, float w256, int lane) {
+__device__ __forceinline__ void q8_block(const Q8Block& b, Q8Wave& w, const u32x4* lds, uint32_t* pl, float w256, int lane) {
     const int c = lane & 15, g = lane >> 4;
     // planes x keys: lane holds plane g of heads r = 0..3, keys 16 t + c
     i32x4_t s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
@@ -289,11 +312,31 @@ __device__ __forceinline__ void q8_block(const Q8Block& b, Q8Wave& w, uint32_t* 
         s0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(w.q[s], __builtin_bit_cast(i32x4_t, b.k[s]), s0, 0, 0, 0);
         s1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(w.q[s], __builtin_bit_cast(i32x4_t, b.k[4 + s]), s1, 0, 0, 0);
     }
+    float y0[4], y1[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        y0[r] = (float)s0[r] * w256;
+        y1[r] = (float)s1[r] * w256;
+    }
+    if (w.low) {
+        s0 = s1 = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const u32x4 o = lds[(c * 4 + s) * 4 + g];
+            s0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, o), __builtin_bit_cast(i32x4_t, b.k[s]), s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, o), __builtin_bit_cast(i32x4_t, b.k[4 + s]), s1, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            y0[r] = fmaf((float)s0[r], w256 * 0x1p-30f, y0[r]);
+            y1[r] = fmaf((float)s1[r], w256 * 0x1p-30f, y1[r]);
+        }
+    }
     // sum of the planes; lane (g, c) ends with key 16 (g & 1) + c of heads
     // 2 (g / 2) and + 1
     float x[4];
 #pragma unroll
-    for (int r = 0; r < 4; r++) x[r] = swap16_add((float)s0[r] * w256, (float)s1[r] * w256);
+    for (int r = 0; r < 4; r++) x[r] = swap16_add(y0[r], y1[r]);
     float sc[2], p[2], f[2];
     bool up = false;
 #pragma unroll
@@ -410,10 +453,10 @@ void decode_q8_kernel(DecodeQ8Args a) {
         uint32_t* pl = sm.w.p[wave];
         for (; b < blk1; b += 2 * kWaves) {
             if (b + kWaves < blk1) q8_load(r1, a.c, trow[b + kWaves], h, lane);
-            q8_block(r0, w, pl, w256, lane);
+            q8_block(r0, w, sm.w.q[wave], pl, w256, lane);
             if (b + kWaves >= blk1) break;
             if (b + 2 * kWaves < blk1) q8_load(r0, a.c, trow[b + 2 * kWaves], h, lane);
-            q8_block(r1, w, pl, w256, lane);
+            q8_block(r1, w, sm.w.q[wave], pl, w256, lane);
         }
         // sum the planes: lane (g, c) ends with dims 16 t + c of the 4 tiles
         // t = i + 4 (g / 2) + 8 (g & 1), i = 0..3
