@@ -364,8 +364,9 @@ int kvc_attn_weights(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * of the tokens that stay, -1 past a shorter seq's length.  acc_out (NULL, or
  * shaped as acc) receives their acc, then zeros up to
  * the old length.  The kept rows are copied, bit for bit (8-bit ones as RNE
- * bf16 of i * s), into fresh bf16 blocks, which must be free beforehand
- * (KVC_ERR_NOMEM otherwise, with no change).
+ * bf16 of i * s), into fresh bf16 blocks, which must be free beforehand or held
+ * by the prefix index alone, which then gives them up (KVC_ERR_NOMEM otherwise,
+ * with no change).
  * dst as for kvc_kv_quantize; in place, a seq of at most budget tokens is left
  * as it is.  len becomes the number of tokens kept, while positions go on:
  * kvc_qkv_append rotates new tokens at kvc_seq_info.position (KVC_ERR_RANGE

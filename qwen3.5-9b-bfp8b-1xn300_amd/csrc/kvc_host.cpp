@@ -214,6 +214,20 @@ bool evict_one(kvc_ctx* c) {
     return false;
 }
 
+// How many blocks evict_one can reclaim: those that only the index holds and
+// that no entry in use descends from (a chain is given up from its leaf on).
+int64_t reclaimable_blocks(const kvc_ctx* c) {
+    std::vector<char> held(c->entries.size(), 0);
+    int64_t n = 0;
+    for (const Entry& en : c->entries) {
+        if (!en.live) continue;
+        n++;
+        if (c->refcnt[en.block] == 1) continue;
+        for (int32_t e = (int32_t)(&en - c->entries.data()); e >= 0 && !held[e]; e = c->entries[e].parent) held[e] = 1;
+    }
+    return n - std::count(held.begin(), held.end(), 1);
+}
+
 void unref_block8(kvc_ctx* c, int32_t b) {
     if (--c->refcnt8[b] == 0) c->free_blocks8.push_back(b);
 }
@@ -1920,27 +1934,21 @@ int kvc_evict(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seq
     if (overlap(acc, acc_bytes, kept, kept_bytes) ||
         (acc_out && (overlap(acc, acc_bytes, acc_out, acc_bytes) || overlap(acc_out, acc_bytes, kept, kept_bytes))))
         return set_err(KVC_ERR_INVALID, "acc, acc_out and kept must not overlap");
-    // fresh blocks for every sequence that changes, before anything is moved
+    // fresh blocks for every sequence that changes, before anything is moved;
+    // counted first, since to allocate one may cost the index an entry
     std::vector<std::vector<int32_t>> fresh(n_seqs);
-    int64_t total = 0;
-    bool fail = false;
-    for (int32_t i = 0; i < n_seqs && !fail; i++) {
+    const auto need = [&](int32_t i) -> int32_t {
         const Seq& s = c->seqs[seqs[i]];
-        if (!dst && s.len <= budget) continue;  // keeps all of its tokens, where they are
-        const int32_t need = (std::min(s.len, budget) + kBlockTok - 1) / kBlockTok;
-        for (int32_t b = 0; b < need; b++) {
-            const int32_t id = alloc_block(c);
-            if (id < 0) { fail = true; break; }
-            fresh[i].push_back(id);
-        }
-        total += need;
-    }
-    if (fail || total * c->cfg.n_attn_layers * 2 * kKvHeads > INT32_MAX) {
-        for (const auto& f : fresh)
-            for (int32_t id : f) unref_block(c, id);
-        if (!fail) return set_err(KVC_ERR_RANGE, "evict too large");
+        if (!dst && s.len <= budget) return 0;  // keeps all of its tokens, where they are
+        return (std::min(s.len, budget) + kBlockTok - 1) / kBlockTok;
+    };
+    int64_t total = 0;
+    for (int32_t i = 0; i < n_seqs; i++) total += need(i);
+    if (total * c->cfg.n_attn_layers * 2 * kKvHeads > INT32_MAX) return set_err(KVC_ERR_RANGE, "evict too large");
+    if (total > (int64_t)c->free_blocks.size() && total > (int64_t)c->free_blocks.size() + reclaimable_blocks(c))
         return set_err(KVC_ERR_NOMEM, "block pool exhausted: eviction writes the kept tokens to fresh blocks");
-    }
+    for (int32_t i = 0; i < n_seqs; i++)
+        for (int32_t b = need(i); b > 0; b--) fresh[i].push_back(alloc_block(c));  // cannot fail: counted above
     for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch) {
         const int32_t n = std::min(kMaxBatch, n_seqs - i0);
         EvictSelectArgs sel{};
