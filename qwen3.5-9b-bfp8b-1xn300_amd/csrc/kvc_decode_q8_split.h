@@ -51,7 +51,7 @@ inline void decode_q8_split(const int32_t* nb, int32_t n, int32_t chunk_blocks, 
     };
     int64_t chunks;
     if (chunk_blocks > 0) {
-        chunks = cut(chunk_blocks);
+        chunks = cut(caller_chunk_blocks(chunk_blocks));
     } else {
         for (cb8 = 4; (chunks = cut(cb8)) > 96 && cb8 < std::min(longest, 20); cb8 += 4) {}
         if (chunks > 96) chunks = cut(std::max(12, (int32_t)std::lround(0.25 * std::sqrt((double)total))));

@@ -1222,7 +1222,7 @@ static int build_decode_args(kvc_ctx* c, int32_t layer, const int32_t* seqs, int
     }
     const bool auto_cb = c->cfg.decode_chunk_blocks <= 0;
     const bool force_split = c->cfg.flags & KVC_FLAG_DECODE_SPLIT_D;
-    int32_t cb = auto_cb ? auto_chunk_blocks(nblk, n, force_split) : c->cfg.decode_chunk_blocks;
+    int32_t cb = auto_cb ? auto_chunk_blocks(nblk, n, force_split) : caller_chunk_blocks(c->cfg.decode_chunk_blocks);
     const int64_t max_chunks = force_split ? kMaxChunks / kMaxDParts : kMaxChunks;
     int64_t total_chunks;
     for (;;) {

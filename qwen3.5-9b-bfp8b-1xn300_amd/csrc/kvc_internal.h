@@ -47,6 +47,9 @@ constexpr size_t kQ8BlockBytes = kQ8UnitBytes * kKvHeads;        // 32 KiB
 
 constexpr int kMaxBatch = 64;        // seqs per kernel launch (argument block)
 constexpr int kMaxChunks = 8192;     // split-K work chunks per decode launch
+// A chunk length set by the caller (kvc_config): up to the blocks of 2^31 tokens,
+// so that 32-bit sums of it and a sequence's blocks hold.
+constexpr int caller_chunk_blocks(int n) { return n < (1 << 26) ? n : 1 << 26; }
 // split-K partial of one work item: acc [4 q heads][256] fp32 then (m, l) per
 // head, padded to whole 128-B lines so no line is shared by two items
 constexpr int kItemFloats = 1056;
