@@ -228,27 +228,32 @@ __device__ __forceinline__ void q8_load_q(Q8Wave& w, const uint16_t* qhead0, flo
     const u32x4* src = reinterpret_cast<const u32x4*>(qhead0 + head * kHeadDim + 64 * sp + 16 * g);
     const u32x4 x0 = src[0], x1 = src[1];
     float f[16];
-    uint32_t mx = 0;
+    // largest magnitude and, less one bit pattern, the smallest that is not 0, of
+    // even and of odd elements (bf16 bits order as integers)
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0}, least = {0xFFFF, 0xFFFF};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        f[2 * i] = bf16lo(x0[i]);
-        f[2 * i + 1] = bf16hi(x0[i]);
-        f[8 + 2 * i] = bf16lo(x1[i]);
-        f[9 + 2 * i] = bf16hi(x1[i]);
-        mx = max(max(mx, x0[i] & 0x7FFFu), max((x0[i] >> 16) & 0x7FFFu, max(x1[i] & 0x7FFFu, (x1[i] >> 16) & 0x7FFFu)));
+    for (int i = 0; i < 8; i++) {
+        const uint32_t w = i < 4 ? x0[i & 3] : x1[i & 3];
+        f[2 * i] = bf16lo(w);
+        f[2 * i + 1] = bf16hi(w);
+        const u16x2 a = __builtin_bit_cast(u16x2, w & 0x7FFF7FFFu);
+        most = __builtin_elementwise_max(most, a);
+        least = __builtin_elementwise_min(least, a - u16x2{1, 1});
     }
-    // the head's maximum over its 16 lanes (c / 4 and g); bf16 bits order as
-    // integers, exact in fp32
+    uint32_t mx = max((uint32_t)most[0], (uint32_t)most[1]);
+    // the head's maximum over its 16 lanes (c / 4 and g); bits are exact in fp32
     float mf = (float)mx;
     mf = fmaxf(mf, dpp<kDppRowRor8>(mf));
     mf = fmaxf(mf, dpp<0x124>(mf));  // row rotate by 4
     mf = max_xor16(mf);
     mf = max_xor32(mf);
     mx = (uint32_t)mf;
-    // 2^e, at least 2^-90
-    const uint32_t e = max(mx >> 7, 127u - 90u) << 23;
+    const uint32_t e = max(mx >> 7, 127u - 90u) << 23;  // 2^e as fp32 bits, at least 2^-90
     const bool bad = mx >= 0x7F80u;
-    const float up = bad ? 0.f : __uint_as_float(((2 * 127 + 29) << 23) - e);  // 2^(29 - e)
+    const float up = __uint_as_float(((2 * 127 + 29) << 23) - e);  // 2^(29 - e)
+    // an element under 2^(e - 22) may have bits below the digits
+    w.low = __builtin_amdgcn_ballot_w64(min((uint32_t)least[0], (uint32_t)least[1]) < (e >> 16) - (22u << 7)) != 0;
     uint32_t dg[16];
     const auto planes = [&] {
 #pragma unroll
@@ -265,14 +270,10 @@ __device__ __forceinline__ void q8_load_q(Q8Wave& w, const uint16_t* qhead0, flo
         }
         wave_lds_sync();
     };
-    bool low = false;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         f[i] = bad ? 0.f : f[i] * up;  // exact
-        const float y = rintf(f[i]);
-        dg[i] = dig30((int)y);
-        f[i] -= y;  // exact, at most 1/2
-        low |= f[i] != 0.f;
+        dg[i] = dig30((int)f[i]);
     }
     planes();
 #pragma unroll
@@ -280,11 +281,10 @@ __device__ __forceinline__ void q8_load_q(Q8Wave& w, const uint16_t* qhead0, flo
         const u32x4 o = lds[(c * 4 + s) * 4 + g];
         w.q[s] = __builtin_bit_cast(i32x4_t, o);
     }
-    w.low = __builtin_amdgcn_ballot_w64(low) != 0;
-    if (w.low) {
+    if (w.low) {  // what the cut left, below 1 in magnitude
         wave_lds_sync();
 #pragma unroll
-        for (int i = 0; i < 16; i++) dg[i] = dig30((int)rintf(f[i] * 0x1p30f));
+        for (int i = 0; i < 16; i++) dg[i] = dig30((int)((f[i] - truncf(f[i])) * 0x1p30f));
         planes();
     }
     const float mine = bad ? nan_f() : __uint_as_float(e) * 0x1p-29f * scale_log2;
