@@ -136,7 +136,8 @@ typedef struct kvc_config {
                                   (64, model_config.h:22); 0 or a power of two
                                   in [8, head_dim] */
     int32_t q8_blocks;         /* 8-bit blocks per layer (kvc_kv_quantize); 0 = none.
-                                  A block of 32 tokens takes 32.1 KiB here, 64 in bf16 */
+                                  A block of 32 tokens takes 64 KiB and 32 B per
+                                  layer here, K and V together, 128 KiB in bf16 */
 } kvc_config;
 
 typedef struct kvc_stats {
@@ -322,7 +323,8 @@ int kvc_gather(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * KVC_ERR_NOMEM, with no change, if they do not suffice.
  * Neither this call nor kvc_evict can be captured into a graph (KVC_ERR_STATE).
  * A sequence with 8-bit blocks is read by kvc_decode_attn (no weight is
- * rounded to bf16), kvc_prefill_attn (weights as three bf16 parts when
+ * rounded to bf16; queries in 60 bits below the head's largest value),
+ * kvc_prefill_attn (weights as three bf16 parts when
  * out_dtype is fp32, as one when it is bf16; a NaN or infinity in a value row of
  * the chunk itself may also reach up to 63 rows before it), kvc_gather (bf16, RNE of i * s),
  * kvc_attn_weights and kvc_evict; kvc_append and kvc_qkv_append add to it.
@@ -370,8 +372,9 @@ int kvc_attn_weights(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * dst as for kvc_kv_quantize; in place, a seq of at most budget tokens is left
  * as it is.  len becomes the number of tokens kept, while positions go on:
  * kvc_qkv_append rotates new tokens at kvc_seq_info.position (KVC_ERR_RANGE
- * once that passes max_seq_len; kvc_evict itself once it nears 2^31), rows of kvc_prefill_attn and kvc_attn_weights
- * still see every cached token up to their own.  The seq no longer feeds the
+ * once that passes max_seq_len; kvc_evict itself once it nears 2^31), rows of
+ * kvc_prefill_attn and kvc_attn_weights still see every cached token up to their
+ * own.  The seq no longer feeds the
  * prefix index; kvc_decode_step, kvc_prefill_step and the snapshots refuse it
  * (KVC_ERR_UNSUPPORTED) until it is reset. */
 int kvc_evict(kvc_ctx* ctx, const int32_t* seqs, const int32_t* dst,

@@ -19,16 +19,18 @@ namespace kvc {
 // shortest multiple of 4 blocks that stays within it, up to 20 or to one chunk
 // per sequence.  Above it a chunk's start, exchange and combine weigh more
 // than the tail of the last workgroups; both shrink the total relatively with
-// the square root of the launch.  us per layer, this rule / chunks of:
-//   1 x 4096 tokens        8.8 / 8: 10.6
-//   1 x 16000             14.3 / 8: 14.4
-//   2 x 6000              12.6 / 8: 12.1, 12: 13.2
-//   4 x 3000..9000        18.6 / 8: 17.2, 16: 17.4
-//   8 x 777..6001         20.5 / 8: 22.2, 16: 21.8
-//   64 x 300              18.4 / 4: 22.1
-//   24 x 100..4000        29.4 / 8: 27.9, 16: 26.5
-//   64 x 500..3000        58.3 / 8: 58.3, 12: 56.3, 24: 57.8
-//   64 x 512..16384      177.7 / 16: 188.7, 24: 183.1, 32: 179.8, 48: 187.4
+// the square root of the launch.  us per layer of calls back to
+// back, this rule / chunks of:
+//   1 x 4096 tokens        9.0 / 8: 10.7
+//   1 x 16000             14.3 / 8: 14.5
+//   2 x 6000              12.7 / 8: 12.2, 12: 13.3
+//   4 x 3000..9000        18.6 / 8: 17.4, 16: 17.5
+//   8 x 777..6001         20.5 / 8: 22.4, 16: 22.0
+//   64 x 300              18.6 / 4: 22.7
+//   24 x 100..4000        29.5 / 8: 28.3, 16: 26.4
+//   64 x 500..3000        58.7 / 8: 58.8, 12: 57.0, 24: 57.8
+//   64 x 512..16384      178.0 / 16: 188.5, 24: 183.3, 32: 180.1, 48: 186.6
+// (behind the best fixed length by up to 11 % between those ends)
 inline void decode_q8_split(const int32_t* nb, int32_t n, int32_t chunk_blocks, DecodeQ8Args& a) {
     int64_t total = 0;  // in 8-bit blocks; a bf16 block has the bytes of two
     int32_t longest = 1;

@@ -20,9 +20,13 @@ namespace kvc {
 // 32 queries 119 us, with LDS 51.)  A lane then has 8 keys of one row.
 //
 // Few rows are bound by memory, or by two launches' latency: 64 sequences of
-// 500..8000 tokens, 1 query, bf16 144 us, 3.9 TB/s, 8-bit 99 us; 1 x 4096 10 us
-// (6 and 4).  Many rows by the exponentials and the row sums: 16 x 32 queries
-// over 500..6000 8-bit tokens 25 and 27 us, twice 13.6 GFLOP and 53 MB.
+// 500..8000 tokens, 1 query, bf16 124 + 22 us, 4.0 TB/s; 1 x 4096 10 us (6 and 4).
+// In 8 bits the 64 sequences take 82 + 22 us, 2.9 TB/s: a wave has one block to
+// ask for and to widen, and waits 59 % of its cycles.  Many rows wait too: 16 x 32
+// queries over 500..6000 8-bit tokens 25 and 27 us, each 11.8 GFLOP and 52 MB;
+// the matrix pipe is busy 20-22 % of the cycles, VALU 31-34 % (exponentials
+// counted as any other instruction), LDS 13-17 %, and the waves spend 48 % of
+// theirs at waits (each workgroup's rows and keys, once, with nothing beside).
 __device__ __forceinline__ void weights_load_k(u32x4 (&kf)[2][8], const MixedCache& c, int id, int h, bool q8, int lane) {
     const int r16 = lane & 15, g = lane >> 4;
     const size_t unit = (size_t)id * kKvHeads + h;

@@ -540,7 +540,10 @@ bool any_q8(kvc_ctx* c, const int32_t* seqs, int32_t n) {
 // Whether an attention launch runs the kernels that read 8-bit blocks.  They
 // hold weights in more than bf16, so with fp32 output a context that has such
 // blocks runs them in every launch: else a sequence would be 1e-3 off or not by
-// whether another one of the launch holds an 8-bit block.
+// whether another one of the launch holds an 8-bit block.  What that costs a
+// launch without one, us per layer, bf16 kernels (bf16 output) / these: decode of
+// 1 sequence of 4096 tokens 8.7 / 10.2, of 8 of 777..6001 25.8 / 33.0; prefill of
+// 32 rows over 4001 keys 21.4 / 27.5, of 16 x 128 rows over 256..6000 172 / 308.
 bool mixed_launch(kvc_ctx* c, const int32_t* seqs, int32_t n, int32_t out_dtype) {
     return any_q8(c, seqs, n) || (c->cfg.q8_blocks > 0 && out_dtype == KVC_DTYPE_F32);
 }

@@ -20,13 +20,13 @@ namespace kvc {
 // B operand: lane half f, product j takes keys 16 j + 4 f + {0..3, 8..11}, the
 // order in which V pieces hold their tokens.
 //
-// Bounds: a step is 2048 cycles of products per SIMD (2 waves x 32 x 32) and 304
-// KB through the LDS port per CU, about as long; softmax and widening another
-// 1500 of VALU issue.  Measured, 16 sequences of 128 rows over 256..6000 keys:
-// 150 us, 650 TFLOP/s, against 1260 of a large matrix product (the clock is near
-// 1.7 GHz); the matrix pipe is busy 37 % of the cycles, VALU 27 %, LDS 24 %, and
-// the two waves per SIMD spend 35 % of their time at waits and barriers.  The
-// fold takes another 21 us.
+// Bounds: a step is 2048 cycles of products per SIMD (2 waves x 32 x 32), 304 KB
+// of LDS access per CU, 1330 cycles by SQ_LDS_IDX_ACTIVE, and 1500 of VALU issue
+// for softmax and widening.  Measured, 16 sequences of 128 rows over 256..6000
+// keys: 150 us, 650 TFLOP/s, against 1260 of a large matrix product (the clock is
+// near 1.7 GHz); the matrix pipe is busy 37 % of the cycles, VALU 27 %, LDS 24 %,
+// and the two waves per SIMD spend 35 % of their time at waits and barriers.  The
+// fold takes another 21 us.  FINE: 231 and 24 us.
 //
 // 8-bit blocks: pieces go from memory straight to LDS as they are
 // (global_load_lds, 3 steps ahead of their use, no registers); during step b

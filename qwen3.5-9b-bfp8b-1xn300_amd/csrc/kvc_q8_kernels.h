@@ -189,9 +189,11 @@ __global__ __launch_bounds__(256) void gather_q8_kernel(GatherQ8Args a) {
 // has rows to spare (4 heads of 16 rows), so the digits are free; the block's
 // 16 KiB cost about 220 VALU instructions and 24 MFMAs.
 // Bound by memory from some tens of sequences on: 64 sequences of 512..16384
-// tokens 178 us, 1037 MB at 5.8 TB/s; 8 of 777..6001 20.5 us a layer, 3.5 TB/s
-// (the run-up of 2 workgroups a CU); below that by latency: 1 x 4096 8.8 us, 1 x
-// 300 6.6 us a layer.
+// tokens 179 us, 1037 MB at 5.8 TB/s; 8 of 777..6001 21 us a layer, 3.4 TB/s
+// (the run-up of 2 workgroups a CU); below that by latency: 1 x 4096 9.5 us, 1 x
+// 300 7.5 us a layer (kernel trace; a layer of calls back to back 9.0 and 6.9).
+// The second planes, with fp32 output: 64 sequences 180 us against 179, 1 x 4096
+// as without.
 //
 // digits: bytes 0..3 of dig30(x) are x's signed base-256 digits
 __device__ __forceinline__ uint32_t dig30(int n) { return ((uint32_t)n + 0x00808080u) ^ 0x00808080u; }
