@@ -201,9 +201,10 @@ def _context(**config):
 
 
 class _Device:
-    """Device memory of the library as an array."""
+    """Device memory of a context as an array, which keeps the context."""
 
-    def __init__(self, ptr, n):
+    def __init__(self, ctx, ptr, n):
+        self.ctx = ctx
         self.__cuda_array_interface__ = {"shape": (n,), "typestr": "<f4", "data": (ptr, False), "version": 2}
 
 
@@ -224,7 +225,7 @@ def _state_at(st, seq):
     """The recurrent state of a sequence: where the library has it now."""
     at = st.ctx.state_ptrs(seq, 0)[0]
     if at not in st.views:
-        st.views[at] = torch.as_tensor(_Device(at, STATE), device="cuda")
+        st.views[at] = torch.as_tensor(_Device(st.ctx, at, STATE), device="cuda")
     return st.views[at]
 
 
