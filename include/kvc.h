@@ -35,6 +35,8 @@
  *                               kvc_prefill_attn and kvc_gather then read (new)
  *   kvc_attn_weights, kvc_evict eviction from a sequence's cache by accumulated
  *                               attention weight (new)
+ *   kvc_seq_fork, kvc_seq_reorder   one sequence continued as several; beams that
+ *                               go on from their parents (new)
  *   kvc_snapshot_save/_restore  prefix-boundary copies of that state (new: the
  *                               reference can only extend one live sequence)
  *
@@ -196,6 +198,26 @@ int kvc_seq_reserve(kvc_ctx* ctx, const int32_t* seqs, int32_t n_seqs,
  * its recurrent state and last segment of K/V is taken on `stream`. */
 int kvc_seq_commit(kvc_ctx* ctx, const int32_t* seqs, int32_t n_seqs,
                    int32_t n_tok, const int32_t* tokens, void* stream);
+
+/* ---- forks (no counterpart in the reference) ------------------------------ */
+/* dst[i] (an empty sequence) becomes a copy of src[i], which may be listed more
+ * than once: the same length, tokens and position, the same K/V blocks, shared
+ * (one that is not full is copied by the kvc_seq_reserve that next writes to it),
+ * and a copy of the recurrent and conv state.  8-bit blocks are shared too, and
+ * evicted tokens stay evicted.  A source may be released afterwards.  No source
+ * may be a destination, and none may have tokens pending (KVC_ERR_STATE). */
+int kvc_seq_fork(kvc_ctx* ctx, const int32_t* src, const int32_t* dst, int32_t n,
+                 void* stream);
+/* Beam search's step back to the parents, in place: seqs[i] becomes what
+ * seqs[parent[i]] was before the call, parent[i] in [0, n).  One child of each
+ * parent goes on with the parent's recurrent state where it is; only the others
+ * get copies.  So pointers from kvc_state_ptrs and graphs captured around
+ * kvc_deltanet_step, kvc_snapshot_* or the attention of these sequences are of
+ * use until the next kvc_seq_reorder only.  Nothing may be pending.
+ * Neither call can be captured into a graph (KVC_ERR_STATE); both launch on the
+ * context's device, which must be current (KVC_ERR_INVALID). */
+int kvc_seq_reorder(kvc_ctx* ctx, const int32_t* seqs, const int32_t* parent,
+                    int32_t n, void* stream);
 
 /* ---- prefix cache (host bookkeeping + device restore) ------------------- */
 /* seq must be empty.  Finds the longest verified block-chain prefix of
@@ -400,7 +422,8 @@ int kvc_kv_checksum(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
 
 /* ---- recurrent state + snapshots ---------------------------------------- */
 /* Live state of seq for Gated-DeltaNet layer ssm_layer: rec = fp32
- * [v_heads][v_dim][k_dim], conv = fp32 [conv_rows][conv_channels]. */
+ * [v_heads][v_dim][k_dim], conv = fp32 [conv_rows][conv_channels].  It stays
+ * there until a kvc_seq_reorder of seq. */
 int kvc_state_ptrs(kvc_ctx* ctx, int32_t seq, int32_t ssm_layer, void** rec,
                    void** conv);
 /* Gated-DeltaNet step of n_tok tokens per seq, in place on the state above

@@ -96,6 +96,7 @@ struct Seq {
     bool state_dirty = false;      // recurrent state must be zeroed before its next use
     int32_t n8 = 0;       // leading blocks that are 8-bit ones (full and committed)
     int32_t evicted = 0;  // tokens evicted: the next token's position is len + evicted
+    int32_t state = 0;    // slot of its recurrent state: kvc_seq_reorder moves these between sequences
 };
 
 struct Entry {
@@ -405,7 +406,7 @@ int clean_states(kvc_ctx* c, const int32_t* seqs, size_t n, void* stream) {
         Seq& s = c->seqs[seqs[i]];
         if (!s.state_dirty) continue;
         s.state_dirty = false;
-        z.slot[z.n_slots++] = seqs[i];
+        z.slot[z.n_slots++] = s.state;
         if (z.n_slots == kMaxBatch || i + 1 == n) {
             int e = launch_zero_state(z, stream);
             if (e) return hip_err((hipError_t)e, "state zero-fill launch");
@@ -448,6 +449,7 @@ int launch_snapshots(kvc_ctx* c, const std::vector<int32_t>& seq_slots,
         a.n_pairs = (int32_t)n;
         for (size_t k = 0; k < n; k++) {
             a.seq_slot[k] = seq_slots[i0 + k];
+            a.state_slot[k] = c->seqs[seq_slots[i0 + k]].state;
             a.snap_slot[k] = snap_slots[i0 + k];
             a.first_block[k] = first_blocks[i0 + k];
         }
@@ -791,6 +793,7 @@ int kvc_create(const kvc_config* cfg, kvc_ctx** out) {
     c->free_blocks8.resize(k.q8_blocks);
     for (int32_t i = 0; i < k.q8_blocks; i++) c->free_blocks8[i] = k.q8_blocks - 1 - i;
     c->seqs.resize(k.max_seqs);
+    for (int32_t i = 0; i < k.max_seqs; i++) c->seqs[i].state = i;
     for (int32_t i = k.max_seqs - 1; i >= 0; i--) c->free_seqs.push_back(i);
     c->snaps.resize(n_snap);
     *out = c;
@@ -831,7 +834,9 @@ int kvc_seq_create(kvc_ctx* c, int32_t* seq) {
     if (c->free_seqs.empty()) return set_err(KVC_ERR_NOMEM, "all %d sequence slots in use", c->cfg.max_seqs);
     const int32_t s = c->free_seqs.back();
     c->free_seqs.pop_back();
+    const int32_t state = c->seqs[s].state;
     c->seqs[s] = Seq();
+    c->seqs[s].state = state;
     c->seqs[s].live = true;
     c->seqs[s].state_dirty = c->cfg.n_ssm_layers > 0;  // the slot may hold an earlier sequence's state
     *seq = s;
@@ -1715,9 +1720,22 @@ static MixedPools mixed_pools(kvc_ctx* c) {
     return p;
 }
 
+// For calls that give sequences other blocks: a graph would replay the blocks of
+// the capture, which others hold by then.
+static int check_table_call(kvc_ctx* c, const char* what, void* stream) {
+    if (!c->has_device) return KVC_OK;
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (stream) {  // (the null stream is never captured)
+        hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &capture);
+        if (e != hipSuccess) return hip_err(e, "hipStreamIsCapturing");
+    }
+    if (capture != hipStreamCaptureStatusNone)
+        return set_err(KVC_ERR_STATE, "%s changes block tables and cannot be captured into a graph", what);
+    return check_current(c);
+}
+
 // The sequences that kvc_kv_quantize / kvc_evict read (and change, unless dst
-// names the empty sequences that receive the result).  A graph would replay the
-// blocks of the capture, which others hold by then.
+// names the empty sequences that receive the result).
 static int check_src_dst(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, const char* what,
                          void* stream) {
     int rc;
@@ -1733,15 +1751,7 @@ static int check_src_dst(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, in
     }
     if (dst && c->cfg.n_ssm_layers > 0)
         return set_err(KVC_ERR_UNSUPPORTED, "%s into other sequences does not copy recurrent state", what);
-    if (!c->has_device) return KVC_OK;
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    if (stream) {  // (the null stream is never captured)
-        hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &capture);
-        if (e != hipSuccess) return hip_err(e, "hipStreamIsCapturing");
-    }
-    if (capture != hipStreamCaptureStatusNone)
-        return set_err(KVC_ERR_STATE, "%s changes block tables and cannot be captured into a graph", what);
-    return check_current(c);
+    return check_table_call(c, what, stream);
 }
 
 int kvc_kv_quantize(kvc_ctx* c, const int32_t* seqs, const int32_t* dst, int32_t n_seqs, int32_t keep_tokens,
@@ -2030,6 +2040,153 @@ int kvc_q8_stats(kvc_ctx* c, int64_t* blocks, int64_t* free_blocks) {
     return KVC_OK;
 }
 
+// ---- forks -------------------------------------------------------------------
+
+// What a copy of s holds besides its recurrent state; its blocks are counted for
+// it once the copy is kept (hold_blocks).
+static Seq copy_of(const Seq& s) {
+    Seq d = s;
+    d.pending = 0;
+    return d;
+}
+
+static void hold_blocks(kvc_ctx* c, const Seq& s) {
+    for (int32_t b = 0; b < (int32_t)s.blocks.size(); b++) (b < s.n8 ? c->refcnt8 : c->refcnt)[s.blocks[b]]++;
+    for (int32_t pin : s.pins)
+        if (pin >= 0) c->refcnt[pin]++;
+}
+
+// The table rows of a and the states (src_slot, dst_slot) of pairs, which are
+// sorted; 64 destinations a launch.
+static int launch_forks(kvc_ctx* c, const std::vector<std::pair<int32_t, int32_t>>& pairs, ForkArgs a, void* stream) {
+    a.state = c->d_state;
+    a.state_bytes = c->state_bytes;
+    a.table = c->d_table;
+    a.table_stride = c->max_blocks;
+    size_t i = 0;
+    do {
+        a.n_src = 0;
+        for (int32_t n = 0; n < kMaxBatch && i < pairs.size(); n++, i++) {
+            if (a.n_src == 0 || a.src[a.n_src - 1] != pairs[i].first) a.src[a.n_src++] = pairs[i].first;
+            a.dst[n] = pairs[i].second;
+            if (n == 0) a.dst_begin[0] = 0;
+            a.dst_begin[a.n_src] = n + 1;
+        }
+        int e = launch_fork(a, stream);
+        if (e) return hip_err((hipError_t)e, "fork launch");
+        a.n_rows = 0;
+    } while (i < pairs.size());
+    return KVC_OK;
+}
+
+int kvc_seq_fork(kvc_ctx* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) try {
+    if (!c) return set_err(KVC_ERR_INVALID, "null context");
+    int rc;
+    if (!src) return set_err(KVC_ERR_INVALID, "fork needs sources");
+    if ((rc = check_seqs(c, dst, n))) return rc;
+    std::vector<char> is_dst(c->seqs.size(), 0);
+    for (int32_t i = 0; i < n; i++) is_dst[dst[i]] = 1;
+    for (int32_t i = 0; i < n; i++) {
+        if (!seq_ok(c, src[i])) return set_err(KVC_ERR_INVALID, "sequence %d is not live", src[i]);
+        if (is_dst[src[i]]) return set_err(KVC_ERR_INVALID, "sequence %d is both source and destination", src[i]);
+        const Seq &s = c->seqs[src[i]], &d = c->seqs[dst[i]];
+        if (s.pending) return set_err(KVC_ERR_STATE, "sequence %d has %d uncommitted tokens", src[i], s.pending);
+        if (d.len || d.pending) return set_err(KVC_ERR_STATE, "destination %d is not empty", dst[i]);
+    }
+    if ((rc = check_table_call(c, "kvc_seq_fork", stream))) return rc;
+    // everything that can run out of memory comes before the first change
+    std::vector<Seq> made(n);
+    std::vector<std::pair<int32_t, int32_t>> states, none;
+    for (int32_t i = 0; i < n; i++) {
+        const Seq& s = c->seqs[src[i]];
+        made[i] = copy_of(s);
+        made[i].state = c->seqs[dst[i]].state;
+        if (!s.state_dirty && c->state_bytes > 0) states.push_back({s.state, made[i].state});
+    }
+    std::sort(states.begin(), states.end());
+    for (int32_t i = 0; i < n; i++) {
+        hold_blocks(c, made[i]);
+        c->seqs[dst[i]] = std::move(made[i]);
+    }
+    if (!c->has_device) return KVC_OK;
+    // a launch copies up to 64 table rows; the states go with the last ones
+    for (int32_t i0 = 0; i0 < n; i0 += kMaxBatch) {
+        ForkArgs a{};
+        const bool last = i0 + kMaxBatch >= n;
+        for (int32_t j = 0; j < kMaxBatch && i0 + j < n; j++) {
+            const int32_t len = (int32_t)c->seqs[src[i0 + j]].blocks.size();
+            if (len == 0) continue;
+            a.row_src[a.n_rows] = src[i0 + j];
+            a.row_dst[a.n_rows] = dst[i0 + j];
+            a.row_len[a.n_rows++] = len;
+        }
+        if ((rc = launch_forks(c, last ? states : none, a, stream))) return rc;
+    }
+    return KVC_OK;
+} catch (const std::bad_alloc&) {
+    return set_err(KVC_ERR_NOMEM, "host allocation failed");
+}
+
+int kvc_seq_reorder(kvc_ctx* c, const int32_t* seqs, const int32_t* parent, int32_t n, void* stream) try {
+    if (!c) return set_err(KVC_ERR_INVALID, "null context");
+    int rc;
+    if (!parent) return set_err(KVC_ERR_INVALID, "reorder needs parents");
+    if ((rc = check_seqs(c, seqs, n))) return rc;
+    for (int32_t i = 0; i < n; i++) {
+        if (parent[i] < 0 || parent[i] >= n)
+            return set_err(KVC_ERR_RANGE, "parent %d of sequence %d is outside [0, %d)", parent[i], seqs[i], n);
+        if (c->seqs[seqs[i]].pending)
+            return set_err(KVC_ERR_STATE, "sequence %d has %d uncommitted tokens", seqs[i], c->seqs[seqs[i]].pending);
+    }
+    if ((rc = check_table_call(c, "kvc_seq_reorder", stream))) return rc;
+    // Of a parent's children one goes on with its state slot (itself, or else
+    // the first), the others get copies in the slots of the childless.
+    std::vector<int32_t> heir(n, -1), slot(n, -1), spare;
+    std::vector<std::pair<int32_t, int32_t>> states;
+    for (int32_t i = 0; i < n; i++)
+        if (heir[parent[i]] < 0 || parent[i] == i) heir[parent[i]] = i;
+    for (int32_t p = 0; p < n; p++) {
+        if (heir[p] >= 0)
+            slot[heir[p]] = c->seqs[seqs[p]].state;
+        else
+            spare.push_back(c->seqs[seqs[p]].state);
+    }
+    for (int32_t i = 0; i < n; i++) {
+        if (slot[i] >= 0) continue;
+        const Seq& s = c->seqs[seqs[parent[i]]];
+        slot[i] = spare.back();
+        spare.pop_back();
+        if (!s.state_dirty && c->state_bytes > 0) states.push_back({s.state, slot[i]});
+    }
+    std::sort(states.begin(), states.end());
+    std::vector<Seq> made(n);
+    size_t updates = c->table_updates.size();
+    for (int32_t i = 0; i < n; i++) {
+        if (parent[i] == i) continue;
+        made[i] = copy_of(c->seqs[seqs[parent[i]]]);
+        updates += made[i].blocks.size();
+    }
+    c->table_updates.reserve(updates);
+    for (int32_t i = 0; i < n; i++)
+        if (parent[i] != i) hold_blocks(c, made[i]);
+    for (int32_t i = 0; i < n; i++) {
+        if (parent[i] != i) {
+            const std::vector<int32_t>&was = c->seqs[seqs[i]].blocks, &now = made[i].blocks;
+            for (size_t b = 0; b < now.size(); b++)
+                if (b >= was.size() || was[b] != now[b]) set_table(c, seqs[i], (int32_t)b, now[b]);
+            release_tail(c, seqs[i], 0);
+            drop_entries(c, c->seqs[seqs[i]], 0);
+            c->seqs[seqs[i]] = std::move(made[i]);
+        }
+        c->seqs[seqs[i]].state = slot[i];
+    }
+    if ((rc = flush_table(c, stream))) return rc;
+    if (states.empty() || !c->has_device) return KVC_OK;
+    return launch_forks(c, states, ForkArgs{}, stream);
+} catch (const std::bad_alloc&) {
+    return set_err(KVC_ERR_NOMEM, "host allocation failed");
+}
+
 // ---- state + snapshots -------------------------------------------------------
 
 int kvc_state_ptrs(kvc_ctx* c, int32_t seq, int32_t ssm_layer, void** rec, void** conv) {
@@ -2044,7 +2201,7 @@ int kvc_state_ptrs(kvc_ctx* c, int32_t seq, int32_t ssm_layer, void** rec, void*
         hipError_t e = hipStreamSynchronize(nullptr);
         if (e != hipSuccess) return hip_err(e, "state zero-fill");
     }
-    uint8_t* base = c->d_state + (int64_t)seq * c->state_bytes + (int64_t)ssm_layer * (c->rec_bytes + c->conv_bytes);
+    uint8_t* base = c->d_state + (int64_t)c->seqs[seq].state * c->state_bytes + (int64_t)ssm_layer * (c->rec_bytes + c->conv_bytes);
     if (rec) *rec = base;
     if (conv) *conv = base + c->rec_bytes;
     return KVC_OK;
@@ -2112,7 +2269,7 @@ int kvc_deltanet_step(kvc_ctx* c, int32_t ssm_layer, const int32_t* seqs, int32_
         d.n_seqs = n;
         d.n_tok = n_tok;
         d.ref_math = !(k.flags & KVC_FLAG_EXACT_MATH);
-        for (int32_t j = 0; j < n; j++) d.slot[j] = seqs[i0 + j];
+        for (int32_t j = 0; j < n; j++) d.slot[j] = c->seqs[seqs[i0 + j]].state;
         if (deltanet_few(n, n_tok)) {
             d.ws = c->d_part;
             d.seg_blocks = std::min((n_tok + kSsmChunk - 1) / kSsmChunk, kDnFewMax / (n * kSsmKHeads));

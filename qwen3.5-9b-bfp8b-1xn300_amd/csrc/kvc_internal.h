@@ -517,7 +517,8 @@ struct SnapshotArgs {
     int32_t do_state;        // copy the recurrent state part
     int32_t do_kv;           // copy the K/V segment part
     int32_t pad;
-    int32_t seq_slot[kMaxBatch];
+    int32_t seq_slot[kMaxBatch];     // block-table row
+    int32_t state_slot[kMaxBatch];   // live state
     int32_t snap_slot[kMaxBatch];
     int32_t first_block[kMaxBatch];  // block-table index of the segment start
 };
@@ -532,8 +533,27 @@ struct BlockCopyArgs {
     int32_t dst[kMaxBatch];
 };
 
+// Recurrent state and block tables of forked sequences: source states that go to
+// several places are read once.
+struct ForkArgs {
+    uint8_t* state;
+    int64_t state_bytes;           // per slot (multiple of 256)
+    int32_t* table;
+    int32_t table_stride;
+    int32_t n_rows;                // table rows copied
+    int32_t n_src;                 // states copied, of them each to dst[dst_begin[i] ..]
+    int32_t wgs_per_state;         // set by the launcher
+    int32_t row_src[kMaxBatch];
+    int32_t row_dst[kMaxBatch];
+    int32_t row_len[kMaxBatch];    // entries
+    int32_t src[kMaxBatch];
+    int32_t dst_begin[kMaxBatch + 1];
+    int32_t dst[kMaxBatch];
+};
+
 static_assert(sizeof(DecodeQ8Args) < 4096 && sizeof(QuantizeArgs) < 4096 && sizeof(GatherQ8Args) < 4096 &&
-                  sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillQ8Args) < 4096 && sizeof(PrefillArgs) < 4096,
+                  sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillQ8Args) < 4096 && sizeof(PrefillArgs) < 4096 &&
+                  sizeof(ForkArgs) < 4096,
               "argument blocks are passed by value");
 
 // ---- launchers (kvc_kernels.hip); return hipError_t as int ---------------
@@ -553,6 +573,7 @@ int launch_gather(const GatherArgs& a, void* stream);
 int launch_checksum(const ChecksumArgs& a, void* stream);
 int launch_prefill(const PrefillArgs& a, void* stream);
 int launch_snapshot(const SnapshotArgs& a, void* stream);
+int launch_fork(const ForkArgs& a, void* stream);
 int launch_block_copy(const BlockCopyArgs& a, void* stream);
 int launch_decode_q8(const DecodeQ8Args& a, void* stream);
 int launch_prefill_q8(const PrefillQ8Args& a, void* stream);

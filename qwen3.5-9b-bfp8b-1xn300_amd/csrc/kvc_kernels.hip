@@ -4182,7 +4182,7 @@ __global__ __launch_bounds__(256) void checksum_kernel(ChecksumArgs a) {
 __global__ __launch_bounds__(256) void snapshot_kernel(SnapshotArgs a) {
     const int p = blockIdx.y;
     const int64_t u0 = snap_units_begin(a), u1 = snap_units_end(a);
-    uint8_t* live = a.state_base + (int64_t)a.seq_slot[p] * a.state_bytes;
+    uint8_t* live = a.state_base + (int64_t)a.state_slot[p] * a.state_bytes;
     uint8_t* snap = a.snap_base + (int64_t)a.snap_slot[p] * a.snap_bytes;
     const int32_t* trow = a.table + (size_t)a.seq_slot[p] * a.table_stride + a.first_block[p];
     const int64_t base = u0 + ((int64_t)blockIdx.x * blockDim.x * kSnapUnroll) + threadIdx.x;
@@ -4267,6 +4267,7 @@ __global__ __launch_bounds__(256) void fill_normal_kernel(uint16_t* dst, int64_t
 #include "kvc_q8_kernels.h"
 #include "kvc_prefill_q8_kernels.h"
 #include "kvc_evict_kernels.h"
+#include "kvc_fork_kernels.h"
 
 namespace kvc {
 

@@ -47,7 +47,7 @@ EXPORTS = [
     "kvc_decode_attn_static", "kvc_decode_step", "kvc_prefill_attn", "kvc_prefill_step", "kvc_gather", "kvc_kv_checksum", "kvc_state_ptrs", "kvc_deltanet_step", "kvc_snapshot_save",
     "kvc_snapshot_restore", "kvc_snapshot_release", "kvc_pool_fill_normal",
     "kvc_fill_normal_bf16", "kvc_sync", "kvc_kv_quantize", "kvc_attn_weights", "kvc_evict", "kvc_seq_get_info",
-    "kvc_q8_stats",
+    "kvc_q8_stats", "kvc_seq_fork", "kvc_seq_reorder",
 ]
 
 
@@ -137,6 +137,8 @@ def lib() -> ctypes.CDLL:
             "kvc_attn_weights": (ctypes.c_int, [P, I32, pI32, I32, I32, P, F32, P, P, I64, P]),
             "kvc_evict": (ctypes.c_int, [P, pI32, pI32, I32, I32, I32, I32, P, P, I64, P, P]),
             "kvc_seq_get_info": (ctypes.c_int, [P, I32, ctypes.POINTER(SeqInfo)]),
+            "kvc_seq_fork": (ctypes.c_int, [P, pI32, pI32, I32, P]),
+            "kvc_seq_reorder": (ctypes.c_int, [P, pI32, pI32, I32, P]),
             "kvc_q8_stats": (ctypes.c_int, [P, ctypes.POINTER(I64), ctypes.POINTER(I64)]),
         }
         for name, (res, args) in sig.items():
@@ -365,6 +367,14 @@ class Context:
             t = np.ascontiguousarray(np.asarray(tokens, dtype=np.int32).reshape(len(seqs), n_tok))
             tp = t.ctypes.data_as(ctypes.POINTER(ctypes.c_int32))
         _check(self.L.kvc_seq_commit(self.ptr, _i32(seqs), len(seqs), n_tok, tp, stream))
+
+    def fork(self, src, dst, stream=None):
+        """dst[i] (empty) becomes a copy of src[i]: blocks shared, recurrent state copied"""
+        _check(self.L.kvc_seq_fork(self.ptr, _i32(src), self._pair(src, dst), len(src), stream))
+
+    def reorder(self, seqs, parents, stream=None):
+        """seqs[i] becomes what seqs[parents[i]] was, in place"""
+        _check(self.L.kvc_seq_reorder(self.ptr, _i32(seqs), self._pair(seqs, parents), len(seqs), stream))
 
     def prefix_match(self, s, tokens, stream=None) -> int:
         t = np.ascontiguousarray(np.asarray(tokens, dtype=np.int32))
