@@ -37,6 +37,8 @@
  *                               attention weight (new)
  *   kvc_seq_fork, kvc_seq_reorder   one sequence continued as several; beams that
  *                               go on from their parents (new)
+ *   kvc_decode_attn_shared      kvc_decode_attn that reads blocks which sequences
+ *                               share once (new)
  *   kvc_snapshot_save/_restore  prefix-boundary copies of that state (new: the
  *                               reference can only extend one live sequence)
  *
@@ -277,6 +279,22 @@ int kvc_decode_attn(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * that workspace: calls that overlap on one GPU (other streams, other
  * contexts, other host threads) race and must be serialised by the caller. */
 int kvc_decode_attn_static(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
+                           int32_t n_seqs, const void* q, const void* k_new,
+                           const void* v_new, const void* gate, void* out,
+                           int32_t out_dtype, float scale, void* stream);
+/* No counterpart in the reference.  kvc_decode_attn for sequences that share
+ * blocks (kvc_seq_fork, kvc_prefix_match): same arguments and semantics, any order
+ * of the sequences, any tree of common prefixes, but a full block that several
+ * sequences of up to 64 of a call hold is read once for all of them.  Launches in
+ * which they share little, or some hold 8-bit blocks, run kvc_decode_attn's
+ * kernels.  With bf16 output weights are rounded to bf16 before the product with
+ * the values; with fp32 output they keep 24 bits in either kind of launch (as
+ * several parts, so an infinite value may make the elements that it enters NaN).  Equal
+ * to kvc_decode_attn within those roundings; the order of sums follows from the
+ * tables and lengths of all sequences that share 64 of a call.  Arrays must be
+ * aligned to 16 bytes, and out must not overlap the inputs.  The context's device
+ * must be current.  Uses the context's split-K workspace. */
+int kvc_decode_attn_shared(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
                            int32_t n_seqs, const void* q, const void* k_new,
                            const void* v_new, const void* gate, void* out,
                            int32_t out_dtype, float scale, void* stream);

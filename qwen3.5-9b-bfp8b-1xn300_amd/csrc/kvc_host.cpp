@@ -29,6 +29,7 @@
 #include "kvc_internal.h"
 #include "kvc_prefill_q8_split.h"
 #include "kvc_prefill_split.h"
+#include "kvc_shared_plan.h"
 
 using namespace kvc;
 
@@ -1426,6 +1427,122 @@ int kvc_decode_attn_static(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
 }
 
 // One prefill launch over sequences of which some may hold 8-bit blocks (at most 64).
+// The launches of kvc_decode_attn_shared for seqs[i0, i0 + n): over the trie of
+// their block tables where that saves enough reads (shared_pays), else those of
+// kvc_decode_attn, of them the ones that hold weights in fp32 for fp32 output.
+// With launch = false only what can be refused is checked.
+static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t i0, int32_t n, const void* q,
+                         const void* k_new, const void* v_new, const void* gate, void* out, int32_t out_dtype,
+                         float scale, bool launch, void* stream) {
+    const bool q8 = any_q8(c, seqs + i0, n);
+    SharedPlan p;
+    const int32_t* tab[kMaxBatch];
+    int32_t keys[kMaxBatch];
+    if (!q8) {
+        for (int32_t j = 0; j < n; j++) {
+            const Seq& s = c->seqs[seqs[i0 + j]];
+            tab[j] = s.blocks.data();
+            keys[j] = s.len + s.pending - (k_new ? 1 : 0);
+        }
+        if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, p);
+    }
+    if (!launch || q8 || !shared_pays(p)) {
+        DecodeArgs a;
+        DecodeQ8Args a8;
+        int rc, e = 0;
+        if (q8 || out_dtype == KVC_DTYPE_F32) {
+            if ((rc = build_decode_q8_args(c, layer, seqs, i0, n, q, k_new, v_new, gate, out, out_dtype, scale, a8)))
+                return rc;
+            if (launch) e = launch_decode_q8(a8, stream);
+        } else {
+            if ((rc = build_decode_args(c, layer, seqs, i0, n, q, k_new, v_new, gate, DecodeProducer{}, out, out_dtype,
+                                        scale, c->d_part, (uint32_t)kPartBytes, c->d_counters,
+                                        (int64_t)kMaxChunks * kKvHeads, "context's split-K workspace", a)))
+                return rc;
+            if (launch) e = launch_decode(a, stream);
+        }
+        return e ? hip_err((hipError_t)e, "decode launch") : KVC_OK;
+    }
+    const size_t qoff = (size_t)i0 * kQHeads * kHeadDim, kvoff = (size_t)i0 * kKvHeads * kHeadDim;
+    SharedArgs a;
+    SharedFoldArgs f;
+    memset(&a, 0, sizeof a);
+    memset(&f, 0, sizeof f);
+    a.kpool = reinterpret_cast<const uint16_t*>(c->d_pool + (int64_t)(layer * 2) * c->layer_kv_bytes);
+    a.vpool = reinterpret_cast<const uint16_t*>(c->d_pool + (int64_t)(layer * 2 + 1) * c->layer_kv_bytes);
+    f.kpool = const_cast<uint16_t*>(a.kpool);
+    f.vpool = const_cast<uint16_t*>(a.vpool);
+    a.table = f.table = c->d_table;
+    a.q = f.q = static_cast<const uint16_t*>(q) + qoff;
+    f.k_new = k_new ? static_cast<const uint16_t*>(k_new) + kvoff : nullptr;
+    f.v_new = v_new ? static_cast<const uint16_t*>(v_new) + kvoff : nullptr;
+    f.gate = gate ? static_cast<const uint16_t*>(gate) + qoff : nullptr;
+    f.out = static_cast<uint8_t*>(out) + qoff * (out_dtype == KVC_DTYPE_BF16 ? 2 : 4);
+    a.stats = c->d_part;  // (a row count is a multiple of 16)
+    a.acc = c->d_part + (size_t)p.rows * 2;
+    f.stats = a.stats;
+    f.acc = a.acc;
+    a.scale_log2 = f.scale_log2 = scale * 1.4426950408889634f;
+    f.out_bf16 = out_dtype == KVC_DTYPE_BF16;
+    f.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
+    a.table_stride = f.table_stride = c->max_blocks;
+    a.n_nodes = p.n_nodes;
+    f.n_seqs = n;
+    for (int32_t j = 0; j < n; j++) {
+        a.slot[j] = f.slot[j] = seqs[i0 + j];
+        a.keys[j] = f.keys[j] = keys[j];
+    }
+    memcpy(a.member, p.member, p.n_members);
+    for (int32_t k = 0; k < p.n_nodes; k++) {
+        const int32_t mb = p.member_begin[k], members = p.member_begin[k + 1] - mb;
+        a.item_begin[k] = p.item_begin[k];
+        a.node[k] = {p.row_begin[k], p.first[k], p.len[k], shared_shape(SharedShape{p.chunk[k], p.kind[k], members, mb})};
+        f.row_begin[k] = p.row_begin[k];
+        f.chunks[k] = (uint32_t)((p.len[k] + p.chunk[k] - 1) / p.chunk[k]) | (uint32_t)members << 16;
+        for (int32_t i = mb; i < mb + members; i++) f.path_begin[p.member[i] + 1]++;
+    }
+    a.item_begin[p.n_nodes] = p.n_items;
+    int32_t at[kMaxBatch];
+    for (int32_t j = 0; j < n; j++) {
+        at[j] = f.path_begin[j];
+        f.path_begin[j + 1] += f.path_begin[j];
+    }
+    for (int32_t k = 0; k < p.n_nodes; k++)
+        for (int32_t i = p.member_begin[k]; i < p.member_begin[k + 1]; i++)
+            f.path[at[p.member[i]]++] = (uint16_t)(k | (i - p.member_begin[k]) << 8);
+    int e = launch_shared(a, p.n_items, f, stream);
+    return e ? hip_err((hipError_t)e, "decode launch (shared blocks)") : KVC_OK;
+}
+
+int kvc_decode_attn_shared(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n_seqs, const void* q,
+                           const void* k_new, const void* v_new, const void* gate, void* out, int32_t out_dtype,
+                           float scale, void* stream) {
+    if (!c) return set_err(KVC_ERR_INVALID, "null context");
+    int rc;
+    if ((rc = check_device(c)) || (rc = check_layer(c, layer)) || (rc = check_seqs(c, seqs, n_seqs))) return rc;
+    if (!q || !out) return set_err(KVC_ERR_INVALID, "decode needs q and out");
+    if ((k_new == nullptr) != (v_new == nullptr)) return set_err(KVC_ERR_INVALID, "k_new and v_new go together");
+    if (out_dtype != KVC_DTYPE_F32 && out_dtype != KVC_DTYPE_BF16) return set_err(KVC_ERR_INVALID, "bad out_dtype");
+    if (!std::isfinite(scale)) return set_err(KVC_ERR_INVALID, "scale must be finite");
+    if (((uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)gate | (uintptr_t)out) & 15)
+        return set_err(KVC_ERR_INVALID, "decode over shared blocks needs arrays aligned to 16 bytes");
+    // (out is written while other heads still read the inputs)
+    const size_t qbytes = (size_t)n_seqs * kQHeads * kHeadDim * 2, kvbytes = (size_t)n_seqs * kKvHeads * kHeadDim * 2;
+    const size_t obytes = out_dtype == KVC_DTYPE_BF16 ? qbytes : 2 * qbytes;
+    const auto meets_out = [&](const void* x, size_t nx) {
+        return x && (uintptr_t)x < (uintptr_t)out + obytes && (uintptr_t)out < (uintptr_t)x + nx;
+    };
+    if (meets_out(q, qbytes) || meets_out(gate, qbytes) || meets_out(k_new, kvbytes) || meets_out(v_new, kvbytes))
+        return set_err(KVC_ERR_INVALID, "out overlaps an input");
+    if ((rc = check_current(c))) return rc;
+    for (int pass = 0; pass < 2; pass++)
+        for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch)
+            if ((rc = shared_launch(c, layer, seqs, i0, std::min(kMaxBatch, n_seqs - i0), q, k_new, v_new, gate, out,
+                                    out_dtype, scale, pass == 1, stream)))
+                return rc;
+    return KVC_OK;
+}
+
 static int prefill_q8_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n, int32_t n_q, const void* q,
                              const void* gate, void* out, int32_t out_dtype, float scale, void* stream) {
     PrefillQ8Args a{};

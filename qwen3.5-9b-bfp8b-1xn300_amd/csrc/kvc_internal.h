@@ -533,6 +533,84 @@ struct BlockCopyArgs {
     int32_t dst[kMaxBatch];
 };
 
+// ---- decode over shared blocks (kvc_shared_plan.h) ------------------------
+// A node's key chunk and one kv head are a workgroup's work, for up to
+// kSharedSeqs members; each leaves a partial per (member, q head): the
+// unnormalised output [256] and (max, sum), in the workspace.
+constexpr int kSharedNodes = 128;
+constexpr int kSharedMembers = 512;
+constexpr int kSharedSeqs = 16;
+constexpr int kSharedMaxChunk = 64;  // blocks whose ids a wave holds
+constexpr int kSharedShort = 8;      // blocks of a node whose workgroup takes all kv heads
+constexpr int kSharedPath = 512;     // partials of one (sequence, q head)
+// who does what in a workgroup of 4 waves
+enum { kSharedRows = 0,   // more than 4 members: a wave takes one q head, 16 members; K and V tiles for all waves
+       kSharedKeys = 1,   // up to 4 members (x 4 q heads = 16 rows): a wave takes every 4th block
+       kSharedHeads = 2 };  // as kSharedKeys, but few blocks: a wave takes one kv head
+constexpr int kSharedMaxRows = (int)(kPartBytes / ((kHeadDim + 2) * 4));
+
+// Records of whole words: a scalar load drops the low two bits of each part of
+// its address, and beside an array of bytes with the same index the compiler has
+// split the address of a word into such parts.
+struct SharedNode {
+    int32_t row_begin;      // first partial row
+    int32_t first;          // block in the members' tables
+    int32_t len;            // blocks
+    uint32_t shape;         // see shared_shape
+};
+struct SharedShape {
+    int chunk, kind, members, member_begin;
+};
+constexpr uint32_t shared_shape(SharedShape s) {
+    return (uint32_t)s.chunk | (uint32_t)s.kind << 10 | (uint32_t)s.members << 12 | (uint32_t)s.member_begin << 20;
+}
+constexpr SharedShape shared_shape(uint32_t w) {
+    return {(int)(w & 1023), (int)(w >> 10 & 3), (int)(w >> 12 & 255), (int)(w >> 20)};
+}
+
+struct SharedArgs {
+    const uint16_t* kpool;
+    const uint16_t* vpool;
+    const int32_t* table;
+    const uint16_t* q;      // [n_seqs][Hq][D]
+    float* acc;             // [row][256]
+    float* stats;           // [row][max, sum]
+    float scale_log2;
+    int32_t table_stride;
+    int32_t n_nodes;
+    int32_t pad;
+    int32_t slot[kMaxBatch];
+    int32_t keys[kMaxBatch];          // attended in the cache (a new token's key is not among them)
+    int32_t item_begin[kSharedNodes + 1];
+    SharedNode node[kSharedNodes];
+    uint8_t member[kSharedMembers];
+};
+
+// Folds the partials; the new token (k_new) is one more and is appended.
+struct SharedFoldArgs {
+    uint16_t* kpool;
+    uint16_t* vpool;
+    const int32_t* table;
+    const uint16_t* q;
+    const uint16_t* k_new;  // [n_seqs][Hkv][D] or null
+    const uint16_t* v_new;
+    const uint16_t* gate;   // [n_seqs][Hq][D] or null
+    void* out;
+    const float* acc;
+    const float* stats;
+    float scale_log2;
+    int32_t out_bf16;
+    int32_t gate_ref;
+    int32_t table_stride;
+    int32_t n_seqs;
+    int32_t slot[kMaxBatch];
+    int32_t keys[kMaxBatch];
+    int32_t path_begin[kMaxBatch + 1];  // nodes of each sequence
+    int32_t row_begin[kSharedNodes];
+    uint32_t chunks[kSharedNodes];      // chunks | members << 16
+    uint16_t path[kSharedMembers];      // node | place among its members << 8
+};
+
 // Recurrent state and block tables of forked sequences: source states that go to
 // several places are read once.
 struct ForkArgs {
@@ -553,7 +631,7 @@ struct ForkArgs {
 
 static_assert(sizeof(DecodeQ8Args) < 4096 && sizeof(QuantizeArgs) < 4096 && sizeof(GatherQ8Args) < 4096 &&
                   sizeof(WeightsArgs) < 4096 && sizeof(EvictCopyArgs) < 4096 && sizeof(PrefillQ8Args) < 4096 && sizeof(PrefillArgs) < 4096 &&
-                  sizeof(ForkArgs) < 4096,
+                  sizeof(ForkArgs) < 4096 && sizeof(SharedArgs) < 4096 && sizeof(SharedFoldArgs) < 4096,
               "argument blocks are passed by value");
 
 // ---- launchers (kvc_kernels.hip); return hipError_t as int ---------------
@@ -572,6 +650,7 @@ int launch_zero_state(const ZeroStateArgs& a, void* stream);
 int launch_gather(const GatherArgs& a, void* stream);
 int launch_checksum(const ChecksumArgs& a, void* stream);
 int launch_prefill(const PrefillArgs& a, void* stream);
+int launch_shared(const SharedArgs& a, int32_t n_items, const SharedFoldArgs& f, void* stream);
 int launch_snapshot(const SnapshotArgs& a, void* stream);
 int launch_fork(const ForkArgs& a, void* stream);
 int launch_block_copy(const BlockCopyArgs& a, void* stream);

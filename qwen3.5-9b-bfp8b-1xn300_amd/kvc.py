@@ -47,7 +47,7 @@ EXPORTS = [
     "kvc_decode_attn_static", "kvc_decode_step", "kvc_prefill_attn", "kvc_prefill_step", "kvc_gather", "kvc_kv_checksum", "kvc_state_ptrs", "kvc_deltanet_step", "kvc_snapshot_save",
     "kvc_snapshot_restore", "kvc_snapshot_release", "kvc_pool_fill_normal",
     "kvc_fill_normal_bf16", "kvc_sync", "kvc_kv_quantize", "kvc_attn_weights", "kvc_evict", "kvc_seq_get_info",
-    "kvc_q8_stats", "kvc_seq_fork", "kvc_seq_reorder",
+    "kvc_q8_stats", "kvc_seq_fork", "kvc_seq_reorder", "kvc_decode_attn_shared",
 ]
 
 
@@ -120,6 +120,7 @@ def lib() -> ctypes.CDLL:
             "kvc_qkv_append": (ctypes.c_int, [P, I32, pI32, I32, I32, P, I32, P, P, P, P, P]),
             "kvc_decode_attn": (ctypes.c_int, [P, I32, pI32, I32, P, P, P, P, P, I32, F32, P]),
             "kvc_decode_attn_static": (ctypes.c_int, [P, I32, pI32, I32, P, P, P, P, P, I32, F32, P]),
+            "kvc_decode_attn_shared": (ctypes.c_int, [P, I32, pI32, I32, P, P, P, P, P, I32, F32, P]),
             "kvc_decode_step": (ctypes.c_int, [P, I32, pI32, I32, P, I32, P, P, P, I32, F32, P]),
             "kvc_kv_checksum": (ctypes.c_int, [P, I32, pI32, I32, P, P]),
             "kvc_prefill_attn": (ctypes.c_int, [P, I32, pI32, I32, I32, P, P, P, I32, F32, P]),
@@ -409,6 +410,13 @@ class Context:
                            out_dtype=DTYPE_F32, scale=1.0 / 16, stream=None):
         """decode_attn on the library's static per-GPU workspace (allocates nothing)"""
         _check(self.L.kvc_decode_attn_static(self.ptr, layer, _i32(seqs), len(seqs), self._p(q), self._p(k_new),
+                                             self._p(v_new), self._p(gate), self._p(out), out_dtype,
+                                             ctypes.c_float(scale), stream))
+
+    def decode_attn_shared(self, layer, seqs, q, out, k_new=None, v_new=None, gate=None,
+                           out_dtype=DTYPE_F32, scale=1.0 / 16, stream=None):
+        """decode_attn that reads the blocks which sequences share once"""
+        _check(self.L.kvc_decode_attn_shared(self.ptr, layer, _i32(seqs), len(seqs), self._p(q), self._p(k_new),
                                              self._p(v_new), self._p(gate), self._p(out), out_dtype,
                                              ctypes.c_float(scale), stream))
 
