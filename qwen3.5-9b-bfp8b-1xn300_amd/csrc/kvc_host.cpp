@@ -1435,6 +1435,7 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
                          const void* k_new, const void* v_new, const void* gate, void* out, int32_t out_dtype,
                          float scale, bool launch, void* stream) {
     const bool q8 = any_q8(c, seqs + i0, n);
+    const int32_t group = shared_group(out_dtype == KVC_DTYPE_F32);
     SharedPlan p;
     const int32_t* tab[kMaxBatch];
     int32_t keys[kMaxBatch];
@@ -1444,7 +1445,7 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
             tab[j] = s.blocks.data();
             keys[j] = s.len + s.pending - (k_new ? 1 : 0);
         }
-        if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, p);
+        if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, group, p);
     }
     if (!launch || q8 || !shared_pays(p)) {
         DecodeArgs a;
@@ -1478,38 +1479,29 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
     f.v_new = v_new ? static_cast<const uint16_t*>(v_new) + kvoff : nullptr;
     f.gate = gate ? static_cast<const uint16_t*>(gate) + qoff : nullptr;
     f.out = static_cast<uint8_t*>(out) + qoff * (out_dtype == KVC_DTYPE_BF16 ? 2 : 4);
-    a.stats = c->d_part;  // (a row count is a multiple of 16)
-    a.acc = c->d_part + (size_t)p.rows * 2;
+    a.stats = c->d_part;  // [row][2], 16 rows a partial
+    a.acc = c->d_part + (size_t)p.parts * kQHeads * 2;
     f.stats = a.stats;
     f.acc = a.acc;
     a.scale_log2 = f.scale_log2 = scale * 1.4426950408889634f;
     f.out_bf16 = out_dtype == KVC_DTYPE_BF16;
     f.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
     a.table_stride = f.table_stride = c->max_blocks;
-    a.n_nodes = p.n_nodes;
     f.n_seqs = n;
+    a.group = group;
     for (int32_t j = 0; j < n; j++) {
-        a.slot[j] = f.slot[j] = seqs[i0 + j];
-        a.keys[j] = f.keys[j] = keys[j];
+        a.seq_row[j] = p.seq_row[j];
+        f.seq[j] = {p.seq_row[j], p.seq_parts[j], seqs[i0 + j], keys[j]};
     }
-    memcpy(a.member, p.member, p.n_members);
+    for (int32_t k = 0; k < kSharedNodes; k++) a.item_end[k] = k < p.n_nodes ? p.item_begin[k + 1] : INT32_MAX;
     for (int32_t k = 0; k < p.n_nodes; k++) {
-        const int32_t mb = p.member_begin[k], members = p.member_begin[k + 1] - mb;
-        a.item_begin[k] = p.item_begin[k];
-        a.node[k] = {p.row_begin[k], p.first[k], p.len[k], shared_shape(SharedShape{p.chunk[k], p.kind[k], members, mb})};
-        f.row_begin[k] = p.row_begin[k];
-        f.chunks[k] = (uint32_t)((p.len[k] + p.chunk[k] - 1) / p.chunk[k]) | (uint32_t)members << 16;
-        for (int32_t i = mb; i < mb + members; i++) f.path_begin[p.member[i] + 1]++;
+        const int32_t mb = p.member_begin[k], members = p.member_begin[k + 1] - mb, s = p.member[mb];
+        // (a node of several members has full blocks only)
+        const int32_t last = std::min(keys[s] - (p.first[k] + p.len[k] - 1) * kBlockTok, kBlockTok);
+        a.node[k] = {p.first[k], (uint32_t)p.len[k] | (uint32_t)last << 26,
+                     shared_shape(SharedShape{p.chunk[k], p.kind[k], members, mb}), seqs[i0 + s]};
     }
-    a.item_begin[p.n_nodes] = p.n_items;
-    int32_t at[kMaxBatch];
-    for (int32_t j = 0; j < n; j++) {
-        at[j] = f.path_begin[j];
-        f.path_begin[j + 1] += f.path_begin[j];
-    }
-    for (int32_t k = 0; k < p.n_nodes; k++)
-        for (int32_t i = p.member_begin[k]; i < p.member_begin[k + 1]; i++)
-            f.path[at[p.member[i]]++] = (uint16_t)(k | (i - p.member_begin[k]) << 8);
+    for (int32_t i = 0; i < p.n_members; i++) a.member[i] = (uint16_t)(p.member[i] | p.part[i] << 6);
     int e = launch_shared(a, p.n_items, f, stream);
     return e ? hip_err((hipError_t)e, "decode launch (shared blocks)") : KVC_OK;
 }

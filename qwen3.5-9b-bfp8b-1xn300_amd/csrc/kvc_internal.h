@@ -534,29 +534,31 @@ struct BlockCopyArgs {
 };
 
 // ---- decode over shared blocks (kvc_shared_plan.h) ------------------------
-// A node's key chunk and one kv head are a workgroup's work, for up to
-// kSharedSeqs members; each leaves a partial per (member, q head): the
-// unnormalised output [256] and (max, sum), in the workspace.
+// A node's key chunk is a workgroup's work, for up to shared_group members and one
+// kv head (or all of them).  It leaves a partial per (member, q head): the
+// unnormalised output [256] and (max, sum), in the workspace, where a sequence's
+// partials stand in a row: partial p of sequence s and q head h is row
+// (seq_row[s] + p) * 16 + h.
 constexpr int kSharedNodes = 128;
 constexpr int kSharedMembers = 512;
-constexpr int kSharedSeqs = 16;
-constexpr int kSharedMaxChunk = 64;  // blocks whose ids a wave holds
-constexpr int kSharedShort = 8;      // blocks of a node whose workgroup takes all kv heads
-constexpr int kSharedPath = 512;     // partials of one (sequence, q head)
-// who does what in a workgroup of 4 waves
-enum { kSharedRows = 0,   // more than 4 members: a wave takes one q head, 16 members; K and V tiles for all waves
-       kSharedKeys = 1,   // up to 4 members (x 4 q heads = 16 rows): a wave takes every 4th block
-       kSharedHeads = 2 };  // as kSharedKeys, but few blocks: a wave takes one kv head
-constexpr int kSharedMaxRows = (int)(kPartBytes / ((kHeadDim + 2) * 4));
+// 4 members are a tile of 16 rows: two tiles fill a wave's registers with weights in
+// one bf16 part, one with weights in three
+constexpr int shared_group(bool f32) { return f32 ? 4 : 8; }
+constexpr int kSharedWaveBlocks = 64;  // blocks whose ids a wave holds
+constexpr int kSharedPath = 512;       // partials of one (sequence, q head)
+// how the 4 waves of a workgroup split it
+enum { kSharedKeys = 0,    // one kv head: a wave takes every 4th block
+       kSharedHeads = 1 }; // all kv heads: a wave takes one
+constexpr int kSharedMaxParts = (int)(kPartBytes / ((kHeadDim + 2) * 4 * kQHeads));  // over all sequences
 
 // Records of whole words: a scalar load drops the low two bits of each part of
 // its address, and beside an array of bytes with the same index the compiler has
 // split the address of a word into such parts.
 struct SharedNode {
-    int32_t row_begin;      // first partial row
     int32_t first;          // block in the members' tables
-    int32_t len;            // blocks
+    uint32_t len;           // blocks | keys in the last one << 26
     uint32_t shape;         // see shared_shape
+    int32_t slot;           // table row of a member
 };
 struct SharedShape {
     int chunk, kind, members, member_begin;
@@ -577,16 +579,21 @@ struct SharedArgs {
     float* stats;           // [row][max, sum]
     float scale_log2;
     int32_t table_stride;
-    int32_t n_nodes;
+    int32_t group;                    // members of a workgroup
     int32_t pad;
-    int32_t slot[kMaxBatch];
-    int32_t keys[kMaxBatch];          // attended in the cache (a new token's key is not among them)
-    int32_t item_begin[kSharedNodes + 1];
+    int32_t item_end[kSharedNodes];   // INT32_MAX behind the last node
     SharedNode node[kSharedNodes];
-    uint8_t member[kSharedMembers];
+    int32_t seq_row[kMaxBatch];
+    uint16_t member[kSharedMembers];  // sequence | its first partial of the node << 6
 };
 
 // Folds the partials; the new token (k_new) is one more and is appended.
+struct SharedSeq {
+    int32_t row;    // seq_row
+    int32_t parts;
+    int32_t slot;
+    int32_t keys;   // attended in the cache: where the new token goes
+};
 struct SharedFoldArgs {
     uint16_t* kpool;
     uint16_t* vpool;
@@ -603,12 +610,8 @@ struct SharedFoldArgs {
     int32_t gate_ref;
     int32_t table_stride;
     int32_t n_seqs;
-    int32_t slot[kMaxBatch];
-    int32_t keys[kMaxBatch];
-    int32_t path_begin[kMaxBatch + 1];  // nodes of each sequence
-    int32_t row_begin[kSharedNodes];
-    uint32_t chunks[kSharedNodes];      // chunks | members << 16
-    uint16_t path[kSharedMembers];      // node | place among its members << 8
+    int32_t pad;
+    SharedSeq seq[kMaxBatch];
 };
 
 // Recurrent state and block tables of forked sequences: source states that go to

@@ -2,25 +2,27 @@
 // shared block read once (included by kvc_kernels.hip).
 //
 // For every trie node (kvc_shared_plan.h) and kv head, the members' query rows
-// (4 q heads each) attend to the node's keys in one product:
+// (4 q heads each, 4 members to a tile of 16 rows) attend to the node's keys in
+// one product per tile:
 //   S^T[32 keys x 16 rows]  = K[keys x 256] . Q^T        (v_mfma_f32_16x16x32_bf16)
 //   P^T = 2^(S^T - m), m the running maximum of the row
 //   O^T[256 x 16 rows]     += V^T[256 x keys] . P^T
 // in the operand layouts of the prefill kernel: a lane stays on one row in both
 // products, P^T leaves the accumulator in operand order, and V^T fragments come
-// from LDS through the transposing read.  A second launch folds the partials
-// (m, l, O) of a row: O = sum 2^(m_p - M) O_p, l likewise, and divides.
+// from LDS through the transposing read.  Every wave streams blocks of its own
+// through LDS units of its own, without barriers, for all tiles of its members, so
+// a K or V fragment is read from LDS once for up to 32 rows.  A second launch folds
+// the partials (m, l, O) of a row: O = sum 2^(m_p - M) O_p, l likewise, and divides.
 #pragma once
 
 namespace kvc {
 
 struct SharedSmem {
-    // kSharedRows: 4 stages of (K, V) units; otherwise (K, V) of each wave.
-    // Rows of 512 B, 16-B chunks swizzled by the row (kswz, vswz).
-    uint16_t unit[8][kBlockTok * kHeadDim];
+    // (K, V) units of each wave: rows of 512 B, 16-B chunks swizzled by the row (kswz, vswz)
+    uint16_t unit[2 * kWaves][kBlockTok * kHeadDim];
     float2 ml[kWaves][16];
 };
-constexpr int kSharedStages = 4;
+constexpr int kShAhead = 3;  // operand fragments read ahead of their MFMAs (4 spill at two tiles)
 constexpr uint32_t kUnitLds = kBlockTok * kHeadDim * 2;
 constexpr int kSharedRowPad = kHeadDim + 4;  // floats between rows of a wave's O in LDS
 static_assert(16 * kSharedRowPad * 4 <= 2 * kUnitLds, "a wave's O fits its two units");
@@ -31,280 +33,318 @@ __device__ __forceinline__ void wait_vm() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// PARTS: bf16 parts of a weight (1 for bf16 output, 3 = 24 bits for fp32 output)
-template <int PARTS>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(SharedArgs a) {
-    __shared__ SharedSmem sm;
+// One workgroup's chunk: blocks [b0, b0 + n_blk) of the node for members
+// [m0, m0 + members) of it (T tiles).
+struct SharedItem {
+    int kind, h, ck, n_blk, mb, members;
+    const int32_t* trow;  // of the chunk's first block
+    int last;             // keys of the chunk's last block
+};
+
+// T: 16-row tiles; PARTS: bf16 parts of a weight (1 for bf16 output, 3 = 24 bits for fp32 output)
+template <int T, int PARTS>
+__device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedItem& it, SharedSmem& sm) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q4 = lane >> 4, r16 = lane & 15;
-    const int item = blockIdx.x;
-    int node;
-    {
-        const int e0 = lane < a.n_nodes ? a.item_begin[lane + 1] : INT32_MAX;
-        const int e1 = lane + 64 < a.n_nodes ? a.item_begin[lane + 65] : INT32_MAX;
-        node = __popcll(__builtin_amdgcn_ballot_w64(e0 <= item)) + __popcll(__builtin_amdgcn_ballot_w64(e1 <= item));
-        node = __builtin_amdgcn_readfirstlane(node);
-    }
-    if (node >= a.n_nodes) return;
-    const SharedNode nd = a.node[node];
-    const SharedShape sh = shared_shape(nd.shape);
-    const int kind = sh.kind, chunk = sh.chunk, mb = sh.member_begin, members = sh.members;
-    const int n_chunks = (nd.len + chunk - 1) / chunk;
-    const int j = item - a.item_begin[node];
-    int unit = j, grp = 0;
-    if (members > kSharedSeqs) {
-        // the groups of 16 members that read the same keys run on one XCD (b % 8), one after the other
-        const int groups = (members + kSharedSeqs - 1) / kSharedSeqs;
-        grp = (j >> 3) % groups;
-        unit = (j >> 3) / groups * 8 + (j & 7);
-        if (unit >= n_chunks * kKvHeads) return;
-    }
-    if (kind == kSharedHeads ? unit >= n_chunks : unit >= n_chunks * kKvHeads) return;  // (padding items)
-    const int h = kind == kSharedHeads ? wave : unit % kKvHeads;
-    const int ck = kind == kSharedHeads ? unit : unit / kKvHeads;
-    const int b0 = ck * chunk, n_blk = min(chunk, nd.len - b0);
-    const int s0 = __builtin_amdgcn_readfirstlane(a.member[mb]);
-    const int32_t* trow = a.table + (size_t)a.slot[s0] * a.table_stride + nd.first + b0;
-
+    const int step = it.kind == kSharedKeys ? kWaves : 1, base = it.kind == kSharedKeys ? wave : 0;
+    const int h = it.h;
     // block ids: lane i holds this wave's i-th block
-    const int step = kind == kSharedKeys ? kWaves : 1, base = kind == kSharedKeys ? wave : 0;
-    const int n_my = (n_blk - base + step - 1) / step;
-    const int idv = lane < n_my ? trow[base + lane * step] : 0;
+    const int n_my = it.kind == kSharedKeys ? (it.n_blk - wave + kWaves - 1) / kWaves : it.n_blk;
+    const int idv = lane < n_my ? it.trow[base + lane * step] : 0;
 
-    // this lane's row: member and q head
-    const bool rows_kind = kind == kSharedRows;
-    const int jm = rows_kind ? kSharedSeqs * grp + r16 : r16 >> 2;
-    const int g = rows_kind ? wave : r16 & 3;
-    const bool real = jm < members;
+    // this lane's rows: member 4 t + r16 / 4, q head r16 % 4
+    const int g = r16 & 3;
     const float c = fabsf(a.scale_log2);
     const uint32_t qflip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-    bf16x8_t qb[8];
-    {
-        const int s = a.member[mb + min(jm, members - 1)];
-        const uint16_t* qr = a.q + ((size_t)s * kQHeads + h * kGroup + g) * kHeadDim;
-        u32x4 x[8];
+    int mem[T];
 #pragma unroll
-        for (int ks = 0; ks < 8; ks++) x[ks] = *reinterpret_cast<const u32x4*>(qr + 32 * ks + 8 * q4);
+    for (int t = 0; t < T; t++) mem[t] = a.member[it.mb + min(4 * t + (r16 >> 2), it.members - 1)];
+    bf16x8_t qb[T][8];
+    {
+        u32x4 x[T][8];
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const uint16_t* qr = a.q + ((size_t)(mem[t] & 63) * kQHeads + h * kGroup + g) * kHeadDim;
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++) x[t][ks] = *reinterpret_cast<const u32x4*>(qr + 32 * ks + 8 * q4);
+        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int ks = 0; ks < 8; ks++) {
+        for (int t = 0; t < T; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[ks][i] ^= qflip;
-            // (waited for here, before the copies are issued: a later wait would cover those too)
-            asm volatile("" : "+v"(x[ks]));
-            qb[ks] = as_bf16x8(x[ks]);
-        }
+            for (int ks = 0; ks < 8; ks++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[t][ks][i] ^= qflip;
+                // (waited for here, before the copies are issued: a later wait would cover those too)
+                asm volatile("" : "+v"(x[t][ks]));
+                qb[t][ks] = as_bf16x8(x[t][ks]);
+            }
     }
-    // keys of the chunk that exist (a node of one member may end inside a block)
-    const int limit = members == 1 ? a.keys[s0] - (nd.first + b0) * kBlockTok : INT32_MAX;
 
-    // copy instruction p of a unit: rows 2p, 2p + 1; lane l fills position l % 32
+    // copy p of a unit: rows 2p, 2p + 1; lane l fills position l % 32
     const uint32_t cbk = (((lane & 31) ^ (lane >> 5)) << 4) + (lane >> 5) * 512;
     const uint32_t cbv = (((lane & 31) ^ ((lane >> 5) << 1)) << 4) + (lane >> 5) * 512;
-    auto copy = [&](const uint16_t* pool, uint32_t cb, int jsh, int id, uint32_t lds, auto p0, auto np) {
+    auto issue = [&](const uint16_t* pool, uint32_t cb, int jsh, int i, uint32_t lds) {
+        const int id = __builtin_amdgcn_readlane(idv, i);
         const uint16_t* src = pool + ((size_t)id * kKvHeads + h) * (kBlockTok * kHeadDim);
 #pragma unroll
-        for (int p = 0; p < decltype(np)::value; p++) {
-            const int pp = p0 + p;
-            lds_dma16s(src + pp * 2 * kHeadDim, cb ^ ((uint32_t)(pp & 7) << jsh), lds + pp * 1024);
-        }
+        for (int p = 0; p < 16; p++) lds_dma16s(src + p * 2 * kHeadDim, cb ^ ((uint32_t)(p & 7) << jsh), lds + p * 1024);
     };
-    const uint32_t lds0 = lds_addr(&sm.unit[0][0]);
-
-    f32x4 o[16], ol = {0.f, 0.f, 0.f, 0.f};  // ol: the row's sum of weights (PARTS 3: ol[0] is the lane's part)
-    float m_run = kNegBig;
-#pragma unroll
-    for (int dt = 0; dt < 16; dt++) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const bf16x8_t ones = as_bf16x8(u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-
-    // operand fragments within a unit: K (kt, ks = 4 hi + jj): ka[jj] + 256 hi + 8192 kt;
-    // V^T (dt, lo/hi): va[dt] + 8192 (hi)
-    uint32_t ka[4], va[16];
-#pragma unroll
-    for (int jj = 0; jj < 4; jj++) ka[jj] = r16 * 512 + 16 * ((4 * jj + q4) ^ r16);
-    {
-        const int w = 4 * q4 + (r16 >> 2);
-#pragma unroll
-        for (int dt = 0; dt < 16; dt++) va[dt] = w * 512 + 16 * (2 * (dt ^ w) + ((r16 & 3) >> 1)) + 8 * (r16 & 1);
+    const uint32_t ku = lds_addr(&sm.unit[2 * wave][0]), vu = ku + kUnitLds;
+    if (n_my > 0) {
+        issue(a.kpool, cbk, 5, 0, ku);
+        issue(a.vpool, cbv, 6, 0, vu);
     }
 
-    f32x4 st[2];
-    auto scores = [&](uint32_t ku) {
-        bf16x8_t kf[kPfAhead];
-        auto read = [&](int i) {
-            const int ks = i >> 1, kt = i & 1;
-            kf[i % kPfAhead] = as_bf16x8(lds_load16(ku + ka[ks & 3], 256 * (ks >> 2) + 8192 * kt));
-        };
+    f32x4 o[T][16];
+    float m_run[T], l[T];  // l: the lane's part of the row's sum of weights
 #pragma unroll
-        for (int i = 0; i < kPfAhead; i++) read(i);
+    for (int t = 0; t < T; t++) {
+        m_run[t] = kNegBig;
+        l[t] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int ks = i >> 1, kt = i & 1;
-            const bf16x8_t x = kf[i % kPfAhead];
-            if (i + kPfAhead < 16) read(i + kPfAhead);
-            st[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qb[ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : st[kt], 0, 0, 0);
+        for (int dt = 0; dt < 16; dt++) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // operand fragments within a unit: K (kt, ks = 4 hi + jj): ka[jj] + 256 hi + 8192 kt;
+    // V^T (dt, lo/hi): va[dt % 4] + vb[dt / 4] + 8192 (hi)
+    uint32_t ka[4], va[4], vb[4];
+#pragma unroll
+    for (int jj = 0; jj < 4; jj++) ka[jj] = ku + r16 * 512 + 16 * ((4 * jj + q4) ^ r16);
+    {
+        const int w = 4 * q4 + (r16 >> 2);  // V row % 16 of this lane; its swizzle takes chunk pair dt to dt ^ w
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            va[j] = vu + w * 512 + 32 * (j ^ (w & 3)) + 16 * ((r16 & 3) >> 1) + 8 * (r16 & 1);
+            vb[j] = 128 * (j ^ (w >> 2));
         }
-    };
-    bf16x8_t pw[PARTS];
-    // weights of a block's scores; its keys from `valid` on do not exist
-    auto weights = [&](int valid) {
-        const bool all = valid >= kBlockTok;
+    }
+
+    for (int i = 0; i < n_my; i++) {
+        const bool more = i + 1 < n_my;
+        // keys of the block that exist (a node of one member may end inside a block)
+        const int valid = base + i * step == it.n_blk - 1 ? it.last : kBlockTok;
+        wait_vm<16>();  // K: the 16 copies after it are V's
+        f32x4 st[T][2];
+        {
+            bf16x8_t kf[kShAhead];
+            auto read = [&](int n) {
+                const int ks = n >> 1, kt = n & 1;
+                kf[n % kShAhead] = as_bf16x8(lds_load16(ka[ks & 3], 256 * (ks >> 2) + 8192 * kt));
+            };
+#pragma unroll
+            for (int n = 0; n < kShAhead; n++) read(n);
+#pragma unroll
+            for (int n = 0; n < 16; n++) {
+                const int ks = n >> 1, kt = n & 1;
+                const bf16x8_t x = kf[n % kShAhead];
+                if (n + kShAhead < 16) read(n + kShAhead);
+#pragma unroll
+                for (int t = 0; t < T; t++)
+                    st[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qb[t][ks],
+                                                                       ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : st[t][kt], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_group_barrier(kSgDsRead, kShAhead, 0);
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+            if (n + kShAhead < 16) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSgMfma, T, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lds();
+        if (more) issue(a.kpool, cbk, 5, i + 1, ku);
+        // weights of the scores
         float cs = c;
-        if (!all) {
+        if (valid < kBlockTok) {  // (one member, one tile)
             asm volatile("");
             cs = 1.f;
 #pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) st[t][kt][e] = 16 * kt + 4 * q4 + e < valid ? st[t][kt][e] * c : kNegBig;
+        }
+        bf16x8_t pw[T][PARTS];
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            float mx = kNegBig;
+#pragma unroll
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) st[kt][i] = 16 * kt + 4 * q4 + i < valid ? st[kt][i] * c : kNegBig;
-        }
-        float mx = kNegBig;
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, st[t][kt][e]);
+            const float mt = max_xor32(max_xor16(mx)) * cs;
+            const bool up = mt > m_run[t] + kRescaleSlack;
+            if (__builtin_amdgcn_ballot_w64(up) != 0) {  // uniform; rows that keep their maximum scale by 1
+                const float cr = up ? fast_exp2(m_run[t] - mt) : 1.f;
+                m_run[t] = up ? mt : m_run[t];
+                // (the scaled values re-enter the accumulators through an MFMA with
+                // zero operands, which keeps them in the MFMA register class)
+                const bf16x8_t z8 = {};
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++)
+                for (int dt = 0; dt < 16; dt++)
+                    o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(z8, z8, o[t][dt] * cr, 0, 0, 0);
+                l[t] *= cr;
+            }
+            const float nm = -m_run[t];
+            u32x4 w[PARTS];
 #pragma unroll
-            for (int i = 0; i < 4; i++) mx = fmaxf(mx, st[kt][i]);
-        mx = max_xor32(max_xor16(mx));
-        const float mt = mx * cs;
-        const bool up = mt > m_run + kRescaleSlack;
-        if (__builtin_amdgcn_ballot_w64(up) != 0) {  // uniform; rows that keep their maximum scale by 1
-            const float cr = up ? fast_exp2(m_run - mt) : 1.f;
-            m_run = up ? mt : m_run;
+            for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-            for (int dt = 0; dt < 16; dt++) o[dt] *= cr;
-            ol *= cr;
-        }
-        const float nm = -m_run;
-        u32x4 w[PARTS];
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float x = fast_exp2(fmaf(st[kt][2 * i], cs, nm)), y = fast_exp2(fmaf(st[kt][2 * i + 1], cs, nm));
-                w[0][2 * kt + i] = cvt_pk_bf16(x, y);
-                if constexpr (PARTS == 3) {
-                    ol[0] += x + y;
-                    const float x1 = x - bf16lo(w[0][2 * kt + i]), y1 = y - bf16hi(w[0][2 * kt + i]);  // exact
-                    w[1][2 * kt + i] = cvt_pk_bf16(x1, y1);
-                    w[2][2 * kt + i] = cvt_pk_bf16(x1 - bf16lo(w[1][2 * kt + i]), y1 - bf16hi(w[1][2 * kt + i]));
+                for (int e = 0; e < 2; e++) {
+                    const float x = fast_exp2(fmaf(st[t][kt][2 * e], cs, nm)), y = fast_exp2(fmaf(st[t][kt][2 * e + 1], cs, nm));
+                    w[0][2 * kt + e] = cvt_pk_bf16(x, y);
+                    if constexpr (PARTS == 1) {
+                        l[t] += bf16lo(w[0][2 * kt + e]) + bf16hi(w[0][2 * kt + e]);  // what the product uses
+                    } else {
+                        l[t] += x + y;
+                        const float x1 = x - bf16lo(w[0][2 * kt + e]), y1 = y - bf16hi(w[0][2 * kt + e]);  // exact
+                        w[1][2 * kt + e] = cvt_pk_bf16(x1, y1);
+                        w[2][2 * kt + e] = cvt_pk_bf16(x1 - bf16lo(w[1][2 * kt + e]), y1 - bf16hi(w[1][2 * kt + e]));
+                    }
                 }
-            }
 #pragma unroll
-        for (int i = 0; i < PARTS; i++) pw[i] = as_bf16x8(w[i]);
-    };
-    auto values = [&](uint32_t vu) {
-        bf16x8_t vf[kPfAhead];
-        auto read = [&](int dt) {
-            const u32x2 lo = lds_load_tr16(vu + va[dt], 0), hi = lds_load_tr16(vu + va[dt], 8192);
-            vf[dt % kPfAhead] = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
-        };
-#pragma unroll
-        for (int i = 0; i < kPfAhead; i++) read(i);
-#pragma unroll
-        for (int dt = 0; dt < 16; dt++) {
-            const bf16x8_t x = vf[dt % kPfAhead];
-            if (dt + kPfAhead < 16) read(dt + kPfAhead);
-#pragma unroll
-            for (int i = 0; i < PARTS; i++) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pw[i], o[dt], 0, 0, 0);
+            for (int p = 0; p < PARTS; p++) pw[t][p] = as_bf16x8(w[p]);
         }
-        if constexpr (PARTS == 1) ol = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pw[0], ol, 0, 0, 0);
-    };
-
-    if (rows_kind) {
-        // K and V of a block, for all waves; each copies an eighth of the rows.
-        // 3 blocks are in flight while one is computed, one barrier a block.
-        auto issue = [&](int i) {
-            const int id = __builtin_amdgcn_readlane(idv, i);
-            const uint32_t lds = lds0 + 2 * (i % kSharedStages) * kUnitLds;
-            copy(a.kpool, cbk, 5, id, lds, 4 * wave, PfBuf<4>{});
-            copy(a.vpool, cbv, 6, id, lds + kUnitLds, 4 * wave, PfBuf<4>{});
-        };
-        for (int i = 0; i < min(n_blk, kSharedStages - 1); i++) issue(i);
-        for (int i = 0; i < n_blk; i++) {
-            const int ahead = n_blk - 1 - i;  // uniform
-            if (ahead >= 2)
-                wait_vm<16>();
-            else if (ahead == 1)
-                wait_vm<8>();
-            else
-                wait_vm<0>();
-            lds_barrier();  // block i is there, and every wave has read block i - 1
-            if (i + kSharedStages - 1 < n_blk) issue(i + kSharedStages - 1);
-            const uint32_t lds = lds0 + 2 * (i % kSharedStages) * kUnitLds;
-            scores(lds);
-            weights(kBlockTok);
-            values(lds + kUnitLds);
-        }
-    } else {
-        // a block of its own per wave: no barrier.  K of the next block is
-        // requested once this one's has been read, V likewise.
-        const uint32_t ku = lds0 + 2 * wave * kUnitLds, vu = ku + kUnitLds;
-        auto issue = [&](const uint16_t* pool, uint32_t cb, int jsh, int i, uint32_t lds) {
-            copy(pool, cb, jsh, __builtin_amdgcn_readlane(idv, i), lds, 0, PfBuf<16>{});
-        };
-        if (n_my > 0) {
-            issue(a.kpool, cbk, 5, 0, ku);
-            issue(a.vpool, cbv, 6, 0, vu);
-        }
-        for (int i = 0; i < n_my; i++) {
-            const bool more = i + 1 < n_my;
-            const int valid = limit - (base + i * step) * kBlockTok;
-            wait_vm<16>();  // K: the 16 copies after it are V's
-            scores(ku);
+        if (more)
+            wait_vm<16>();
+        else
+            wait_vm<0>();
+        if (valid < kBlockTok) {  // rows that do not exist may hold anything: 0 times it must be 0
+            for (int r = valid; r < kBlockTok; r++)
+                *reinterpret_cast<u32x2*>(&sm.unit[2 * wave + 1][r * kHeadDim + lane * 4]) = u32x2{0u, 0u};
             wait_lds();
-            if (more) issue(a.kpool, cbk, 5, i + 1, ku);
-            weights(valid);
-            if (more)
-                wait_vm<16>();
-            else
-                wait_vm<0>();
-            if (valid < kBlockTok) {  // rows that do not exist may hold anything: 0 times it must be 0
-                for (int r = max(valid, 0); r < kBlockTok; r++)
-                    *reinterpret_cast<u32x2*>(&sm.unit[2 * wave + 1][r * kHeadDim + lane * 4]) = u32x2{0u, 0u};
-                wait_lds();
-            }
-            values(vu);
-            wait_lds();
-            if (more) issue(a.vpool, cbv, 6, i + 1, vu);
         }
+        {
+            bf16x8_t vf[kShAhead];
+            auto read = [&](int dt) {
+                const uint32_t at = va[dt & 3] + vb[dt >> 2];
+                const u32x2 lo = lds_load_tr16(at, 0), hi = lds_load_tr16(at, 8192);
+                vf[dt % kShAhead] = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
+            };
+#pragma unroll
+            for (int n = 0; n < kShAhead; n++) read(n);
+#pragma unroll
+            for (int dt = 0; dt < 16; dt++) {
+                const bf16x8_t x = vf[dt % kShAhead];
+                if (dt + kShAhead < 16) read(dt + kShAhead);
+#pragma unroll
+                for (int t = 0; t < T; t++)
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++)
+                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pw[t][p], o[t][dt], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2 * kShAhead, 1);
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+            if (n + kShAhead < 16) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2, 1);
+            __builtin_amdgcn_sched_group_barrier(kSgMfma, T * PARTS, 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lds();
+        if (more) issue(a.vpool, cbv, 6, i + 1, vu);
     }
-    float l = ol[0];
-    if constexpr (PARTS == 3) l = sum_xor32(sum_xor16(l));
-
-    const size_t row0 = (size_t)nd.row_begin + (size_t)(ck * kKvHeads + h) * members * kGroup;
-    if (kind != kSharedKeys) {
-        if (!real) return;
-        const size_t row = row0 + jm * kGroup + g;
-        float* acc = a.acc + row * kHeadDim + 4 * q4;
 #pragma unroll
-        for (int dt = 0; dt < 16; dt++) *reinterpret_cast<f32x4*>(acc + 16 * dt) = o[dt];
-        if (q4 == 0) *reinterpret_cast<float2*>(a.stats + row * 2) = make_float2(m_run, l);
+    for (int t = 0; t < T; t++) l[t] = sum_xor32(sum_xor16(l[t]));
+
+    if (it.kind == kSharedHeads) {
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            if (4 * t + (r16 >> 2) >= it.members) continue;
+            const size_t row = (size_t)(a.seq_row[mem[t] & 63] + (mem[t] >> 6) + it.ck) * kQHeads + h * kGroup + g;
+            float* acc = a.acc + row * kHeadDim + 4 * q4;
+#pragma unroll
+            for (int dt = 0; dt < 16; dt++) *reinterpret_cast<f32x4*>(acc + 16 * dt) = o[t][dt];
+            if (q4 == 0) *reinterpret_cast<float2*>(a.stats + row * 2) = make_float2(m_run[t], l[t]);
+        }
         return;
     }
-    // fold the 4 waves' keys: O through LDS (each wave into its own units, which it alone read)
+    // fold the 4 waves' keys, tile by tile: O through LDS (each wave into its own units, which it alone read)
     float* own = reinterpret_cast<float*>(sm.unit[2 * wave]);
 #pragma unroll
-    for (int dt = 0; dt < 16; dt++) *reinterpret_cast<f32x4*>(own + r16 * kSharedRowPad + 16 * dt + 4 * q4) = o[dt];
-    if (q4 == 0) sm.ml[wave][r16] = make_float2(m_run, l);
-    __syncthreads();
-    for (int r = wave; r < members * kGroup; r += kWaves) {
-        float2 ml[kWaves];
-        float m = kNegBig, lt = 0.f;
+    for (int t = 0; t < T; t++) {
+        if (t > 0) __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            ml[w] = sm.ml[w][r];
-            m = fmaxf(m, ml[w].x);
-        }
-        f32x4 t = {0.f, 0.f, 0.f, 0.f};
+        for (int dt = 0; dt < 16; dt++) *reinterpret_cast<f32x4*>(own + r16 * kSharedRowPad + 16 * dt + 4 * q4) = o[t][dt];
+        if (q4 == 0) sm.ml[wave][r16] = make_float2(m_run[t], l[t]);
+        __syncthreads();
+        for (int r = wave; r < min(16, (it.members - 4 * t) * kGroup); r += kWaves) {
+            float2 ml[kWaves];
+            float m = kNegBig, lt = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float f = fast_exp2(ml[w].x - m);
-            lt = fmaf(f, ml[w].y, lt);
-            t += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(sm.unit[2 * w]) + r * kSharedRowPad + lane * 4);
+            for (int w = 0; w < kWaves; w++) {
+                ml[w] = sm.ml[w][r];
+                m = fmaxf(m, ml[w].x);
+            }
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const float f = fast_exp2(ml[w].x - m);
+                lt = fmaf(f, ml[w].y, lt);
+                x += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(sm.unit[2 * w]) + r * kSharedRowPad + lane * 4);
+            }
+            const int mr = __builtin_amdgcn_readlane(mem[t], r);  // lane r holds row r's member
+            const size_t row = (size_t)(a.seq_row[mr & 63] + (mr >> 6) + it.ck) * kQHeads + h * kGroup + (r & 3);
+            *reinterpret_cast<f32x4*>(a.acc + row * kHeadDim + lane * 4) = x;
+            if (lane == 0) *reinterpret_cast<float2*>(a.stats + row * 2) = make_float2(m, lt);
         }
-        *reinterpret_cast<f32x4*>(a.acc + (row0 + r) * kHeadDim + lane * 4) = t;
-        if (lane == 0) *reinterpret_cast<float2*>(a.stats + (row0 + r) * 2) = make_float2(m, lt);
     }
+}
+
+template <int PARTS>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(SharedArgs a) {
+    __shared__ SharedSmem sm;
+    const int lane = threadIdx.x & 63;
+    const int item = blockIdx.x;
+    // which node: every lane looks at two; both records are requested with their
+    // ends, so that one trip to the arguments gives all
+    const int e0 = a.item_end[lane], e1 = a.item_end[lane + 64];
+    const int4 n0 = *reinterpret_cast<const int4*>(&a.node[lane]), n1 = *reinterpret_cast<const int4*>(&a.node[lane + 64]);
+    const int c0 = __popcll(__builtin_amdgcn_ballot_w64(e0 <= item)), c1 = __popcll(__builtin_amdgcn_ballot_w64(e1 <= item));
+    const int node = c0 + c1, at = node & 63;
+    if (node >= kSharedNodes) return;
+    const bool hi = node >= 64;
+    const int first = hi ? __builtin_amdgcn_readlane(n1.x, at) : __builtin_amdgcn_readlane(n0.x, at);
+    const uint32_t lw = hi ? __builtin_amdgcn_readlane(n1.y, at) : __builtin_amdgcn_readlane(n0.y, at);
+    const uint32_t sw = hi ? __builtin_amdgcn_readlane(n1.z, at) : __builtin_amdgcn_readlane(n0.z, at);
+    const int slot = hi ? __builtin_amdgcn_readlane(n1.w, at) : __builtin_amdgcn_readlane(n0.w, at);
+    const int begin = node == 0 ? 0 : node <= 64 ? __builtin_amdgcn_readlane(e0, node - 1) : __builtin_amdgcn_readlane(e1, node - 65);
+    const SharedShape sh = shared_shape(sw);
+    const int len = lw & ((1 << 26) - 1);
+    if (sh.members == 0) return;  // (behind the last node)
+    SharedItem it;
+    it.kind = sh.kind;
+    const int n_chunks = (len + sh.chunk - 1) / sh.chunk, units = it.kind == kSharedHeads ? n_chunks : n_chunks * kKvHeads;
+    const int groups = (sh.members + a.group - 1) / a.group;
+    int j = item - begin, grp = 0;
+    if (groups > 1) {
+        // (the node starts on a multiple of 8; the groups of members that read the
+        // same keys run on one XCD, workgroup number % 8, one after the other)
+        j = item - (begin + 7) / 8 * 8;
+        if (j < 0) return;
+        const int r = j >> 3;
+        grp = r % groups;
+        j = r / groups * 8 + (j & 7);
+    }
+    if (j >= units) return;  // (padding)
+    it.h = it.kind == kSharedHeads ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : j % kKvHeads;
+    it.ck = it.kind == kSharedHeads ? j : j / kKvHeads;
+    const int b0 = it.ck * sh.chunk;
+    it.n_blk = min(sh.chunk, len - b0);
+    it.last = b0 + it.n_blk == len ? (int)(lw >> 26) : kBlockTok;
+    it.mb = sh.member_begin + grp * a.group;
+    it.members = min(a.group, sh.members - grp * a.group);
+    it.trow = a.table + (size_t)slot * a.table_stride + first + b0;
+    if constexpr (PARTS == 1) {
+        if (it.members > 4) {
+            shared_item<2, PARTS>(a, it, sm);
+            return;
+        }
+    }
+    shared_item<1, PARTS>(a, it, sm);
 }
 
 // One workgroup folds a (sequence, q head): each wave every 4th partial, its
@@ -312,21 +352,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // a partial of its own, (score, 1, v), and is written to the cache.
 constexpr int kSharedFold = 16;
 __global__ __launch_bounds__(256) void shared_fold_kernel(SharedFoldArgs a) {
-    __shared__ int rows[kSharedPath];
     __shared__ float wgt[kSharedPath];
     __shared__ float red[kWaves][2];
     __shared__ f32x4 part[kWaves][64];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int s = blockIdx.x / kQHeads, head = blockIdx.x % kQHeads, h = head / kGroup, g = head % kGroup;
-    int np = 0;
-    for (int e = a.path_begin[s]; e < a.path_begin[s + 1]; e++) {
-        const int pe = __builtin_amdgcn_readfirstlane(a.path[e]), node = pe & 255;
-        const int nc = a.chunks[node] & 0xFFFF, mg = (a.chunks[node] >> 16) * kGroup;
-        const int row = a.row_begin[node] + h * mg + (pe >> 8) * kGroup + g;
-        for (int k = tid; k < nc; k += 256) rows[np + k] = row + k * kKvHeads * mg;
-        np += nc;
-    }
+    const SharedSeq sq = a.seq[s];
+    const int np = sq.parts;
+    const size_t row0 = (size_t)sq.row * kQHeads + head;
     const size_t qrow = ((size_t)s * kQHeads + head) * kHeadDim;
     const bool has_gate = a.gate != nullptr;
     uint2 gw = make_uint2(0u, 0u);
@@ -338,12 +372,11 @@ __global__ __launch_bounds__(256) void shared_fold_kernel(SharedFoldArgs a) {
         kw = *reinterpret_cast<const uint2*>(a.k_new + krow);
         vw = *reinterpret_cast<const uint2*>(a.v_new + krow);
     }
-    __syncthreads();
     f32x4 x[kSharedFold];
     if (np > 0) {
 #pragma unroll
         for (int k = 0; k < kSharedFold; k++)
-            x[k] = *reinterpret_cast<const f32x4*>(a.acc + (size_t)rows[min(wave + kWaves * k, np - 1)] * kHeadDim + lane * 4);
+            x[k] = *reinterpret_cast<const f32x4*>(a.acc + (row0 + (size_t)min(wave + kWaves * k, np - 1) * kQHeads) * kHeadDim + lane * 4);
     }
     float ms[kSharedPath / 256], ls[kSharedPath / 256], m = kNegBig;
 #pragma unroll
@@ -351,7 +384,7 @@ __global__ __launch_bounds__(256) void shared_fold_kernel(SharedFoldArgs a) {
         ms[i] = kNegBig;
         ls[i] = 0.f;
         if (tid + 256 * i < np) {
-            const float2 t = *reinterpret_cast<const float2*>(a.stats + (size_t)rows[tid + 256 * i] * 2);
+            const float2 t = *reinterpret_cast<const float2*>(a.stats + (row0 + (size_t)(tid + 256 * i) * kQHeads) * 2);
             ms[i] = t.x;
             ls[i] = t.y;
         }
@@ -382,7 +415,7 @@ __global__ __launch_bounds__(256) void shared_fold_kernel(SharedFoldArgs a) {
     for (int k = 0; k < kSharedFold; k++)
         if (wave + kWaves * k < np) t += wgt[wave + kWaves * k] * x[k];
     for (int p = wave + kWaves * kSharedFold; p < np; p += kWaves)
-        t += wgt[p] * *reinterpret_cast<const f32x4*>(a.acc + (size_t)rows[p] * kHeadDim + lane * 4);
+        t += wgt[p] * *reinterpret_cast<const f32x4*>(a.acc + (row0 + (size_t)p * kQHeads) * kHeadDim + lane * 4);
     part[wave][lane] = t;
     __syncthreads();
     if (wave != 0) return;
@@ -397,8 +430,8 @@ __global__ __launch_bounds__(256) void shared_fold_kernel(SharedFoldArgs a) {
         A[2] = fmaf(f, bf16lo(vw.y), A[2]);
         A[3] = fmaf(f, bf16hi(vw.y), A[3]);
         if (g == 0) {
-            const int pos = a.keys[s];
-            const int blk = a.table[(size_t)a.slot[s] * a.table_stride + pos / kBlockTok];
+            const int pos = sq.keys;
+            const int blk = a.table[(size_t)sq.slot * a.table_stride + pos / kBlockTok];
             const size_t off = (((size_t)blk * kKvHeads + h) * kBlockTok + pos % kBlockTok) * kHeadDim + lane * 4;
             *reinterpret_cast<uint2*>(a.kpool + off) = kw;
             *reinterpret_cast<uint2*>(a.vpool + off) = vw;

@@ -19,17 +19,19 @@ namespace kvc {
 struct SharedPlan {
     int32_t n_nodes = 0, n_members = 0;
     int32_t n_items = 0;               // workgroups
-    int32_t rows = 0;                  // partial rows
-    int32_t path = 0;                  // most partials of one (sequence, q head)
+    int32_t parts = 0;                 // partials per q head, of all sequences
+    int32_t path = 0;                  // most of them of one sequence
     int64_t blocks = 0, blocks_apart = 0;  // read by the plan, and sequence by sequence
     int32_t first[kSharedNodes];       // of the node's blocks, in its members' tables
     int32_t len[kSharedNodes];         // blocks
     int32_t item_begin[kSharedNodes + 1];
-    int32_t row_begin[kSharedNodes];
     uint16_t chunk[kSharedNodes];      // blocks per workgroup
     uint16_t member_begin[kSharedNodes + 1];
     uint8_t kind[kSharedNodes];
     uint8_t member[kSharedMembers];    // index of the sequence in the launch
+    uint16_t part[kSharedMembers];     // its first partial of this node
+    int32_t seq_row[kMaxBatch];        // its first partial in the workspace
+    int32_t seq_parts[kMaxBatch];
 };
 
 // A node is worth its own partials from this many saved block reads on.
@@ -109,62 +111,57 @@ class SharedPlanner {
     int32_t left_ = 0;  // sequences without a leaf
 };
 
-inline int32_t shared_groups(int32_t members) { return (members + kSharedSeqs - 1) / kSharedSeqs; }
-
-// Items of the nodes, for the chunk length c (blocks of a workgroup).
-inline void shared_items(SharedPlan& p, int32_t c, int32_t n) {
-    int32_t chunks_of[kMaxBatch] = {};
-    int64_t items = 0, rows = 0;
+// Workgroups of the nodes, `group` members each at most, where a wave takes up to w blocks of a node: a node of
+// at most w blocks goes to workgroups that take all kv heads.
+inline void shared_items(SharedPlan& p, int32_t w, int32_t n, int32_t group) {
+    for (int32_t i = 0; i < n; i++) p.seq_parts[i] = 0;
+    int64_t items = 0;
     for (int32_t k = 0; k < p.n_nodes; k++) {
-        const int32_t members = p.member_begin[k + 1] - p.member_begin[k], groups = shared_groups(members);
-        int32_t chunk;
-        if (members > 4) {
-            p.kind[k] = kSharedRows;
-            chunk = std::min(c, kSharedMaxChunk);
-        } else if (p.len[k] <= kSharedShort) {
-            p.kind[k] = kSharedHeads;
-            chunk = p.len[k];
-        } else {
-            p.kind[k] = kSharedKeys;
-            chunk = std::min((c + 3) / 4 * 4, 4 * kSharedMaxChunk);
-        }
-        const int32_t n_chunks = (p.len[k] + chunk - 1) / chunk;
+        const int32_t members = p.member_begin[k + 1] - p.member_begin[k], groups = (members + group - 1) / group;
+        p.kind[k] = p.len[k] <= w ? kSharedHeads : kSharedKeys;
+        const int32_t chunk = p.kind[k] == kSharedHeads ? p.len[k] : 4 * w;
+        const int32_t n_chunks = (p.len[k] + chunk - 1) / chunk, units = n_chunks * (p.kind[k] == kSharedHeads ? 1 : kKvHeads);
         p.chunk[k] = (uint16_t)chunk;
+        // (the groups of a unit run on one XCD: such nodes start on a multiple of 8)
+        if (groups > 1) items = (items + 7) / 8 * 8;
         p.item_begin[k] = (int32_t)items;
-        p.row_begin[k] = (int32_t)rows;
-        if (groups > 1)
-            items += (int64_t)(n_chunks * kKvHeads + 7) / 8 * 8 * groups;
-        else
-            items += p.kind[k] == kSharedHeads ? n_chunks : n_chunks * kKvHeads;
-        // (nodes of one group start anywhere, those of several on a multiple of 8)
-        if (k + 1 < p.n_nodes && p.member_begin[k + 2] - p.member_begin[k + 1] > kSharedSeqs) items = (items + 7) / 8 * 8;
-        rows += (int64_t)n_chunks * kQHeads * members;
-        for (int32_t i = p.member_begin[k]; i < p.member_begin[k + 1]; i++) chunks_of[p.member[i]] += n_chunks;
+        items += groups > 1 ? (int64_t)(units + 7) / 8 * 8 * groups : units;
+        for (int32_t i = p.member_begin[k]; i < p.member_begin[k + 1]; i++) {
+            p.part[i] = (uint16_t)std::min(p.seq_parts[p.member[i]], kSharedPath);
+            p.seq_parts[p.member[i]] += n_chunks;
+        }
     }
     p.item_begin[p.n_nodes] = (int32_t)items;
     p.n_items = (int32_t)items;
-    p.rows = (int32_t)std::min<int64_t>(rows, INT32_MAX);
     p.path = 0;
-    for (int32_t i = 0; i < n; i++) p.path = std::max(p.path, chunks_of[i]);
+    int64_t parts = 0;
+    for (int32_t i = 0; i < n; i++) {
+        p.seq_row[i] = (int32_t)parts;
+        parts = std::min<int64_t>(parts + p.seq_parts[i], INT32_MAX);
+        p.path = std::max(p.path, p.seq_parts[i]);
+    }
+    p.parts = (int32_t)parts;
 }
 
 // Whether the plan beats reading sequence by sequence, and fits.
 inline bool shared_pays(const SharedPlan& p) {
-    return p.path <= kSharedPath && p.rows <= kSharedMaxRows && p.blocks_apart - p.blocks >= 16;
+    return p.path <= kSharedPath && p.parts <= kSharedMaxParts && p.blocks_apart - p.blocks >= 16;
 }
 
-// The work of a launch of n sequences (n <= kMaxBatch): caller_chunk > 0 is a
-// chunk length that the caller set.
-inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, SharedPlan& p) {
+// The work of a launch of n sequences (n <= kMaxBatch), `group` members a
+// workgroup; caller_chunk > 0 is a chunk length that the caller set.
+inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, int32_t group,
+                        SharedPlan& p) {
     SharedPlanner(tab, keys, n, p);
     int64_t work = 0;
     for (int32_t k = 0; k < p.n_nodes; k++)
-        work += (int64_t)p.len[k] * shared_groups(p.member_begin[k + 1] - p.member_begin[k]) * kKvHeads;
-    int32_t c = caller_chunk > 0 ? std::min(caller_chunk, 4 * kSharedMaxChunk) : (int32_t)std::max<int64_t>(2, (work + 255) / 256);
+        work += (int64_t)p.len[k] * ((p.member_begin[k + 1] - p.member_begin[k] + group - 1) / group);
+    int32_t w = caller_chunk > 0 ? (std::min(caller_chunk, 4 * kSharedWaveBlocks) + 3) / 4
+                                 : (int32_t)std::min<int64_t>(kSharedWaveBlocks, std::max<int64_t>(1, (work + 255) / 256));
     for (;;) {
-        shared_items(p, c, n);
-        if ((p.path <= kSharedPath && p.rows <= kSharedMaxRows) || c >= 4 * kSharedMaxChunk) break;
-        c *= 2;
+        shared_items(p, w, n, group);
+        if ((p.path <= kSharedPath && p.parts <= kSharedMaxParts) || w >= kSharedWaveBlocks) break;
+        w = std::min(2 * w, kSharedWaveBlocks);
     }
 }
 

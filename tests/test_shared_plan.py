@@ -13,18 +13,18 @@ import pytest
 CSRC = Path(__file__).resolve().parents[1] / "qwen3.5-9b-bfp8b-1xn300_amd" / "csrc"
 CXX = shutil.which("g++")
 pytestmark = pytest.mark.skipif(CXX is None, reason="needs g++")
-BT, HEADS, QHEADS, SEQS, SHORT = 32, 4, 16, 16, 8
-ROWS, KEYS, ALL_HEADS = 0, 1, 2  # kinds
+BT, HEADS = 32, 4
+KEYS, ALL_HEADS = 0, 1  # kinds
 
-# stdin: launches as "n chunk", then per sequence "keys nblk id id ..."; stdout: the plan
+# stdin: launches as "n chunk group", then per sequence "keys nblk id id ..."; stdout: the plan
 PROGRAM = r"""
 #include <cstdio>
 #include <iostream>
 #include <vector>
 #include "kvc_shared_plan.h"
 int main() {
-    int n, chunk;
-    while (std::cin >> n >> chunk) {
+    int n, chunk, group;
+    while (std::cin >> n >> chunk >> group) {
         std::vector<std::vector<int32_t>> t(n);
         std::vector<int32_t> keys(n);
         std::vector<const int32_t*> tab(n);
@@ -36,13 +36,13 @@ int main() {
             tab[i] = t[i].data();
         }
         kvc::SharedPlan p;
-        kvc::shared_plan(tab.data(), keys.data(), n, chunk, p);
-        std::printf("%d %d %d %d %lld %lld %d\n", p.n_nodes, p.n_items, p.rows, p.path, (long long)p.blocks,
+        kvc::shared_plan(tab.data(), keys.data(), n, chunk, group, p);
+        std::printf("%d %d %d %d %lld %lld %d\n", p.n_nodes, p.n_items, p.parts, p.path, (long long)p.blocks,
                     (long long)p.blocks_apart, (int)kvc::shared_pays(p));
         for (int k = 0; k < p.n_nodes; k++) {
-            std::printf("%d %d %d %d %d %d %d", p.first[k], p.len[k], p.item_begin[k], p.row_begin[k], p.chunk[k], p.kind[k],
-                        p.item_begin[k + 1]);
-            for (int i = p.member_begin[k]; i < p.member_begin[k + 1]; i++) std::printf(" %d", p.member[i]);
+            std::printf("%d %d %d %d %d %d", p.first[k], p.len[k], p.item_begin[k], p.chunk[k], p.kind[k], p.item_begin[k + 1]);
+            for (int i = p.member_begin[k]; i < p.member_begin[k + 1]; i++)
+                std::printf(" %d %d", p.member[i], p.seq_row[p.member[i]] + p.part[i]);
             std::printf("\n");
         }
     }
@@ -58,18 +58,18 @@ def plans(tmp_path_factory):
                     "-fno-sanitize-recover=undefined", f"-I{CSRC}", str(d / "plan.cpp"), "-o", str(d / "plan")], check=True)
 
     def run(launches):
-        """launches: (chunk, [(keys, table), ...])"""
-        text = "\n".join("\n".join([f"{len(seqs)} {chunk}"] + [" ".join(map(str, (k, len(t), *t))) for k, t in seqs])
-                         for chunk, seqs in launches)
+        """launches: (chunk, members of a workgroup, [(keys, table), ...])"""
+        text = "\n".join("\n".join([f"{len(seqs)} {chunk} {group}"] + [" ".join(map(str, (k, len(t), *t))) for k, t in seqs])
+                         for chunk, group, seqs in launches)
         out = subprocess.run([str(d / "plan")], input=text, capture_output=True, text=True, check=True).stdout
         lines = iter(out.splitlines())
         got = []
         for _ in launches:
-            head = dict(zip(("n_nodes", "n_items", "rows", "path", "blocks", "apart", "pays"), map(int, next(lines).split())))
+            head = dict(zip(("n_nodes", "n_items", "parts", "path", "blocks", "apart", "pays"), map(int, next(lines).split())))
             nodes = []
             for _ in range(head["n_nodes"]):
                 x = list(map(int, next(lines).split()))
-                nodes.append(dict(zip(("first", "len", "item", "row", "chunk", "kind", "end"), x[:7]), members=x[7:]))
+                nodes.append(dict(zip(("first", "len", "item", "chunk", "kind", "end"), x[:6]), members=x[6::2], rows=x[7::2]))
             got.append((head, nodes))
         return got
 
@@ -101,48 +101,55 @@ def tree(rng, n, depth_blocks, ids):
     return seqs
 
 
-def check(head, nodes, seqs):
+def check(head, nodes, group, seqs):
     path = {i: [] for i in range(len(seqs))}
-    rows = 0
-    for k, x in enumerate(nodes):
+    used = set()  # partials
+    for x in nodes:
         assert x["len"] > 0 and len(set(x["members"])) == len(x["members"])
-        assert x["row"] == rows
         chunks = -(-x["len"] // x["chunk"])
-        rows += chunks * QHEADS * len(x["members"])
+        units = chunks * (1 if x["kind"] == ALL_HEADS else HEADS)
         # the kernel's reading of its item number
         seen = set()
-        groups = -(-len(x["members"]) // SEQS)
-        for j in range(x["end"] - x["item"]):
-            unit, grp = j, 0
+        groups = -(-len(x["members"]) // group)
+        begin = 0 if x is nodes[0] else nodes[nodes.index(x) - 1]["end"]
+        for item in range(begin, x["end"]):
+            j, grp = item - begin, 0
             if groups > 1:
-                assert x["item"] % 8 == 0
-                grp, unit = (j >> 3) % groups, (j >> 3) // groups * 8 + (j & 7)
-            if unit >= chunks * (1 if x["kind"] == ALL_HEADS else HEADS):
+                j = item - (begin + 7) // 8 * 8
+                if j < 0:
+                    continue
+                grp, j = (j >> 3) % groups, (j >> 3) // groups * 8 + (j & 7)
+            if j >= units:
                 continue
-            assert (unit, grp) not in seen
-            seen.add((unit, grp))
-        assert len(seen) == chunks * groups * (1 if x["kind"] == ALL_HEADS else HEADS)
-        assert (x["kind"] == ROWS) == (len(x["members"]) > 4)
-        assert x["chunk"] <= {ROWS: 64, KEYS: 256, ALL_HEADS: SHORT}[x["kind"]]  # ids that a wave holds
-        for m in x["members"]:
+            assert (j, grp) not in seen
+            seen.add((j, grp))
+        assert len(seen) == units * groups
+        assert x["chunk"] <= {KEYS: 4 * 64, ALL_HEADS: 64}[x["kind"]]  # ids that a wave holds
+        for m, row in zip(x["members"], x["rows"]):
             keys, t = seqs[m]
             path[m].append((x["first"], x["len"], chunks))
+            if head["pays"]:
+                rows = set(range(row, row + chunks))
+                assert not rows & used
+                used |= rows
             first = seqs[x["members"][0]][1]
             assert t[x["first"]:x["first"] + x["len"]] == first[x["first"]:x["first"] + x["len"]]
             if len(x["members"]) > 1:  # whole blocks only
                 assert (x["first"] + x["len"]) * BT <= keys
-    assert head["rows"] == rows and head["n_items"] == (nodes[-1]["end"] if nodes else 0)
+    assert head["n_items"] == (nodes[-1]["end"] if nodes else 0)
     for i, (keys, t) in enumerate(seqs):
         at = 0
         for first, n, _ in path[i]:  # in order, once each
             assert first == at
             at += n
         assert at == -(-keys // BT)
-    assert head["path"] == max([sum(c for _, _, c in p) for p in path.values()], default=0)
+    parts = [sum(c for _, _, c in p) for p in path.values()]
+    assert head["path"] == max(parts, default=0) and head["parts"] == sum(parts)
     assert head["blocks"] == sum(x["len"] for x in nodes)
     assert head["apart"] == sum(-(-k // BT) for k, _ in seqs)
     if head["pays"]:
-        assert head["path"] <= 512 and rows * 258 * 4 <= 8192 * 4 * 1056 * 4
+        assert used == set(range(head["parts"]))
+        assert head["path"] <= 512 and head["parts"] * 16 * 258 * 4 <= 8192 * 4 * 1056 * 4
 
 
 @pytest.mark.parametrize("seed", range(8))
@@ -151,9 +158,9 @@ def test_random_tries(plans, seed):
     launches = []
     for _ in range(60):
         ids = iter(rng.sample(range(100000), 20000))
-        launches.append((rng.choice([0, 0, 0, 1, 3, 40, 1 << 20]), tree(rng, rng.randint(1, 64), rng.choice([3, 20, 150]), ids)))
-    for (head, nodes), (_, seqs) in zip(plans(launches), launches):
-        check(head, nodes, seqs)
+        launches.append((rng.choice([0, 0, 0, 1, 3, 40, 1 << 20]), rng.choice([4, 8]), tree(rng, rng.randint(1, 64), rng.choice([3, 20, 150]), ids)))
+    for (head, nodes), (_, group, seqs) in zip(plans(launches), launches):
+        check(head, nodes, group, seqs)
 
 
 def common(n, prefix_blocks, tail_blocks):
@@ -164,16 +171,16 @@ def common(n, prefix_blocks, tail_blocks):
 
 def test_a_common_prefix_is_read_once(plans):
     for n in (2, 4, 5, 16, 17, 64):
-        (head, nodes), = plans([(0, common(n, 128, 3))])
-        check(head, nodes, common(n, 128, 3))
+        (head, nodes), = plans([(0, 8, common(n, 128, 3))])
+        check(head, nodes, 8, common(n, 128, 3))
         assert head["blocks"] == 128 + 3 * n and head["pays"]
-        assert nodes[0]["members"] == list(range(n)) and nodes[0]["kind"] == (ROWS if n > 4 else KEYS)
+        assert nodes[0]["members"] == list(range(n)) and nodes[0]["kind"] == KEYS
 
 
 def test_nothing_in_common(plans):
     seqs = [(100, [4 * i, 4 * i + 1, 4 * i + 2, 4 * i + 3]) for i in range(10)]
-    (head, nodes), = plans([(0, seqs)])
-    check(head, nodes, seqs)
+    (head, nodes), = plans([(0, 8, seqs)])
+    check(head, nodes, 8, seqs)
     assert head["blocks"] == head["apart"] == 40 and not head["pays"]
 
 
@@ -183,13 +190,13 @@ def test_ladders_and_long_prefixes(plans):
     ids = list(range(2000))
     ladder = [((8 * i + 9) * BT, ids[:8 * i + 8] + [5000 + i]) for i in range(64)]
     long = common(64, 8192, 1)
-    for (head, nodes), seqs in zip(plans([(0, ladder), (0, long), (1, long)]), (ladder, long, long)):
-        check(head, nodes, seqs)
+    for (head, nodes), seqs in zip(plans([(0, 8, ladder), (0, 8, long), (1, 8, long)]), (ladder, long, long)):
+        check(head, nodes, 8, seqs)
         assert sum(len(x["members"]) for x in nodes) <= 512 and head["n_nodes"] <= 128
 
 
 def test_only_new_tokens(plans):
-    (head, nodes), = plans([(0, [(0, [1]), (0, [2])])])
+    (head, nodes), = plans([(0, 8, [(0, [1]), (0, [2])])])
     assert head["n_nodes"] == 0 and head["n_items"] == 0 and not head["pays"]
 
 
@@ -198,6 +205,6 @@ def test_same_sequence_many_times_over_ends_in_a_shared_block(plans):
     attends it alone."""
     t = list(range(20))
     seqs = [(20 * BT - 5, t) for _ in range(9)]
-    (head, nodes), = plans([(0, seqs)])
-    check(head, nodes, seqs)
+    (head, nodes), = plans([(0, 8, seqs)])
+    check(head, nodes, 8, seqs)
     assert nodes[0]["len"] == 19 and head["blocks"] == 19 + 9
