@@ -1494,14 +1494,18 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
         f.seq[j] = {p.seq_row[j], p.seq_parts[j], seqs[i0 + j], keys[j]};
     }
     for (int32_t k = 0; k < kSharedNodes; k++) a.item_end[k] = k < p.n_nodes ? p.item_begin[k + 1] : INT32_MAX;
+    int32_t listed = 0;
     for (int32_t k = 0; k < p.n_nodes; k++) {
         const int32_t mb = p.member_begin[k], members = p.member_begin[k + 1] - mb, s = p.member[mb];
         // (a node of several members has full blocks only)
         const int32_t last = std::min(keys[s] - (p.first[k] + p.len[k] - 1) * kBlockTok, kBlockTok);
-        a.node[k] = {p.first[k], (uint32_t)p.len[k] | (uint32_t)last << 26,
-                     shared_shape(SharedShape{p.chunk[k], p.kind[k], members, mb}), seqs[i0 + s]};
+        const auto entry = [&](int32_t i) { return (uint16_t)(p.member[i] | p.part[i] << 6); };
+        a.node[k] = {(uint32_t)p.first[k] | (uint32_t)p.kind[k] << 26, (uint32_t)p.len[k] | (uint32_t)(last - 1) << 26,
+                     (uint32_t)p.chunk[k] | (uint32_t)(members - 1) << 10 | (members == 1 ? entry(mb) : (uint32_t)listed / 8) << 16,
+                     seqs[i0 + s]};
+        if (members == 1) continue;
+        for (int32_t i = 0; i < (members + 7) / 8 * 8; i++) a.member[listed++] = entry(mb + std::min(i, members - 1));
     }
-    for (int32_t i = 0; i < p.n_members; i++) a.member[i] = (uint16_t)(p.member[i] | p.part[i] << 6);
     int e = launch_shared(a, p.n_items, f, stream);
     return e ? hip_err((hipError_t)e, "decode launch (shared blocks)") : KVC_OK;
 }

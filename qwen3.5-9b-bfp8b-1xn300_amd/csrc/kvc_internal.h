@@ -551,24 +551,16 @@ enum { kSharedKeys = 0,    // one kv head: a wave takes every 4th block
        kSharedHeads = 1 }; // all kv heads: a wave takes one
 constexpr int kSharedMaxParts = (int)(kPartBytes / ((kHeadDim + 2) * 4 * kQHeads));  // over all sequences
 
-// Records of whole words: a scalar load drops the low two bits of each part of
-// its address, and beside an array of bytes with the same index the compiler has
+// A node's record.  Whole words: a scalar load drops the low two bits of each part
+// of its address, and beside an array of bytes with the same index the compiler has
 // split the address of a word into such parts.
 struct SharedNode {
-    int32_t first;          // block in the members' tables
-    uint32_t len;           // blocks | keys in the last one << 26
-    uint32_t shape;         // see shared_shape
-    int32_t slot;           // table row of a member
+    uint32_t first;  // block in the members' tables | kind << 26
+    uint32_t len;    // blocks | (keys in the last one - 1) << 26
+    uint32_t who;    // chunk (blocks of a workgroup) | (members - 1) << 10 | and << 16:
+                     // of one member its entry, else where their list starts, / 8
+    int32_t slot;    // table row of a member
 };
-struct SharedShape {
-    int chunk, kind, members, member_begin;
-};
-constexpr uint32_t shared_shape(SharedShape s) {
-    return (uint32_t)s.chunk | (uint32_t)s.kind << 10 | (uint32_t)s.members << 12 | (uint32_t)s.member_begin << 20;
-}
-constexpr SharedShape shared_shape(uint32_t w) {
-    return {(int)(w & 1023), (int)(w >> 10 & 3), (int)(w >> 12 & 255), (int)(w >> 20)};
-}
 
 struct SharedArgs {
     const uint16_t* kpool;
@@ -584,7 +576,8 @@ struct SharedArgs {
     int32_t item_end[kSharedNodes];   // INT32_MAX behind the last node
     SharedNode node[kSharedNodes];
     int32_t seq_row[kMaxBatch];
-    uint16_t member[kSharedMembers];  // sequence | its first partial of the node << 6
+    uint16_t member[kSharedMembers];  // sequence | its first partial of the node << 6; a node's list starts at
+                                      // a multiple of 8 and is filled up to one with its last member
 };
 
 // Folds the partials; the new token (k_new) is one more and is appended.

@@ -20,12 +20,10 @@ namespace kvc {
 struct SharedSmem {
     // (K, V) units of each wave: rows of 512 B, 16-B chunks swizzled by the row (kswz, vswz)
     uint16_t unit[2 * kWaves][kBlockTok * kHeadDim];
-    float2 ml[kWaves][16];
+    float2 ml[kWaves][32];
 };
-constexpr int kShAhead = 3;  // operand fragments read ahead of their MFMAs (4 spill at two tiles)
+constexpr int kShAhead = 3;  // operand fragments read ahead of their MFMAs
 constexpr uint32_t kUnitLds = kBlockTok * kHeadDim * 2;
-constexpr int kSharedRowPad = kHeadDim + 4;  // floats between rows of a wave's O in LDS
-static_assert(16 * kSharedRowPad * 4 <= 2 * kUnitLds, "a wave's O fits its two units");
 
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -36,14 +34,15 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // One workgroup's chunk: blocks [b0, b0 + n_blk) of the node for members
 // [m0, m0 + members) of it (T tiles).
 struct SharedItem {
-    int kind, h, ck, n_blk, mb, members;
+    int kind, h, ck, n_blk, members;
     const int32_t* trow;  // of the chunk's first block
     int last;             // keys of the chunk's last block
+    uint32_t who[4];      // the members' entries, two a word
 };
 
 // T: 16-row tiles; PARTS: bf16 parts of a weight (1 for bf16 output, 3 = 24 bits for fp32 output)
 template <int T, int PARTS>
-__device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedItem& it, SharedSmem& sm) {
+__device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedItem& it, int seq_row, SharedSmem& sm) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q4 = lane >> 4, r16 = lane & 15;
@@ -57,15 +56,13 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
     const int g = r16 & 3;
     const float c = fabsf(a.scale_log2);
     const uint32_t qflip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-    int mem[T];
-#pragma unroll
-    for (int t = 0; t < T; t++) mem[t] = a.member[it.mb + min(4 * t + (r16 >> 2), it.members - 1)];
+    const auto entry = [&](int t) { return (((r16 & 8) ? it.who[2 * t + 1] : it.who[2 * t]) >> ((r16 & 4) * 4)) & 0xFFFF; };
     bf16x8_t qb[T][8];
     {
         u32x4 x[T][8];
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            const uint16_t* qr = a.q + ((size_t)(mem[t] & 63) * kQHeads + h * kGroup + g) * kHeadDim;
+            const uint16_t* qr = a.q + ((size_t)(entry(t) & 63) * kQHeads + h * kGroup + g) * kHeadDim;
 #pragma unroll
             for (int ks = 0; ks < 8; ks++) x[t][ks] = *reinterpret_cast<const u32x4*>(qr + 32 * ks + 8 * q4);
         }
@@ -107,31 +104,24 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
         for (int dt = 0; dt < 16; dt++) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // operand fragments within a unit: K (kt, ks = 4 hi + jj): ka[jj] + 256 hi + 8192 kt;
-    // V^T (dt, lo/hi): va[dt % 4] + vb[dt / 4] + 8192 (hi)
-    uint32_t ka[4], va[4], vb[4];
-#pragma unroll
-    for (int jj = 0; jj < 4; jj++) ka[jj] = ku + r16 * 512 + 16 * ((4 * jj + q4) ^ r16);
-    {
-        const int w = 4 * q4 + (r16 >> 2);  // V row % 16 of this lane; its swizzle takes chunk pair dt to dt ^ w
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            va[j] = vu + w * 512 + 32 * (j ^ (w & 3)) + 16 * ((r16 & 3) >> 1) + 8 * (r16 & 1);
-            vb[j] = 128 * (j ^ (w >> 2));
-        }
-    }
+    // operand fragments within a unit: K (kt, ks = 4 hi + jj): (ka ^ 64 jj) + 256 hi + 8192 kt;
+    // V^T (dt, lo/hi): (va ^ 32 dt) + 8192 (hi); the swizzles are in ka and va
+    const int vr = 4 * q4 + (r16 >> 2);  // V row % 16 of this lane
+    uint32_t ka = ku + r16 * 512 + 16 * (q4 ^ r16);
+    uint32_t va = vu + vr * (512 + 32) + 8 * (r16 & 3);
 
     for (int i = 0; i < n_my; i++) {
         const bool more = i + 1 < n_my;
         // keys of the block that exist (a node of one member may end inside a block)
         const int valid = base + i * step == it.n_blk - 1 ? it.last : kBlockTok;
+        asm volatile("" : "+v"(ka), "+v"(va));  // (the fragments' addresses are not kept over the loop)
         wait_vm<16>();  // K: the 16 copies after it are V's
         f32x4 st[T][2];
         {
             bf16x8_t kf[kShAhead];
             auto read = [&](int n) {
                 const int ks = n >> 1, kt = n & 1;
-                kf[n % kShAhead] = as_bf16x8(lds_load16(ka[ks & 3], 256 * (ks >> 2) + 8192 * kt));
+                kf[n % kShAhead] = as_bf16x8(lds_load16(ka ^ (64 * (ks & 3)), 256 * (ks >> 2) + 8192 * kt));
             };
 #pragma unroll
             for (int n = 0; n < kShAhead; n++) read(n);
@@ -220,7 +210,7 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
         {
             bf16x8_t vf[kShAhead];
             auto read = [&](int dt) {
-                const uint32_t at = va[dt & 3] + vb[dt >> 2];
+                const uint32_t at = va ^ (32 * dt);
                 const u32x2 lo = lds_load_tr16(at, 0), hi = lds_load_tr16(at, 8192);
                 vf[dt % kShAhead] = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
             };
@@ -247,82 +237,99 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
         wait_lds();
         if (more) issue(a.vpool, cbv, 6, i + 1, vu);
     }
+    int row[T];  // of the lane's partial
 #pragma unroll
-    for (int t = 0; t < T; t++) l[t] = sum_xor32(sum_xor16(l[t]));
+    for (int t = 0; t < T; t++) {
+        l[t] = sum_xor32(sum_xor16(l[t]));
+        const int e = entry(t), r0 = __builtin_amdgcn_ds_bpermute((e & 63) * 4, seq_row);  // lane s holds sequence s's
+        row[t] = (r0 + (e >> 6) + it.ck) * kQHeads + h * kGroup + g;
+    }
 
     if (it.kind == kSharedHeads) {
 #pragma unroll
         for (int t = 0; t < T; t++) {
             if (4 * t + (r16 >> 2) >= it.members) continue;
-            const size_t row = (size_t)(a.seq_row[mem[t] & 63] + (mem[t] >> 6) + it.ck) * kQHeads + h * kGroup + g;
-            float* acc = a.acc + row * kHeadDim + 4 * q4;
+            float* acc = a.acc + (size_t)row[t] * kHeadDim + 4 * q4;
 #pragma unroll
             for (int dt = 0; dt < 16; dt++) *reinterpret_cast<f32x4*>(acc + 16 * dt) = o[t][dt];
-            if (q4 == 0) *reinterpret_cast<float2*>(a.stats + row * 2) = make_float2(m_run[t], l[t]);
+            if (q4 == 0) *reinterpret_cast<float2*>(a.stats + (size_t)row[t] * 2) = make_float2(m_run[t], l[t]);
         }
         return;
     }
-    // fold the 4 waves' keys, tile by tile: O through LDS (each wave into its own units, which it alone read)
-    float* own = reinterpret_cast<float*>(sm.unit[2 * wave]);
+    // fold the 4 waves' keys: O through LDS (each wave into its own units, which it
+    // alone read), 16-B chunks swizzled by the row; then a wave takes a member
+    uint8_t* own = reinterpret_cast<uint8_t*>(sm.unit[2 * wave]);
 #pragma unroll
     for (int t = 0; t < T; t++) {
-        if (t > 0) __syncthreads();
 #pragma unroll
-        for (int dt = 0; dt < 16; dt++) *reinterpret_cast<f32x4*>(own + r16 * kSharedRowPad + 16 * dt + 4 * q4) = o[t][dt];
-        if (q4 == 0) sm.ml[wave][r16] = make_float2(m_run[t], l[t]);
-        __syncthreads();
-        for (int r = wave; r < min(16, (it.members - 4 * t) * kGroup); r += kWaves) {
+        for (int dt = 0; dt < 16; dt++)
+            *reinterpret_cast<f32x4*>(own + (16 * t + r16) * 1024 + (((4 * dt + q4) ^ r16) << 4)) = o[t][dt];
+        if (q4 == 0) sm.ml[wave][16 * t + r16] = make_float2(m_run[t], l[t]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        if (4 * t + wave >= it.members) break;  // uniform
+#pragma unroll
+        for (int rr = 0; rr < kGroup; rr++) {
+            const int r = kGroup * wave + rr;
             float2 ml[kWaves];
-            float m = kNegBig, lt = 0.f;
+            f32x4 x[kWaves];
 #pragma unroll
             for (int w = 0; w < kWaves; w++) {
-                ml[w] = sm.ml[w][r];
-                m = fmaxf(m, ml[w].x);
+                ml[w] = sm.ml[w][16 * t + r];
+                x[w] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(sm.unit[2 * w]) + (16 * t + r) * 1024 + ((lane ^ r) << 4));
             }
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            const float m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+            float lt = 0.f;
+            f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < kWaves; w++) {
                 const float f = fast_exp2(ml[w].x - m);
                 lt = fmaf(f, ml[w].y, lt);
-                x += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(sm.unit[2 * w]) + r * kSharedRowPad + lane * 4);
+                y += f * x[w];
             }
-            const int mr = __builtin_amdgcn_readlane(mem[t], r);  // lane r holds row r's member
-            const size_t row = (size_t)(a.seq_row[mr & 63] + (mr >> 6) + it.ck) * kQHeads + h * kGroup + (r & 3);
-            *reinterpret_cast<f32x4*>(a.acc + row * kHeadDim + lane * 4) = x;
-            if (lane == 0) *reinterpret_cast<float2*>(a.stats + row * 2) = make_float2(m, lt);
+            const size_t to = (size_t)__builtin_amdgcn_readlane(row[t], r);  // lane r holds row r's
+            *reinterpret_cast<f32x4*>(a.acc + to * kHeadDim + lane * 4) = y;
+            if (lane == 0) *reinterpret_cast<float2*>(a.stats + to * 2) = make_float2(m, lt);
         }
     }
 }
 
 template <int PARTS>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(SharedArgs a) {
-    __shared__ SharedSmem sm;
+    __shared__ __align__(1024) SharedSmem sm;  // (the XORs with a fragment's number need it)
     const int lane = threadIdx.x & 63;
     const int item = blockIdx.x;
-    // which node: every lane looks at two; both records are requested with their
-    // ends, so that one trip to the arguments gives all
-    const int e0 = a.item_end[lane], e1 = a.item_end[lane + 64];
-    const int4 n0 = *reinterpret_cast<const int4*>(&a.node[lane]), n1 = *reinterpret_cast<const int4*>(&a.node[lane + 64]);
-    const int c0 = __popcll(__builtin_amdgcn_ballot_w64(e0 <= item)), c1 = __popcll(__builtin_amdgcn_ballot_w64(e1 <= item));
-    const int node = c0 + c1, at = node & 63;
+    // one trip to the arguments: every lane asks for the ends and records of two
+    // nodes, 8 list entries and a sequence's first partial
+    int e0 = a.item_end[lane], e1 = a.item_end[lane + 64];
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    i32x4 n0 = *reinterpret_cast<const i32x4*>(&a.node[lane]), n1 = *reinterpret_cast<const i32x4*>(&a.node[lane + 64]);
+    i32x4 mw = *reinterpret_cast<const i32x4*>(&a.member[8 * lane]);
+    int seq_row = a.seq_row[lane];
+    asm volatile("" : "+v"(e0), "+v"(e1), "+v"(n0), "+v"(n1), "+v"(mw), "+v"(seq_row));  // all of it, here
+    const int node = __popcll(__builtin_amdgcn_ballot_w64(e0 <= item)) + __popcll(__builtin_amdgcn_ballot_w64(e1 <= item));
     if (node >= kSharedNodes) return;
-    const bool hi = node >= 64;
-    const int first = hi ? __builtin_amdgcn_readlane(n1.x, at) : __builtin_amdgcn_readlane(n0.x, at);
-    const uint32_t lw = hi ? __builtin_amdgcn_readlane(n1.y, at) : __builtin_amdgcn_readlane(n0.y, at);
-    const uint32_t sw = hi ? __builtin_amdgcn_readlane(n1.z, at) : __builtin_amdgcn_readlane(n0.z, at);
-    const int slot = hi ? __builtin_amdgcn_readlane(n1.w, at) : __builtin_amdgcn_readlane(n0.w, at);
+    const int at = node & 63;
+    const bool up = node >= 64;
+    const uint32_t w0 = up ? __builtin_amdgcn_readlane(n1.x, at) : __builtin_amdgcn_readlane(n0.x, at);
+    const uint32_t w1 = up ? __builtin_amdgcn_readlane(n1.y, at) : __builtin_amdgcn_readlane(n0.y, at);
+    const uint32_t w2 = up ? __builtin_amdgcn_readlane(n1.z, at) : __builtin_amdgcn_readlane(n0.z, at);
+    const int slot = up ? __builtin_amdgcn_readlane(n1.w, at) : __builtin_amdgcn_readlane(n0.w, at);
     const int begin = node == 0 ? 0 : node <= 64 ? __builtin_amdgcn_readlane(e0, node - 1) : __builtin_amdgcn_readlane(e1, node - 65);
-    const SharedShape sh = shared_shape(sw);
-    const int len = lw & ((1 << 26) - 1);
-    if (sh.members == 0) return;  // (behind the last node)
+    constexpr uint32_t kLow26 = (1u << 26) - 1;
+    const int first = w0 & kLow26, len = w1 & kLow26, chunk = w2 & 1023;
+    if (len == 0) return;  // (behind the last node)
+    const int all = (w2 >> 10 & 63) + 1;  // members of the node
     SharedItem it;
-    it.kind = sh.kind;
-    const int n_chunks = (len + sh.chunk - 1) / sh.chunk, units = it.kind == kSharedHeads ? n_chunks : n_chunks * kKvHeads;
-    const int groups = (sh.members + a.group - 1) / a.group;
+    it.kind = w0 >> 26;
+    const int n_chunks = (len + chunk - 1) / chunk, units = it.kind == kSharedHeads ? n_chunks : n_chunks * kKvHeads;
     int j = item - begin, grp = 0;
-    if (groups > 1) {
+    if (all > a.group) {
         // (the node starts on a multiple of 8; the groups of members that read the
         // same keys run on one XCD, workgroup number % 8, one after the other)
+        const int groups = (all + a.group - 1) / a.group;
         j = item - (begin + 7) / 8 * 8;
         if (j < 0) return;
         const int r = j >> 3;
@@ -332,19 +339,31 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (j >= units) return;  // (padding)
     it.h = it.kind == kSharedHeads ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : j % kKvHeads;
     it.ck = it.kind == kSharedHeads ? j : j / kKvHeads;
-    const int b0 = it.ck * sh.chunk;
-    it.n_blk = min(sh.chunk, len - b0);
-    it.last = b0 + it.n_blk == len ? (int)(lw >> 26) : kBlockTok;
-    it.mb = sh.member_begin + grp * a.group;
-    it.members = min(a.group, sh.members - grp * a.group);
+    const int b0 = it.ck * chunk;
+    it.n_blk = min(chunk, len - b0);
+    it.last = b0 + it.n_blk == len ? (int)(w1 >> 26) + 1 : kBlockTok;
+    it.members = min(a.group, all - grp * a.group);
     it.trow = a.table + (size_t)slot * a.table_stride + first + b0;
+    if (all == 1) {
+        it.who[0] = it.who[1] = it.who[2] = it.who[3] = (w2 >> 16) * 0x10001u;
+    } else {
+        const int e = (w2 >> 16) * 8 + grp * a.group, from = e >> 3;  // lane that holds them
+        it.who[0] = __builtin_amdgcn_readlane(mw.x, from);
+        it.who[1] = __builtin_amdgcn_readlane(mw.y, from);
+        it.who[2] = __builtin_amdgcn_readlane(mw.z, from);
+        it.who[3] = __builtin_amdgcn_readlane(mw.w, from);
+        if (e & 4) {  // (groups of 4)
+            it.who[0] = it.who[2];
+            it.who[1] = it.who[3];
+        }
+    }
     if constexpr (PARTS == 1) {
         if (it.members > 4) {
-            shared_item<2, PARTS>(a, it, sm);
+            shared_item<2, PARTS>(a, it, seq_row, sm);
             return;
         }
     }
-    shared_item<1, PARTS>(a, it, sm);
+    shared_item<1, PARTS>(a, it, seq_row, sm);
 }
 
 // One workgroup folds a (sequence, q head): each wave every 4th partial, its

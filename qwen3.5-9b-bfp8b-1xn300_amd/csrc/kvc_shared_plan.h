@@ -18,6 +18,7 @@ namespace kvc {
 
 struct SharedPlan {
     int32_t n_nodes = 0, n_members = 0;
+    int32_t listed = 0;                // of them in nodes of several, each filled up to a multiple of 8
     int32_t n_items = 0;               // workgroups
     int32_t parts = 0;                 // partials per q head, of all sequences
     int32_t path = 0;                  // most of them of one sequence
@@ -28,8 +29,8 @@ struct SharedPlan {
     uint16_t chunk[kSharedNodes];      // blocks per workgroup
     uint16_t member_begin[kSharedNodes + 1];
     uint8_t kind[kSharedNodes];
-    uint8_t member[kSharedMembers];    // index of the sequence in the launch
-    uint16_t part[kSharedMembers];     // its first partial of this node
+    uint8_t member[kSharedMembers + kMaxBatch];  // index of the sequence in the launch
+    uint16_t part[kSharedMembers + kMaxBatch];   // its first partial of this node
     int32_t seq_row[kMaxBatch];        // its first partial in the workspace
     int32_t seq_parts[kMaxBatch];
 };
@@ -41,13 +42,12 @@ class SharedPlanner {
   public:
     // tab[i]: block ids of sequence i; keys[i]: keys attended (0 allowed)
     SharedPlanner(const int32_t* const* tab, const int32_t* keys, int32_t n, SharedPlan& p) : tab_(tab), keys_(keys), p_(p) {
-        p_.n_nodes = p_.n_members = 0;
+        p_.n_nodes = p_.n_members = p_.listed = 0;
         p_.blocks = p_.blocks_apart = 0;
         for (int32_t i = 0; i < n; i++) {
             order_[i] = (uint8_t)i;
             p_.blocks_apart += total(i);
         }
-        left_ = n;
         walk(0, n, 0, 0);
         p_.member_begin[p_.n_nodes] = (uint16_t)p_.n_members;
     }
@@ -71,21 +71,20 @@ class SharedPlanner {
         p_.member_begin[k] = (uint16_t)p_.n_members;
         for (int32_t i = lo; i < hi; i++) p_.member[p_.n_members++] = order_[i];
         p_.blocks += to - from;
+        if (hi - lo > 1) p_.listed += (hi - lo + 7) / 8 * 8;
     }
 
     // order_[lo, hi) run together up to block `at`; their blocks from `from` on
     // (<= at) have no node yet.
     void walk(int32_t lo, int32_t hi, int32_t from, int32_t at) {
         if (hi - lo == 1) {
-            left_--;
             if (total(order_[lo]) > from) emit(lo, hi, from, total(order_[lo]));
             return;
         }
         int32_t end = full(order_[lo]);
         for (int32_t i = lo + 1; i < hi; i++)
             end = common(order_[lo], order_[i], at, std::min(end, full(order_[i])));
-        // (a leaf for each sequence that has none yet still has to fit)
-        if ((int64_t)(end - from) * (hi - lo - 1) >= kSharedMinSaved && p_.n_members + (hi - lo) + left_ <= kSharedMembers) {
+        if ((int64_t)(end - from) * (hi - lo - 1) >= kSharedMinSaved && p_.listed + (hi - lo + 7) / 8 * 8 <= kSharedMembers) {
             emit(lo, hi, from, end);
             from = end;
         }
@@ -108,7 +107,6 @@ class SharedPlanner {
     const int32_t* keys_;
     SharedPlan& p_;
     uint8_t order_[kMaxBatch];
-    int32_t left_ = 0;  // sequences without a leaf
 };
 
 // Workgroups of the nodes, `group` members each at most, where a wave takes up to w blocks of a node: a node of
