@@ -1435,7 +1435,6 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
                          const void* k_new, const void* v_new, const void* gate, void* out, int32_t out_dtype,
                          float scale, bool launch, void* stream) {
     const bool q8 = any_q8(c, seqs + i0, n);
-    const int32_t group = shared_group(out_dtype == KVC_DTYPE_F32);
     SharedPlan p;
     const int32_t* tab[kMaxBatch];
     int32_t keys[kMaxBatch];
@@ -1445,7 +1444,7 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
             tab[j] = s.blocks.data();
             keys[j] = s.len + s.pending - (k_new ? 1 : 0);
         }
-        if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, group, p);
+        if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, p);
     }
     if (!launch || q8 || !shared_pays(p)) {
         DecodeArgs a;
@@ -1488,7 +1487,6 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
     f.gate_ref = !(c->cfg.flags & KVC_FLAG_EXACT_MATH);
     a.table_stride = f.table_stride = c->max_blocks;
     f.n_seqs = n;
-    a.group = group;
     for (int32_t j = 0; j < n; j++) {
         a.seq_row[j] = p.seq_row[j];
         f.seq[j] = {p.seq_row[j], p.seq_parts[j], seqs[i0 + j], keys[j]};
@@ -1501,10 +1499,10 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
         const int32_t last = std::min(keys[s] - (p.first[k] + p.len[k] - 1) * kBlockTok, kBlockTok);
         const auto entry = [&](int32_t i) { return (uint16_t)(p.member[i] | p.part[i] << 6); };
         a.node[k] = {(uint32_t)p.first[k] | (uint32_t)p.kind[k] << 26, (uint32_t)p.len[k] | (uint32_t)(last - 1) << 26,
-                     (uint32_t)p.chunk[k] | (uint32_t)(members - 1) << 10 | (members == 1 ? entry(mb) : (uint32_t)listed / 8) << 16,
+                     (uint32_t)p.chunk[k] | (uint32_t)(members - 1) << 10 | (members == 1 ? entry(mb) : (uint32_t)listed / kSharedSeqs) << 16,
                      seqs[i0 + s]};
         if (members == 1) continue;
-        for (int32_t i = 0; i < (members + 7) / 8 * 8; i++) a.member[listed++] = entry(mb + std::min(i, members - 1));
+        for (int32_t i = 0; i < (members + kSharedSeqs - 1) / kSharedSeqs * kSharedSeqs; i++) a.member[listed++] = entry(mb + std::min(i, members - 1));
     }
     int e = launch_shared(a, p.n_items, f, stream);
     return e ? hip_err((hipError_t)e, "decode launch (shared blocks)") : KVC_OK;

@@ -534,20 +534,18 @@ struct BlockCopyArgs {
 };
 
 // ---- decode over shared blocks (kvc_shared_plan.h) ------------------------
-// A node's key chunk is a workgroup's work, for up to shared_group members and one
+// A node's key chunk is a workgroup's work, for up to kSharedSeqs members and one
 // kv head (or all of them).  It leaves a partial per (member, q head): the
 // unnormalised output [256] and (max, sum), in the workspace, where a sequence's
 // partials stand in a row: partial p of sequence s and q head h is row
 // (seq_row[s] + p) * 16 + h.
 constexpr int kSharedNodes = 128;
 constexpr int kSharedMembers = 512;
-// 4 members are a tile of 16 rows: two tiles fill a wave's registers with weights in
-// one bf16 part, one with weights in three
-constexpr int shared_group(bool f32) { return f32 ? 4 : 8; }
-constexpr int kSharedWaveBlocks = 64;  // blocks whose ids a wave holds
+constexpr int kSharedSeqs = 8;         // 4 members are a tile of 16 rows; two tiles fill a wave's registers
+constexpr int kSharedWaveBlocks = 32;  // blocks whose ids a wave holds, one for each half
 constexpr int kSharedPath = 512;       // partials of one (sequence, q head)
 // how the 4 waves of a workgroup split it
-enum { kSharedKeys = 0,    // one kv head: a wave takes every 4th block
+enum { kSharedKeys = 0,    // one kv head: a wave takes every 4th half block
        kSharedHeads = 1 }; // all kv heads: a wave takes one
 constexpr int kSharedMaxParts = (int)(kPartBytes / ((kHeadDim + 2) * 4 * kQHeads));  // over all sequences
 
@@ -571,8 +569,7 @@ struct SharedArgs {
     float* stats;           // [row][max, sum]
     float scale_log2;
     int32_t table_stride;
-    int32_t group;                    // members of a workgroup
-    int32_t pad;
+    int32_t pad[2];
     int32_t item_end[kSharedNodes];   // INT32_MAX behind the last node
     SharedNode node[kSharedNodes];
     int32_t seq_row[kMaxBatch];

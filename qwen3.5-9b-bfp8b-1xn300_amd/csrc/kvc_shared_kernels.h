@@ -4,26 +4,30 @@
 // For every trie node (kvc_shared_plan.h) and kv head, the members' query rows
 // (4 q heads each, 4 members to a tile of 16 rows) attend to the node's keys in
 // one product per tile:
-//   S^T[32 keys x 16 rows]  = K[keys x 256] . Q^T        (v_mfma_f32_16x16x32_bf16)
+//   S^T[16 keys x 16 rows]  = K[keys x 256] . Q^T        (v_mfma_f32_16x16x32_bf16)
 //   P^T = 2^(S^T - m), m the running maximum of the row
-//   O^T[256 x 16 rows]     += V^T[256 x keys] . P^T
+//   O^T[256 x 16 rows]     += V^T[256 x keys] . P^T      (v_mfma_f32_16x16x16_bf16)
 // in the operand layouts of the prefill kernel: a lane stays on one row in both
 // products, P^T leaves the accumulator in operand order, and V^T fragments come
-// from LDS through the transposing read.  Every wave streams blocks of its own
-// through LDS units of its own, without barriers, for all tiles of its members, so
-// a K or V fragment is read from LDS once for up to 32 rows.  A second launch folds
-// the partials (m, l, O) of a row: O = sum 2^(m_p - M) O_p, l likewise, and divides.
+// from LDS through the transposing read.  Every wave streams half blocks (16 keys)
+// of its own through LDS units of its own, without barriers, for all tiles of its
+// members, so a K or V fragment is read from LDS once for up to 32 rows, and two
+// workgroups fit on a CU: while waves of one wait for a copy or fold, the other's
+// run.  A second launch folds the partials (m, l, O) of a row: O = sum 2^(m_p - M)
+// O_p, l likewise, and divides.
 #pragma once
 
 namespace kvc {
 
+constexpr int kSharedTok = 16;  // keys of a unit: half a block
 struct SharedSmem {
     // (K, V) units of each wave: rows of 512 B, 16-B chunks swizzled by the row (kswz, vswz)
-    uint16_t unit[2 * kWaves][kBlockTok * kHeadDim];
-    float2 ml[kWaves][32];
+    uint16_t unit[2 * kWaves][kSharedTok * kHeadDim];
+    float2 ml[kWaves][16];
 };
 constexpr int kShAhead = 3;  // operand fragments read ahead of their MFMAs
-constexpr uint32_t kUnitLds = kBlockTok * kHeadDim * 2;
+constexpr uint32_t kUnitLds = kSharedTok * kHeadDim * 2;
+typedef short bf16x4_t __attribute__((ext_vector_type(4)));  // (the 16x16x16 product's operand type)
 
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -31,12 +35,11 @@ __device__ __forceinline__ void wait_vm() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// One workgroup's chunk: blocks [b0, b0 + n_blk) of the node for members
-// [m0, m0 + members) of it (T tiles).
+// One workgroup's work: a chunk of a node for up to kSharedSeqs of its members.
 struct SharedItem {
-    int kind, h, ck, n_blk, members;
-    const int32_t* trow;  // of the chunk's first block
-    int last;             // keys of the chunk's last block
+    int kind, h, ck, members;
+    int keys;             // of the chunk
+    const int32_t* trow;  // of its first block
     uint32_t who[4];      // the members' entries, two a word
 };
 
@@ -48,9 +51,10 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
     const int q4 = lane >> 4, r16 = lane & 15;
     const int step = it.kind == kSharedKeys ? kWaves : 1, base = it.kind == kSharedKeys ? wave : 0;
     const int h = it.h;
-    // block ids: lane i holds this wave's i-th block
-    const int n_my = it.kind == kSharedKeys ? (it.n_blk - wave + kWaves - 1) / kWaves : it.n_blk;
-    const int idv = lane < n_my ? it.trow[base + lane * step] : 0;
+    // block ids: lane i holds that of this wave's i-th half block
+    const int n_half = (it.keys + kSharedTok - 1) / kSharedTok;
+    const int n_my = it.kind == kSharedKeys ? (n_half - wave + kWaves - 1) / kWaves : n_half;
+    const int idv = lane < n_my ? it.trow[(base + lane * step) >> 1] : 0;
 
     // this lane's rows: member 4 t + r16 / 4, q head r16 % 4
     const int g = r16 & 3;
@@ -84,9 +88,10 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
     const uint32_t cbv = (((lane & 31) ^ ((lane >> 5) << 1)) << 4) + (lane >> 5) * 512;
     auto issue = [&](const uint16_t* pool, uint32_t cb, int jsh, int i, uint32_t lds) {
         const int id = __builtin_amdgcn_readlane(idv, i);
-        const uint16_t* src = pool + ((size_t)id * kKvHeads + h) * (kBlockTok * kHeadDim);
+        const int half = (base + i * step) & 1;
+        const uint16_t* src = pool + (((size_t)id * kKvHeads + h) * kBlockTok + half * kSharedTok) * kHeadDim;
 #pragma unroll
-        for (int p = 0; p < 16; p++) lds_dma16s(src + p * 2 * kHeadDim, cb ^ ((uint32_t)(p & 7) << jsh), lds + p * 1024);
+        for (int p = 0; p < 8; p++) lds_dma16s(src + p * 2 * kHeadDim, cb ^ ((uint32_t)p << jsh), lds + p * 1024);
     };
     const uint32_t ku = lds_addr(&sm.unit[2 * wave][0]), vu = ku + kUnitLds;
     if (n_my > 0) {
@@ -104,42 +109,38 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
         for (int dt = 0; dt < 16; dt++) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // operand fragments within a unit: K (kt, ks = 4 hi + jj): (ka ^ 64 jj) + 256 hi + 8192 kt;
-    // V^T (dt, lo/hi): (va ^ 32 dt) + 8192 (hi); the swizzles are in ka and va
+    // operand fragments within a unit: K (ks = 4 hi + jj): (ka ^ 64 jj) + 256 hi;
+    // V^T (dt): va ^ 32 dt; the swizzles are in ka and va
     const int vr = 4 * q4 + (r16 >> 2);  // V row % 16 of this lane
     uint32_t ka = ku + r16 * 512 + 16 * (q4 ^ r16);
     uint32_t va = vu + vr * (512 + 32) + 8 * (r16 & 3);
 
     for (int i = 0; i < n_my; i++) {
         const bool more = i + 1 < n_my;
-        // keys of the block that exist (a node of one member may end inside a block)
-        const int valid = base + i * step == it.n_blk - 1 ? it.last : kBlockTok;
+        const int valid = it.keys - (base + i * step) * kSharedTok;  // keys from the half block's first on
         asm volatile("" : "+v"(ka), "+v"(va));  // (the fragments' addresses are not kept over the loop)
-        wait_vm<16>();  // K: the 16 copies after it are V's
-        f32x4 st[T][2];
+        wait_vm<8>();  // K: the 8 copies after it are V's
+        f32x4 st[T];
         {
             bf16x8_t kf[kShAhead];
-            auto read = [&](int n) {
-                const int ks = n >> 1, kt = n & 1;
-                kf[n % kShAhead] = as_bf16x8(lds_load16(ka ^ (64 * (ks & 3)), 256 * (ks >> 2) + 8192 * kt));
+            auto read = [&](int ks) {
+                kf[ks % kShAhead] = as_bf16x8(lds_load16(ka ^ (64 * (ks & 3)), 256 * (ks >> 2)));
             };
 #pragma unroll
             for (int n = 0; n < kShAhead; n++) read(n);
 #pragma unroll
-            for (int n = 0; n < 16; n++) {
-                const int ks = n >> 1, kt = n & 1;
-                const bf16x8_t x = kf[n % kShAhead];
-                if (n + kShAhead < 16) read(n + kShAhead);
+            for (int ks = 0; ks < 8; ks++) {
+                const bf16x8_t x = kf[ks % kShAhead];
+                if (ks + kShAhead < 8) read(ks + kShAhead);
 #pragma unroll
                 for (int t = 0; t < T; t++)
-                    st[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qb[t][ks],
-                                                                       ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : st[t][kt], 0, 0, 0);
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qb[t][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : st[t], 0, 0, 0);
             }
         }
         __builtin_amdgcn_sched_group_barrier(kSgDsRead, kShAhead, 0);
 #pragma unroll
-        for (int n = 0; n < 16; n++) {
-            if (n + kShAhead < 16) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 1, 0);
+        for (int n = 0; n < 8; n++) {
+            if (n + kShAhead < 8) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 1, 0);
             __builtin_amdgcn_sched_group_barrier(kSgMfma, T, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -147,90 +148,74 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
         if (more) issue(a.kpool, cbk, 5, i + 1, ku);
         // weights of the scores
         float cs = c;
-        if (valid < kBlockTok) {  // (one member, one tile)
+        if (valid < kSharedTok) {  // (one member, one tile)
             asm volatile("");
             cs = 1.f;
 #pragma unroll
             for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) st[t][kt][e] = 16 * kt + 4 * q4 + e < valid ? st[t][kt][e] * c : kNegBig;
+                for (int e = 0; e < 4; e++) st[t][e] = 4 * q4 + e < valid ? st[t][e] * c : kNegBig;
         }
-        bf16x8_t pw[T][PARTS];
+        bf16x4_t pw[T][PARTS];
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            float mx = kNegBig;
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, st[t][kt][e]);
+            const float mx = fmaxf(fmaxf(st[t][0], st[t][1]), fmaxf(st[t][2], st[t][3]));
             const float mt = max_xor32(max_xor16(mx)) * cs;
             const bool up = mt > m_run[t] + kRescaleSlack;
             if (__builtin_amdgcn_ballot_w64(up) != 0) {  // uniform; rows that keep their maximum scale by 1
                 const float cr = up ? fast_exp2(m_run[t] - mt) : 1.f;
                 m_run[t] = up ? mt : m_run[t];
-                // (the scaled values re-enter the accumulators through an MFMA with
-                // zero operands, which keeps them in the MFMA register class)
-                const bf16x8_t z8 = {};
 #pragma unroll
-                for (int dt = 0; dt < 16; dt++)
-                    o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(z8, z8, o[t][dt] * cr, 0, 0, 0);
+                for (int dt = 0; dt < 16; dt++) o[t][dt] *= cr;
                 l[t] *= cr;
             }
             const float nm = -m_run[t];
-            u32x4 w[PARTS];
+            u32x2 w[PARTS];
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const float x = fast_exp2(fmaf(st[t][kt][2 * e], cs, nm)), y = fast_exp2(fmaf(st[t][kt][2 * e + 1], cs, nm));
-                    w[0][2 * kt + e] = cvt_pk_bf16(x, y);
-                    if constexpr (PARTS == 1) {
-                        l[t] += bf16lo(w[0][2 * kt + e]) + bf16hi(w[0][2 * kt + e]);  // what the product uses
-                    } else {
-                        l[t] += x + y;
-                        const float x1 = x - bf16lo(w[0][2 * kt + e]), y1 = y - bf16hi(w[0][2 * kt + e]);  // exact
-                        w[1][2 * kt + e] = cvt_pk_bf16(x1, y1);
-                        w[2][2 * kt + e] = cvt_pk_bf16(x1 - bf16lo(w[1][2 * kt + e]), y1 - bf16hi(w[1][2 * kt + e]));
-                    }
+            for (int e = 0; e < 2; e++) {
+                const float x = fast_exp2(fmaf(st[t][2 * e], cs, nm)), y = fast_exp2(fmaf(st[t][2 * e + 1], cs, nm));
+                w[0][e] = cvt_pk_bf16(x, y);
+                if constexpr (PARTS == 1) {
+                    l[t] += bf16lo(w[0][e]) + bf16hi(w[0][e]);  // what the product uses
+                } else {
+                    l[t] += x + y;
+                    const float x1 = x - bf16lo(w[0][e]), y1 = y - bf16hi(w[0][e]);  // exact
+                    w[1][e] = cvt_pk_bf16(x1, y1);
+                    w[2][e] = cvt_pk_bf16(x1 - bf16lo(w[1][e]), y1 - bf16hi(w[1][e]));
                 }
+            }
 #pragma unroll
-            for (int p = 0; p < PARTS; p++) pw[t][p] = as_bf16x8(w[p]);
+            for (int p = 0; p < PARTS; p++) pw[t][p] = __builtin_bit_cast(bf16x4_t, w[p]);
         }
         if (more)
-            wait_vm<16>();
+            wait_vm<8>();
         else
             wait_vm<0>();
-        if (valid < kBlockTok) {  // rows that do not exist may hold anything: 0 times it must be 0
-            for (int r = valid; r < kBlockTok; r++)
+        if (valid < kSharedTok) {  // rows that do not exist may hold anything: 0 times it must be 0
+            for (int r = valid; r < kSharedTok; r++)
                 *reinterpret_cast<u32x2*>(&sm.unit[2 * wave + 1][r * kHeadDim + lane * 4]) = u32x2{0u, 0u};
             wait_lds();
         }
         {
-            bf16x8_t vf[kShAhead];
-            auto read = [&](int dt) {
-                const uint32_t at = va ^ (32 * dt);
-                const u32x2 lo = lds_load_tr16(at, 0), hi = lds_load_tr16(at, 8192);
-                vf[dt % kShAhead] = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
-            };
+            bf16x4_t vf[kShAhead];
+            auto read = [&](int dt) { vf[dt % kShAhead] = __builtin_bit_cast(bf16x4_t, lds_load_tr16(va ^ (32 * dt), 0)); };
 #pragma unroll
             for (int n = 0; n < kShAhead; n++) read(n);
 #pragma unroll
             for (int dt = 0; dt < 16; dt++) {
-                const bf16x8_t x = vf[dt % kShAhead];
+                const bf16x4_t x = vf[dt % kShAhead];
                 if (dt + kShAhead < 16) read(dt + kShAhead);
 #pragma unroll
                 for (int t = 0; t < T; t++)
 #pragma unroll
                     for (int p = 0; p < PARTS; p++)
-                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pw[t][p], o[t][dt], 0, 0, 0);
+                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x, pw[t][p], o[t][dt], 0, 0, 0);
             }
         }
-        __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2 * kShAhead, 1);
+        __builtin_amdgcn_sched_group_barrier(kSgDsRead, kShAhead, 1);
 #pragma unroll
         for (int n = 0; n < 16; n++) {
-            if (n + kShAhead < 16) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2, 1);
+            if (n + kShAhead < 16) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 1, 1);
             __builtin_amdgcn_sched_group_barrier(kSgMfma, T * PARTS, 1);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -256,20 +241,19 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
         }
         return;
     }
-    // fold the 4 waves' keys: O through LDS (each wave into its own units, which it
-    // alone read), 16-B chunks swizzled by the row; then a wave takes a member
+    // fold the 4 waves' keys, tile by tile: O through LDS (each wave into its own
+    // units, which it alone read), 16-B chunks swizzled by the row; then a wave takes
+    // a member
     uint8_t* own = reinterpret_cast<uint8_t*>(sm.unit[2 * wave]);
 #pragma unroll
     for (int t = 0; t < T; t++) {
+        if (t > 0) __syncthreads();
 #pragma unroll
         for (int dt = 0; dt < 16; dt++)
-            *reinterpret_cast<f32x4*>(own + (16 * t + r16) * 1024 + (((4 * dt + q4) ^ r16) << 4)) = o[t][dt];
-        if (q4 == 0) sm.ml[wave][16 * t + r16] = make_float2(m_run[t], l[t]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < T; t++) {
-        if (4 * t + wave >= it.members) break;  // uniform
+            *reinterpret_cast<f32x4*>(own + r16 * 1024 + (((4 * dt + q4) ^ r16) << 4)) = o[t][dt];
+        if (q4 == 0) sm.ml[wave][r16] = make_float2(m_run[t], l[t]);
+        __syncthreads();
+        if (4 * t + wave >= it.members) continue;  // uniform
 #pragma unroll
         for (int rr = 0; rr < kGroup; rr++) {
             const int r = kGroup * wave + rr;
@@ -277,8 +261,8 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
             f32x4 x[kWaves];
 #pragma unroll
             for (int w = 0; w < kWaves; w++) {
-                ml[w] = sm.ml[w][16 * t + r];
-                x[w] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(sm.unit[2 * w]) + (16 * t + r) * 1024 + ((lane ^ r) << 4));
+                ml[w] = sm.ml[w][r];
+                x[w] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(sm.unit[2 * w]) + r * 1024 + ((lane ^ r) << 4));
             }
             const float m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
             float lt = 0.f;
@@ -326,10 +310,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     it.kind = w0 >> 26;
     const int n_chunks = (len + chunk - 1) / chunk, units = it.kind == kSharedHeads ? n_chunks : n_chunks * kKvHeads;
     int j = item - begin, grp = 0;
-    if (all > a.group) {
+    if (all > kSharedSeqs) {
         // (the node starts on a multiple of 8; the groups of members that read the
         // same keys run on one XCD, workgroup number % 8, one after the other)
-        const int groups = (all + a.group - 1) / a.group;
+        const int groups = (all + kSharedSeqs - 1) / kSharedSeqs;
         j = item - (begin + 7) / 8 * 8;
         if (j < 0) return;
         const int r = j >> 3;
@@ -340,30 +324,23 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     it.h = it.kind == kSharedHeads ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : j % kKvHeads;
     it.ck = it.kind == kSharedHeads ? j : j / kKvHeads;
     const int b0 = it.ck * chunk;
-    it.n_blk = min(chunk, len - b0);
-    it.last = b0 + it.n_blk == len ? (int)(w1 >> 26) + 1 : kBlockTok;
-    it.members = min(a.group, all - grp * a.group);
+    const int n_blk = min(chunk, len - b0);
+    it.keys = n_blk * kBlockTok - (b0 + n_blk == len ? kBlockTok - 1 - (int)(w1 >> 26) : 0);
+    it.members = min(kSharedSeqs, all - grp * kSharedSeqs);
     it.trow = a.table + (size_t)slot * a.table_stride + first + b0;
     if (all == 1) {
         it.who[0] = it.who[1] = it.who[2] = it.who[3] = (w2 >> 16) * 0x10001u;
     } else {
-        const int e = (w2 >> 16) * 8 + grp * a.group, from = e >> 3;  // lane that holds them
+        const int from = (w2 >> 16) + grp;  // lane that holds them
         it.who[0] = __builtin_amdgcn_readlane(mw.x, from);
         it.who[1] = __builtin_amdgcn_readlane(mw.y, from);
         it.who[2] = __builtin_amdgcn_readlane(mw.z, from);
         it.who[3] = __builtin_amdgcn_readlane(mw.w, from);
-        if (e & 4) {  // (groups of 4)
-            it.who[0] = it.who[2];
-            it.who[1] = it.who[3];
-        }
     }
-    if constexpr (PARTS == 1) {
-        if (it.members > 4) {
-            shared_item<2, PARTS>(a, it, seq_row, sm);
-            return;
-        }
-    }
-    shared_item<1, PARTS>(a, it, seq_row, sm);
+    if (it.members > 4)
+        shared_item<2, PARTS>(a, it, seq_row, sm);
+    else
+        shared_item<1, PARTS>(a, it, seq_row, sm);
 }
 
 // One workgroup folds a (sequence, q head): each wave every 4th partial, its

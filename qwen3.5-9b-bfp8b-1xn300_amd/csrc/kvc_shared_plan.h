@@ -71,7 +71,7 @@ class SharedPlanner {
         p_.member_begin[k] = (uint16_t)p_.n_members;
         for (int32_t i = lo; i < hi; i++) p_.member[p_.n_members++] = order_[i];
         p_.blocks += to - from;
-        if (hi - lo > 1) p_.listed += (hi - lo + 7) / 8 * 8;
+        if (hi - lo > 1) p_.listed += (hi - lo + kSharedSeqs - 1) / kSharedSeqs * kSharedSeqs;
     }
 
     // order_[lo, hi) run together up to block `at`; their blocks from `from` on
@@ -84,7 +84,7 @@ class SharedPlanner {
         int32_t end = full(order_[lo]);
         for (int32_t i = lo + 1; i < hi; i++)
             end = common(order_[lo], order_[i], at, std::min(end, full(order_[i])));
-        if ((int64_t)(end - from) * (hi - lo - 1) >= kSharedMinSaved && p_.listed + (hi - lo + 7) / 8 * 8 <= kSharedMembers) {
+        if ((int64_t)(end - from) * (hi - lo - 1) >= kSharedMinSaved && p_.listed + (hi - lo + kSharedSeqs - 1) / kSharedSeqs * kSharedSeqs <= kSharedMembers) {
             emit(lo, hi, from, end);
             from = end;
         }
@@ -109,13 +109,15 @@ class SharedPlanner {
     uint8_t order_[kMaxBatch];
 };
 
-// Workgroups of the nodes, `group` members each at most, where a wave takes up to w blocks of a node: a node of
+inline int32_t shared_groups(int32_t members) { return (members + kSharedSeqs - 1) / kSharedSeqs; }
+
+// Workgroups of the nodes, where a wave takes up to w blocks of a node: a node of
 // at most w blocks goes to workgroups that take all kv heads.
-inline void shared_items(SharedPlan& p, int32_t w, int32_t n, int32_t group) {
+inline void shared_items(SharedPlan& p, int32_t w, int32_t n) {
     for (int32_t i = 0; i < n; i++) p.seq_parts[i] = 0;
     int64_t items = 0;
     for (int32_t k = 0; k < p.n_nodes; k++) {
-        const int32_t members = p.member_begin[k + 1] - p.member_begin[k], groups = (members + group - 1) / group;
+        const int32_t members = p.member_begin[k + 1] - p.member_begin[k], groups = shared_groups(members);
         p.kind[k] = p.len[k] <= w ? kSharedHeads : kSharedKeys;
         const int32_t chunk = p.kind[k] == kSharedHeads ? p.len[k] : 4 * w;
         const int32_t n_chunks = (p.len[k] + chunk - 1) / chunk, units = n_chunks * (p.kind[k] == kSharedHeads ? 1 : kKvHeads);
@@ -146,18 +148,17 @@ inline bool shared_pays(const SharedPlan& p) {
     return p.path <= kSharedPath && p.parts <= kSharedMaxParts && p.blocks_apart - p.blocks >= 16;
 }
 
-// The work of a launch of n sequences (n <= kMaxBatch), `group` members a
-// workgroup; caller_chunk > 0 is a chunk length that the caller set.
-inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, int32_t group,
-                        SharedPlan& p) {
+// The work of a launch of n sequences (n <= kMaxBatch): caller_chunk > 0 is a
+// chunk length that the caller set.
+inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, SharedPlan& p) {
     SharedPlanner(tab, keys, n, p);
     int64_t work = 0;
     for (int32_t k = 0; k < p.n_nodes; k++)
-        work += (int64_t)p.len[k] * ((p.member_begin[k + 1] - p.member_begin[k] + group - 1) / group);
+        work += (int64_t)p.len[k] * shared_groups(p.member_begin[k + 1] - p.member_begin[k]);
     int32_t w = caller_chunk > 0 ? (std::min(caller_chunk, 4 * kSharedWaveBlocks) + 3) / 4
                                  : (int32_t)std::min<int64_t>(kSharedWaveBlocks, std::max<int64_t>(1, (work + 255) / 256));
     for (;;) {
-        shared_items(p, w, n, group);
+        shared_items(p, w, n);
         if ((p.path <= kSharedPath && p.parts <= kSharedMaxParts) || w >= kSharedWaveBlocks) break;
         w = std::min(2 * w, kSharedWaveBlocks);
     }

@@ -13,18 +13,18 @@ import pytest
 CSRC = Path(__file__).resolve().parents[1] / "qwen3.5-9b-bfp8b-1xn300_amd" / "csrc"
 CXX = shutil.which("g++")
 pytestmark = pytest.mark.skipif(CXX is None, reason="needs g++")
-BT, HEADS = 32, 4
+BT, HEADS, SEQS = 32, 4, 8
 KEYS, ALL_HEADS = 0, 1  # kinds
 
-# stdin: launches as "n chunk group", then per sequence "keys nblk id id ..."; stdout: the plan
+# stdin: launches as "n chunk", then per sequence "keys nblk id id ..."; stdout: the plan
 PROGRAM = r"""
 #include <cstdio>
 #include <iostream>
 #include <vector>
 #include "kvc_shared_plan.h"
 int main() {
-    int n, chunk, group;
-    while (std::cin >> n >> chunk >> group) {
+    int n, chunk;
+    while (std::cin >> n >> chunk) {
         std::vector<std::vector<int32_t>> t(n);
         std::vector<int32_t> keys(n);
         std::vector<const int32_t*> tab(n);
@@ -36,7 +36,7 @@ int main() {
             tab[i] = t[i].data();
         }
         kvc::SharedPlan p;
-        kvc::shared_plan(tab.data(), keys.data(), n, chunk, group, p);
+        kvc::shared_plan(tab.data(), keys.data(), n, chunk, p);
         std::printf("%d %d %d %d %lld %lld %d\n", p.n_nodes, p.n_items, p.parts, p.path, (long long)p.blocks,
                     (long long)p.blocks_apart, (int)kvc::shared_pays(p));
         for (int k = 0; k < p.n_nodes; k++) {
@@ -58,9 +58,9 @@ def plans(tmp_path_factory):
                     "-fno-sanitize-recover=undefined", f"-I{CSRC}", str(d / "plan.cpp"), "-o", str(d / "plan")], check=True)
 
     def run(launches):
-        """launches: (chunk, members of a workgroup, [(keys, table), ...])"""
-        text = "\n".join("\n".join([f"{len(seqs)} {chunk} {group}"] + [" ".join(map(str, (k, len(t), *t))) for k, t in seqs])
-                         for chunk, group, seqs in launches)
+        """launches: (chunk, [(keys, table), ...])"""
+        text = "\n".join("\n".join([f"{len(seqs)} {chunk}"] + [" ".join(map(str, (k, len(t), *t))) for k, t in seqs])
+                         for chunk, seqs in launches)
         out = subprocess.run([str(d / "plan")], input=text, capture_output=True, text=True, check=True).stdout
         lines = iter(out.splitlines())
         got = []
@@ -101,7 +101,7 @@ def tree(rng, n, depth_blocks, ids):
     return seqs
 
 
-def check(head, nodes, group, seqs):
+def check(head, nodes, seqs):
     path = {i: [] for i in range(len(seqs))}
     used = set()  # partials
     for x in nodes:
@@ -110,7 +110,7 @@ def check(head, nodes, group, seqs):
         units = chunks * (1 if x["kind"] == ALL_HEADS else HEADS)
         # the kernel's reading of its item number
         seen = set()
-        groups = -(-len(x["members"]) // group)
+        groups = -(-len(x["members"]) // SEQS)
         begin = 0 if x is nodes[0] else nodes[nodes.index(x) - 1]["end"]
         for item in range(begin, x["end"]):
             j, grp = item - begin, 0
@@ -124,7 +124,7 @@ def check(head, nodes, group, seqs):
             assert (j, grp) not in seen
             seen.add((j, grp))
         assert len(seen) == units * groups
-        assert x["chunk"] <= {KEYS: 4 * 64, ALL_HEADS: 64}[x["kind"]]  # ids that a wave holds
+        assert x["chunk"] <= {KEYS: 4 * 32, ALL_HEADS: 32}[x["kind"]]  # ids that a wave holds
         for m, row in zip(x["members"], x["rows"]):
             keys, t = seqs[m]
             path[m].append((x["first"], x["len"], chunks))
@@ -158,9 +158,9 @@ def test_random_tries(plans, seed):
     launches = []
     for _ in range(60):
         ids = iter(rng.sample(range(100000), 20000))
-        launches.append((rng.choice([0, 0, 0, 1, 3, 40, 1 << 20]), rng.choice([4, 8]), tree(rng, rng.randint(1, 64), rng.choice([3, 20, 150]), ids)))
-    for (head, nodes), (_, group, seqs) in zip(plans(launches), launches):
-        check(head, nodes, group, seqs)
+        launches.append((rng.choice([0, 0, 0, 1, 3, 40, 1 << 20]), tree(rng, rng.randint(1, 64), rng.choice([3, 20, 150]), ids)))
+    for (head, nodes), (_, seqs) in zip(plans(launches), launches):
+        check(head, nodes, seqs)
 
 
 def common(n, prefix_blocks, tail_blocks):
@@ -171,16 +171,16 @@ def common(n, prefix_blocks, tail_blocks):
 
 def test_a_common_prefix_is_read_once(plans):
     for n in (2, 4, 5, 16, 17, 64):
-        (head, nodes), = plans([(0, 8, common(n, 128, 3))])
-        check(head, nodes, 8, common(n, 128, 3))
+        (head, nodes), = plans([(0, common(n, 128, 3))])
+        check(head, nodes, common(n, 128, 3))
         assert head["blocks"] == 128 + 3 * n and head["pays"]
         assert nodes[0]["members"] == list(range(n)) and nodes[0]["kind"] == KEYS
 
 
 def test_nothing_in_common(plans):
     seqs = [(100, [4 * i, 4 * i + 1, 4 * i + 2, 4 * i + 3]) for i in range(10)]
-    (head, nodes), = plans([(0, 8, seqs)])
-    check(head, nodes, 8, seqs)
+    (head, nodes), = plans([(0, seqs)])
+    check(head, nodes, seqs)
     assert head["blocks"] == head["apart"] == 40 and not head["pays"]
 
 
@@ -190,13 +190,13 @@ def test_ladders_and_long_prefixes(plans):
     ids = list(range(2000))
     ladder = [((8 * i + 9) * BT, ids[:8 * i + 8] + [5000 + i]) for i in range(64)]
     long = common(64, 8192, 1)
-    for (head, nodes), seqs in zip(plans([(0, 8, ladder), (0, 8, long), (1, 8, long)]), (ladder, long, long)):
-        check(head, nodes, 8, seqs)
+    for (head, nodes), seqs in zip(plans([(0, ladder), (0, long), (1, long)]), (ladder, long, long)):
+        check(head, nodes, seqs)
         assert sum(-(-len(x["members"]) // 8) * 8 for x in nodes if len(x["members"]) > 1) <= 512 and head["n_nodes"] <= 128
 
 
 def test_only_new_tokens(plans):
-    (head, nodes), = plans([(0, 8, [(0, [1]), (0, [2])])])
+    (head, nodes), = plans([(0, [(0, [1]), (0, [2])])])
     assert head["n_nodes"] == 0 and head["n_items"] == 0 and not head["pays"]
 
 
@@ -205,6 +205,6 @@ def test_same_sequence_many_times_over_ends_in_a_shared_block(plans):
     attends it alone."""
     t = list(range(20))
     seqs = [(20 * BT - 5, t) for _ in range(9)]
-    (head, nodes), = plans([(0, 8, seqs)])
-    check(head, nodes, 8, seqs)
+    (head, nodes), = plans([(0, seqs)])
+    check(head, nodes, seqs)
     assert nodes[0]["len"] == 19 and head["blocks"] == 19 + 9
