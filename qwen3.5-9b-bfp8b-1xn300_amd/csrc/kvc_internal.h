@@ -542,11 +542,13 @@ struct BlockCopyArgs {
 constexpr int kSharedNodes = 128;
 constexpr int kSharedMembers = 512;
 constexpr int kSharedSeqs = 8;         // 4 members are a tile of 16 rows; two tiles fill a wave's registers
-constexpr int kSharedWaveBlocks = 32;  // blocks whose ids a wave holds, one for each half
+constexpr int kSharedHalves = 64;      // half blocks of a wave: the ids it holds
+constexpr int kSharedOneMax = 1023;    // blocks of a kSharedOne workgroup
 constexpr int kSharedPath = 512;       // partials of one (sequence, q head)
 // how the 4 waves of a workgroup split it
 enum { kSharedKeys = 0,    // one kv head: a wave takes every 4th half block
-       kSharedHeads = 1 }; // all kv heads: a wave takes one
+       kSharedHeads = 1,   // all kv heads: a wave takes one
+       kSharedOne = 2 };   // one member, one kv head: kvc_decode_attn's walk, a wave takes 8 tokens of each block
 constexpr int kSharedMaxParts = (int)(kPartBytes / ((kHeadDim + 2) * 4 * kQHeads));  // over all sequences
 
 // A node's record.  Whole words: a scalar load drops the low two bits of each part
@@ -555,7 +557,7 @@ constexpr int kSharedMaxParts = (int)(kPartBytes / ((kHeadDim + 2) * 4 * kQHeads
 struct SharedNode {
     uint32_t first;  // block in the members' tables | kind << 26
     uint32_t len;    // blocks | (keys in the last one - 1) << 26
-    uint32_t who;    // chunk (blocks of a workgroup) | (members - 1) << 10 | and << 16:
+    uint32_t who;    // chunk (blocks of a workgroup, up to 1023) | (members - 1) << 10 | and << 16:
                      // of one member its entry, else where their list starts, / 8
     int32_t slot;    // table row of a member
 };

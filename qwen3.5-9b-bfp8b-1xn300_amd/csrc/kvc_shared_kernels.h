@@ -1,7 +1,7 @@
 // kvc_shared_kernels.h -- decode attention for sequences that share blocks, each
 // shared block read once (included by kvc_kernels.hip).
 //
-// For every trie node (kvc_shared_plan.h) and kv head, the members' query rows
+// For every trie node (kvc_shared_plan.h) of several members and kv head, the members' query rows
 // (4 q heads each, 4 members to a tile of 16 rows) attend to the node's keys in
 // one product per tile:
 //   S^T[16 keys x 16 rows]  = K[keys x 256] . Q^T        (v_mfma_f32_16x16x32_bf16)
@@ -35,6 +35,11 @@ __device__ __forceinline__ void wait_vm() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+struct SharedOneSmem {
+    DecodeSmem d;
+    __align__(16) float p[kWaves][32];  // a block's weights of 8 tokens and 4 heads
+};
+
 // One workgroup's work: a chunk of a node for up to kSharedSeqs of its members.
 struct SharedItem {
     int kind, h, ck, members;
@@ -52,7 +57,7 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
     const int step = it.kind == kSharedKeys ? kWaves : 1, base = it.kind == kSharedKeys ? wave : 0;
     const int h = it.h;
     // block ids: lane i holds that of this wave's i-th half block
-    const int n_half = (it.keys + kSharedTok - 1) / kSharedTok;
+    const int n_half = it.keys / kSharedTok;  // (whole blocks)
     const int n_my = it.kind == kSharedKeys ? (n_half - wave + kWaves - 1) / kWaves : n_half;
     const int idv = lane < n_my ? it.trow[(base + lane * step) >> 1] : 0;
 
@@ -117,7 +122,6 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
 
     for (int i = 0; i < n_my; i++) {
         const bool more = i + 1 < n_my;
-        const int valid = it.keys - (base + i * step) * kSharedTok;  // keys from the half block's first on
         asm volatile("" : "+v"(ka), "+v"(va));  // (the fragments' addresses are not kept over the loop)
         wait_vm<8>();  // K: the 8 copies after it are V's
         f32x4 st[T];
@@ -147,20 +151,11 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
         wait_lds();
         if (more) issue(a.kpool, cbk, 5, i + 1, ku);
         // weights of the scores
-        float cs = c;
-        if (valid < kSharedTok) {  // (one member, one tile)
-            asm volatile("");
-            cs = 1.f;
-#pragma unroll
-            for (int t = 0; t < T; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) st[t][e] = 4 * q4 + e < valid ? st[t][e] * c : kNegBig;
-        }
         bf16x4_t pw[T][PARTS];
 #pragma unroll
         for (int t = 0; t < T; t++) {
             const float mx = fmaxf(fmaxf(st[t][0], st[t][1]), fmaxf(st[t][2], st[t][3]));
-            const float mt = max_xor32(max_xor16(mx)) * cs;
+            const float mt = max_xor32(max_xor16(mx)) * c;
             const bool up = mt > m_run[t] + kRescaleSlack;
             if (__builtin_amdgcn_ballot_w64(up) != 0) {  // uniform; rows that keep their maximum scale by 1
                 const float cr = up ? fast_exp2(m_run[t] - mt) : 1.f;
@@ -173,7 +168,7 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
             u32x2 w[PARTS];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float x = fast_exp2(fmaf(st[t][2 * e], cs, nm)), y = fast_exp2(fmaf(st[t][2 * e + 1], cs, nm));
+                const float x = fast_exp2(fmaf(st[t][2 * e], c, nm)), y = fast_exp2(fmaf(st[t][2 * e + 1], c, nm));
                 w[0][e] = cvt_pk_bf16(x, y);
                 if constexpr (PARTS == 1) {
                     l[t] += bf16lo(w[0][e]) + bf16hi(w[0][e]);  // what the product uses
@@ -191,11 +186,6 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
             wait_vm<8>();
         else
             wait_vm<0>();
-        if (valid < kSharedTok) {  // rows that do not exist may hold anything: 0 times it must be 0
-            for (int r = valid; r < kSharedTok; r++)
-                *reinterpret_cast<u32x2*>(&sm.unit[2 * wave + 1][r * kHeadDim + lane * 4]) = u32x2{0u, 0u};
-            wait_lds();
-        }
         {
             bf16x4_t vf[kShAhead];
             auto read = [&](int dt) { vf[dt % kShAhead] = __builtin_bit_cast(bf16x4_t, lds_load_tr16(va ^ (32 * dt), 0)); };
@@ -280,9 +270,34 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
     }
 }
 
+// A chunk of one sequence: 4 rows, read from memory once.  The walk of
+// kvc_decode_attn holds twice the bytes in flight that the tiles' LDS does.
+template <int PARTS>
+__device__ __forceinline__ void shared_one(const SharedArgs& a, const SharedItem& it, int seq_row, SharedOneSmem& sm) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n_blk = (it.keys + kBlockTok - 1) / kBlockTok, e = it.who[0] & 0xFFFF;
+    const int ids = lane < min(64, n_blk) ? it.trow[lane] : 0;
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t qv[kGroup][2][4];
+    load_q(qv, a.q + ((size_t)(e & 63) * kQHeads + it.h * kGroup) * kHeadDim, lane);
+    WaveState st;
+    init_state(st);
+    walk_blocks<1, false, PARTS != 1>(a.kpool, a.vpool, it.trow, it.h, 0, n_blk, it.keys, qv, a.scale_log2,
+                                      reinterpret_cast<uint16_t*>(sm.p[wave]), st, wave, lane, 0, ids, [] {});
+    finalize_l(st);
+    float m, l, A[4];
+    merge_waves(st, sm.d, wave, lane, m, l, A);  // head `wave`, dims 4 lane ..
+    const size_t row = (size_t)(__builtin_amdgcn_readlane(seq_row, e & 63) + (e >> 6) + it.ck) * kQHeads + it.h * kGroup + wave;
+    *reinterpret_cast<float4*>(a.acc + row * kHeadDim + lane * 4) = make_float4(A[0], A[1], A[2], A[3]);
+    if (lane == 0) *reinterpret_cast<float2*>(a.stats + row * 2) = make_float2(m, l);
+}
+
 template <int PARTS>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(SharedArgs a) {
-    __shared__ __align__(1024) SharedSmem sm;  // (the XORs with a fragment's number need it)
+    __shared__ __align__(1024) union {  // (the XORs with a fragment's number need it)
+        SharedSmem tiles;
+        SharedOneSmem one;
+    } sm;
     const int lane = threadIdx.x & 63;
     const int item = blockIdx.x;
     // one trip to the arguments: every lane asks for the ends and records of two
@@ -337,10 +352,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         it.who[2] = __builtin_amdgcn_readlane(mw.z, from);
         it.who[3] = __builtin_amdgcn_readlane(mw.w, from);
     }
-    if (it.members > 4)
-        shared_item<2, PARTS>(a, it, seq_row, sm);
+    if (it.kind == kSharedOne)
+        shared_one<PARTS>(a, it, seq_row, sm.one);
+    else if (it.members > 4)
+        shared_item<2, PARTS>(a, it, seq_row, sm.tiles);
     else
-        shared_item<1, PARTS>(a, it, seq_row, sm);
+        shared_item<1, PARTS>(a, it, seq_row, sm.tiles);
 }
 
 // One workgroup folds a (sequence, q head): each wave every 4th partial, its

@@ -111,15 +111,16 @@ class SharedPlanner {
 
 inline int32_t shared_groups(int32_t members) { return (members + kSharedSeqs - 1) / kSharedSeqs; }
 
-// Workgroups of the nodes, where a wave takes up to w blocks of a node: a node of
-// at most w blocks goes to workgroups that take all kv heads.
-inline void shared_items(SharedPlan& p, int32_t w, int32_t n) {
+// Workgroups of the nodes: of several members, up to `halves` half blocks a wave
+// (a node that has no more goes to workgroups that take all kv heads), of one
+// member `one` blocks each.
+inline void shared_items(SharedPlan& p, int32_t halves, int32_t one, int32_t n) {
     for (int32_t i = 0; i < n; i++) p.seq_parts[i] = 0;
     int64_t items = 0;
     for (int32_t k = 0; k < p.n_nodes; k++) {
         const int32_t members = p.member_begin[k + 1] - p.member_begin[k], groups = shared_groups(members);
-        p.kind[k] = p.len[k] <= w ? kSharedHeads : kSharedKeys;
-        const int32_t chunk = p.kind[k] == kSharedHeads ? p.len[k] : 4 * w;
+        p.kind[k] = members == 1 ? kSharedOne : 2 * p.len[k] <= halves ? kSharedHeads : kSharedKeys;
+        const int32_t chunk = members == 1 ? one : p.kind[k] == kSharedHeads ? p.len[k] : 2 * halves;
         const int32_t n_chunks = (p.len[k] + chunk - 1) / chunk, units = n_chunks * (p.kind[k] == kSharedHeads ? 1 : kKvHeads);
         p.chunk[k] = (uint16_t)chunk;
         // (the groups of a unit run on one XCD: such nodes start on a multiple of 8)
@@ -143,6 +144,11 @@ inline void shared_items(SharedPlan& p, int32_t w, int32_t n) {
     p.parts = (int32_t)parts;
 }
 
+// us of a workgroup per block while another one runs on its CU: of a node of one
+// member (a chunk streams from memory), of 8 members of a node (from L2, bound by
+// LDS), and the least that is worth a workgroup
+constexpr double kSharedOneUs = 1.3, kSharedTilesUs = 1.0, kSharedMinUs = 3.0;
+
 // Whether the plan beats reading sequence by sequence, and fits.
 inline bool shared_pays(const SharedPlan& p) {
     return p.path <= kSharedPath && p.parts <= kSharedMaxParts && p.blocks_apart - p.blocks >= 16;
@@ -152,15 +158,25 @@ inline bool shared_pays(const SharedPlan& p) {
 // chunk length that the caller set.
 inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, SharedPlan& p) {
     SharedPlanner(tab, keys, n, p);
-    int64_t work = 0;
-    for (int32_t k = 0; k < p.n_nodes; k++)
-        work += (int64_t)p.len[k] * shared_groups(p.member_begin[k + 1] - p.member_begin[k]);
-    int32_t w = caller_chunk > 0 ? (std::min(caller_chunk, 4 * kSharedWaveBlocks) + 3) / 4
-                                 : (int32_t)std::min<int64_t>(kSharedWaveBlocks, std::max<int64_t>(1, (work + 255) / 256));
+    double us = 0;  // of a workgroup's place on a CU, two to a CU
+    for (int32_t k = 0; k < p.n_nodes; k++) {
+        const int32_t members = p.member_begin[k + 1] - p.member_begin[k];
+        us += (double)p.len[k] * kKvHeads * (members == 1 ? kSharedOneUs : shared_groups(members) * kSharedTilesUs);
+    }
+    us = std::max(us / 512, kSharedMinUs);
+    int32_t halves, one;
+    if (caller_chunk > 0) {
+        halves = (std::min(caller_chunk, 2 * kSharedHalves) + 1) / 2;
+        one = std::min(caller_chunk, kSharedOneMax);
+    } else {
+        halves = (int32_t)std::min<double>(kSharedHalves, us / kSharedTilesUs / 2 + 1);
+        one = (int32_t)std::min<double>(kSharedOneMax, us / kSharedOneUs + 1);
+    }
     for (;;) {
-        shared_items(p, w, n);
-        if ((p.path <= kSharedPath && p.parts <= kSharedMaxParts) || w >= kSharedWaveBlocks) break;
-        w = std::min(2 * w, kSharedWaveBlocks);
+        shared_items(p, halves, one, n);
+        if ((p.path <= kSharedPath && p.parts <= kSharedMaxParts) || (halves >= kSharedHalves && one >= kSharedOneMax)) break;
+        halves = std::min(2 * halves, kSharedHalves);
+        one = std::min(2 * one, kSharedOneMax);
     }
 }
 

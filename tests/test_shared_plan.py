@@ -14,7 +14,7 @@ CSRC = Path(__file__).resolve().parents[1] / "qwen3.5-9b-bfp8b-1xn300_amd" / "cs
 CXX = shutil.which("g++")
 pytestmark = pytest.mark.skipif(CXX is None, reason="needs g++")
 BT, HEADS, SEQS = 32, 4, 8
-KEYS, ALL_HEADS = 0, 1  # kinds
+KEYS, ALL_HEADS, ONE = 0, 1, 2  # kinds
 
 # stdin: launches as "n chunk", then per sequence "keys nblk id id ..."; stdout: the plan
 PROGRAM = r"""
@@ -124,7 +124,8 @@ def check(head, nodes, seqs):
             assert (j, grp) not in seen
             seen.add((j, grp))
         assert len(seen) == units * groups
-        assert x["chunk"] <= {KEYS: 4 * 32, ALL_HEADS: 32}[x["kind"]]  # ids that a wave holds
+        assert x["chunk"] <= {KEYS: 2 * 64, ALL_HEADS: 32, ONE: 1023}[x["kind"]]  # ids that a wave holds
+        assert (x["kind"] == ONE) == (len(x["members"]) == 1)
         for m, row in zip(x["members"], x["rows"]):
             keys, t = seqs[m]
             path[m].append((x["first"], x["len"], chunks))
