@@ -94,6 +94,9 @@ enum { KVC_DTYPE_F32 = 0, KVC_DTYPE_BF16 = 1 };
  * each other. */
 #define KVC_FLAG_DECODE_SPLIT_D 0x2u
 #define KVC_FLAG_DECODE_NO_SPLIT_D 0x4u
+/* kvc_decode_attn_shared goes over shared blocks wherever sequences share any, also
+ * where it estimates reading them per sequence to be faster (tuning and test hook). */
+#define KVC_FLAG_DECODE_SHARE 0x10u
 /* Transcendentals.  By default the library computes the reference's
  * Schraudolph (1999) approximations (src/engine.cpp:2349-2376): the output
  * gate sigma(gate) of decode and prefill attention (:3563, :2923), bit-exact
@@ -285,9 +288,9 @@ int kvc_decode_attn_static(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
 /* No counterpart in the reference.  kvc_decode_attn for sequences that share
  * blocks (kvc_seq_fork, kvc_prefix_match): same arguments and semantics, any order
  * of the sequences, any tree of common prefixes, but a full block that several
- * sequences of up to 64 of a call hold is read once for all of them.  Launches in
- * which they share little, or some hold 8-bit blocks, run kvc_decode_attn's
- * kernels.  With bf16 output weights are rounded to bf16 before the product with
+ * sequences of up to 64 of a call hold is read once for all of them.  Launches
+ * for which that is estimated to be slower (a few short sequences, little in
+ * common), or in which some hold 8-bit blocks, run kvc_decode_attn's kernels.  With bf16 output weights are rounded to bf16 before the product with
  * the values; with fp32 output they keep 24 bits in either kind of launch (as
  * several parts, so an infinite value may make the elements that it enters NaN).  Equal
  * to kvc_decode_attn within those roundings; the order of sums follows from the

@@ -1446,7 +1446,7 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
         }
         if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, p);
     }
-    if (!launch || q8 || !shared_pays(p)) {
+    if (!launch || q8 || !shared_pays(p, c->cfg.flags & KVC_FLAG_DECODE_SHARE)) {
         DecodeArgs a;
         DecodeQ8Args a8;
         int rc, e = 0;
@@ -1494,7 +1494,7 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
     for (int32_t k = 0; k < kSharedNodes; k++) a.item_end[k] = k < p.n_nodes ? p.item_begin[k + 1] : INT32_MAX;
     int32_t listed = 0;
     for (int32_t k = 0; k < p.n_nodes; k++) {
-        const int32_t mb = p.member_begin[k], members = p.member_begin[k + 1] - mb, s = p.member[mb];
+        const int32_t mb = p.member_begin[k], members = p.members[k], s = p.member[mb];
         // (a node of several members has full blocks only)
         const int32_t last = std::min(keys[s] - (p.first[k] + p.len[k] - 1) * kBlockTok, kBlockTok);
         const auto entry = [&](int32_t i) { return (uint16_t)(p.member[i] | p.part[i] << 6); };

@@ -82,7 +82,9 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const SharedIte
             for (int ks = 0; ks < 8; ks++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[t][ks][i] ^= qflip;
-                // (waited for here, before the copies are issued: a later wait would cover those too)
+                // waited for here, before the copies are issued: a later wait would
+                // cover those too (8 sequences on 65536 tokens 58.9 us a layer, with
+                // the wait behind the first copies 62.8)
                 asm volatile("" : "+v"(x[t][ks]));
                 qb[t][ks] = as_bf16x8(x[t][ks]);
             }
@@ -364,6 +366,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // first kSharedFold requested before the weights are known.  The new token is
 // a partial of its own, (score, 1, v), and is written to the cache.
 constexpr int kSharedFold = 16;
+constexpr int kSharedFew = 16;
 __global__ __launch_bounds__(256) void shared_fold_kernel(SharedFoldArgs a) {
     __shared__ float wgt[kSharedPath];
     __shared__ float red[kWaves][2];
@@ -455,6 +458,68 @@ __global__ __launch_bounds__(256) void shared_fold_kernel(SharedFoldArgs a) {
     write_out(a.out, a.out_bf16, qrow, lane * 4, has_gate, gs, l, A);
 }
 
+// The same for few partials: a wave folds a q head alone, a workgroup a kv head.
+__global__ __launch_bounds__(256) void shared_fold_few_kernel(SharedFoldArgs a) {
+    const int lane = threadIdx.x & 63, g = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int s = blockIdx.x / kKvHeads, h = blockIdx.x % kKvHeads, head = h * kGroup + g;
+    const SharedSeq sq = a.seq[s];
+    const int np = sq.parts;
+    const size_t row0 = (size_t)sq.row * kQHeads + head;
+    const size_t qrow = ((size_t)s * kQHeads + head) * kHeadDim;
+    const bool has_gate = a.gate != nullptr;
+    uint2 gw = make_uint2(0u, 0u), qw = gw, kw = gw, vw = gw;
+    if (has_gate) gw = *reinterpret_cast<const uint2*>(a.gate + qrow + lane * 4);
+    int blk = 0;
+    if (a.k_new) {
+        const size_t krow = ((size_t)s * kKvHeads + h) * kHeadDim + lane * 4;
+        qw = *reinterpret_cast<const uint2*>(a.q + qrow + lane * 4);
+        kw = *reinterpret_cast<const uint2*>(a.k_new + krow);
+        vw = *reinterpret_cast<const uint2*>(a.v_new + krow);
+        if (g == 0) blk = a.table[(size_t)sq.slot * a.table_stride + sq.keys / kBlockTok];
+    }
+    float2 ml = make_float2(kNegBig, 0.f);
+    f32x4 x[kSharedFew];
+    if (np > 0) {
+        if (lane < np) ml = *reinterpret_cast<const float2*>(a.stats + (row0 + (size_t)lane * kQHeads) * 2);
+#pragma unroll
+        for (int k = 0; k < kSharedFew; k++)
+            x[k] = *reinterpret_cast<const f32x4*>(a.acc + (row0 + (size_t)min(k, np - 1) * kQHeads) * kHeadDim + lane * 4);
+    }
+    float m = wave_max(ml.x), sc = kNegBig;
+    if (a.k_new) {
+        sc = wave_sum(bf16lo(qw.x) * bf16lo(kw.x) + bf16hi(qw.x) * bf16hi(kw.x) + bf16lo(qw.y) * bf16lo(kw.y) +
+                      bf16hi(qw.y) * bf16hi(kw.y)) * a.scale_log2;
+        m = fmaxf(m, sc);
+    }
+    const float f = lane < np ? fast_exp2(ml.x - m) : 0.f;
+    float l = wave_sum(f * ml.y);
+    float A[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kSharedFew; k++) {
+        if (k < np) {  // uniform
+            const float w = readlane(f, k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) A[i] = fmaf(w, x[k][i], A[i]);
+        }
+    }
+    if (a.k_new) {
+        const float w = fast_exp2(sc - m);
+        l += w;
+        A[0] = fmaf(w, bf16lo(vw.x), A[0]);
+        A[1] = fmaf(w, bf16hi(vw.x), A[1]);
+        A[2] = fmaf(w, bf16lo(vw.y), A[2]);
+        A[3] = fmaf(w, bf16hi(vw.y), A[3]);
+        if (g == 0) {
+            const size_t off = (((size_t)blk * kKvHeads + h) * kBlockTok + sq.keys % kBlockTok) * kHeadDim + lane * 4;
+            *reinterpret_cast<uint2*>(a.kpool + off) = kw;
+            *reinterpret_cast<uint2*>(a.vpool + off) = vw;
+        }
+    }
+    float gs[4] = {1.f, 1.f, 1.f, 1.f};
+    if (has_gate) gate_factors(gw, a.gate_ref, gs);
+    write_out(a.out, a.out_bf16, qrow, lane * 4, has_gate, gs, l, A);
+}
+
 int launch_shared(const SharedArgs& a, int32_t n_items, const SharedFoldArgs& f, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
     if (n_items > 0) {
@@ -465,7 +530,12 @@ int launch_shared(const SharedArgs& a, int32_t n_items, const SharedFoldArgs& f,
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(shared_fold_kernel, dim3(f.n_seqs * kQHeads), dim3(256), 0, st, f);
+    int32_t parts = 0;
+    for (int32_t i = 0; i < f.n_seqs; i++) parts = f.seq[i].parts > parts ? f.seq[i].parts : parts;
+    if (parts <= kSharedFew)
+        hipLaunchKernelGGL(shared_fold_few_kernel, dim3(f.n_seqs * kKvHeads), dim3(256), 0, st, f);
+    else
+        hipLaunchKernelGGL(shared_fold_kernel, dim3(f.n_seqs * kQHeads), dim3(256), 0, st, f);
     return (int)hipGetLastError();
 }
 

@@ -23,11 +23,13 @@ struct SharedPlan {
     int32_t parts = 0;                 // partials per q head, of all sequences
     int32_t path = 0;                  // most of them of one sequence
     int64_t blocks = 0, blocks_apart = 0;  // read by the plan, and sequence by sequence
+    int64_t tile_work = 0;             // blocks of a kv head for up to kSharedSeqs members
     int32_t first[kSharedNodes];       // of the node's blocks, in its members' tables
     int32_t len[kSharedNodes];         // blocks
     int32_t item_begin[kSharedNodes + 1];
     uint16_t chunk[kSharedNodes];      // blocks per workgroup
-    uint16_t member_begin[kSharedNodes + 1];
+    uint16_t member_begin[kSharedNodes];
+    uint8_t members[kSharedNodes];
     uint8_t kind[kSharedNodes];
     uint8_t member[kSharedMembers + kMaxBatch];  // index of the sequence in the launch
     uint16_t part[kSharedMembers + kMaxBatch];   // its first partial of this node
@@ -49,7 +51,6 @@ class SharedPlanner {
             p_.blocks_apart += total(i);
         }
         walk(0, n, 0, 0);
-        p_.member_begin[p_.n_nodes] = (uint16_t)p_.n_members;
     }
 
   private:
@@ -69,6 +70,7 @@ class SharedPlanner {
         p_.first[k] = from;
         p_.len[k] = to - from;
         p_.member_begin[k] = (uint16_t)p_.n_members;
+        p_.members[k] = (uint8_t)(hi - lo);
         for (int32_t i = lo; i < hi; i++) p_.member[p_.n_members++] = order_[i];
         p_.blocks += to - from;
         if (hi - lo > 1) p_.listed += (hi - lo + kSharedSeqs - 1) / kSharedSeqs * kSharedSeqs;
@@ -111,23 +113,45 @@ class SharedPlanner {
 
 inline int32_t shared_groups(int32_t members) { return (members + kSharedSeqs - 1) / kSharedSeqs; }
 
-// Workgroups of the nodes: of several members, up to `halves` half blocks a wave
-// (a node that has no more goes to workgroups that take all kv heads), of one
+// Nodes of several members first, then the long ones: what runs last is short.
+inline void shared_sort(SharedPlan& p) {
+    uint8_t order[kSharedNodes];
+    for (int32_t k = 0; k < p.n_nodes; k++) order[k] = (uint8_t)k;
+    const SharedPlan was = p;
+    std::sort(order, order + p.n_nodes, [&](uint8_t a, uint8_t b) {
+        const bool x = was.members[a] > 1, y = was.members[b] > 1;
+        return x != y ? x : was.len[a] != was.len[b] ? was.len[a] > was.len[b] : a < b;
+    });
+    for (int32_t k = 0; k < p.n_nodes; k++) {
+        p.first[k] = was.first[order[k]];
+        p.len[k] = was.len[order[k]];
+        p.member_begin[k] = was.member_begin[order[k]];
+        p.members[k] = was.members[order[k]];
+    }
+}
+
+// Cuts the nodes into workgroups: of several members, up to `halves` half blocks a
+// wave (a node that has no more goes to workgroups that take all kv heads), of one
 // member `one` blocks each.
 inline void shared_items(SharedPlan& p, int32_t halves, int32_t one, int32_t n) {
     for (int32_t i = 0; i < n; i++) p.seq_parts[i] = 0;
     int64_t items = 0;
     for (int32_t k = 0; k < p.n_nodes; k++) {
-        const int32_t members = p.member_begin[k + 1] - p.member_begin[k], groups = shared_groups(members);
+        const int32_t members = p.members[k], groups = shared_groups(members);
         p.kind[k] = members == 1 ? kSharedOne : 2 * p.len[k] <= halves ? kSharedHeads : kSharedKeys;
-        const int32_t chunk = members == 1 ? one : p.kind[k] == kSharedHeads ? p.len[k] : 2 * halves;
-        const int32_t n_chunks = (p.len[k] + chunk - 1) / chunk, units = n_chunks * (p.kind[k] == kSharedHeads ? 1 : kKvHeads);
+        int32_t chunk = members == 1 ? one : p.kind[k] == kSharedHeads ? p.len[k] : 2 * halves;
+        int32_t n_chunks = (p.len[k] + chunk - 1) / chunk;
+        // equal ones, of whole rounds of the 4 waves
+        chunk = (p.len[k] + n_chunks - 1) / n_chunks;
+        if (p.kind[k] == kSharedKeys) chunk = (chunk + 1) / 2 * 2;
+        n_chunks = (p.len[k] + chunk - 1) / chunk;
+        const int32_t units = n_chunks * (p.kind[k] == kSharedHeads ? 1 : kKvHeads);
         p.chunk[k] = (uint16_t)chunk;
         // (the groups of a unit run on one XCD: such nodes start on a multiple of 8)
         if (groups > 1) items = (items + 7) / 8 * 8;
         p.item_begin[k] = (int32_t)items;
         items += groups > 1 ? (int64_t)(units + 7) / 8 * 8 * groups : units;
-        for (int32_t i = p.member_begin[k]; i < p.member_begin[k + 1]; i++) {
+        for (int32_t i = p.member_begin[k]; i < p.member_begin[k] + members; i++) {
             p.part[i] = (uint16_t)std::min(p.seq_parts[p.member[i]], kSharedPath);
             p.seq_parts[p.member[i]] += n_chunks;
         }
@@ -144,39 +168,45 @@ inline void shared_items(SharedPlan& p, int32_t halves, int32_t one, int32_t n) 
     p.parts = (int32_t)parts;
 }
 
-// us of a workgroup per block while another one runs on its CU: of a node of one
-// member (a chunk streams from memory), of 8 members of a node (from L2, bound by
-// LDS), and the least that is worth a workgroup
-constexpr double kSharedOneUs = 1.3, kSharedTilesUs = 1.0, kSharedMinUs = 3.0;
+// Whether the partials fit.
+inline bool shared_fits(const SharedPlan& p) { return p.path <= kSharedPath && p.parts <= kSharedMaxParts; }
 
-// Whether the plan beats reading sequence by sequence, and fits.
-inline bool shared_pays(const SharedPlan& p) {
-    return p.path <= kSharedPath && p.parts <= kSharedMaxParts && p.blocks_apart - p.blocks >= 16;
+// Whether the plan beats kvc_decode_attn's launch, by the us that either takes: a
+// fixed part (here two launches), blocks from memory, blocks that sequence by
+// sequence come from the caches, and the tiles' LDS.  us per layer, kvc_decode_attn /
+// shared: 4 sequences on 300 tokens 9.2 / 12.4, 8 on 1000 9.5 / 12.8, 2 on 4096 11.5
+// / 12.7, 8 on 4096 17.6 / 16.6, 16 on 2000 17.0 / 15.2, 64 on 1000 28.3 / 17.3, 64
+// with 96 tokens in common of 1031 47.7 / 53.6, 64 on 65536 1228 / 141.
+// `always`: wherever blocks are shared.
+inline bool shared_pays(const SharedPlan& p, bool always) {
+    if (!shared_fits(p) || p.blocks == p.blocks_apart) return false;
+    if (always) return true;
+    constexpr double kBlockUs = 2.0 * kBlockBytes * 1e-6;  // of a block, K and V, at 1 TB/s
+    const double shared = 12 + std::max(p.blocks * kBlockUs / 5.5, 0.002 * p.tile_work);
+    const double apart = 7 + std::max(p.blocks * kBlockUs / 6.5, p.blocks_apart * kBlockUs / 12);
+    return shared < apart;
 }
 
 // The work of a launch of n sequences (n <= kMaxBatch): caller_chunk > 0 is a
-// chunk length that the caller set.
+// chunk length that the caller set.  Otherwise nodes of several members and of one
+// are each cut into about a workgroup per CU.  (Two fit, but those on tiles then
+// share its LDS and take twice the time, and shorter chunks leave more partials to
+// fold.)
 inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, SharedPlan& p) {
     SharedPlanner(tab, keys, n, p);
-    double us = 0;  // of a workgroup's place on a CU, two to a CU
-    for (int32_t k = 0; k < p.n_nodes; k++) {
-        const int32_t members = p.member_begin[k + 1] - p.member_begin[k];
-        us += (double)p.len[k] * kKvHeads * (members == 1 ? kSharedOneUs : shared_groups(members) * kSharedTilesUs);
-    }
-    us = std::max(us / 512, kSharedMinUs);
-    int32_t halves, one;
-    if (caller_chunk > 0) {
-        halves = (std::min(caller_chunk, 2 * kSharedHalves) + 1) / 2;
-        one = std::min(caller_chunk, kSharedOneMax);
-    } else {
-        halves = (int32_t)std::min<double>(kSharedHalves, us / kSharedTilesUs / 2 + 1);
-        one = (int32_t)std::min<double>(kSharedOneMax, us / kSharedOneUs + 1);
-    }
-    for (;;) {
-        shared_items(p, halves, one, n);
-        if ((p.path <= kSharedPath && p.parts <= kSharedMaxParts) || (halves >= kSharedHalves && one >= kSharedOneMax)) break;
+    shared_sort(p);
+    int64_t work[2] = {0, 0};  // blocks of all kv heads, of nodes of one member and of several
+    for (int32_t k = 0; k < p.n_nodes; k++)
+        work[p.members[k] > 1] += (int64_t)p.len[k] * kKvHeads * shared_groups(p.members[k]);
+    p.tile_work = work[1];
+    const int64_t tiles = caller_chunk > 0 ? caller_chunk : std::max<int64_t>(4, (work[1] + 255) / 256);
+    int32_t halves = (int32_t)std::min<int64_t>(kSharedHalves, (tiles + 1) / 2);
+    int32_t one = (int32_t)std::min<int64_t>(kSharedOneMax, caller_chunk > 0 ? caller_chunk : std::max<int64_t>(3, (work[0] + 255) / 256));
+    shared_items(p, halves, one, n);
+    while (!shared_fits(p) && (halves < kSharedHalves || one < kSharedOneMax)) {
         halves = std::min(2 * halves, kSharedHalves);
         one = std::min(2 * one, kSharedOneMax);
+        shared_items(p, halves, one, n);
     }
 }
 

@@ -45,7 +45,8 @@ class Forest(Q.Filled):
 
         n = count(spec)
         cfg = dict(max_seqs=2 * n + 4, max_seq_len=deepest(spec) + extra + 32,
-                   pool_blocks=tokens(spec) // 32 + n * (extra // 32 + 3) + 8, q8_blocks=0)
+                   pool_blocks=tokens(spec) // 32 + n * (extra // 32 + 3) + 8, q8_blocks=0,
+                   flags=kvc.FLAG_EXACT_MATH | kvc.FLAG_DECODE_SHARE)  # however little is shared
         super().__init__([0], layers=layers, seed=seed, **{**cfg, **over})
         self.ctx.seq_release(self.seqs.pop())
 
@@ -154,6 +155,29 @@ def test_scales(scale):
     with Forest([(600, 6)], seed=14) as f:
         f.check(f.seqs, "bf16", scale=scale)
         f.check(f.seqs, "fp32", scale=scale, bf16_out=False, seed=9)
+
+
+@pytest.mark.parametrize("name", ["pair", "sixty_four"])
+@pytest.mark.parametrize("bf16_out", [True, False])
+def test_where_the_rule_decides(name, bf16_out):
+    """without the flag: too little in common for one, enough for the other"""
+    say(f"shared decode {name} by the rule")
+    with Forest(SPECS[name], seed=26, flags=kvc.FLAG_EXACT_MATH) as f:
+        f.check(f.seqs, "fused, gated", bf16_out=bf16_out)
+
+
+def test_reference_gate():
+    """the default gate: the reference's sigmoid, within its own error of the exact one"""
+    say("shared decode with the reference's gate")
+    with Forest([(600, 6)], seed=27, flags=kvc.FLAG_DECODE_SHARE) as f:
+        gate = O.normal_bf16(6 * NQ * D, 5).reshape(6, NQ, D)
+        q = O.normal_bf16(6 * NQ * D, 6).reshape(6, NQ, D)
+        outs = [f.run(lambda qb, gb, ob: f.ctx.decode_attn_shared(0, f.seqs, qb, ob, gate=gb), (6, NQ, D), np.float32, q, g)
+                for g in (gate, None)]
+        # out = plain * sigma(gate), sigma bit for bit the reference's (the model tests/_oracle.py holds)
+        sig = np.array([O.sigmoid_ref_model(float(x)) for x in Q.f64(gate).reshape(-1)], np.float32).reshape(gate.shape)
+        want = outs[1].astype(np.float64) * sig
+        assert (np.abs(outs[0] - want) <= np.abs(want) * 2.0 ** -23).all()
 
 
 def test_large_scores():

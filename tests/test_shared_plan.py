@@ -16,15 +16,15 @@ pytestmark = pytest.mark.skipif(CXX is None, reason="needs g++")
 BT, HEADS, SEQS = 32, 4, 8
 KEYS, ALL_HEADS, ONE = 0, 1, 2  # kinds
 
-# stdin: launches as "n chunk", then per sequence "keys nblk id id ..."; stdout: the plan
+# stdin: launches as "n chunk share", then per sequence "keys nblk id id ..."; stdout: the plan
 PROGRAM = r"""
 #include <cstdio>
 #include <iostream>
 #include <vector>
 #include "kvc_shared_plan.h"
 int main() {
-    int n, chunk;
-    while (std::cin >> n >> chunk) {
+    int n, chunk, share;
+    while (std::cin >> n >> chunk >> share) {
         std::vector<std::vector<int32_t>> t(n);
         std::vector<int32_t> keys(n);
         std::vector<const int32_t*> tab(n);
@@ -38,10 +38,10 @@ int main() {
         kvc::SharedPlan p;
         kvc::shared_plan(tab.data(), keys.data(), n, chunk, p);
         std::printf("%d %d %d %d %lld %lld %d\n", p.n_nodes, p.n_items, p.parts, p.path, (long long)p.blocks,
-                    (long long)p.blocks_apart, (int)kvc::shared_pays(p));
+                    (long long)p.blocks_apart, (int)kvc::shared_pays(p, share));
         for (int k = 0; k < p.n_nodes; k++) {
             std::printf("%d %d %d %d %d %d", p.first[k], p.len[k], p.item_begin[k], p.chunk[k], p.kind[k], p.item_begin[k + 1]);
-            for (int i = p.member_begin[k]; i < p.member_begin[k + 1]; i++)
+            for (int i = p.member_begin[k]; i < p.member_begin[k] + p.members[k]; i++)
                 std::printf(" %d %d", p.member[i], p.seq_row[p.member[i]] + p.part[i]);
             std::printf("\n");
         }
@@ -57,9 +57,9 @@ def plans(tmp_path_factory):
     subprocess.run([CXX, "-O1", "-g", "-std=c++17", "-Wall", "-Wextra", "-fsanitize=address,undefined",
                     "-fno-sanitize-recover=undefined", f"-I{CSRC}", str(d / "plan.cpp"), "-o", str(d / "plan")], check=True)
 
-    def run(launches):
-        """launches: (chunk, [(keys, table), ...])"""
-        text = "\n".join("\n".join([f"{len(seqs)} {chunk}"] + [" ".join(map(str, (k, len(t), *t))) for k, t in seqs])
+    def run(launches, share=True):
+        """launches: (chunk, [(keys, table), ...]); share: over shared blocks wherever there are any"""
+        text = "\n".join("\n".join([f"{len(seqs)} {chunk} {int(share)}"] + [" ".join(map(str, (k, len(t), *t))) for k, t in seqs])
                          for chunk, seqs in launches)
         out = subprocess.run([str(d / "plan")], input=text, capture_output=True, text=True, check=True).stdout
         lines = iter(out.splitlines())
@@ -140,7 +140,7 @@ def check(head, nodes, seqs):
     assert head["n_items"] == (nodes[-1]["end"] if nodes else 0)
     for i, (keys, t) in enumerate(seqs):
         at = 0
-        for first, n, _ in path[i]:  # in order, once each
+        for first, n, _ in sorted(path[i]):  # once each
             assert first == at
             at += n
         assert at == -(-keys // BT)
@@ -209,3 +209,12 @@ def test_same_sequence_many_times_over_ends_in_a_shared_block(plans):
     (head, nodes), = plans([(0, seqs)])
     check(head, nodes, seqs)
     assert nodes[0]["len"] == 19 and head["blocks"] == 19 + 9
+
+
+@pytest.mark.parametrize("n,prefix,tail,shares", [(4, 9, 1, False), (8, 31, 1, False), (2, 128, 1, False),
+                                                  (8, 128, 1, True), (16, 62, 2, True), (64, 31, 1, True),
+                                                  (64, 3, 30, False), (64, 256, 24, True), (4, 500, 1, True)])
+def test_where_it_is_worth_it(plans, n, prefix, tail, shares):
+    """the measured side (us per layer in the rule's comment)"""
+    (head, _), = plans([(0, common(n, prefix, tail))], share=False)
+    assert bool(head["pays"]) == shares
