@@ -37,6 +37,7 @@
  *                               attention weight (new)
  *   kvc_seq_fork, kvc_seq_reorder   one sequence continued as several; beams that
  *                               go on from their parents (new)
+ *   kvc_beam_select             beam search's choice over beams and vocabulary (new)
  *   kvc_decode_attn_shared      kvc_decode_attn that reads blocks which sequences
  *                               share once (new)
  *   kvc_snapshot_save/_restore  prefix-boundary copies of that state (new: the
@@ -440,6 +441,26 @@ int kvc_q8_stats(kvc_ctx* ctx, int64_t* blocks, int64_t* free_blocks);
  * floor and a counter calibration of known size. */
 int kvc_kv_checksum(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
                     int32_t n_seqs, uint64_t* out, void* stream);
+
+/* ---- beam search (no counterpart in the reference) ------------------------- */
+/* Of every group (a prompt's beams) the n_out greatest of
+ *   scores[g][b] + logits[g][b][t] - log sum_u exp logits[g][b][u]
+ * over its beams b and tokens t, greatest first: the sums, in 64 bits, to
+ * out_scores (fp32), b and t to out_beams and out_tokens, device [n_groups][n_out]
+ * each.  Of equal sums the lower beam comes first, then the lower token.  A logit
+ * of -inf or NaN is never chosen; a beam whose score is not finite, or whose
+ * greatest logit is not, gives nothing; where fewer than n_out values are left the
+ * rest of a group's outputs is -inf, -1, -1.  logits: device, fp32 or bf16 by dtype,
+ * rows of vocab tokens row_stride apart, at any address of their element.  scores:
+ * device fp32 [n_groups][n_beams], NULL for zeros; it may be out_scores if n_out =
+ * n_beams.  Otherwise no two arrays may overlap.  n_beams <= 64, n_out <= 128;
+ * n_beams * vocab is bounded by the context's workspace (1 B per 64 tokens and a
+ * little; KVC_ERR_RANGE).  The next step: kvc_seq_reorder by the beams chosen. */
+int kvc_beam_select(kvc_ctx* ctx, const void* logits, int32_t dtype,
+                    int64_t row_stride, int32_t n_groups, int32_t n_beams,
+                    int32_t vocab, const void* scores, int32_t n_out,
+                    void* out_scores, int32_t* out_beams, int32_t* out_tokens,
+                    void* stream);
 
 /* ---- recurrent state + snapshots ---------------------------------------- */
 /* Live state of seq for Gated-DeltaNet layer ssm_layer: rec = fp32

@@ -1,0 +1,401 @@
+// kvc_beam_kernels.h -- beam search's choice: of each group (prompt) the n_out
+// greatest of score_b + x_bt - log sum_u exp x_bu over its beams b and tokens t, in
+// order (included by kvc_kernels.hip).
+//
+// Within a beam the order is that of the logits, so the first launch needs one pass
+// over them: the maximum of every 256-token segment, and the sum of exponentials.
+// The n_out greatest values of a group lie in the n_out segments with the greatest
+// maxima (ties: the lower beam, then the lower segment): a value in any other
+// segment has n_out segment maxima before it.  So the second launch, a workgroup per
+// group, chooses among the maxima and reads n_out segments again, no more.
+#pragma once
+
+namespace kvc {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 16 B at any element's address: rows are cut by token, not by address, so that equal
+// rows have equal sums wherever they lie.  The hardware takes such loads whole; of a
+// wave's 1024 B they touch nine 128-B lines instead of eight.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+template <bool BF16>
+__device__ __forceinline__ float beam_logit(const void* row, int t) {
+    const float x = BF16 ? bf16f(static_cast<const uint16_t*>(row)[t]) : static_cast<const float*>(row)[t];
+    return x != x ? -INFINITY : x;
+}
+
+// One chunk of a row: 4 waves x STEPS loads of 16 B a lane, all in flight at once.
+template <bool BF16, int STEPS>
+__global__ __launch_bounds__(256) void beam_max_kernel(BeamArgs a) {
+    constexpr int E = BF16 ? 8 : 4;            // tokens of a lane's load
+    constexpr int kSegLanes = kBeamSeg / E;    // 32 or 64
+    __shared__ float2 red[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const size_t row = blockIdx.y;
+    const uint8_t* base = static_cast<const uint8_t*>(a.logits) + row * (size_t)a.stride * (BF16 ? 2 : 4);
+    const int64_t at = ((int64_t)blockIdx.x * 4 + wave) * STEPS * (64 * E);  // of the wave
+    u32x4 w[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int64_t t = at + k * (64 * E) + lane * E;
+        if (t + E <= a.vocab) {
+            w[k] = *reinterpret_cast<const u32x4_any*>(base + t * (BF16 ? 2 : 4));
+        } else {  // the row's end: token by token, -inf behind it
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (BF16) {
+                    const uint32_t lo = t + 2 * i < a.vocab ? reinterpret_cast<const uint16_t*>(base)[t + 2 * i] : 0xFF80u;
+                    const uint32_t hi = t + 2 * i + 1 < a.vocab ? reinterpret_cast<const uint16_t*>(base)[t + 2 * i + 1] : 0xFF80u;
+                    w[k][i] = lo | hi << 16;
+                } else {
+                    w[k][i] = t + i < a.vocab ? reinterpret_cast<const uint32_t*>(base)[t + i] : 0xFF800000u;
+                }
+            }
+        }
+    }
+    float m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        float x[E];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (BF16) {
+                x[2 * i] = bf16lo(w[k][i]);
+                x[2 * i + 1] = bf16hi(w[k][i]);
+            } else {
+                x[i] = __uint_as_float(w[k][i]);
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            x[i] = x[i] != x[i] ? -INFINITY : x[i];
+            mx = fmaxf(mx, x[i]);
+        }
+        float seg = mx;  // over the segment's lanes
+        seg = fmaxf(seg, dpp<kDppXor1>(seg));
+        seg = fmaxf(seg, dpp<kDppXor2>(seg));
+        seg = fmaxf(seg, dpp<kDppHalfMirror>(seg));
+        seg = fmaxf(seg, dpp<kDppRowRor8>(seg));
+        seg = max_xor16(seg);
+        if constexpr (kSegLanes == 64) seg = max_xor32(seg);
+        const int64_t j = (at + k * (64 * E) + lane * E) / kBeamSeg;
+        if (lane % kSegLanes == 0 && j < a.n_seg) a.seg_max[row * a.n_seg + j] = seg;
+        // running sum of exp(x - m); a row of -inf so far has m = -inf and sum 0
+        const float m2 = fmaxf(m, mx), me = m2 == -INFINITY ? 0.f : m2;
+        s *= fast_exp2((m - me) * kLog2e);
+        m = m2;
+#pragma unroll
+        for (int i = 0; i < E; i++) s += fast_exp2((x[i] - me) * kLog2e);
+    }
+    const float wm = wave_max(m), we = wm == -INFINITY ? 0.f : wm;
+    s = wave_sum(s * fast_exp2((m - we) * kLog2e));
+    if (lane == 0) red[wave] = make_float2(wm, s);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const float M = fmaxf(fmaxf(red[0].x, red[1].x), fmaxf(red[2].x, red[3].x)), me = M == -INFINITY ? 0.f : M;
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) t += red[i].y * fast_exp2((red[i].x - me) * kLog2e);
+        *reinterpret_cast<float2*>(a.chunk_sum + (row * a.n_chunks + blockIdx.x) * 2) = make_float2(M, t);
+    }
+}
+
+// Doubles as integers of the same order; 0 for -inf, which is never chosen.
+__device__ __forceinline__ uint64_t beam_key(double v) {
+    if (!(v > -INFINITY)) return 0;
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);  // (-0 is 0)
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double beam_value(uint64_t k) {
+    return __longlong_as_double((int64_t)(k >> 63 ? k & ~(1ull << 63) : ~k));
+}
+
+constexpr int kBeamThreads = 1024, kBeamWaves = kBeamThreads / 64;
+constexpr int kBeamCached = 8192;  // keys of segments held in LDS
+constexpr int kBeamCands = 1024;   // values that the last step sorts
+struct BeamSmem {
+    uint64_t keys[kBeamCached];
+    double off[kBeamMaxBeams];      // score - log sum exp(x - max); -inf for a beam that gives nothing
+    double max[kBeamMaxBeams];
+    uint64_t red[2 * kBeamWaves];
+    int32_t hist[kBeamThreads];
+    int32_t wsum[kBeamWaves];
+    int32_t list[kBeamMaxOut];      // chosen segments
+    uint64_t cand[kBeamCands];      // key of a value, and where it is: beam << 32 | token
+    uint64_t where[kBeamCands];
+    int32_t count, bin, above;
+};
+
+__device__ __forceinline__ int beam_scan(BeamSmem& sm, int x, int tid) {  // sum over threads >= tid
+    const int lane = tid & 63, wave = tid >> 6;
+    int v = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_down(v, d);
+        v += lane + d < 64 ? y : 0;
+    }
+    if (lane == 0) sm.wsum[wave] = v;
+    __syncthreads();
+    for (int w = wave + 1; w < kBeamWaves; w++) v += sm.wsum[w];
+    __syncthreads();
+    return v;
+}
+
+// Of n keys (0: none) the `want` greatest: those above *cut, and of those equal to
+// it the first *ties.  All threads; want >= 1.
+template <typename Key>
+__device__ __forceinline__ void beam_cut(BeamSmem& sm, int n, int want, Key&& key, uint64_t* cut, int* ties) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint64_t lo = ~0ull, hi = 0;
+    int alive = 0;
+    for (int p = tid; p < n; p += kBeamThreads) {
+        const uint64_t k = key(p);
+        if (k == 0) continue;
+        alive++;
+        lo = k < lo ? k : lo;
+        hi = k > hi ? k : hi;
+    }
+#pragma unroll
+    for (int d = 32; d; d /= 2) {
+        const uint64_t l2 = __shfl_xor(lo, d), h2 = __shfl_xor(hi, d);
+        lo = l2 < lo ? l2 : lo;
+        hi = h2 > hi ? h2 : hi;
+    }
+    if (lane == 0) {
+        sm.red[2 * wave] = lo;
+        sm.red[2 * wave + 1] = hi;
+    }
+    const int total = beam_scan(sm, alive, tid);  // (thread 0's is the sum of all; its barriers order red)
+    if (tid == 0) sm.above = total;
+    for (int w = 0; w < kBeamWaves; w++) {
+        lo = sm.red[2 * w] < lo ? sm.red[2 * w] : lo;
+        hi = sm.red[2 * w + 1] > hi ? sm.red[2 * w + 1] : hi;
+    }
+    __syncthreads();
+    if (sm.above <= want) {  // all that there are
+        *cut = 1;
+        *ties = n;
+        __syncthreads();
+        return;
+    }
+    // narrow [lo, hi] to the 1024th part that holds the want-th greatest, until it
+    // is taken whole or is one value (4 rounds at least of 64 bits; 2 or 3 in use)
+    int need = want;
+    for (;;) {
+        const uint64_t width = hi - lo;
+        const int bits = width ? 64 - __clzll((long long)width) : 0;
+        const int sh = bits > 10 ? bits - 10 : 0;
+        __syncthreads();
+        sm.hist[tid] = 0;
+        __syncthreads();
+        for (int p = tid; p < n; p += kBeamThreads) {
+            const uint64_t k = key(p);
+            if (k >= lo && k <= hi) atomicAdd(&sm.hist[(int)((k - lo) >> sh)], 1);
+        }
+        __syncthreads();
+        const int h = sm.hist[tid];
+        const int from = beam_scan(sm, h, tid);  // in this part and above
+        if (from >= need && from - h < need) {
+            sm.bin = tid;
+            sm.above = from - h;
+            sm.count = h;
+        }
+        __syncthreads();
+        const int bin = sm.bin, inside = sm.count;
+        need -= sm.above;
+        lo += (uint64_t)bin << sh;
+        const uint64_t top = lo + ((1ull << sh) - 1);
+        hi = top < hi ? top : hi;
+        if (inside == need || sh == 0) break;
+    }
+    __syncthreads();
+    // one value left: its first `need` places; a part taken whole: all from lo on
+    if (lo == hi) {
+        *cut = lo;
+        *ties = need;
+    } else {
+        *cut = lo;
+        *ties = n;
+    }
+}
+
+// emit(p) for the chosen of n keys, in no order.
+template <typename Key, typename Emit>
+__device__ __forceinline__ void beam_collect(BeamSmem& sm, int n, uint64_t cut, int ties, Key&& key, Emit&& emit) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (ties >= n) {
+        for (int p = tid; p < n; p += kBeamThreads) {
+            const uint64_t k = key(p);
+            if (k >= cut && k) emit(p, k);
+        }
+        return;
+    }
+    int before = 0;  // equal ones in earlier rounds
+    for (int p0 = 0; p0 < n; p0 += kBeamThreads) {
+        const int p = p0 + tid;
+        const uint64_t k = p < n ? key(p) : 0;
+        const bool eq = k == cut;
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(eq);
+        if (lane == 0) sm.wsum[wave] = __popcll(mask);
+        __syncthreads();
+        int r = before + __popcll(mask & ((1ull << lane) - 1));
+        for (int w = 0; w < kBeamWaves; w++) {
+            if (w < wave) r += sm.wsum[w];
+            before += sm.wsum[w];
+        }
+        if (k > cut || (eq && r < ties)) emit(p, k);
+        __syncthreads();
+    }
+}
+
+// A workgroup per group.
+template <bool BF16>
+__global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
+    __shared__ BeamSmem sm;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t row0 = (size_t)blockIdx.x * a.n_beams;
+    // A value is (score - log sum exp(x - max)) + (x - max), in 64 bits: large logits
+    // cancel before the small sums join them.
+    for (int b = wave; b < a.n_beams; b += kBeamWaves) {
+        const float* cs = a.chunk_sum + (row0 + b) * (size_t)a.n_chunks * 2;
+        float m = -INFINITY;
+        for (int c = lane; c < a.n_chunks; c += 64) m = fmaxf(m, cs[2 * c]);
+        m = wave_max(m);
+        const bool fine = m > -INFINITY && m < INFINITY;
+        double s = 0.0;
+        for (int c = lane; fine && c < a.n_chunks; c += 64) s += cs[2 * c + 1] * exp((double)cs[2 * c] - m);
+#pragma unroll
+        for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
+        if (lane == 0) {
+            const float score = a.scores ? a.scores[row0 + b] : 0.f;
+            sm.off[b] = fine && score > -INFINITY && score < INFINITY ? score - log(s) : -INFINITY;
+            sm.max[b] = fine ? m : 0.0;
+        }
+    }
+    __syncthreads();
+    const int n_seg = a.n_seg, n = a.n_beams * n_seg;
+    const float* seg = a.seg_max + row0 * n_seg;
+    const auto beam_of = [&](int p) { return (int)((unsigned)p / (unsigned)n_seg); };
+    const auto key_of = [&](int b, float x) { return beam_key(sm.off[b] + ((double)x - sm.max[b])); };
+    const auto seg_key = [&](int p) { return key_of(beam_of(p), seg[p]); };
+    const bool cached = n <= kBeamCached;
+    if (cached) {
+        for (int p = tid; p < n; p += kBeamThreads) sm.keys[p] = seg_key(p);
+        __syncthreads();
+    }
+    const auto key = [&](int p) { return cached ? sm.keys[p] : seg_key(p); };
+    uint64_t cut;
+    int ties;
+    beam_cut(sm, n, a.n_out, key, &cut, &ties);
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
+    beam_collect(sm, n, cut, ties, key, [&](int p, uint64_t) { sm.list[atomicAdd(&sm.count, 1)] = p; });
+    __syncthreads();
+    const int n_list = sm.count;
+    __syncthreads();
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
+    // values of the chosen segments from the least chosen maximum on
+    const size_t esz = BF16 ? 2 : 4;
+    const uint8_t* rows = static_cast<const uint8_t*>(a.logits) + row0 * (size_t)a.stride * esz;
+    const auto place = [&](int p, int i, int* b, int64_t* t) -> const void* {
+        *b = beam_of(p);
+        const void* row = rows + (size_t)*b * (size_t)a.stride * esz;
+        *t = (int64_t)(p - *b * n_seg) * kBeamSeg + i;
+        return row;
+    };
+    for (int k = wave; k < n_list; k += kBeamWaves) {
+        const int p = sm.list[k];
+#pragma unroll
+        for (int i = 0; i < kBeamSeg / 64; i++) {
+            int b;
+            int64_t t;
+            const void* row = place(p, 64 * i + lane, &b, &t);
+            if (t >= a.vocab) continue;
+            const uint64_t v = key_of(b, beam_logit<BF16>(row, (int)t));
+            if (v == 0 || v < cut) continue;
+            const int c = atomicAdd(&sm.count, 1);
+            if (c < kBeamCands) {
+                sm.cand[c] = v;
+                sm.where[c] = (uint64_t)b << 32 | (uint32_t)t;
+            }
+        }
+    }
+    __syncthreads();
+    int n_cand = sm.count;
+    __syncthreads();
+    if (n_cand > kBeamCands) {
+        // many equal or close values: the segments in order of place, then exactly
+        // the n_out greatest, of equal ones the first
+        if (tid < n_list) {
+            const int p = sm.list[tid];
+            int r = 0;
+            for (int k = 0; k < n_list; k++) r += sm.list[k] < p;
+            sm.hist[r] = p;
+        }
+        __syncthreads();
+        if (tid < n_list) sm.list[tid] = sm.hist[tid];
+        __syncthreads();
+        const auto value = [&](int q) -> uint64_t {
+            int b;
+            int64_t t;
+            const void* row = place(sm.list[q / kBeamSeg], q % kBeamSeg, &b, &t);
+            return t >= a.vocab ? 0 : key_of(b, beam_logit<BF16>(row, (int)t));
+        };
+        uint64_t vcut;
+        int vties;
+        beam_cut(sm, n_list * kBeamSeg, a.n_out, value, &vcut, &vties);
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+        beam_collect(sm, n_list * kBeamSeg, vcut, vties, value, [&](int q, uint64_t v) {
+            const int c = atomicAdd(&sm.count, 1);
+            int b;
+            int64_t t;
+            place(sm.list[q / kBeamSeg], q % kBeamSeg, &b, &t);
+            sm.cand[c] = v;
+            sm.where[c] = (uint64_t)b << 32 | (uint32_t)t;
+        });
+        __syncthreads();
+        n_cand = sm.count;
+    }
+    // in order: greatest first, then the lower beam, then the lower token
+    const size_t o = (size_t)blockIdx.x * a.n_out;
+    if (tid < n_cand) {
+        const uint64_t v = sm.cand[tid], w = sm.where[tid];
+        int r = 0;
+        for (int k = 0; k < n_cand; k++) r += sm.cand[k] > v || (sm.cand[k] == v && sm.where[k] < w);
+        if (r < a.n_out) {
+            a.out_scores[o + r] = (float)beam_value(v);
+            a.out_beams[o + r] = (int32_t)(w >> 32);
+            a.out_tokens[o + r] = (int32_t)(uint32_t)w;
+        }
+    }
+    if (tid >= n_cand && tid < a.n_out) {  // fewer than n_out
+        a.out_scores[o + tid] = -INFINITY;
+        a.out_beams[o + tid] = a.out_tokens[o + tid] = -1;
+    }
+}
+
+int launch_beam_select(const BeamArgs& a, void* stream) {
+    const hipStream_t st = (hipStream_t)stream;
+    const dim3 grid(a.n_chunks, a.n_groups * a.n_beams);
+    if (a.bf16 && a.steps == 4)
+        hipLaunchKernelGGL((beam_max_kernel<true, 4>), grid, dim3(256), 0, st, a);
+    else if (a.bf16)
+        hipLaunchKernelGGL((beam_max_kernel<true, 1>), grid, dim3(256), 0, st, a);
+    else if (a.steps == 4)
+        hipLaunchKernelGGL((beam_max_kernel<false, 4>), grid, dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((beam_max_kernel<false, 1>), grid, dim3(256), 0, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    if (a.bf16)
+        hipLaunchKernelGGL(beam_select_kernel<true>, dim3(a.n_groups), dim3(kBeamThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(beam_select_kernel<false>, dim3(a.n_groups), dim3(kBeamThreads), 0, st, a);
+    return (int)hipGetLastError();
+}
+
+}  // namespace kvc

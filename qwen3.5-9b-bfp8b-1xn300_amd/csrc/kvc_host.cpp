@@ -2151,6 +2151,80 @@ int kvc_q8_stats(kvc_ctx* c, int64_t* blocks, int64_t* free_blocks) {
     return KVC_OK;
 }
 
+// ---- beam selection -----------------------------------------------------------
+
+int kvc_beam_select(kvc_ctx* c, const void* logits, int32_t dtype, int64_t row_stride, int32_t n_groups,
+                    int32_t n_beams, int32_t vocab, const void* scores, int32_t n_out, void* out_scores,
+                    int32_t* out_beams, int32_t* out_tokens, void* stream) {
+    if (!c) return set_err(KVC_ERR_INVALID, "null context");
+    if (!logits || !out_scores || !out_beams || !out_tokens)
+        return set_err(KVC_ERR_INVALID, "beam selection needs logits and its three outputs");
+    if (dtype != KVC_DTYPE_F32 && dtype != KVC_DTYPE_BF16) return set_err(KVC_ERR_INVALID, "bad dtype");
+    if (n_groups <= 0 || n_beams <= 0 || vocab <= 0 || n_out <= 0)
+        return set_err(KVC_ERR_INVALID, "beam selection needs positive counts");
+    if (row_stride < vocab) return set_err(KVC_ERR_INVALID, "row_stride %lld is less than vocab %d", (long long)row_stride, vocab);
+    if (n_beams > kBeamMaxBeams || n_out > kBeamMaxOut)
+        return set_err(KVC_ERR_RANGE, "%d beams, %d chosen: at most %d and %d", n_beams, n_out, kBeamMaxBeams, kBeamMaxOut);
+    const bool bf16 = dtype == KVC_DTYPE_BF16;
+    const size_t esz = bf16 ? 2 : 4;
+    if (((uintptr_t)logits & (esz - 1)) ||
+        (((uintptr_t)scores | (uintptr_t)out_scores | (uintptr_t)out_beams | (uintptr_t)out_tokens) & 3))
+        return set_err(KVC_ERR_INVALID, "beam selection needs arrays aligned to their elements");
+    // (a group's scores are read before its choice is written: in place where the shapes are equal)
+    const int64_t rows = (int64_t)n_groups * n_beams;
+    if (rows > INT32_MAX || row_stride > INT64_MAX / 4 / rows) return set_err(KVC_ERR_RANGE, "beam selection too large");
+    const size_t lbytes = ((size_t)(rows - 1) * (size_t)row_stride + (size_t)vocab) * esz, obytes = (size_t)n_groups * n_out * 4;
+    const auto meet = [](const void* x, size_t nx, const void* y, size_t ny) {
+        return x && (uintptr_t)x < (uintptr_t)y + ny && (uintptr_t)y < (uintptr_t)x + nx;
+    };
+    const void* outs[3] = {out_scores, out_beams, out_tokens};
+    for (int i = 0; i < 3; i++) {
+        const bool in_place = i == 0 && scores == out_scores && n_out == n_beams;
+        if (meet(logits, lbytes, outs[i], obytes) || (!in_place && meet(scores, (size_t)rows * 4, outs[i], obytes)))
+            return set_err(KVC_ERR_INVALID, "an output of the beam selection overlaps an input");
+        for (int j = 0; j < i; j++)
+            if (meet(outs[i], obytes, outs[j], obytes))
+                return set_err(KVC_ERR_INVALID, "outputs of the beam selection overlap");
+    }
+    const int64_t n_seg = ((int64_t)vocab + kBeamSeg - 1) / kBeamSeg;
+    // short chunks for few rows, so that every CU has some
+    const auto chunks_of = [&](int steps) {
+        const int64_t tokens = beam_chunk_tokens(bf16, steps);
+        return (vocab + tokens - 1) / tokens;
+    };
+    const int steps = rows * chunks_of(4) >= 512 ? 4 : 1;
+    const int64_t n_chunks = chunks_of(steps);
+    const int64_t group_bytes = n_beams * (n_seg * 4 + n_chunks * 8);
+    if (group_bytes > (int64_t)kPartBytes || n_beams * n_seg > INT32_MAX)
+        return set_err(KVC_ERR_RANGE, "the maxima of %d beams of %d tokens exceed the workspace", n_beams, vocab);
+    int rc;
+    if ((rc = check_device(c)) || (rc = check_current(c))) return rc;
+    const int32_t at_once = (int32_t)std::min<int64_t>(std::min<int64_t>(n_groups, (int64_t)kPartBytes / group_bytes), 65535 / n_beams);
+    for (int32_t g0 = 0; g0 < n_groups; g0 += at_once) {
+        BeamArgs a{};
+        const size_t row0 = (size_t)g0 * n_beams;
+        a.n_groups = std::min(at_once, n_groups - g0);
+        a.logits = static_cast<const uint8_t*>(logits) + row0 * (size_t)row_stride * esz;
+        a.scores = scores ? static_cast<const float*>(scores) + row0 : nullptr;
+        a.out_scores = static_cast<float*>(out_scores) + (size_t)g0 * n_out;
+        a.out_beams = out_beams + (size_t)g0 * n_out;
+        a.out_tokens = out_tokens + (size_t)g0 * n_out;
+        a.chunk_sum = c->d_part;
+        a.seg_max = c->d_part + (size_t)a.n_groups * n_beams * n_chunks * 2;
+        a.stride = row_stride;
+        a.bf16 = bf16;
+        a.vocab = vocab;
+        a.n_beams = n_beams;
+        a.n_out = n_out;
+        a.n_seg = (int32_t)n_seg;
+        a.n_chunks = (int32_t)n_chunks;
+        a.steps = steps;
+        int e = launch_beam_select(a, stream);
+        if (e) return hip_err((hipError_t)e, "beam selection launch");
+    }
+    return KVC_OK;
+}
+
 // ---- forks -------------------------------------------------------------------
 
 // What a copy of s holds besides its recurrent state; its blocks are counted for

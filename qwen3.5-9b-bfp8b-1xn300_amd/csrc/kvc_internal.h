@@ -606,6 +606,33 @@ struct SharedFoldArgs {
     SharedSeq seq[kMaxBatch];
 };
 
+// ---- beam selection --------------------------------------------------------
+// A row is one beam's logits, cut into segments of 256 tokens; the first launch
+// leaves each segment's maximum and, per chunk of segments, (max, sum of exp).
+constexpr int kBeamSeg = 256;
+constexpr int kBeamMaxBeams = 64;
+constexpr int kBeamMaxOut = 128;
+struct BeamArgs {
+    const void* logits;     // [groups][beams][stride], bf16 or fp32
+    const float* scores;    // [groups][beams] or null (zeros)
+    float* out_scores;      // [groups][n_out]
+    int32_t* out_beams;
+    int32_t* out_tokens;
+    float* seg_max;         // [row][n_seg]
+    float* chunk_sum;       // [row][n_chunks][max, sum]
+    int64_t stride;
+    int32_t bf16;
+    int32_t vocab;
+    int32_t n_groups;
+    int32_t n_beams;
+    int32_t n_out;
+    int32_t n_seg;          // segments of a row
+    int32_t n_chunks;
+    int32_t steps;          // 16-B loads of a lane per chunk: 1 or 4
+};
+constexpr int beam_step_tokens(bool bf16) { return bf16 ? 512 : 256; }  // of a wave's load
+constexpr int beam_chunk_tokens(bool bf16, int steps) { return 4 * steps * beam_step_tokens(bf16); }
+
 // Recurrent state and block tables of forked sequences: source states that go to
 // several places are read once.
 struct ForkArgs {
@@ -645,6 +672,7 @@ int launch_zero_state(const ZeroStateArgs& a, void* stream);
 int launch_gather(const GatherArgs& a, void* stream);
 int launch_checksum(const ChecksumArgs& a, void* stream);
 int launch_prefill(const PrefillArgs& a, void* stream);
+int launch_beam_select(const BeamArgs& a, void* stream);
 int launch_shared(const SharedArgs& a, int32_t n_items, const SharedFoldArgs& f, void* stream);
 int launch_snapshot(const SnapshotArgs& a, void* stream);
 int launch_fork(const ForkArgs& a, void* stream);

@@ -4269,6 +4269,7 @@ __global__ __launch_bounds__(256) void fill_normal_kernel(uint16_t* dst, int64_t
 #include "kvc_evict_kernels.h"
 #include "kvc_fork_kernels.h"
 #include "kvc_shared_kernels.h"
+#include "kvc_beam_kernels.h"
 
 namespace kvc {
 

@@ -48,7 +48,7 @@ EXPORTS = [
     "kvc_decode_attn_static", "kvc_decode_step", "kvc_prefill_attn", "kvc_prefill_step", "kvc_gather", "kvc_kv_checksum", "kvc_state_ptrs", "kvc_deltanet_step", "kvc_snapshot_save",
     "kvc_snapshot_restore", "kvc_snapshot_release", "kvc_pool_fill_normal",
     "kvc_fill_normal_bf16", "kvc_sync", "kvc_kv_quantize", "kvc_attn_weights", "kvc_evict", "kvc_seq_get_info",
-    "kvc_q8_stats", "kvc_seq_fork", "kvc_seq_reorder", "kvc_decode_attn_shared",
+    "kvc_q8_stats", "kvc_seq_fork", "kvc_seq_reorder", "kvc_decode_attn_shared", "kvc_beam_select",
 ]
 
 
@@ -121,6 +121,7 @@ def lib() -> ctypes.CDLL:
             "kvc_qkv_append": (ctypes.c_int, [P, I32, pI32, I32, I32, P, I32, P, P, P, P, P]),
             "kvc_decode_attn": (ctypes.c_int, [P, I32, pI32, I32, P, P, P, P, P, I32, F32, P]),
             "kvc_decode_attn_static": (ctypes.c_int, [P, I32, pI32, I32, P, P, P, P, P, I32, F32, P]),
+            "kvc_beam_select": (ctypes.c_int, [P, P, I32, I64, I32, I32, I32, P, I32, P, P, P, P]),
             "kvc_decode_attn_shared": (ctypes.c_int, [P, I32, pI32, I32, P, P, P, P, P, I32, F32, P]),
             "kvc_decode_step": (ctypes.c_int, [P, I32, pI32, I32, P, I32, P, P, P, I32, F32, P]),
             "kvc_kv_checksum": (ctypes.c_int, [P, I32, pI32, I32, P, P]),
@@ -420,6 +421,13 @@ class Context:
         _check(self.L.kvc_decode_attn_shared(self.ptr, layer, _i32(seqs), len(seqs), self._p(q), self._p(k_new),
                                              self._p(v_new), self._p(gate), self._p(out), out_dtype,
                                              ctypes.c_float(scale), stream))
+
+    def beam_select(self, logits, n_groups, n_beams, vocab, n_out, out_scores, out_beams, out_tokens, scores=None,
+                    row_stride=None, dtype=DTYPE_F32, stream=None):
+        """the n_out greatest of scores + log_softmax(logits) of every group, in order"""
+        _check(self.L.kvc_beam_select(self.ptr, self._p(logits), dtype, vocab if row_stride is None else row_stride,
+                                      n_groups, n_beams, vocab, self._p(scores), n_out, self._p(out_scores),
+                                      self._p(out_beams), self._p(out_tokens), stream))
 
     def decode_step(self, layer, seqs, qkv, q_norm, k_norm, out, in_dtype=DTYPE_BF16, out_dtype=DTYPE_F32,
                     scale=1.0 / 16, stream=None):
