@@ -25,28 +25,33 @@ __device__ __forceinline__ float beam_logit(const void* row, int t) {
     return x != x ? -INFINITY : x;
 }
 
+__device__ __forceinline__ float beam_clean(float x) { return x != x ? -INFINITY : x; }
+
 // One chunk of a row: 4 waves x STEPS loads of 16 B a lane, all in flight at once.
+// A segment's lanes are neighbours, and STEPS loads of theirs cover it.
 template <bool BF16, int STEPS>
 __global__ __launch_bounds__(256) void beam_max_kernel(BeamArgs a) {
-    constexpr int E = BF16 ? 8 : 4;            // tokens of a lane's load
-    constexpr int kSegLanes = kBeamSeg / E;    // 32 or 64
+    constexpr int E = BF16 ? 8 : 4;                    // tokens of a lane's load
+    constexpr int kSegLanes = kBeamSeg / (E * STEPS);  // 8 to 64
     __shared__ float2 red[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const size_t row = blockIdx.y;
     const uint8_t* base = static_cast<const uint8_t*>(a.logits) + row * (size_t)a.stride * (BF16 ? 2 : 4);
-    const int64_t at = ((int64_t)blockIdx.x * 4 + wave) * STEPS * (64 * E);  // of the wave
+    const int64_t j = ((int64_t)blockIdx.x * 4 + wave) * (64 / kSegLanes) + lane / kSegLanes;  // the lane's segment
+    const int64_t t0 = j * kBeamSeg + lane % kSegLanes * E;
     u32x4 w[STEPS];
 #pragma unroll
     for (int k = 0; k < STEPS; k++) {
-        const int64_t t = at + k * (64 * E) + lane * E;
+        const int64_t t = t0 + k * kSegLanes * E;
         if (t + E <= a.vocab) {
             w[k] = *reinterpret_cast<const u32x4_any*>(base + t * (BF16 ? 2 : 4));
         } else {  // the row's end: token by token, -inf behind it
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if constexpr (BF16) {
-                    const uint32_t lo = t + 2 * i < a.vocab ? reinterpret_cast<const uint16_t*>(base)[t + 2 * i] : 0xFF80u;
-                    const uint32_t hi = t + 2 * i + 1 < a.vocab ? reinterpret_cast<const uint16_t*>(base)[t + 2 * i + 1] : 0xFF80u;
+                    const uint16_t* x = reinterpret_cast<const uint16_t*>(base);
+                    const uint32_t lo = t + 2 * i < a.vocab ? x[t + 2 * i] : 0xFF80u;
+                    const uint32_t hi = t + 2 * i + 1 < a.vocab ? x[t + 2 * i + 1] : 0xFF80u;
                     w[k][i] = lo | hi << 16;
                 } else {
                     w[k][i] = t + i < a.vocab ? reinterpret_cast<const uint32_t*>(base)[t + i] : 0xFF800000u;
@@ -54,50 +59,50 @@ __global__ __launch_bounds__(256) void beam_max_kernel(BeamArgs a) {
             }
         }
     }
+    const auto logit = [&](int k, int i) {
+        if constexpr (BF16) return i & 1 ? bf16hi(w[k][i / 2]) : bf16lo(w[k][i / 2]);
+        return __uint_as_float(w[k][i]);
+    };
     float m = -INFINITY, s = 0.f;
 #pragma unroll
-    for (int k = 0; k < STEPS; k++) {
-        float x[E];
+    for (int k = 0; k < STEPS; k++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (BF16) {
-                x[2 * i] = bf16lo(w[k][i]);
-                x[2 * i + 1] = bf16hi(w[k][i]);
-            } else {
-                x[i] = __uint_as_float(w[k][i]);
-            }
-        }
-        float mx = -INFINITY;
+        for (int i = 0; i < E; i++) m = fmaxf(m, logit(k, i));
+    float me = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            x[i] = x[i] != x[i] ? -INFINITY : x[i];
-            mx = fmaxf(mx, x[i]);
-        }
-        float seg = mx;  // over the segment's lanes
-        seg = fmaxf(seg, dpp<kDppXor1>(seg));
-        seg = fmaxf(seg, dpp<kDppXor2>(seg));
-        seg = fmaxf(seg, dpp<kDppHalfMirror>(seg));
-        seg = fmaxf(seg, dpp<kDppRowRor8>(seg));
-        seg = max_xor16(seg);
-        if constexpr (kSegLanes == 64) seg = max_xor32(seg);
-        const int64_t j = (at + k * (64 * E) + lane * E) / kBeamSeg;
-        if (lane % kSegLanes == 0 && j < a.n_seg) a.seg_max[row * a.n_seg + j] = seg;
-        // running sum of exp(x - m); a row of -inf so far has m = -inf and sum 0
-        const float m2 = fmaxf(m, mx), me = m2 == -INFINITY ? 0.f : m2;
-        s *= fast_exp2((m - me) * kLog2e);
-        m = m2;
+    for (int k = 0; k < STEPS; k++)
 #pragma unroll
-        for (int i = 0; i < E; i++) s += fast_exp2((x[i] - me) * kLog2e);
+        for (int i = 0; i < E; i++) s += fast_exp2((logit(k, i) - me) * kLog2e);
+    if (s != s) {  // a NaN counts as -inf; so does +inf here, whose sum nobody reads
+        m = -INFINITY;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+#pragma unroll
+            for (int i = 0; i < E; i++) m = fmaxf(m, beam_clean(logit(k, i)));
+        me = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+#pragma unroll
+            for (int i = 0; i < E; i++) s += fast_exp2((beam_clean(logit(k, i)) - me) * kLog2e);
     }
+    float seg = m;  // over the segment's lanes
+    seg = fmaxf(seg, dpp<kDppXor1>(seg));
+    seg = fmaxf(seg, dpp<kDppXor2>(seg));
+    seg = fmaxf(seg, dpp<kDppHalfMirror>(seg));
+    if constexpr (kSegLanes >= 16) seg = fmaxf(seg, dpp<kDppRowRor8>(seg));
+    if constexpr (kSegLanes >= 32) seg = max_xor16(seg);
+    if constexpr (kSegLanes == 64) seg = max_xor32(seg);
+    if (lane % kSegLanes == 0 && j < a.n_seg) a.seg_max[row * a.n_seg + j] = seg;
     const float wm = wave_max(m), we = wm == -INFINITY ? 0.f : wm;
     s = wave_sum(s * fast_exp2((m - we) * kLog2e));
     if (lane == 0) red[wave] = make_float2(wm, s);
     __syncthreads();
     if (threadIdx.x == 0) {
-        const float M = fmaxf(fmaxf(red[0].x, red[1].x), fmaxf(red[2].x, red[3].x)), me = M == -INFINITY ? 0.f : M;
+        const float M = fmaxf(fmaxf(red[0].x, red[1].x), fmaxf(red[2].x, red[3].x)), e = M == -INFINITY ? 0.f : M;
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) t += red[i].y * fast_exp2((red[i].x - me) * kLog2e);
+        for (int i = 0; i < 4; i++) t += red[i].y * fast_exp2((red[i].x - e) * kLog2e);
         *reinterpret_cast<float2*>(a.chunk_sum + (row * a.n_chunks + blockIdx.x) * 2) = make_float2(M, t);
     }
 }
@@ -113,18 +118,18 @@ __device__ __forceinline__ double beam_value(uint64_t k) {
 }
 
 constexpr int kBeamThreads = 1024, kBeamWaves = kBeamThreads / 64;
-constexpr int kBeamCached = 8192;  // keys of segments held in LDS
-constexpr int kBeamCands = 1024;   // values that the last step sorts
+constexpr int kBeamHeld = 8;      // a thread's segment maxima in registers
+constexpr int kBeamCands = 1024;  // segments, then values, that are looked at one by one
 struct BeamSmem {
-    uint64_t keys[kBeamCached];
-    double off[kBeamMaxBeams];      // score - log sum exp(x - max); -inf for a beam that gives nothing
+    uint64_t cand[kBeamCands];   // key of a value, and where it is: beam << 32 | token
+    uint64_t where[kBeamCands];
+    double off[kBeamMaxBeams];   // score - log sum exp(x - max); -inf for a beam that gives nothing
     double max[kBeamMaxBeams];
     uint64_t red[2 * kBeamWaves];
+    int32_t list[kBeamCands];    // chosen segments
     int32_t hist[kBeamThreads];
     int32_t wsum[kBeamWaves];
-    int32_t list[kBeamMaxOut];      // chosen segments
-    uint64_t cand[kBeamCands];      // key of a value, and where it is: beam << 32 | token
-    uint64_t where[kBeamCands];
+    float wmax[kBeamWaves];
     int32_t count, bin, above;
 };
 
@@ -250,86 +255,149 @@ __device__ __forceinline__ void beam_collect(BeamSmem& sm, int n, uint64_t cut, 
     }
 }
 
-// A workgroup per group.
+// Distances from the greatest value, 32 parts to an octave from 2^-16 to 2^16.
+__device__ __forceinline__ int beam_part(double top, double v) {
+    const float d = (float)(top - v);
+    const int i = (int)(__float_as_uint(d > 0.f ? d : 0.f) >> 18) - (111 << 5);
+    return i < 0 ? 0 : i > 1023 ? 1023 : i;
+}
+
+// A workgroup per group.  A histogram of the segment maxima's distances from the
+// greatest finds a part that n_out of them reach; the values that reach it are among
+// those segments' and are few, since a part is 3 % of a distance: they are ranked by
+// counting.  Where they are more than can be held (rows of one level, say), the
+// n_out greatest maxima and then values are found exactly, equal ones by place.
 template <bool BF16>
 __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     __shared__ BeamSmem sm;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t row0 = (size_t)blockIdx.x * a.n_beams;
+    const int n_seg = a.n_seg, n = a.n_beams * n_seg;
+    const float* seg = a.seg_max + row0 * n_seg;
+    float held[kBeamHeld];
+#pragma unroll
+    for (int i = 0; i < kBeamHeld; i++) {
+        const int p = i * kBeamThreads + tid;
+        held[i] = p < n ? seg[p] : -INFINITY;
+    }
+    sm.hist[tid] = 0;
+    if (tid == 0) {
+        sm.count = 0;
+        sm.bin = kBeamThreads - 1;
+    }
     // A value is (score - log sum exp(x - max)) + (x - max), in 64 bits: large logits
     // cancel before the small sums join them.
     for (int b = wave; b < a.n_beams; b += kBeamWaves) {
-        const float* cs = a.chunk_sum + (row0 + b) * (size_t)a.n_chunks * 2;
-        float m = -INFINITY;
-        for (int c = lane; c < a.n_chunks; c += 64) m = fmaxf(m, cs[2 * c]);
+        const float2* cs = reinterpret_cast<const float2*>(a.chunk_sum) + (row0 + b) * (size_t)a.n_chunks;
+        const float score = a.scores ? a.scores[row0 + b] : 0.f;
+        const float2 first = lane < a.n_chunks ? cs[lane] : make_float2(-INFINITY, 0.f);
+        float m = first.x;
+        for (int c = lane + 64; c < a.n_chunks; c += 64) m = fmaxf(m, cs[c].x);
         m = wave_max(m);
         const bool fine = m > -INFINITY && m < INFINITY;
         double s = 0.0;
-        for (int c = lane; fine && c < a.n_chunks; c += 64) s += cs[2 * c + 1] * exp((double)cs[2 * c] - m);
+        if (fine) {
+            s = first.y * fast_exp2((first.x - m) * kLog2e);
+            for (int c = lane + 64; c < a.n_chunks; c += 64) s += cs[c].y * fast_exp2((cs[c].x - m) * kLog2e);
+        }
 #pragma unroll
         for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
         if (lane == 0) {
-            const float score = a.scores ? a.scores[row0 + b] : 0.f;
             sm.off[b] = fine && score > -INFINITY && score < INFINITY ? score - log(s) : -INFINITY;
             sm.max[b] = fine ? m : 0.0;
         }
     }
     __syncthreads();
-    const int n_seg = a.n_seg, n = a.n_beams * n_seg;
-    const float* seg = a.seg_max + row0 * n_seg;
     const auto beam_of = [&](int p) { return (int)((unsigned)p / (unsigned)n_seg); };
-    const auto key_of = [&](int b, float x) { return beam_key(sm.off[b] + ((double)x - sm.max[b])); };
-    const auto seg_key = [&](int p) { return key_of(beam_of(p), seg[p]); };
-    const bool cached = n <= kBeamCached;
-    if (cached) {
-        for (int p = tid; p < n; p += kBeamThreads) sm.keys[p] = seg_key(p);
+    const auto value_of = [&](int b, float x) { return sm.off[b] + ((double)x - sm.max[b]); };
+    const auto each = [&](auto&& f) {  // f(segment, its greatest value)
+#pragma unroll
+        for (int i = 0; i < kBeamHeld; i++) {
+            const int p = i * kBeamThreads + tid;
+            if (i * kBeamThreads >= n) break;
+            f(p, value_of(p < n ? beam_of(p) : 0, held[i]));
+        }
+        for (int p = kBeamHeld * kBeamThreads + tid; p < n; p += kBeamThreads) f(p, value_of(beam_of(p), seg[p]));
+    };
+    float top = -__FLT_MAX__;
+    each([&](int, double v) { top = fmaxf(top, (float)v); });
+    top = wave_max(top);
+    if (lane == 0) sm.wmax[wave] = top;
+    __syncthreads();
+    top = wave_max(sm.wmax[lane % kBeamWaves]);
+    each([&](int, double v) {
+        if (v > -INFINITY) atomicAdd(&sm.hist[beam_part(top, v)], 1);
+    });
+    __syncthreads();
+    {
+        const int h = sm.hist[tid];
+        int to = h;  // in this part and before it
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int y = __shfl_up(to, d);
+            to += lane >= d ? y : 0;
+        }
+        if (lane == 63) sm.wsum[wave] = to;
         __syncthreads();
+        for (int w = 0; w < wave; w++) to += sm.wsum[w];
+        if (to >= a.n_out && to - h < a.n_out) sm.bin = tid;
     }
-    const auto key = [&](int p) { return cached ? sm.keys[p] : seg_key(p); };
-    uint64_t cut;
-    int ties;
-    beam_cut(sm, n, a.n_out, key, &cut, &ties);
-    if (tid == 0) sm.count = 0;
     __syncthreads();
-    beam_collect(sm, n, cut, ties, key, [&](int p, uint64_t) { sm.list[atomicAdd(&sm.count, 1)] = p; });
+    const int last = sm.bin;
+    each([&](int p, double v) {
+        if (v > -INFINITY && beam_part(top, v) <= last) {
+            const int c = atomicAdd(&sm.count, 1);
+            if (c < kBeamCands) sm.list[c] = p;
+        }
+    });
     __syncthreads();
-    const int n_list = sm.count;
-    __syncthreads();
-    if (tid == 0) sm.count = 0;
-    __syncthreads();
-    // values of the chosen segments from the least chosen maximum on
     const size_t esz = BF16 ? 2 : 4;
     const uint8_t* rows = static_cast<const uint8_t*>(a.logits) + row0 * (size_t)a.stride * esz;
     const auto place = [&](int p, int i, int* b, int64_t* t) -> const void* {
         *b = beam_of(p);
-        const void* row = rows + (size_t)*b * (size_t)a.stride * esz;
         *t = (int64_t)(p - *b * n_seg) * kBeamSeg + i;
-        return row;
+        return rows + (size_t)*b * (size_t)a.stride * esz;
     };
-    for (int k = wave; k < n_list; k += kBeamWaves) {
-        const int p = sm.list[k];
-#pragma unroll
-        for (int i = 0; i < kBeamSeg / 64; i++) {
+    int n_list = sm.count, n_cand = kBeamCands + 1;
+    __syncthreads();
+    if (n_list <= kBeamCands) {
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+        constexpr int kPer = kBeamSeg / 64;
+        for (int k = wave; k < n_list; k += kBeamWaves) {
+            const int p = __builtin_amdgcn_readfirstlane(sm.list[k]);
             int b;
             int64_t t;
-            const void* row = place(p, 64 * i + lane, &b, &t);
-            if (t >= a.vocab) continue;
-            const uint64_t v = key_of(b, beam_logit<BF16>(row, (int)t));
-            if (v == 0 || v < cut) continue;
-            const int c = atomicAdd(&sm.count, 1);
-            if (c < kBeamCands) {
-                sm.cand[c] = v;
-                sm.where[c] = (uint64_t)b << 32 | (uint32_t)t;
+            const void* row = place(p, lane, &b, &t);
+            float x[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; i++) x[i] = t + 64 * i < a.vocab ? beam_logit<BF16>(row, (int)(t + 64 * i)) : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const double v = value_of(b, x[i]);
+                if (!(v > -INFINITY) || beam_part(top, v) > last) continue;
+                const int c = atomicAdd(&sm.count, 1);
+                if (c < kBeamCands) {
+                    sm.cand[c] = beam_key(v);
+                    sm.where[c] = (uint64_t)b << 32 | (uint32_t)(t + 64 * i);
+                }
             }
         }
+        __syncthreads();
+        n_cand = sm.count;
+        __syncthreads();
     }
-    __syncthreads();
-    int n_cand = sm.count;
-    __syncthreads();
     if (n_cand > kBeamCands) {
-        // many equal or close values: the segments in order of place, then exactly
-        // the n_out greatest, of equal ones the first
-        if (tid < n_list) {
+        const auto seg_key = [&](int p) { return beam_key(value_of(beam_of(p), seg[p])); };
+        uint64_t cut;
+        int ties;
+        beam_cut(sm, n, a.n_out, seg_key, &cut, &ties);
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+        beam_collect(sm, n, cut, ties, seg_key, [&](int p, uint64_t) { sm.list[atomicAdd(&sm.count, 1)] = p; });
+        __syncthreads();
+        n_list = sm.count;
+        if (tid < n_list) {  // in order of place
             const int p = sm.list[tid];
             int r = 0;
             for (int k = 0; k < n_list; k++) r += sm.list[k] < p;
@@ -338,18 +406,16 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
         __syncthreads();
         if (tid < n_list) sm.list[tid] = sm.hist[tid];
         __syncthreads();
-        const auto value = [&](int q) -> uint64_t {
+        const auto key = [&](int q) -> uint64_t {
             int b;
             int64_t t;
             const void* row = place(sm.list[q / kBeamSeg], q % kBeamSeg, &b, &t);
-            return t >= a.vocab ? 0 : key_of(b, beam_logit<BF16>(row, (int)t));
+            return t >= a.vocab ? 0 : beam_key(value_of(b, beam_logit<BF16>(row, (int)t)));
         };
-        uint64_t vcut;
-        int vties;
-        beam_cut(sm, n_list * kBeamSeg, a.n_out, value, &vcut, &vties);
+        beam_cut(sm, n_list * kBeamSeg, a.n_out, key, &cut, &ties);
         if (tid == 0) sm.count = 0;
         __syncthreads();
-        beam_collect(sm, n_list * kBeamSeg, vcut, vties, value, [&](int q, uint64_t v) {
+        beam_collect(sm, n_list * kBeamSeg, cut, ties, key, [&](int q, uint64_t v) {
             const int c = atomicAdd(&sm.count, 1);
             int b;
             int64_t t;
@@ -360,13 +426,18 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
         __syncthreads();
         n_cand = sm.count;
     }
-    // in order: greatest first, then the lower beam, then the lower token
+    // in order: greatest first, then the lower beam, then the lower token; a value's
+    // rank is counted by as many neighbouring lanes as there are threads for
     const size_t o = (size_t)blockIdx.x * a.n_out;
-    if (tid < n_cand) {
-        const uint64_t v = sm.cand[tid], w = sm.where[tid];
+    int lanes = 64;
+    while (lanes > 1 && lanes * n_cand > kBeamThreads) lanes /= 2;
+    const int c = tid / lanes;
+    if (tid - lane < n_cand * lanes) {  // (the wave has some)
+        const uint64_t v = c < n_cand ? sm.cand[c] : 0, w = c < n_cand ? sm.where[c] : 0;
         int r = 0;
-        for (int k = 0; k < n_cand; k++) r += sm.cand[k] > v || (sm.cand[k] == v && sm.where[k] < w);
-        if (r < a.n_out) {
+        for (int k = tid % lanes; k < n_cand; k += lanes) r += sm.cand[k] > v || (sm.cand[k] == v && sm.where[k] < w);
+        for (int d = 1; d < lanes; d *= 2) r += __shfl_xor(r, d);
+        if (c < n_cand && tid % lanes == 0 && r < a.n_out) {
             a.out_scores[o + r] = (float)beam_value(v);
             a.out_beams[o + r] = (int32_t)(w >> 32);
             a.out_tokens[o + r] = (int32_t)(uint32_t)w;
