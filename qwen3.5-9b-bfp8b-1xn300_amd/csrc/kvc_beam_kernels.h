@@ -27,6 +27,31 @@ __device__ __forceinline__ float beam_logit(const void* row, int t) {
 
 __device__ __forceinline__ float beam_clean(float x) { return x != x ? -INFINITY : x; }
 
+// A lane's 16 B of a row from token t on; -inf behind the row's end.
+template <bool BF16>
+__device__ __forceinline__ u32x4 beam_load(const uint8_t* row, int64_t t, int vocab) {
+    constexpr int E = BF16 ? 8 : 4;
+    if (t + E <= vocab) return *reinterpret_cast<const u32x4_any*>(row + t * (BF16 ? 2 : 4));
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (BF16) {
+            const uint16_t* x = reinterpret_cast<const uint16_t*>(row);
+            const uint32_t lo = t + 2 * i < vocab ? x[t + 2 * i] : 0xFF80u;
+            const uint32_t hi = t + 2 * i + 1 < vocab ? x[t + 2 * i + 1] : 0xFF80u;
+            w[i] = lo | hi << 16;
+        } else {
+            w[i] = t + i < vocab ? reinterpret_cast<const uint32_t*>(row)[t + i] : 0xFF800000u;
+        }
+    }
+    return w;
+}
+template <bool BF16>
+__device__ __forceinline__ float beam_word(const u32x4& w, int i) {
+    if constexpr (BF16) return i & 1 ? bf16hi(w[i / 2]) : bf16lo(w[i / 2]);
+    return __uint_as_float(w[i]);
+}
+
 // One chunk of a row: 4 waves x STEPS loads of 16 B a lane, all in flight at once.
 // A segment's lanes are neighbours, and STEPS loads of theirs cover it.
 template <bool BF16, int STEPS>
@@ -41,28 +66,8 @@ __global__ __launch_bounds__(256) void beam_max_kernel(BeamArgs a) {
     const int64_t t0 = j * kBeamSeg + lane % kSegLanes * E;
     u32x4 w[STEPS];
 #pragma unroll
-    for (int k = 0; k < STEPS; k++) {
-        const int64_t t = t0 + k * kSegLanes * E;
-        if (t + E <= a.vocab) {
-            w[k] = *reinterpret_cast<const u32x4_any*>(base + t * (BF16 ? 2 : 4));
-        } else {  // the row's end: token by token, -inf behind it
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (BF16) {
-                    const uint16_t* x = reinterpret_cast<const uint16_t*>(base);
-                    const uint32_t lo = t + 2 * i < a.vocab ? x[t + 2 * i] : 0xFF80u;
-                    const uint32_t hi = t + 2 * i + 1 < a.vocab ? x[t + 2 * i + 1] : 0xFF80u;
-                    w[k][i] = lo | hi << 16;
-                } else {
-                    w[k][i] = t + i < a.vocab ? reinterpret_cast<const uint32_t*>(base)[t + i] : 0xFF800000u;
-                }
-            }
-        }
-    }
-    const auto logit = [&](int k, int i) {
-        if constexpr (BF16) return i & 1 ? bf16hi(w[k][i / 2]) : bf16lo(w[k][i / 2]);
-        return __uint_as_float(w[k][i]);
-    };
+    for (int k = 0; k < STEPS; k++) w[k] = beam_load<BF16>(base, t0 + k * kSegLanes * E, a.vocab);
+    const auto logit = [&](int k, int i) { return beam_word<BF16>(w[k], i); };
     float m = -INFINITY, s = 0.f;
 #pragma unroll
     for (int k = 0; k < STEPS; k++)
@@ -262,8 +267,8 @@ __device__ __forceinline__ int beam_part(double top, double v) {
     return i < 0 ? 0 : i > 1023 ? 1023 : i;
 }
 
-// A workgroup per group.  A histogram of the segment maxima's distances from the
-// greatest finds a part that n_out of them reach; the values that reach it are among
+// A workgroup per group.  A histogram of the threads' greatest segment maxima, by their
+// distance from the greatest of all, finds a part that n_out of them reach; the values that reach it are among
 // those segments' and are few, since a part is 3 % of a distance: they are ranked by
 // counting.  Where they are more than can be held (rows of one level, say), the
 // n_out greatest maxima and then values are found exactly, equal ones by place.
@@ -295,39 +300,38 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
         for (int c = lane + 64; c < a.n_chunks; c += 64) m = fmaxf(m, cs[c].x);
         m = wave_max(m);
         const bool fine = m > -INFINITY && m < INFINITY;
-        double s = 0.0;
+        float s = 0.f;
         if (fine) {
             s = first.y * fast_exp2((first.x - m) * kLog2e);
             for (int c = lane + 64; c < a.n_chunks; c += 64) s += cs[c].y * fast_exp2((cs[c].x - m) * kLog2e);
         }
-#pragma unroll
-        for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
+        s = wave_sum(s);
         if (lane == 0) {
-            sm.off[b] = fine && score > -INFINITY && score < INFINITY ? score - log(s) : -INFINITY;
+            sm.off[b] = fine && score > -INFINITY && score < INFINITY ? score - log((double)s) : -INFINITY;
             sm.max[b] = fine ? m : 0.0;
         }
     }
     __syncthreads();
     const auto beam_of = [&](int p) { return (int)((unsigned)p / (unsigned)n_seg); };
     const auto value_of = [&](int b, float x) { return sm.off[b] + ((double)x - sm.max[b]); };
-    const auto each = [&](auto&& f) {  // f(segment, its greatest value)
+    double val[kBeamHeld];
+    double mine = -INFINITY;  // the thread's greatest
 #pragma unroll
-        for (int i = 0; i < kBeamHeld; i++) {
-            const int p = i * kBeamThreads + tid;
-            if (i * kBeamThreads >= n) break;
-            f(p, value_of(p < n ? beam_of(p) : 0, held[i]));
-        }
-        for (int p = kBeamHeld * kBeamThreads + tid; p < n; p += kBeamThreads) f(p, value_of(beam_of(p), seg[p]));
-    };
-    float top = -__FLT_MAX__;
-    each([&](int, double v) { top = fmaxf(top, (float)v); });
-    top = wave_max(top);
+    for (int i = 0; i < kBeamHeld; i++) {
+        const int p = i * kBeamThreads + tid;
+        val[i] = -INFINITY;
+        if (i * kBeamThreads < n) val[i] = value_of(p < n ? beam_of(p) : 0, held[i]);
+        mine = val[i] > mine ? val[i] : mine;
+    }
+    for (int p = kBeamHeld * kBeamThreads + tid; p < n; p += kBeamThreads) {
+        const double v = value_of(beam_of(p), seg[p]);
+        mine = v > mine ? v : mine;
+    }
+    float top = wave_max(fmaxf((float)mine, -__FLT_MAX__));
     if (lane == 0) sm.wmax[wave] = top;
     __syncthreads();
     top = wave_max(sm.wmax[lane % kBeamWaves]);
-    each([&](int, double v) {
-        if (v > -INFINITY) atomicAdd(&sm.hist[beam_part(top, v)], 1);
-    });
+    if (mine > -INFINITY) atomicAdd(&sm.hist[beam_part(top, mine)], 1);
     __syncthreads();
     {
         const int h = sm.hist[tid];
@@ -344,16 +348,20 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     }
     __syncthreads();
     const int last = sm.bin;
-    each([&](int p, double v) {
-        if (v > -INFINITY && beam_part(top, v) <= last) {
-            const int c = atomicAdd(&sm.count, 1);
-            if (c < kBeamCands) sm.list[c] = p;
-        }
-    });
+    const auto choose = [&](int p, double v) {
+        if (!(v > -INFINITY) || beam_part(top, v) > last) return;
+        const int c = atomicAdd(&sm.count, 1);
+        if (c < kBeamCands) sm.list[c] = p;
+    };
+    if (mine > -INFINITY && beam_part(top, mine) <= last) {
+#pragma unroll
+        for (int i = 0; i < kBeamHeld; i++) choose(i * kBeamThreads + tid, val[i]);
+        for (int p = kBeamHeld * kBeamThreads + tid; p < n; p += kBeamThreads) choose(p, value_of(beam_of(p), seg[p]));
+    }
     __syncthreads();
     const size_t esz = BF16 ? 2 : 4;
     const uint8_t* rows = static_cast<const uint8_t*>(a.logits) + row0 * (size_t)a.stride * esz;
-    const auto place = [&](int p, int i, int* b, int64_t* t) -> const void* {
+    const auto place = [&](int p, int i, int* b, int64_t* t) -> const uint8_t* {
         *b = beam_of(p);
         *t = (int64_t)(p - *b * n_seg) * kBeamSeg + i;
         return rows + (size_t)*b * (size_t)a.stride * esz;
@@ -363,23 +371,20 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     if (n_list <= kBeamCands) {
         if (tid == 0) sm.count = 0;
         __syncthreads();
-        constexpr int kPer = kBeamSeg / 64;
-        for (int k = wave; k < n_list; k += kBeamWaves) {
-            const int p = __builtin_amdgcn_readfirstlane(sm.list[k]);
+        constexpr int E = BF16 ? 8 : 4, kLanes = kBeamSeg / E;
+        for (int k = tid / kLanes; k < n_list; k += kBeamThreads / kLanes) {
             int b;
             int64_t t;
-            const void* row = place(p, lane, &b, &t);
-            float x[kPer];
+            const uint8_t* row = place(sm.list[k], tid % kLanes * E, &b, &t);
+            const u32x4 w = beam_load<BF16>(row, t, a.vocab);
 #pragma unroll
-            for (int i = 0; i < kPer; i++) x[i] = t + 64 * i < a.vocab ? beam_logit<BF16>(row, (int)(t + 64 * i)) : -INFINITY;
-#pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const double v = value_of(b, x[i]);
+            for (int i = 0; i < E; i++) {
+                const double v = value_of(b, beam_clean(beam_word<BF16>(w, i)));
                 if (!(v > -INFINITY) || beam_part(top, v) > last) continue;
                 const int c = atomicAdd(&sm.count, 1);
                 if (c < kBeamCands) {
                     sm.cand[c] = beam_key(v);
-                    sm.where[c] = (uint64_t)b << 32 | (uint32_t)(t + 64 * i);
+                    sm.where[c] = (uint64_t)b << 32 | (uint32_t)(t + i);
                 }
             }
         }
