@@ -58,6 +58,12 @@ float* d_norm_w = nullptr;  // fp32 [n_attn][2][256]: q_norm, k_norm
 float* d_ssm_w = nullptr;   // fp32 [n_ssm][kSsmW]
 uint16_t *d_qkv = nullptr, *d_q = nullptr, *d_gate = nullptr, *d_out = nullptr;
 uint16_t *d_ssm_in = nullptr, *d_ssm_out = nullptr;
+// beam search: logits of every beam, their scores, and what was chosen of them
+uint16_t* d_logits = nullptr;  // bf16 [max_beams][kVocab]
+float* d_scores = nullptr;     // fp32 [max_beams]
+int32_t* d_picked = nullptr;   // [beams | tokens]
+int g_max_beams = 0;
+std::vector<StepOutput> g_beam_steps;
 const std::vector<int> kNoTokens;
 const std::vector<StepOutput> kNoSteps;
 
@@ -281,16 +287,20 @@ bool process_tokens(Session& ss, const int* tok, int n, int pos0) {
 }
 
 void free_device() {
-    for (uint16_t** p : {&d_qkv, &d_q, &d_gate, &d_out, &d_ssm_in, &d_ssm_out})
+    for (uint16_t** p : {&d_qkv, &d_q, &d_gate, &d_out, &d_ssm_in, &d_ssm_out, &d_logits})
         if (*p) {
             (void)hipFree(*p);
             *p = nullptr;
         }
-    for (float** p : {&d_norm_w, &d_ssm_w})
+    for (float** p : {&d_norm_w, &d_ssm_w, &d_scores})
         if (*p) {
             (void)hipFree(*p);
             *p = nullptr;
         }
+    if (d_picked) {
+        (void)hipFree(d_picked);
+        d_picked = nullptr;
+    }
 }
 
 // Context budget of a prompt (src/engine.cpp:4048-4056): it keeps its last
@@ -308,6 +318,182 @@ bool reset_one(Session& ss) {
     ss.cached_tokens.clear();
     ss.out_digest = 0;
     return kvc_ok(kvc_seq_reset(g_ctx, ss.seq), "kvc_seq_reset");
+}
+
+Session* open_session(int session, const char* what) {
+    if (!g_loaded) {
+        fprintf(stderr, "%s: no model loaded\n", what);
+        return nullptr;
+    }
+    Session* ss = session_at(session);
+    if (!ss) fprintf(stderr, "%s: session %d is not open\n", what, session);
+    return ss;
+}
+
+// The prompt of a request, truncated to its budget, through every layer of the
+// session: what is cached is reused, the rest is prefilled in batches.
+bool prefill_prompt(Session& ss, int session, const std::vector<int>& prompt_tokens, int max_tokens, const char* what,
+                    std::vector<int>& tokens) {
+    ss.steps.clear();
+
+    const int budget = prompt_budget(max_tokens);
+    const size_t cut = prompt_tokens.size() > (size_t)budget ? prompt_tokens.size() - (size_t)budget : 0;
+    if (cut && g_cfg.verbose)
+        printf("  [prompt of %zu tokens: the first %zu dropped, context %d]\n", prompt_tokens.size(), cut, g_max_ctx);
+    tokens.assign(prompt_tokens.begin() + (std::ptrdiff_t)cut, prompt_tokens.end());
+    if (tokens.empty()) {
+        fprintf(stderr, "%s: empty prompt\n", what);
+        return false;
+    }
+
+    // Prefix reuse (src/engine.cpp:4058-4080).  The reference keeps one token
+    // list and reuses it only when it is a strict prefix of the prompt; the
+    // library matches against every block any session has committed, at
+    // 32-token block granularity and, with recurrent layers, at a state
+    // snapshot boundary, and never the whole prompt (one token must run to
+    // produce logits).
+    if (!reset_one(ss)) return false;
+    std::vector<int32_t> t32(tokens.begin(), tokens.end());
+    int32_t reuse = 0;
+    if (!kvc_ok(kvc_prefix_match(g_ctx, ss.seq, t32.data(), (int32_t)t32.size(), &reuse, nullptr),
+                "kvc_prefix_match"))
+        return false;
+    ss.last_prefix = reuse;
+    ss.cached_tokens.assign(tokens.begin(), tokens.begin() + reuse);
+    // the recurrent layers resume from the restored snapshot state; with
+    // verify_restore it is checked against the hash taken at that boundary
+    if (g_cfg.verify_restore && reuse > 0 && g_cfg.n_ssm_layers > 0) {
+        auto it = g_boundary_state.find(token_prefix_hash(tokens.data(), reuse));
+        if (it != g_boundary_state.end()) {
+            uint64_t h = 0;
+            if (!state_hash(ss.seq, &h)) return false;
+            g_checks++;
+            if (h != it->second) g_mismatches++;
+        }
+    }
+    const int n_prompt = (int)tokens.size();
+    if (reuse > 0 && g_cfg.verbose)
+        printf("  [session %d: %d cached tokens reused, %d to prefill]\n", session, reuse, n_prompt - reuse);
+
+    const auto t0 = std::chrono::high_resolution_clock::now();
+    for (int at = reuse; at < n_prompt;) {
+        const int batch = std::min(kPrefillBatch, n_prompt - at);
+        if (!process_tokens(ss, tokens.data() + at, batch, at)) return false;
+        ss.cached_tokens.insert(ss.cached_tokens.end(), tokens.begin() + at, tokens.begin() + at + batch);
+        at += batch;
+    }
+    g_last_prefill_ms = std::chrono::duration<double, std::milli>(std::chrono::high_resolution_clock::now() - t0).count();
+    if (g_cfg.verbose) printf("  [prefill: %.1f ms for %d tokens]\n", g_last_prefill_ms, n_prompt - reuse);
+    return true;
+}
+
+// ---- beam search -------------------------------------------------------------
+
+// Logits of beam i, from the tokens before them alone, so that a search does not
+// depend on how its attention was rounded.
+bool synthetic_logits(int i, const std::vector<int>& history) {
+    const uint64_t seed = mix64(g_cfg.seed ^ token_prefix_hash(history.data(), (int)history.size()));
+    mark(i, 5);
+    return kvc_ok(kvc_fill_normal_bf16(g_ctx, d_logits + (size_t)i * kVocab, kVocab, seed, 3.0f, nullptr),
+                  "kvc_fill_normal_bf16");
+}
+
+// The next token of every beam, at position p, through every layer: the batched
+// decode step, whose attention reads the blocks that beams share once.
+bool process_beams(const std::vector<int32_t>& seqs, const std::vector<int>& tok, int p, std::vector<StepOutput>& steps) {
+    const int n = (int)seqs.size();
+    if (!kvc_ok(kvc_seq_reserve(g_ctx, seqs.data(), n, 1, nullptr), "kvc_seq_reserve")) return false;
+    steps.assign(n, StepOutput());
+    for (int i = 0; i < n; i++) {
+        steps[i].pos = p;
+        steps[i].token = tok[i];
+        steps[i].digest = 0x73746570ULL;
+        if (g_cfg.keep_outputs) {
+            steps[i].out.resize(g_cfg.n_attn_layers);
+            steps[i].ssm_out.resize(g_cfg.n_ssm_layers);
+        }
+    }
+    std::vector<uint16_t> rows((size_t)n * std::max(kQkvRow, kSsmRow)), out((size_t)n * kQRow);
+    for (int layer = 0; layer < g_cfg.n_attn_layers; layer++) {
+        for (int i = 0; i < n; i++)
+            normal_bf16(projection_key(layer, tok[i], p, 0), &rows[(size_t)i * kQkvRow], kQkvRow);
+        mark(layer, 4);
+        const float* nw = d_norm_w + (size_t)layer * 2 * kHeadDim;
+        if (!hip_ok(hipMemcpy(d_qkv, rows.data(), (size_t)n * kQkvRow * 2, hipMemcpyHostToDevice), "upload qkv") ||
+            !kvc_ok(kvc_qkv_append(g_ctx, layer, seqs.data(), n, 1, d_qkv, KVC_DTYPE_BF16, nw, nw + kHeadDim, d_q, d_gate,
+                                   nullptr),
+                    "kvc_qkv_append") ||
+            !kvc_ok(kvc_decode_attn_shared(g_ctx, layer, seqs.data(), n, d_q, nullptr, nullptr, d_gate, d_out,
+                                           KVC_DTYPE_BF16, kAttnScale, nullptr),
+                    "kvc_decode_attn_shared"))
+            return false;
+        mark(layer, 1);
+        if (!hip_ok(hipMemcpy(out.data(), d_out, out.size() * 2, hipMemcpyDeviceToHost), "download out")) return false;
+        for (int i = 0; i < n; i++) {
+            const auto row = out.begin() + (size_t)i * kQRow;
+            steps[i].digest = hash_bytes(&*row, kQRow * 2, steps[i].digest);
+            if (g_cfg.keep_outputs) steps[i].out[layer].assign(row, row + kQRow);
+        }
+    }
+    out.resize((size_t)n * kSsmOut);
+    for (int l = 0; l < g_cfg.n_ssm_layers; l++) {
+        for (int i = 0; i < n; i++)
+            normal_bf16(projection_key(1000 + l, tok[i], p, 4), &rows[(size_t)i * kSsmRow], kSsmRow);
+        mark(1000 + l, 4);
+        const float* w = d_ssm_w + (size_t)l * kSsmW;
+        if (!hip_ok(hipMemcpy(d_ssm_in, rows.data(), (size_t)n * kSsmRow * 2, hipMemcpyHostToDevice), "upload ssm") ||
+            !kvc_ok(kvc_deltanet_step(g_ctx, l, seqs.data(), n, 1, d_ssm_in, KVC_DTYPE_BF16, w, w + 4 * kSsmC,
+                                      w + 4 * kSsmC + kSsmVHeads, w + 4 * kSsmC + 2 * kSsmVHeads, d_ssm_out,
+                                      KVC_DTYPE_BF16, nullptr),
+                    "kvc_deltanet_step"))
+            return false;
+        mark(l, 2);
+        if (!hip_ok(hipMemcpy(out.data(), d_ssm_out, out.size() * 2, hipMemcpyDeviceToHost), "download ssm out"))
+            return false;
+        for (int i = 0; i < n; i++) {
+            const auto row = out.begin() + (size_t)i * kSsmOut;
+            steps[i].digest = hash_bytes(&*row, kSsmOut * 2, steps[i].digest);
+            if (g_cfg.keep_outputs) steps[i].ssm_out[l].assign(row, row + kSsmOut);
+        }
+    }
+    return kvc_ok(kvc_seq_commit(g_ctx, seqs.data(), n, 1, tok.data(), nullptr), "kvc_seq_commit");
+}
+
+// One choice: the `want` best continuations of `beams` (behind `prompt`) replace
+// them; parents[i] is what beam i continues.  The scores so far are d_scores; the
+// first choice has none.
+bool choose_beams(const std::vector<int>& prompt, bool first, int want, std::vector<Beam>& beams,
+                  std::vector<int32_t>& parents) {
+    const int from = (int)beams.size();
+    std::vector<int> history(prompt);
+    for (int i = 0; i < from; i++) {
+        history.resize(prompt.size());
+        history.insert(history.end(), beams[i].tokens.begin(), beams[i].tokens.end());
+        if (!synthetic_logits(i, history)) return false;
+    }
+    if (!kvc_ok(kvc_beam_select(g_ctx, d_logits, KVC_DTYPE_BF16, kVocab, 1, from, kVocab, first ? nullptr : d_scores, want, d_scores, d_picked,
+                                d_picked + want, nullptr),
+                "kvc_beam_select"))
+        return false;
+    std::vector<float> score(want);
+    std::vector<int32_t> picked(2 * (size_t)want);
+    mark(want, 5);
+    if (!hip_ok(hipMemcpy(score.data(), d_scores, (size_t)want * 4, hipMemcpyDeviceToHost), "download scores") ||
+        !hip_ok(hipMemcpy(picked.data(), d_picked, picked.size() * 4, hipMemcpyDeviceToHost), "download beams"))
+        return false;
+    std::vector<Beam> next(want);
+    parents.assign(picked.begin(), picked.begin() + want);
+    for (int i = 0; i < want; i++) {
+        if (parents[i] < 0) {
+            fprintf(stderr, "kvc_beam_select: fewer than %d continuations\n", want);
+            return false;
+        }
+        next[i].tokens = beams[parents[i]].tokens;
+        next[i].tokens.push_back(picked[(size_t)want + i]);
+        next[i].score = score[i];
+    }
+    beams = std::move(next);
+    return true;
 }
 
 }  // namespace
@@ -340,11 +526,12 @@ bool load_model_and_tokenizer(const char* model_path, int max_ctx) {
     g_cfg.seed = model_seed(model_path);
     g_max_ctx = max_ctx;
     const int n_sessions = std::max(1, g_cfg.max_sessions);
+    g_max_beams = std::min(std::max(0, g_cfg.max_beams), kPrefillBatch);  // (the staging holds a batch)
     kvc_config kc;
     kvc_config_default(&kc);
     kc.n_attn_layers = g_cfg.n_attn_layers;
     kc.n_ssm_layers = g_cfg.n_ssm_layers;
-    kc.max_seqs = n_sessions;
+    kc.max_seqs = n_sessions + g_max_beams;
     kc.max_seq_len = max_ctx;
     kc.pool_blocks = g_cfg.pool_blocks;
     kc.pool_fraction = g_cfg.pool_fraction;
@@ -358,6 +545,10 @@ bool load_model_and_tokenizer(const char* model_path, int max_ctx) {
               hip_ok(hipMalloc((void**)&d_out, B * kQRow * 2), "hipMalloc") &&
               hip_ok(hipMalloc((void**)&d_ssm_in, B * kSsmRow * 2), "hipMalloc") &&
               hip_ok(hipMalloc((void**)&d_ssm_out, B * kSsmOut * 2), "hipMalloc") &&
+              (g_max_beams == 0 ||
+               (hip_ok(hipMalloc((void**)&d_logits, (size_t)g_max_beams * kVocab * 2), "hipMalloc") &&
+                hip_ok(hipMalloc((void**)&d_scores, (size_t)g_max_beams * 4), "hipMalloc") &&
+                hip_ok(hipMalloc((void**)&d_picked, (size_t)g_max_beams * 8), "hipMalloc"))) &&
               hip_ok(hipMalloc((void**)&d_norm_w, (size_t)std::max(1, g_cfg.n_attn_layers) * 2 * kHeadDim * 4),
                      "hipMalloc") &&
               hip_ok(hipMalloc((void**)&d_ssm_w, (size_t)std::max(1, g_cfg.n_ssm_layers) * kSsmW * 4), "hipMalloc");
@@ -383,6 +574,7 @@ bool load_model_and_tokenizer(const char* model_path, int max_ctx) {
         return false;
     }
     g_boundary_state.clear();
+    g_beam_steps.clear();
     g_mismatches = g_checks = 0;
     mark(-1, 0);
     return true;
@@ -443,67 +635,11 @@ int generate(const std::vector<int>& prompt_tokens, int max_tokens, float temper
 
 int generate_session(int session, const std::vector<int>& prompt_tokens, int max_tokens, float temperature,
                      TokenCallback cb, StopReason* stop_reason) {
-    if (!g_loaded) {
-        fprintf(stderr, "generate: no model loaded\n");
-        return 0;
-    }
-    Session* sp = session_at(session);
-    if (!sp) {
-        fprintf(stderr, "generate: session %d is not open\n", session);
-        return 0;
-    }
+    Session* sp = open_session(session, "generate");
+    std::vector<int> tokens;
+    if (!sp || !prefill_prompt(*sp, session, prompt_tokens, max_tokens, "generate", tokens)) return 0;
     Session& ss = *sp;
-    ss.steps.clear();
-
-    const int budget = prompt_budget(max_tokens);
-    const size_t cut = prompt_tokens.size() > (size_t)budget ? prompt_tokens.size() - (size_t)budget : 0;
-    if (cut && g_cfg.verbose)
-        printf("  [prompt of %zu tokens: the first %zu dropped, context %d]\n", prompt_tokens.size(), cut, g_max_ctx);
-    const std::vector<int> tokens(prompt_tokens.begin() + (std::ptrdiff_t)cut, prompt_tokens.end());
-    if (tokens.empty()) {
-        fprintf(stderr, "generate: empty prompt\n");
-        return 0;
-    }
-
-    // Prefix reuse (src/engine.cpp:4058-4080).  The reference keeps one token
-    // list and reuses it only when it is a strict prefix of the prompt; the
-    // library matches against every block any session has committed, at
-    // 32-token block granularity and, with recurrent layers, at a state
-    // snapshot boundary, and never the whole prompt (one token must run to
-    // produce logits).
-    if (!reset_one(ss)) return 0;
-    std::vector<int32_t> t32(tokens.begin(), tokens.end());
-    int32_t reuse = 0;
-    if (!kvc_ok(kvc_prefix_match(g_ctx, ss.seq, t32.data(), (int32_t)t32.size(), &reuse, nullptr),
-                "kvc_prefix_match"))
-        return 0;
-    ss.last_prefix = reuse;
-    ss.cached_tokens.assign(tokens.begin(), tokens.begin() + reuse);
-    // the recurrent layers resume from the restored snapshot state; with
-    // verify_restore it is checked against the hash taken at that boundary
-    if (g_cfg.verify_restore && reuse > 0 && g_cfg.n_ssm_layers > 0) {
-        auto it = g_boundary_state.find(token_prefix_hash(tokens.data(), reuse));
-        if (it != g_boundary_state.end()) {
-            uint64_t h = 0;
-            if (!state_hash(ss.seq, &h)) return 0;
-            g_checks++;
-            if (h != it->second) g_mismatches++;
-        }
-    }
-    const int n_prompt = (int)tokens.size();
-    if (reuse > 0 && g_cfg.verbose)
-        printf("  [session %d: %d cached tokens reused, %d to prefill]\n", session, reuse, n_prompt - reuse);
-
-    const auto t0 = std::chrono::high_resolution_clock::now();
-    for (int at = reuse; at < n_prompt;) {
-        const int batch = std::min(kPrefillBatch, n_prompt - at);
-        if (!process_tokens(ss, tokens.data() + at, batch, at)) return 0;
-        ss.cached_tokens.insert(ss.cached_tokens.end(), tokens.begin() + at, tokens.begin() + at + batch);
-        at += batch;
-    }
-    int next_token = sample_token(ss, tokens.back(), n_prompt, temperature);
-    g_last_prefill_ms = std::chrono::duration<double, std::milli>(std::chrono::high_resolution_clock::now() - t0).count();
-    if (g_cfg.verbose) printf("  [prefill: %.1f ms for %d tokens]\n", g_last_prefill_ms, n_prompt - reuse);
+    int next_token = sample_token(ss, tokens.back(), (int)tokens.size(), temperature);
 
     // decode loop (src/engine.cpp:4128-4154): every emitted token is fed back
     int emitted = 0;
@@ -521,6 +657,47 @@ int generate_session(int session, const std::vector<int>& prompt_tokens, int max
     }
     if (stop_reason) *stop_reason = why;
     return emitted;
+}
+
+int generate_beams(int session, const std::vector<int>& prompt_tokens, int n_beams, int max_tokens,
+                   std::vector<Beam>& beams) {
+    beams.clear();
+    g_beam_steps.clear();
+    Session* ss = open_session(session, "generate_beams");
+    if (!ss) return 0;
+    if (n_beams < 1 || n_beams > g_max_beams || max_tokens < 1) {
+        fprintf(stderr, "generate_beams: %d beams of %d tokens (at most %d beams)\n", n_beams, max_tokens, g_max_beams);
+        return 0;
+    }
+    std::vector<int> tokens;
+    if (!prefill_prompt(*ss, session, prompt_tokens, max_tokens, "generate_beams", tokens)) return 0;
+    // the first choice is among the continuations of the prompt alone; then every
+    // beam takes a sequence of its own, a fork of the session's
+    std::vector<Beam> cur(1);
+    std::vector<int32_t> parents, seqs(n_beams, -1);
+    bool ok = choose_beams(tokens, true, n_beams, cur, parents);
+    for (int i = 0; ok && i < n_beams; i++) ok = kvc_ok(kvc_seq_create(g_ctx, &seqs[i]), "kvc_seq_create");
+    if (ok && max_tokens > 1) {
+        const std::vector<int32_t> src(n_beams, ss->seq);
+        ok = kvc_ok(kvc_seq_fork(g_ctx, src.data(), seqs.data(), n_beams, nullptr), "kvc_seq_fork");
+    }
+    std::vector<StepOutput> steps;
+    int n = 1;
+    for (; ok && n < max_tokens && (int)tokens.size() + n - 1 < g_max_ctx; n++) {
+        std::vector<int> last(n_beams);
+        for (int i = 0; i < n_beams; i++) last[i] = cur[i].tokens.back();
+        ok = process_beams(seqs, last, (int)tokens.size() + n - 1, steps) &&
+             choose_beams(tokens, false, n_beams, cur, parents) &&
+             kvc_ok(kvc_seq_reorder(g_ctx, seqs.data(), parents.data(), n_beams, nullptr), "kvc_seq_reorder");
+        if (!ok) break;
+        g_beam_steps.clear();
+        for (int i = 0; i < n_beams; i++) g_beam_steps.push_back(steps[parents[i]]);
+    }
+    for (int32_t s : seqs)
+        if (s >= 0) ok = kvc_ok(kvc_seq_release(g_ctx, s), "kvc_seq_release") && ok;
+    if (!ok) return 0;
+    beams = std::move(cur);
+    return n;
 }
 
 int pos(int session) {
@@ -544,6 +721,7 @@ int32_t sequence(int session) {
     const Session* ss = session_at(session);
     return ss ? ss->seq : -1;
 }
+const std::vector<StepOutput>& beam_outputs() { return g_beam_steps; }
 const std::vector<StepOutput>& step_outputs(int session) {
     const Session* ss = session_at(session);
     return ss ? ss->steps : kNoSteps;

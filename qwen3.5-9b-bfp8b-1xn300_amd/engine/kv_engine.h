@@ -68,6 +68,7 @@ struct EngineConfig {
     bool verify_restore = false; // hash the recurrent state at snapshot boundaries and
                                  // check restored states against it (costly)
     bool verbose = false;        // print the reference's progress lines
+    int max_beams = 0;           // beams of generate_beams(): libkvc sequences of their own, at most 32
 };
 
 // Synthetic vocabulary size (Qwen tokenizer ids are < 151936).
@@ -89,7 +90,8 @@ void shutdown();
 // :4182-4185).  op: 0 none, 1 attention output read (layer = attention layer),
 // 2 Gated-DeltaNet output read (layer = recurrent layer), 3 recurrent-state
 // read of verify_restore (layer = recurrent layer), 4 projection-row upload
-// (layer = attention layer, or 1000 + recurrent layer).  The reference's op
+// (layer = attention layer, or 1000 + recurrent layer), 5 beam selection (layer =
+// beam).  The reference's op
 // numbers name its Tensix reads; these name this engine's blocking HIP calls.
 void get_hang_info(int& layer, int& op);
 double get_last_prefill_ms();
@@ -102,6 +104,21 @@ bool release_session(int session);
 bool reset_session(int session);   // reset_state() of one session
 int generate_session(int session, const std::vector<int>& prompt_tokens, int max_tokens, float temperature,
                      TokenCallback cb, StopReason* stop_reason = nullptr);
+
+// Beam search (no counterpart in the reference, which samples one continuation):
+// the prompt as in generate_session(), then the n_beams best continuations by the
+// sum of their tokens' log probabilities, kept step by step.  The beams fork the
+// session's sequence, decode together (kvc_decode_attn_shared), are chosen by
+// kvc_beam_select and follow their parents by kvc_seq_reorder; the session itself
+// stays at the prompt.  The logits are synthetic, N(0, 3) from the seed and the
+// tokens before them alone.  Returns the tokens per beam (max_tokens, or what the
+// context holds) with the beams best first, 0 on error.
+struct Beam {
+    std::vector<int> tokens;
+    float score = 0.f;
+};
+int generate_beams(int session, const std::vector<int>& prompt_tokens, int n_beams, int max_tokens,
+                   std::vector<Beam>& beams);
 
 // ---- KV-path introspection (tests); session 0 unless given ---------------------
 int pos(int session = 0);                                // g_pos
@@ -127,6 +144,9 @@ struct StepOutput {
     std::vector<std::vector<uint16_t>> ssm_out;  // [ssm layer][32 * 128]
     std::vector<std::vector<uint16_t>> q, gate;  // [attn layer][16 * 256], decode steps only
 };
+// the last position that the last generate_beams() processed of each beam (that of
+// its last token but one); empty if it stopped at the first choice
+const std::vector<StepOutput>& beam_outputs();
 // positions processed by the session's last generate
 const std::vector<StepOutput>& step_outputs(int session = 0);
 
