@@ -333,7 +333,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     top = wave_max(sm.wmax[lane % kBeamWaves]);
     if (mine > -INFINITY) atomicAdd(&sm.hist[beam_part(top, mine)], 1);
     __syncthreads();
-    {
+    const auto reached = [&] {  // the first part that n_out of those counted reach, or the last
         const int h = sm.hist[tid];
         int to = h;  // in this part and before it
 #pragma unroll
@@ -345,9 +345,10 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
         __syncthreads();
         for (int w = 0; w < wave; w++) to += sm.wsum[w];
         if (to >= a.n_out && to - h < a.n_out) sm.bin = tid;
-    }
-    __syncthreads();
-    const int last = sm.bin;
+        __syncthreads();
+        return sm.bin;
+    };
+    const int last = reached();
     const auto choose = [&](int p, double v) {
         if (!(v > -INFINITY) || beam_part(top, v) > last) return;
         const int c = atomicAdd(&sm.count, 1);
@@ -369,27 +370,61 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     int n_list = sm.count, n_cand = kBeamCands + 1;
     __syncthreads();
     if (n_list <= kBeamCands) {
-        if (tid == 0) sm.count = 0;
-        __syncthreads();
         constexpr int E = BF16 ? 8 : 4, kLanes = kBeamSeg / E;
-        for (int k = tid / kLanes; k < n_list; k += kBeamThreads / kLanes) {
-            int b;
-            int64_t t;
-            const uint8_t* row = place(sm.list[k], tid % kLanes * E, &b, &t);
-            const u32x4 w = beam_load<BF16>(row, t, a.vocab);
+        const auto walk = [&](int to, auto&& f) {  // f(beam, token, value, part) of the values that reach part `to`
+            for (int k = tid / kLanes; k < n_list; k += kBeamThreads / kLanes) {
+                int b;
+                int64_t t;
+                const uint8_t* row = place(sm.list[k], tid % kLanes * E, &b, &t);
+                const u32x4 w = beam_load<BF16>(row, t, a.vocab);
 #pragma unroll
-            for (int i = 0; i < E; i++) {
-                const double v = value_of(b, beam_clean(beam_word<BF16>(w, i)));
-                if (!(v > -INFINITY) || beam_part(top, v) > last) continue;
-                const int c = atomicAdd(&sm.count, 1);
-                if (c < kBeamCands) {
-                    sm.cand[c] = beam_key(v);
-                    sm.where[c] = (uint64_t)b << 32 | (uint32_t)(t + i);
+                for (int i = 0; i < E; i++) {
+                    const double v = value_of(b, beam_clean(beam_word<BF16>(w, i)));
+                    const int part = beam_part(top, v);
+                    if (v > -INFINITY && part <= to) f(b, (int)(t + i), v, part);
                 }
             }
-        }
+        };
+        const auto keep = [&](uint64_t key, uint64_t where) {
+            const int c = atomicAdd(&sm.count, 1);
+            if (c < kBeamCands) {
+                sm.cand[c] = key;
+                sm.where[c] = where;
+            }
+        };
+        const auto keep_value = [&](int b, int t, double v, int) { keep(beam_key(v), (uint64_t)b << 32 | (uint32_t)t); };
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+        walk(last, keep_value);
         __syncthreads();
         n_cand = sm.count;
+        if (n_cand > 2 * a.n_out + 64) {
+            // few segments, or many values in each that reach the part: count again,
+            // among the values (ranking costs the square: 1024 of them 30 us)
+            const bool here = n_cand <= kBeamCands;
+            const uint64_t key = here && tid < n_cand ? sm.cand[tid] : 0, where = here && tid < n_cand ? sm.where[tid] : 0;
+            const int part = key ? beam_part(top, beam_value(key)) : kBeamThreads;
+            __syncthreads();
+            sm.hist[tid] = 0;
+            if (tid == 0) {
+                sm.count = 0;
+                sm.bin = kBeamThreads - 1;
+            }
+            __syncthreads();
+            if (here) {
+                if (key) atomicAdd(&sm.hist[part], 1);
+            } else {
+                walk(last, [&](int, int, double, int p) { atomicAdd(&sm.hist[p], 1); });
+            }
+            __syncthreads();
+            const int to = reached();
+            if (!here)
+                walk(to, keep_value);
+            else if (part <= to)
+                keep(key, where);
+            __syncthreads();
+            n_cand = sm.count;
+        }
         __syncthreads();
     }
     if (n_cand > kBeamCands) {

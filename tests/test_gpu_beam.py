@@ -130,6 +130,9 @@ SHAPES = {  # groups, beams, vocab, n_out, pad, at
     "long_chunks": (8, 8, 70001, 16, 0, 1),
     "vocabulary": (2, 3, 151936, 16, 64, 0),
     "many_segments": (1, 48, 60000, 7, 0, 0),
+    "fewer_segments_than_asked": (3, 4, 400, 30, 5, 0),  # values are counted again,
+    "more_values_than_held": (2, 17, 2622, 120, 71, 1),  # from the logits
+    "some_values": (2, 10, 66, 13, 0, 0),
     "many_groups": (70000, 1, 2, 1, 0, 0),
 }
 
