@@ -291,13 +291,16 @@ int kvc_decode_attn_static(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * of the sequences, any tree of common prefixes, but a full block that several
  * sequences of up to 64 of a call hold is read once for all of them.  Launches
  * for which that is estimated to be slower (a few short sequences, little in
- * common), or in which some hold 8-bit blocks, run kvc_decode_attn's kernels.  With bf16 output weights are rounded to bf16 before the product with
- * the values; with fp32 output they keep 24 bits in either kind of launch (as
- * several parts, so an infinite value may make the elements that it enters NaN).  Equal
- * to kvc_decode_attn within those roundings; the order of sums follows from the
- * tables and lengths of all sequences that share 64 of a call.  Arrays must be
+ * common), or in which some hold 8-bit blocks, run kvc_decode_attn's kernels.
+ * With bf16 output weights are rounded to bf16 before the product with the values;
+ * with fp32 output they keep 24 bits in either kind of launch (as several parts, so
+ * an infinite value may make the elements that it enters NaN).  Equal to
+ * kvc_decode_attn within those roundings; the order of sums follows from the tables
+ * and lengths of the up to 64 sequences that are launched together.  Arrays must be
  * aligned to 16 bytes, and out must not overlap the inputs.  The context's device
- * must be current.  Uses the context's split-K workspace. */
+ * must be current.  Uses the context's split-K workspace.  A graph captured around
+ * a call replays its division into blocks: of use while the tables and lengths
+ * stay. */
 int kvc_decode_attn_shared(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
                            int32_t n_seqs, const void* q, const void* k_new,
                            const void* v_new, const void* gate, void* out,
@@ -455,7 +458,9 @@ int kvc_kv_checksum(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * device fp32 [n_groups][n_beams], NULL for zeros; it may be out_scores if n_out =
  * n_beams.  Otherwise no two arrays may overlap.  n_beams <= 64, n_out <= 128;
  * n_beams * vocab is bounded by the context's workspace (1 B per 64 tokens and a
- * little; KVC_ERR_RANGE).  The next step: kvc_seq_reorder by the beams chosen. */
+ * little; KVC_ERR_RANGE).  It uses the context's split-K workspace and no
+ * sequence; the context's device must be current.  The next step: kvc_seq_reorder
+ * by the beams chosen. */
 int kvc_beam_select(kvc_ctx* ctx, const void* logits, int32_t dtype,
                     int64_t row_stride, int32_t n_groups, int32_t n_beams,
                     int32_t vocab, const void* scores, int32_t n_out,

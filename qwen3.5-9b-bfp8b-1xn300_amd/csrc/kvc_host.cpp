@@ -1499,7 +1499,7 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
         const int32_t last = std::min(keys[s] - (p.first[k] + p.len[k] - 1) * kBlockTok, kBlockTok);
         const auto entry = [&](int32_t i) { return (uint16_t)(p.member[i] | p.part[i] << 6); };
         a.node[k] = {(uint32_t)p.first[k] | (uint32_t)p.kind[k] << 26, (uint32_t)p.len[k] | (uint32_t)(last - 1) << 26,
-                     (uint32_t)p.chunk[k] | (uint32_t)(members - 1) << 10 | (members == 1 ? entry(mb) : (uint32_t)listed / kSharedSeqs) << 16,
+                     (uint32_t)p.chunk[k] | (uint32_t)(members - 1) << 10 | (members == 1 ? entry(mb) : (uint32_t)listed / kSharedSeqs | (p.group == kSharedTile ? 64u : 0u)) << 16,
                      seqs[i0 + s]};
         if (members == 1) continue;
         for (int32_t i = 0; i < (members + kSharedSeqs - 1) / kSharedSeqs * kSharedSeqs; i++) a.member[listed++] = entry(mb + std::min(i, members - 1));

@@ -541,7 +541,9 @@ struct BlockCopyArgs {
 // (seq_row[s] + p) * 16 + h.
 constexpr int kSharedNodes = 128;
 constexpr int kSharedMembers = 512;
-constexpr int kSharedSeqs = 8;         // 4 members are a tile of 16 rows; two tiles fill a wave's registers
+constexpr int kSharedTile = 4;         // members of a tile of 16 rows
+constexpr int kSharedSeqs = 8;         // of two tiles, which fill a wave's registers
+constexpr int kSharedCus = 256;
 constexpr int kSharedHalves = 64;      // half blocks of a wave: the ids it holds
 constexpr int kSharedOneMax = 1023;    // blocks of a kSharedOne workgroup
 constexpr int kSharedPath = 512;       // partials of one (sequence, q head)
@@ -557,8 +559,8 @@ constexpr int kSharedMaxParts = (int)(kPartBytes / ((kHeadDim + 2) * 4 * kQHeads
 struct SharedNode {
     uint32_t first;  // block in the members' tables | kind << 26
     uint32_t len;    // blocks | (keys in the last one - 1) << 26
-    uint32_t who;    // chunk (blocks of a workgroup, up to 1023) | (members - 1) << 10 | and << 16:
-                     // of one member its entry, else where their list starts, / 8
+    uint32_t who;    // chunk (blocks of a workgroup, up to 1023) | (members - 1) << 10 | and << 16: of one
+                     // member its entry, else where their list starts, / 8, and 64 for groups of 4
     int32_t slot;    // table row of a member
 };
 

@@ -326,11 +326,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     SharedItem it;
     it.kind = w0 >> 26;
     const int n_chunks = (len + chunk - 1) / chunk, units = it.kind == kSharedHeads ? n_chunks : n_chunks * kKvHeads;
+    const int size = all > 1 && (w2 >> 22 & 1) ? kSharedTile : kSharedSeqs;  // of a group
     int j = item - begin, grp = 0;
-    if (all > kSharedSeqs) {
+    if (all > size) {
         // (the node starts on a multiple of 8; the groups of members that read the
         // same keys run on one XCD, workgroup number % 8, one after the other)
-        const int groups = (all + kSharedSeqs - 1) / kSharedSeqs;
+        const int groups = (all + size - 1) / size;
         j = item - (begin + 7) / 8 * 8;
         if (j < 0) return;
         const int r = j >> 3;
@@ -343,16 +344,20 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int b0 = it.ck * chunk;
     const int n_blk = min(chunk, len - b0);
     it.keys = n_blk * kBlockTok - (b0 + n_blk == len ? kBlockTok - 1 - (int)(w1 >> 26) : 0);
-    it.members = min(kSharedSeqs, all - grp * kSharedSeqs);
+    it.members = min(size, all - grp * size);
     it.trow = a.table + (size_t)slot * a.table_stride + first + b0;
     if (all == 1) {
         it.who[0] = it.who[1] = it.who[2] = it.who[3] = (w2 >> 16) * 0x10001u;
     } else {
-        const int from = (w2 >> 16) + grp;  // lane that holds them
+        const int from = (w2 >> 16 & 63) + grp * size / 8;  // lane that holds them
         it.who[0] = __builtin_amdgcn_readlane(mw.x, from);
         it.who[1] = __builtin_amdgcn_readlane(mw.y, from);
         it.who[2] = __builtin_amdgcn_readlane(mw.z, from);
         it.who[3] = __builtin_amdgcn_readlane(mw.w, from);
+        if (size == kSharedTile && (grp & 1)) {  // the list's second half
+            it.who[0] = it.who[2];
+            it.who[1] = it.who[3];
+        }
     }
     if (it.kind == kSharedOne)
         shared_one<PARTS>(a, it, seq_row, sm.one);

@@ -22,6 +22,7 @@ struct SharedPlan {
     int32_t n_items = 0;               // workgroups
     int32_t parts = 0;                 // partials per q head, of all sequences
     int32_t path = 0;                  // most of them of one sequence
+    int32_t group = kSharedSeqs;       // members of a workgroup: 4 (a tile) or 8
     int64_t blocks = 0, blocks_apart = 0;  // read by the plan, and sequence by sequence
     int64_t tile_work = 0;             // blocks of a kv head for up to kSharedSeqs members
     int32_t first[kSharedNodes];       // of the node's blocks, in its members' tables
@@ -111,7 +112,7 @@ class SharedPlanner {
     uint8_t order_[kMaxBatch];
 };
 
-inline int32_t shared_groups(int32_t members) { return (members + kSharedSeqs - 1) / kSharedSeqs; }
+inline int32_t shared_groups(const SharedPlan& p, int32_t members) { return (members + p.group - 1) / p.group; }
 
 // Nodes of several members first, then the long ones: what runs last is short.
 inline void shared_sort(SharedPlan& p) {
@@ -137,7 +138,7 @@ inline void shared_items(SharedPlan& p, int32_t halves, int32_t one, int32_t n) 
     for (int32_t i = 0; i < n; i++) p.seq_parts[i] = 0;
     int64_t items = 0;
     for (int32_t k = 0; k < p.n_nodes; k++) {
-        const int32_t members = p.members[k], groups = shared_groups(members);
+        const int32_t members = p.members[k], groups = shared_groups(p, members);
         p.kind[k] = members == 1 ? kSharedOne : 2 * p.len[k] <= halves ? kSharedHeads : kSharedKeys;
         int32_t chunk = members == 1 ? one : p.kind[k] == kSharedHeads ? p.len[k] : 2 * halves;
         int32_t n_chunks = (p.len[k] + chunk - 1) / chunk;
@@ -187,22 +188,52 @@ inline bool shared_pays(const SharedPlan& p, bool always) {
     return shared < apart;
 }
 
+// Blocks of all kv heads that workgroups read in nodes of one member [0] and of
+// several [1].
+inline void shared_work(const SharedPlan& p, int64_t* work) {
+    work[0] = work[1] = 0;
+    for (int32_t k = 0; k < p.n_nodes; k++)
+        work[p.members[k] > 1] += (int64_t)p.len[k] * kKvHeads * shared_groups(p, p.members[k]);
+}
+
 // The work of a launch of n sequences (n <= kMaxBatch): caller_chunk > 0 is a
 // chunk length that the caller set.  Otherwise nodes of several members and of one
 // are each cut into about a workgroup per CU.  (Two fit, but those on tiles then
 // share its LDS and take twice the time, and shorter chunks leave more partials to
 // fold.)
+//
+// Groups of 4 members are one tile: half of the registers, of the fold of the waves
+// and of the work of a chunk, and the blocks are read from L2 twice as often.  That
+// pays for nodes of up to 8 and in small launches; us per layer in groups of 4 / 8: 8
+// sequences on 4096 tokens 14.9 / 16.0, 16 on 2000 13.5 / 14.9, 32 on 4096 18.7 / 21.3,
+// 8 on 32768 34.4 / 36.9; 64 on 4096 23.8 / 22.4, 64 on 8192 62 / 58, 16 on 65536 83 /
+// 63.  Chunks of 8 blocks at least (4, 8 and 12 blocks: 16 on 2000 15.6, 13.5, 14.0),
+// or of 12 where not all workgroups then have a CU of their own (16 on 4096: 8 blocks
+// 16.0, 12 14.4).
 inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, SharedPlan& p) {
     SharedPlanner(tab, keys, n, p);
     shared_sort(p);
-    int64_t work[2] = {0, 0};  // blocks of all kv heads, of nodes of one member and of several
-    for (int32_t k = 0; k < p.n_nodes; k++)
-        work[p.members[k] > 1] += (int64_t)p.len[k] * kKvHeads * shared_groups(p.members[k]);
+    int64_t work[2];
+    p.group = kSharedSeqs;
+    shared_work(p, work);
     p.tile_work = work[1];
-    const int64_t tiles = caller_chunk > 0 ? caller_chunk : std::max<int64_t>(4, (work[1] + 255) / 256);
+    int32_t most = 0;
+    for (int32_t k = 0; k < p.n_nodes; k++) most = std::max<int32_t>(most, p.members[k]);
+    p.group = kSharedTile;
+    shared_work(p, work);
+    if (most > kSharedSeqs && work[1] > 16 * kSharedCus) {
+        p.group = kSharedSeqs;
+        shared_work(p, work);
+    }
+    const auto per_cu = [](int64_t w, int64_t least) { return std::max(least, (w + kSharedCus - 1) / kSharedCus); };
+    const int64_t tiles = caller_chunk > 0 ? caller_chunk : per_cu(work[1], 8);
     int32_t halves = (int32_t)std::min<int64_t>(kSharedHalves, (tiles + 1) / 2);
-    int32_t one = (int32_t)std::min<int64_t>(kSharedOneMax, caller_chunk > 0 ? caller_chunk : std::max<int64_t>(3, (work[0] + 255) / 256));
+    int32_t one = (int32_t)std::min<int64_t>(kSharedOneMax, caller_chunk > 0 ? caller_chunk : per_cu(work[0], 3));
     shared_items(p, halves, one, n);
+    if (caller_chunk <= 0 && p.group == kSharedTile && p.n_items > kSharedCus && halves < 6) {
+        halves = 6;
+        shared_items(p, halves, one, n);
+    }
     while (!shared_fits(p) && (halves < kSharedHalves || one < kSharedOneMax)) {
         halves = std::min(2 * halves, kSharedHalves);
         one = std::min(2 * one, kSharedOneMax);

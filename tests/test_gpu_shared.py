@@ -120,6 +120,7 @@ SPECS = {
     "sixty_four": [(160, [(5, 33), (500, 31)])],
     "tree": [(100, [(300, [(20, 3), (0, 2), (333, 2)]), (64, [(64, 6), (1, 1)])])],
     "apart": [(400, 6), (300, 2), (33, 1), (1, 1)],
+    "wide": [(6600, [(5, 9), (40, 9)])],  # work for groups of two tiles
     "long": [(5000, [(1, 2), (700, 1)])],
 }
 

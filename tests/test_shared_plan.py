@@ -13,7 +13,7 @@ import pytest
 CSRC = Path(__file__).resolve().parents[1] / "qwen3.5-9b-bfp8b-1xn300_amd" / "csrc"
 CXX = shutil.which("g++")
 pytestmark = pytest.mark.skipif(CXX is None, reason="needs g++")
-BT, HEADS, SEQS = 32, 4, 8
+BT, HEADS = 32, 4
 KEYS, ALL_HEADS, ONE = 0, 1, 2  # kinds
 
 # stdin: launches as "n chunk share", then per sequence "keys nblk id id ..."; stdout: the plan
@@ -37,8 +37,8 @@ int main() {
         }
         kvc::SharedPlan p;
         kvc::shared_plan(tab.data(), keys.data(), n, chunk, p);
-        std::printf("%d %d %d %d %lld %lld %d\n", p.n_nodes, p.n_items, p.parts, p.path, (long long)p.blocks,
-                    (long long)p.blocks_apart, (int)kvc::shared_pays(p, share));
+        std::printf("%d %d %d %d %lld %lld %d %d\n", p.n_nodes, p.n_items, p.parts, p.path, (long long)p.blocks,
+                    (long long)p.blocks_apart, (int)kvc::shared_pays(p, share), p.group);
         for (int k = 0; k < p.n_nodes; k++) {
             std::printf("%d %d %d %d %d %d", p.first[k], p.len[k], p.item_begin[k], p.chunk[k], p.kind[k], p.item_begin[k + 1]);
             for (int i = p.member_begin[k]; i < p.member_begin[k] + p.members[k]; i++)
@@ -65,7 +65,7 @@ def plans(tmp_path_factory):
         lines = iter(out.splitlines())
         got = []
         for _ in launches:
-            head = dict(zip(("n_nodes", "n_items", "parts", "path", "blocks", "apart", "pays"), map(int, next(lines).split())))
+            head = dict(zip(("n_nodes", "n_items", "parts", "path", "blocks", "apart", "pays", "group"), map(int, next(lines).split())))
             nodes = []
             for _ in range(head["n_nodes"]):
                 x = list(map(int, next(lines).split()))
@@ -110,7 +110,7 @@ def check(head, nodes, seqs):
         units = chunks * (1 if x["kind"] == ALL_HEADS else HEADS)
         # the kernel's reading of its item number
         seen = set()
-        groups = -(-len(x["members"]) // SEQS)
+        groups = -(-len(x["members"]) // head["group"])
         begin = 0 if x is nodes[0] else nodes[nodes.index(x) - 1]["end"]
         for item in range(begin, x["end"]):
             j, grp = item - begin, 0
@@ -137,7 +137,7 @@ def check(head, nodes, seqs):
             assert t[x["first"]:x["first"] + x["len"]] == first[x["first"]:x["first"] + x["len"]]
             if len(x["members"]) > 1:  # whole blocks only
                 assert (x["first"] + x["len"]) * BT <= keys
-    assert head["n_items"] == (nodes[-1]["end"] if nodes else 0)
+    assert head["n_items"] == (nodes[-1]["end"] if nodes else 0) and head["group"] in (4, 8)
     for i, (keys, t) in enumerate(seqs):
         at = 0
         for first, n, _ in sorted(path[i]):  # once each
