@@ -1446,7 +1446,7 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
         }
         if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, p);
     }
-    if (!launch || q8 || !shared_pays(p, c->cfg.flags & KVC_FLAG_DECODE_SHARE)) {
+    if (!launch || q8 || !shared_pays(p, n, c->cfg.flags & KVC_FLAG_DECODE_SHARE)) {
         DecodeArgs a;
         DecodeQ8Args a8;
         int rc, e = 0;

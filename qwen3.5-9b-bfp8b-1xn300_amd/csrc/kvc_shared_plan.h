@@ -173,17 +173,18 @@ inline void shared_items(SharedPlan& p, int32_t halves, int32_t one, int32_t n) 
 inline bool shared_fits(const SharedPlan& p) { return p.path <= kSharedPath && p.parts <= kSharedMaxParts; }
 
 // Whether the plan beats kvc_decode_attn's launch, by the us that either takes: a
-// fixed part (here two launches), blocks from memory, blocks that sequence by
-// sequence come from the caches, and the tiles' LDS.  us per layer, kvc_decode_attn /
-// shared: 4 sequences on 300 tokens 9.2 / 12.4, 8 on 1000 9.5 / 12.8, 2 on 4096 11.5
-// / 12.7, 8 on 4096 17.6 / 16.6, 16 on 2000 17.0 / 15.2, 64 on 1000 28.3 / 17.3, 64
-// with 96 tokens in common of 1031 47.7 / 53.6, 64 on 65536 1228 / 141.
+// fixed part (here two launches, the first longer for more members), blocks from
+// memory, blocks that sequence by sequence come from the caches, and the tiles' LDS.
+// us per layer, kvc_decode_attn / shared: 4 sequences on 300 tokens 9.2 / 12.4, 4 on
+// 4096 13.4 / 12.1, 2 on 4096 11.5 / 12.7, 8 on 1000 9.5 / 13.0, 8 on 2000 12.4 / 13.4, 8
+// on 4096 17.6 / 14.5, 16 on 1000 12.2 / 14.0, 16 on 2000 17.0 / 13.0, 64 on 2000 47 /
+// 19.4, 64 with 96 tokens in common of 1031 47.7 / 53.6, 64 on 65536 1228 / 141.
 // `always`: wherever blocks are shared.
-inline bool shared_pays(const SharedPlan& p, bool always) {
+inline bool shared_pays(const SharedPlan& p, int32_t n, bool always) {
     if (!shared_fits(p) || p.blocks == p.blocks_apart) return false;
     if (always) return true;
     constexpr double kBlockUs = 2.0 * kBlockBytes * 1e-6;  // of a block, K and V, at 1 TB/s
-    const double shared = 12 + std::max(p.blocks * kBlockUs / 5.5, 0.002 * p.tile_work);
+    const double shared = 6.8 + std::min(0.6 * n, 5.7) + std::max(p.blocks * kBlockUs / 5.5, 0.002 * p.tile_work);
     const double apart = 7 + std::max(p.blocks * kBlockUs / 6.5, p.blocks_apart * kBlockUs / 12);
     return shared < apart;
 }
@@ -207,9 +208,9 @@ inline void shared_work(const SharedPlan& p, int64_t* work) {
 // pays for nodes of up to 8 and in small launches; us per layer in groups of 4 / 8: 8
 // sequences on 4096 tokens 14.9 / 16.0, 16 on 2000 13.5 / 14.9, 32 on 4096 18.7 / 21.3,
 // 8 on 32768 34.4 / 36.9; 64 on 4096 23.8 / 22.4, 64 on 8192 62 / 58, 16 on 65536 83 /
-// 63.  Chunks of 8 blocks at least (4, 8 and 12 blocks: 16 on 2000 15.6, 13.5, 14.0),
-// or of 12 where not all workgroups then have a CU of their own (16 on 4096: 8 blocks
-// 16.0, 12 14.4).
+// 63.  Chunks of 8 blocks at least (4, 8 and 12 blocks: 16 on 2000 15.6, 13.5, 14.0), or
+// of 12 where those of three and more groups nearly fill the GPU (8 and 12: 16 on 4096
+// 16.0, 14.4; 12 on 3000 13.7, 13.7; but 8 on 8192, in two groups, 16.7, 18.1).
 inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t n, int32_t caller_chunk, SharedPlan& p) {
     SharedPlanner(tab, keys, n, p);
     shared_sort(p);
@@ -226,14 +227,10 @@ inline void shared_plan(const int32_t* const* tab, const int32_t* keys, int32_t 
         shared_work(p, work);
     }
     const auto per_cu = [](int64_t w, int64_t least) { return std::max(least, (w + kSharedCus - 1) / kSharedCus); };
-    const int64_t tiles = caller_chunk > 0 ? caller_chunk : per_cu(work[1], 8);
+    const int64_t tiles = caller_chunk > 0 ? caller_chunk : per_cu(work[1], most > kSharedSeqs && work[1] > 6 * kSharedCus ? 12 : 8);
     int32_t halves = (int32_t)std::min<int64_t>(kSharedHalves, (tiles + 1) / 2);
     int32_t one = (int32_t)std::min<int64_t>(kSharedOneMax, caller_chunk > 0 ? caller_chunk : per_cu(work[0], 3));
     shared_items(p, halves, one, n);
-    if (caller_chunk <= 0 && p.group == kSharedTile && p.n_items > kSharedCus && halves < 6) {
-        halves = 6;
-        shared_items(p, halves, one, n);
-    }
     while (!shared_fits(p) && (halves < kSharedHalves || one < kSharedOneMax)) {
         halves = std::min(2 * halves, kSharedHalves);
         one = std::min(2 * one, kSharedOneMax);

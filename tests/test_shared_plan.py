@@ -38,7 +38,7 @@ int main() {
         kvc::SharedPlan p;
         kvc::shared_plan(tab.data(), keys.data(), n, chunk, p);
         std::printf("%d %d %d %d %lld %lld %d %d\n", p.n_nodes, p.n_items, p.parts, p.path, (long long)p.blocks,
-                    (long long)p.blocks_apart, (int)kvc::shared_pays(p, share), p.group);
+                    (long long)p.blocks_apart, (int)kvc::shared_pays(p, n, share), p.group);
         for (int k = 0; k < p.n_nodes; k++) {
             std::printf("%d %d %d %d %d %d", p.first[k], p.len[k], p.item_begin[k], p.chunk[k], p.kind[k], p.item_begin[k + 1]);
             for (int i = p.member_begin[k]; i < p.member_begin[k] + p.members[k]; i++)
@@ -213,7 +213,8 @@ def test_same_sequence_many_times_over_ends_in_a_shared_block(plans):
 
 @pytest.mark.parametrize("n,prefix,tail,shares", [(4, 9, 1, False), (8, 31, 1, False), (2, 128, 1, False),
                                                   (8, 128, 1, True), (16, 62, 2, True), (64, 31, 1, True),
-                                                  (64, 3, 30, False), (64, 256, 24, True), (4, 500, 1, True)])
+                                                  (64, 3, 30, False), (64, 256, 24, True), (4, 500, 1, True),
+                                                  (4, 128, 1, True), (8, 62, 1, False), (16, 31, 1, False)])
 def test_where_it_is_worth_it(plans, n, prefix, tail, shares):
     """the measured side (us per layer in the rule's comment)"""
     (head, _), = plans([(0, common(n, prefix, tail))], share=False)
