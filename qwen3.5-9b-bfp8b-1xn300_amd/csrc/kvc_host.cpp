@@ -2187,7 +2187,7 @@ int kvc_beam_select(kvc_ctx* c, const void* logits, int32_t dtype, int64_t row_s
                 return set_err(KVC_ERR_INVALID, "outputs of the beam selection overlap");
     }
     const int64_t n_seg = ((int64_t)vocab + kBeamSeg - 1) / kBeamSeg;
-    // short chunks for few rows, so that every CU has some
+    // short chunks for few rows, so that every CU has some (beam_max_kernel's figures)
     const auto chunks_of = [&](int steps) {
         const int64_t tokens = beam_chunk_tokens(bf16, steps);
         return (vocab + tokens - 1) / tokens;

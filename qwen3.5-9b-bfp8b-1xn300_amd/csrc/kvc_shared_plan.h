@@ -176,7 +176,7 @@ inline bool shared_fits(const SharedPlan& p) { return p.path <= kSharedPath && p
 // fixed part (here two launches, the first longer for more members), blocks from
 // memory, blocks that sequence by sequence come from the caches, and the tiles' LDS.
 // us per layer, kvc_decode_attn / shared: 4 sequences on 300 tokens 9.2 / 12.4, 4 on
-// 4096 13.4 / 12.1, 2 on 4096 11.5 / 12.7, 8 on 1000 9.5 / 13.0, 8 on 2000 12.4 / 13.4, 8
+// 4096 13.4 / 13.1, 2 on 4096 11.5 / 12.7, 8 on 1000 9.5 / 13.0, 8 on 2000 12.4 / 13.4, 8
 // on 4096 17.6 / 14.5, 16 on 1000 12.2 / 14.0, 16 on 2000 17.0 / 13.0, 64 on 2000 47 /
 // 19.4, 64 with 96 tokens in common of 1031 47.7 / 53.6, 64 on 65536 1228 / 141.
 // `always`: wherever blocks are shared.
