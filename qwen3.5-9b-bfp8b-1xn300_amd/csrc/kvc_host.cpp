@@ -1426,7 +1426,6 @@ int kvc_decode_attn_static(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
                        kStaticItems, "static decode workspace");
 }
 
-// One prefill launch over sequences of which some may hold 8-bit blocks (at most 64).
 // The launches of kvc_decode_attn_shared for seqs[i0, i0 + n): over the trie of
 // their block tables where that saves enough reads (shared_pays), else those of
 // kvc_decode_attn, of them the ones that hold weights in fp32 for fp32 output.
@@ -1537,6 +1536,7 @@ int kvc_decode_attn_shared(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
     return KVC_OK;
 }
 
+// One prefill launch over sequences of which some may hold 8-bit blocks (at most 64).
 static int prefill_q8_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t n, int32_t n_q, const void* q,
                              const void* gate, void* out, int32_t out_dtype, float scale, void* stream) {
     PrefillQ8Args a{};

@@ -165,6 +165,17 @@ def test_equal_logits(ctx, dtype, levels):
             assert [(int(i), int(j)) for i, j in zip(b[g], t[g])] == flat
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("levels", [1, 3])
+def test_more_equal_segments_than_are_listed(ctx, dtype, levels):
+    say(f"beam select of {levels} levels in thousands of segments")
+    x = (np.random.default_rng(21).integers(0, levels, (1, 48, 60000)) * 0.5).astype(np.float32)
+    with Case(x, dtype, np.zeros((1, 48), np.float32), 128) as c:
+        _, b, t = c.run(ctx)
+        if levels == 1:  # equal sums everywhere
+            assert (b == 0).all() and t[0].tolist() == list(range(128))
+
+
 def test_more_close_values_than_are_sorted(ctx):
     """Above the least chosen maximum stand more values than the last step sorts."""
     say("beam select of a crowded top")
