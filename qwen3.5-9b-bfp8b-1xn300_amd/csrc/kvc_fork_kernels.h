@@ -7,10 +7,10 @@ namespace kvc {
 // The first n_rows workgroups copy a block-table row each, the others pieces of
 // the states: a piece is read once and stored to every sequence that gets it.
 // Nothing is both read and written (a destination is nobody's source).  HBM-bound:
-// 52.7 MB read a source and written a copy; one state to four sequences 48.6 us (5.4
-// TB/s read + written), 13 copies of 5 169 us (5.6).  Loads and stores pass the caches
-// by (nontemporal): the states are larger, and the K/V in them stays.
-constexpr int kForkUnroll = 4;  // 16-byte loads of a thread
+// 52.7 MB read a source and written a copy; one state to four sequences 49 us (5.4
+// TB/s read + written), 13 copies of 5 163 us (5.8).  A thread moves one 16-B piece: 2,
+// 4 and 8 took 168, 169 and 193 us for the 163.  Loads and stores are nontemporal: the
+// states are larger than the caches, and the K/V in them stays (time the same without).
 __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
     int b = blockIdx.x;
     if (b < a.n_rows) {
@@ -22,23 +22,16 @@ __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
     b -= a.n_rows;
     const int p = b / a.wgs_per_state;
     const size_t n = (size_t)a.state_bytes / 16;
-    const size_t u0 = (size_t)(b - p * a.wgs_per_state) * (256 * kForkUnroll) + threadIdx.x;
-    const u32x4* src = reinterpret_cast<const u32x4*>(a.state + (size_t)a.src[p] * a.state_bytes);
-    u32x4 x[kForkUnroll];
-#pragma unroll
-    for (int k = 0; k < kForkUnroll; k++)
-        if (u0 + 256 * k < n) x[k] = __builtin_nontemporal_load(src + u0 + 256 * k);
-    for (int d = a.dst_begin[p]; d < a.dst_begin[p + 1]; d++) {
-        u32x4* dst = reinterpret_cast<u32x4*>(a.state + (size_t)a.dst[d] * a.state_bytes);
-#pragma unroll
-        for (int k = 0; k < kForkUnroll; k++)
-            if (u0 + 256 * k < n) __builtin_nontemporal_store(x[k], dst + u0 + 256 * k);
-    }
+    const size_t u = (size_t)(b - p * a.wgs_per_state) * 256 + threadIdx.x;
+    if (u >= n) return;
+    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.state + (size_t)a.src[p] * a.state_bytes) + u);
+    for (int d = a.dst_begin[p]; d < a.dst_begin[p + 1]; d++)
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(a.state + (size_t)a.dst[d] * a.state_bytes) + u);
 }
 
 int launch_fork(const ForkArgs& a, void* stream) {
     ForkArgs f = a;
-    f.wgs_per_state = (int32_t)((a.state_bytes / 16 + 256 * kForkUnroll - 1) / (256 * kForkUnroll));
+    f.wgs_per_state = (int32_t)((a.state_bytes / 16 + 255) / 256);
     const int64_t grid = a.n_rows + (int64_t)a.n_src * f.wgs_per_state;
     if (grid <= 0) return 0;
     if (grid > INT32_MAX) return (int)hipErrorInvalidConfiguration;
