@@ -9,10 +9,10 @@
 // segment has n_out segment maxima before it.  So the second launch, a workgroup per
 // group, chooses among the maxima and reads few segments again.
 //
-// Measured: 32 groups of 8 beams of 151936 bf16 logits, 16 of each 24.7 us: the first
-// launch 15.1 for 77.8 MB (5.1 TB/s; its VALU is busy for 10 of them, four tenths of
-// that with the exponentials), the second 10.2, a chain of some ten trips to memory and
-// barriers that a workgroup per group cannot hide.  One group of 4 beams 10.5: 2.9 + 7.9.
+// Measured: 32 groups of 8 beams of 151936 bf16 logits, 16 of each 23.0 us: the first
+// launch 15.2 for 77.8 MB (5.1 TB/s; its VALU is busy for 10 of them, four tenths of
+// that with the exponentials), the second 8.8, a chain of some ten trips to memory and
+// barriers that a workgroup per group cannot hide.  One group of 4 beams 9.3: 2.8 + 6.5.
 #pragma once
 
 namespace kvc {
@@ -59,7 +59,7 @@ __device__ __forceinline__ float beam_word(const u32x4& w, int i) {
 
 // One chunk of a row: 4 waves x STEPS loads of 16 B a lane, all in flight at once.
 // A segment's lanes are neighbours, and STEPS loads of theirs cover it.  A workgroup
-// per chunk: loops over chunks with the next loads in flight took 16-21 us for the 15.1
+// per chunk: loops over chunks with the next loads in flight took 16-21 us for the 15.2
 // above.  STEPS 1, 2, 4, 8: 19.4, 15.5, 15.2, 16.2 us there, 2.8, 3.2, 4.1, 5.7 for one
 // group of 4 beams.
 template <bool BF16, int STEPS>
@@ -130,6 +130,14 @@ __device__ __forceinline__ double beam_value(uint64_t k) {
     return __longlong_as_double((int64_t)(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
 
+// log x of a finite x >= 1: the exponent's part in 64 bits, the mantissa's, below 1, off
+// by 2^-23 at most.
+__device__ __forceinline__ double beam_log(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const float f = __uint_as_float((u & 0x7FFFFFu) | 0x3F800000u);  // in [1, 2)
+    return ((double)((int)(u >> 23) - 127) + (double)__builtin_amdgcn_logf(f)) * 0.6931471805599453;
+}
+
 constexpr int kBeamThreads = 1024, kBeamWaves = kBeamThreads / 64;
 constexpr int kBeamHeld = 8;      // a thread's segment maxima in registers
 constexpr int kBeamCands = 1024;  // segments, then values, that are looked at one by one
@@ -143,7 +151,7 @@ struct BeamSmem {
     int32_t hist[kBeamThreads];
     int32_t wsum[kBeamWaves];
     float wmax[kBeamWaves];
-    int32_t count, bin, above;
+    int32_t count, listed, kept, bin, above;
 };
 
 __device__ __forceinline__ int beam_scan(BeamSmem& sm, int x, int tid) {  // sum over threads >= tid
@@ -159,6 +167,22 @@ __device__ __forceinline__ int beam_scan(BeamSmem& sm, int x, int tid) {  // sum
     for (int w = wave + 1; w < kBeamWaves; w++) v += sm.wsum[w];
     __syncthreads();
     return v;
+}
+
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int dpp_or_0(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+// Sum over the wave's lanes up to this one: by shifts within rows of 16, then of a
+// row's last lane to the next row, and of lane 31 to the upper half.
+__device__ __forceinline__ int wave_prefix(int x) {
+    x += dpp_or_0<0x111>(x);
+    x += dpp_or_0<0x112>(x);
+    x += dpp_or_0<0x114>(x);
+    x += dpp_or_0<0x118>(x);
+    x += dpp_or_0<0x142, 0xA>(x);
+    x += dpp_or_0<0x143, 0xC>(x);
+    return x;
 }
 
 // Of n keys (0: none) the `want` greatest: those above *cut, and of those equal to
@@ -295,7 +319,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     }
     sm.hist[tid] = 0;
     if (tid == 0) {
-        sm.count = 0;
+        sm.count = sm.listed = sm.kept = 0;
         sm.bin = kBeamThreads - 1;
     }
     // A value is (score - log sum exp(x - max)) + (x - max), in 64 bits: large logits
@@ -303,24 +327,29 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     for (int b = wave; b < a.n_beams; b += kBeamWaves) {
         const float2* cs = reinterpret_cast<const float2*>(a.chunk_sum) + (row0 + b) * (size_t)a.n_chunks;
         const float score = a.scores ? a.scores[row0 + b] : 0.f;
-        const float2 first = lane < a.n_chunks ? cs[lane] : make_float2(-INFINITY, 0.f);
-        float m = first.x;
-        for (int c = lane + 64; c < a.n_chunks; c += 64) m = fmaxf(m, cs[c].x);
+        const float2 none = make_float2(-INFINITY, 0.f);
+        const float2 c0 = lane < a.n_chunks ? cs[lane] : none, c1 = lane + 64 < a.n_chunks ? cs[lane + 64] : none;
+        float m = fmaxf(c0.x, c1.x);
+        for (int c = lane + 128; c < a.n_chunks; c += 64) m = fmaxf(m, cs[c].x);
         m = wave_max(m);
         const bool fine = m > -INFINITY && m < INFINITY;
         float s = 0.f;
         if (fine) {
-            s = first.y * fast_exp2((first.x - m) * kLog2e);
-            for (int c = lane + 64; c < a.n_chunks; c += 64) s += cs[c].y * fast_exp2((cs[c].x - m) * kLog2e);
+            s = c0.y * fast_exp2((c0.x - m) * kLog2e) + c1.y * fast_exp2((c1.x - m) * kLog2e);
+            for (int c = lane + 128; c < a.n_chunks; c += 64) s += cs[c].y * fast_exp2((cs[c].x - m) * kLog2e);
         }
         s = wave_sum(s);
         if (lane == 0) {
-            sm.off[b] = fine && score > -INFINITY && score < INFINITY ? score - log((double)s) : -INFINITY;
+            sm.off[b] = fine && score > -INFINITY && score < INFINITY ? score - beam_log(s) : -INFINITY;
             sm.max[b] = fine ? m : 0.0;
         }
     }
     __syncthreads();
-    const auto beam_of = [&](int p) { return (int)((unsigned)p / (unsigned)n_seg); };
+    const float per_seg = 1.f / (float)n_seg;
+    // (the quotient is at least 0.5 / n_seg from an integer, and off by 2^-22 of itself)
+    const auto beam_of = [&](int p) {
+        return p < 1 << 20 ? (int)(((float)p + 0.5f) * per_seg) : (int)((unsigned)p / (unsigned)n_seg);
+    };
     const auto value_of = [&](int b, float x) { return sm.off[b] + ((double)x - sm.max[b]); };
     double val[kBeamHeld];
     double mine = -INFINITY;  // the thread's greatest
@@ -343,12 +372,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     __syncthreads();
     const auto reached = [&] {  // the first part that n_out of those counted reach, or the last
         const int h = sm.hist[tid];
-        int to = h;  // in this part and before it
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int y = __shfl_up(to, d);
-            to += lane >= d ? y : 0;
-        }
+        int to = wave_prefix(h);  // in this part and before it
         if (lane == 63) sm.wsum[wave] = to;
         __syncthreads();
         for (int w = 0; w < wave; w++) to += sm.wsum[w];
@@ -359,7 +383,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     const int last = reached();
     const auto choose = [&](int p, double v) {
         if (!(v > -INFINITY) || beam_part(top, v) > last) return;
-        const int c = atomicAdd(&sm.count, 1);
+        const int c = atomicAdd(&sm.listed, 1);
         if (c < kBeamCands) sm.list[c] = p;
     };
     if (mine > -INFINITY && beam_part(top, mine) <= last) {
@@ -375,8 +399,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
         *t = (int64_t)(p - *b * n_seg) * kBeamSeg + i;
         return rows + (size_t)*b * (size_t)a.stride * esz;
     };
-    int n_list = sm.count, n_cand = kBeamCands + 1;
-    __syncthreads();
+    int n_list = sm.listed, n_cand = kBeamCands + 1;
     if (n_list <= kBeamCands) {
         constexpr int E = BF16 ? 8 : 4, kLanes = kBeamSeg / E;
         const auto walk = [&](int to, auto&& f) {  // f(beam, token, value, part) of the values that reach part `to`
@@ -393,17 +416,15 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
                 }
             }
         };
-        const auto keep = [&](uint64_t key, uint64_t where) {
-            const int c = atomicAdd(&sm.count, 1);
+        const auto keep = [&](int32_t& count, uint64_t key, uint64_t where) {
+            const int c = atomicAdd(&count, 1);
             if (c < kBeamCands) {
                 sm.cand[c] = key;
                 sm.where[c] = where;
             }
         };
-        const auto keep_value = [&](int b, int t, double v, int) { keep(beam_key(v), (uint64_t)b << 32 | (uint32_t)t); };
-        if (tid == 0) sm.count = 0;
-        __syncthreads();
-        walk(last, keep_value);
+        const auto place_of = [](int b, int t) { return (uint64_t)b << 32 | (uint32_t)t; };
+        walk(last, [&](int b, int t, double v, int) { keep(sm.count, beam_key(v), place_of(b, t)); });
         __syncthreads();
         n_cand = sm.count;
         if (n_cand > 2 * a.n_out + 64) {
@@ -414,10 +435,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
             const int part = key ? beam_part(top, beam_value(key)) : kBeamThreads;
             __syncthreads();
             sm.hist[tid] = 0;
-            if (tid == 0) {
-                sm.count = 0;
-                sm.bin = kBeamThreads - 1;
-            }
+            if (tid == 0) sm.bin = kBeamThreads - 1;
             __syncthreads();
             if (here) {
                 if (key) atomicAdd(&sm.hist[part], 1);
@@ -427,18 +445,18 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
             __syncthreads();
             const int to = reached();
             if (!here)
-                walk(to, keep_value);
+                walk(to, [&](int b, int t, double v, int) { keep(sm.kept, beam_key(v), place_of(b, t)); });
             else if (part <= to)
-                keep(key, where);
+                keep(sm.kept, key, where);
             __syncthreads();
-            n_cand = sm.count;
+            n_cand = sm.kept;
         }
-        __syncthreads();
     }
     if (n_cand > kBeamCands) {
         const auto seg_key = [&](int p) { return beam_key(value_of(beam_of(p), seg[p])); };
         uint64_t cut;
         int ties;
+        __syncthreads();
         beam_cut(sm, n, a.n_out, seg_key, &cut, &ties);
         if (tid == 0) sm.count = 0;
         __syncthreads();
@@ -477,15 +495,21 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
     // in order: greatest first, then the lower beam, then the lower token; a value's
     // rank is counted by as many neighbouring lanes as there are threads for
     const size_t o = (size_t)blockIdx.x * a.n_out;
-    int lanes = 64;
-    while (lanes > 1 && lanes * n_cand > kBeamThreads) lanes /= 2;
-    const int c = tid / lanes;
+    const int lanes = n_cand <= 64 ? 16 : n_cand <= 256 ? 4 : 1, part = tid & (lanes - 1);
+    const int c = n_cand <= 64 ? tid >> 4 : n_cand <= 256 ? tid >> 2 : tid;
     if (tid - lane < n_cand * lanes) {  // (the wave has some)
         const uint64_t v = c < n_cand ? sm.cand[c] : 0, w = c < n_cand ? sm.where[c] : 0;
         int r = 0;
-        for (int k = tid % lanes; k < n_cand; k += lanes) r += sm.cand[k] > v || (sm.cand[k] == v && sm.where[k] < w);
-        for (int d = 1; d < lanes; d *= 2) r += __shfl_xor(r, d);
-        if (c < n_cand && tid % lanes == 0 && r < a.n_out) {
+        for (int k = part; k < n_cand; k += lanes) r += sm.cand[k] > v || (sm.cand[k] == v && sm.where[k] < w);
+        if (lanes > 1) {
+            r += dpp_or_0<kDppXor1>(r);
+            r += dpp_or_0<kDppXor2>(r);
+        }
+        if (lanes > 4) {
+            r += dpp_or_0<kDppHalfMirror>(r);
+            r += dpp_or_0<kDppRowRor8>(r);
+        }
+        if (c < n_cand && part == 0 && r < a.n_out) {
             a.out_scores[o + r] = (float)beam_value(v);
             a.out_beams[o + r] = (int32_t)(w >> 32);
             a.out_tokens[o + r] = (int32_t)(uint32_t)w;

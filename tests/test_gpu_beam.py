@@ -5,8 +5,8 @@ between beams they follow sums whose log sum of exponentials is taken in 32 bits
 Its relative error, in units of 2^-24: 1.5 |x - max| for the argument of the
 exponential (a product and a constant, both rounded; |x - max| <= 88, beyond which
 terms vanish), which sums to the same through the rescalings; 2 for each of at most
-4 exponentials and 1 for each product with one; 52 additions one after another.
-That is 132 + 12 + 52 < 200, so log sum is off by at most 200 x 2^-24, and a
+4 exponentials and 1 for each product with one; 52 additions one after another; 2 for
+the logarithm of the mantissa.  That is 132 + 12 + 52 + 2 < 200, so log sum is off by at most 200 x 2^-24, and a
 score by that and half a step of fp32, |score| 2^-24."""
 import numpy as np
 import pytest
