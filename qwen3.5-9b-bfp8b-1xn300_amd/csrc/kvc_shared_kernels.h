@@ -18,9 +18,10 @@
 // kvc_decode_attn does it, would put all members of a group on one workgroup.)
 //
 // Measured, us per layer with bf16 output (kvc_decode_attn beside it): 8 sequences on
-// 4096 common tokens 14.5 (17.6): this launch 10.2, mostly one trip after the other to
-// the arguments, the block ids and queries, the keys, and the fold of the waves; the
-// second launch 4.2.  64 on 8192, with tails of up to 1500 58 (194): this launch 54.8 for
+// 4096 common tokens 14.5 (17.6): this launch 10.2, one trip after the other to the
+// arguments (0.8), the block ids and queries (1.1), the keys (3.9, at 5 TB/s: twice the
+// half blocks in flight took 15.0) and the fold of the waves (1.5); the second launch
+// 4.2.  64 on 8192, with tails of up to 1500 58 (194): this launch 54.8 for
 // 240 MB from HBM, the products 5 of them.  64 on 65536 141 (1228): bound by the
 // blocks' eight trips from L2 to LDS.  30 in a tree of prompts, fp32 output 22.5 (36).
 #pragma once

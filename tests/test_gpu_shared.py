@@ -144,6 +144,14 @@ def test_chunk_lengths(chunk):
         f.check(f.seqs, "fp32", bf16_out=False, seed=9)
 
 
+@pytest.mark.parametrize("chunk", [20, 128])
+@pytest.mark.parametrize("bf16_out", [True, False])
+def test_two_tiles(chunk, bf16_out):
+    say(f"shared decode of two tiles, chunks of {chunk}")
+    with Forest(SPECS["wide"], seed=33, decode_chunk_blocks=chunk) as f:
+        f.check(f.seqs, f"chunk {chunk}", bf16_out=bf16_out)
+
+
 def test_more_than_one_launch_and_layers():
     say("shared decode of 70 sequences, second layer")
     with Forest([(300, [(7, 30), (90, 40)])], seed=13, layers=2) as f:
