@@ -184,3 +184,42 @@ def test_against_a_model_of_shared_blocks(seed):
         for s in model:
             c.seq_release(s)
         assert c.stats().free_blocks == 400
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_reordered_beams_feed_the_prefix_index(seed):
+    """Beams commit tokens between reorders; every full block of every path that
+    was ever committed is found again, and only those."""
+    def common(a, b):
+        return next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))
+
+    rng = random.Random(seed)
+    with ctx() as c:
+        root = fill(c, 70, np.arange(70, dtype=np.int32))
+        seqs = [c.seq_create() for _ in range(4)]
+        c.fork([root] * 4, seqs)
+        path = {s: list(range(70)) for s in seqs}
+        seen = {tuple(range(70))}
+        for step in range(8):
+            n = rng.choice([1, 7, 32, 45])
+            new = {s: [1000 * step + 10 * rng.randrange(3) + 7 * i for i in range(n)] for s in seqs}
+            c.reserve(seqs, n)
+            c.commit(seqs, n, np.array([new[s] for s in seqs], dtype=np.int32))
+            for s in seqs:
+                path[s] = path[s] + new[s]
+                seen.add(tuple(path[s]))
+            parent = [rng.randrange(4) for _ in seqs]
+            c.reorder(seqs, parent)
+            path = {s: path[seqs[p]] for s, p in zip(seqs, parent)}
+            assert [c.seq_len(s) for s in seqs] == [len(path[s]) for s in seqs]
+        probe = c.seq_create()
+        for p in sorted(seen):
+            for tail in ([5], [path[seqs[0]][len(p) - 1] + 1]):
+                prompt = list(p) + tail
+                best = max(common(q, prompt) for q in seen)
+                assert c.prefix_match(probe, np.array(prompt, dtype=np.int32)) == min(best, len(prompt) - 1) // BT * BT
+                c.seq_reset(probe)
+        for s in [root, probe] + seqs:
+            c.seq_release(s)
+        st = c.stats()
+        assert st.indexed_blocks == st.cached_blocks == 400 - st.free_blocks
