@@ -201,7 +201,8 @@ int kvc_seq_reserve(kvc_ctx* ctx, const int32_t* seqs, int32_t n_seqs,
  * [n_seqs][n_tok] (host) extends the token history so full blocks enter the
  * prefix index; NULL commits without indexing (synthetic fills).  When a seq
  * lands on a multiple of snapshot_interval and tokens != NULL, a snapshot of
- * its recurrent state and last segment of K/V is taken on `stream`. */
+ * its recurrent state and last segment of K/V is taken on `stream`; where more
+ * seqs of the call do than there are slots, of the first ones. */
 int kvc_seq_commit(kvc_ctx* ctx, const int32_t* seqs, int32_t n_seqs,
                    int32_t n_tok, const int32_t* tokens, void* stream);
 

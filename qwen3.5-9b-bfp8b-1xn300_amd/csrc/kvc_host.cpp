@@ -460,12 +460,15 @@ int launch_snapshots(kvc_ctx* c, const std::vector<int32_t>& seq_slots,
     return KVC_OK;
 }
 
-// Free or LRU-evictable snapshot slot, or -1.
-int32_t alloc_snapshot(kvc_ctx* c) {
+// Free or LRU-evictable snapshot slot, or -1.  A snapshot that was taken or found
+// after `until` is not evicted: one launch copies all snapshots of a call, so that
+// a slot given out twice in the call would be written by two sequences at once.
+int32_t alloc_snapshot(kvc_ctx* c, uint64_t until = UINT64_MAX) {
     int32_t victim = -1;
     for (int32_t i = 0; i < (int32_t)c->snaps.size(); i++) {
         if (!c->snaps[i].live) return i;
-        if (!c->snaps[i].pinned && (victim < 0 || c->snaps[i].tick < c->snaps[victim].tick)) victim = i;
+        if (!c->snaps[i].pinned && c->snaps[i].tick <= until && (victim < 0 || c->snaps[i].tick < c->snaps[victim].tick))
+            victim = i;
     }
     if (victim >= 0) {
         Snapshot& sn = c->snaps[victim];
@@ -962,6 +965,7 @@ int kvc_seq_commit(kvc_ctx* c, const int32_t* seqs, int32_t n_seqs, int32_t n_to
             return set_err(KVC_ERR_STATE, "sequence %d: commit of %d tokens but %d reserved", seqs[i], n_tok,
                            c->seqs[seqs[i]].pending);
     std::vector<int32_t> snap_seq, snap_slot, snap_first;
+    const uint64_t before = c->tick;
     const int iv = c->cfg.snapshot_interval;
     for (int32_t i = 0; i < n_seqs; i++) {
         Seq& s = c->seqs[seqs[i]];
@@ -983,7 +987,7 @@ int kvc_seq_commit(kvc_ctx* c, const int32_t* seqs, int32_t n_seqs, int32_t n_to
                 c->snaps[have].tick = ++c->tick;
                 continue;
             }
-            const int32_t id = alloc_snapshot(c);
+            const int32_t id = alloc_snapshot(c, before);
             if (id < 0) continue;
             Snapshot& sn = c->snaps[id];
             sn.live = true;
