@@ -209,7 +209,8 @@ int kvc_seq_commit(kvc_ctx* ctx, const int32_t* seqs, int32_t n_seqs,
 /* ---- forks (no counterpart in the reference) ------------------------------ */
 /* dst[i] (an empty sequence) becomes a copy of src[i], which may be listed more
  * than once: the same length, tokens and position, the same K/V blocks, shared
- * (one that is not full is copied by the kvc_seq_reserve that next writes to it),
+ * (one that is not full is copied by the kvc_seq_reserve that next writes to it,
+ * unless all other holders got their copies before or in the same call),
  * and a copy of the recurrent and conv state.  8-bit blocks are shared too, and
  * evicted tokens stay evicted.  A source may be released afterwards.  No source
  * may be a destination, and none may have tokens pending (KVC_ERR_STATE). */

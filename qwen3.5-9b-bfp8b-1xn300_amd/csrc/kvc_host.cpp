@@ -916,16 +916,22 @@ int kvc_seq_reserve(kvc_ctx* c, const int32_t* seqs, int32_t n_seqs, int32_t n_t
     // allocate everything first so a failure leaves no partial reservation
     struct Grant { int32_t seq, idx, block, cow_src; };
     std::vector<Grant> grants;
+    std::unordered_map<int32_t, int32_t> left;  // holders of a shared block that have no copy yet
     bool fail = false;
     for (int32_t i = 0; i < n_seqs && !fail; i++) {
         const Seq& s = c->seqs[seqs[i]];
         if (s.len % kBlockTok) {
             const int32_t idx = s.len / kBlockTok;
             const int32_t b = s.blocks[idx];
-            if (c->refcnt[b] > 1) {  // shared partial block: copy before writing
+            // Shared partial block: copied before it is written.  A holder for which
+            // all others took copies in this call keeps the block; its writes follow
+            // the copies on the stream.  (The references are given up below only, so
+            // that no block is reclaimed that a copy still reads.)
+            if (c->refcnt[b] > 1 && left.emplace(b, c->refcnt[b]).first->second > 1) {
                 const int32_t nb = alloc_block(c);
                 if (nb < 0) { fail = true; break; }
                 grants.push_back({seqs[i], idx, nb, b});
+                left[b]--;
             }
         }
         const int32_t need = (s.len + n_tok + kBlockTok - 1) / kBlockTok;
