@@ -1439,10 +1439,11 @@ int kvc_decode_attn_static(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
 // The launches of kvc_decode_attn_shared for seqs[i0, i0 + n): over the trie of
 // their block tables where that saves enough reads (shared_pays), else those of
 // kvc_decode_attn, of them the ones that hold weights in fp32 for fp32 output.
-// With launch = false only what can be refused is checked.
+// (Either's chunks grow until the launch fits the context's workspace: what the
+// caller checked beforehand is not refused here.)
 static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t i0, int32_t n, const void* q,
                          const void* k_new, const void* v_new, const void* gate, void* out, int32_t out_dtype,
-                         float scale, bool launch, void* stream) {
+                         float scale, void* stream) {
     const bool q8 = any_q8(c, seqs + i0, n);
     SharedPlan p;
     const int32_t* tab[kMaxBatch];
@@ -1453,22 +1454,22 @@ static int shared_launch(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32_t
             tab[j] = s.blocks.data();
             keys[j] = s.len + s.pending - (k_new ? 1 : 0);
         }
-        if (launch) shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, p);
+        shared_plan(tab, keys, n, c->cfg.decode_chunk_blocks, p);
     }
-    if (!launch || q8 || !shared_pays(p, n, c->cfg.flags & KVC_FLAG_DECODE_SHARE)) {
+    if (q8 || !shared_pays(p, n, c->cfg.flags & KVC_FLAG_DECODE_SHARE)) {
         DecodeArgs a;
         DecodeQ8Args a8;
         int rc, e = 0;
         if (q8 || out_dtype == KVC_DTYPE_F32) {
             if ((rc = build_decode_q8_args(c, layer, seqs, i0, n, q, k_new, v_new, gate, out, out_dtype, scale, a8)))
                 return rc;
-            if (launch) e = launch_decode_q8(a8, stream);
+            e = launch_decode_q8(a8, stream);
         } else {
             if ((rc = build_decode_args(c, layer, seqs, i0, n, q, k_new, v_new, gate, DecodeProducer{}, out, out_dtype,
                                         scale, c->d_part, (uint32_t)kPartBytes, c->d_counters,
                                         (int64_t)kMaxChunks * kKvHeads, "context's split-K workspace", a)))
                 return rc;
-            if (launch) e = launch_decode(a, stream);
+            e = launch_decode(a, stream);
         }
         return e ? hip_err((hipError_t)e, "decode launch") : KVC_OK;
     }
@@ -1538,11 +1539,16 @@ int kvc_decode_attn_shared(kvc_ctx* c, int32_t layer, const int32_t* seqs, int32
     if (meets_out(q, qbytes) || meets_out(gate, qbytes) || meets_out(k_new, kvbytes) || meets_out(v_new, kvbytes))
         return set_err(KVC_ERR_INVALID, "out overlaps an input");
     if ((rc = check_current(c))) return rc;
-    for (int pass = 0; pass < 2; pass++)
-        for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch)
-            if ((rc = shared_launch(c, layer, seqs, i0, std::min(kMaxBatch, n_seqs - i0), q, k_new, v_new, gate, out,
-                                    out_dtype, scale, pass == 1, stream)))
-                return rc;
+    for (int32_t i = 0; i < n_seqs; i++) {
+        const Seq& s = c->seqs[seqs[i]];
+        if (s.len + s.pending <= 0) return set_err(KVC_ERR_STATE, "sequence %d has no keys to attend", seqs[i]);
+        if (k_new && s.pending < 1)
+            return set_err(KVC_ERR_STATE, "sequence %d: fused append needs a reserved token", seqs[i]);
+    }
+    for (int32_t i0 = 0; i0 < n_seqs; i0 += kMaxBatch)
+        if ((rc = shared_launch(c, layer, seqs, i0, std::min(kMaxBatch, n_seqs - i0), q, k_new, v_new, gate, out,
+                                out_dtype, scale, stream)))
+            return rc;
     return KVC_OK;
 }
 
