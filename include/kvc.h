@@ -450,11 +450,15 @@ int kvc_kv_checksum(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
 /* ---- beam search (no counterpart in the reference) ------------------------- */
 /* Of every group (a prompt's beams) the n_out greatest of
  *   scores[g][b] + logits[g][b][t] - log sum_u exp logits[g][b][u]
- * over its beams b and tokens t, greatest first: the sums, in 64 bits, to
- * out_scores (fp32), b and t to out_beams and out_tokens, device [n_groups][n_out]
- * each.  Of equal sums the lower beam comes first, then the lower token.  A logit
- * of -inf or NaN is never chosen; a beam whose score is not finite, or whose
- * greatest logit is not, gives nothing; where fewer than n_out values are left the
+ * over its beams b and tokens t, greatest first: the sums to out_scores (fp32), b
+ * and t to out_beams and out_tokens, device [n_groups][n_out] each.  Scores and
+ * logits are added in 64 bits; the sum of exponentials is taken in 32, which leaves
+ * a row's log sum off by at most (2.22 log vocab + 24) 2^-24 (3e-6 of 151936 logits;
+ * below 1e-7 as a rule): beams whose sums are closer than that may come in either
+ * order.  Within a beam the order is the logits' own.  Of equal sums (of two beams:
+ * where scores and logits are the same) the lower beam comes first, then the lower
+ * token.  A logit of -inf or NaN is never chosen; a beam whose score is not
+ * finite, or whose greatest logit is not, gives nothing; where fewer than n_out values are left the
  * rest of a group's outputs is -inf, -1, -1.  logits: device, fp32 or bf16 by dtype,
  * rows of vocab tokens row_stride apart, at any address of their element.  scores:
  * device fp32 [n_groups][n_beams], NULL for zeros; it may be out_scores if n_out =

@@ -3,16 +3,17 @@
 // order (included by kvc_kernels.hip).
 //
 // Within a beam the order is that of the logits, so the first launch needs one pass
-// over them: the maximum of every 256-token segment, and the sum of exponentials.
+// over them: the maximum of every 256-token segment, and the sum of exponentials, in 32
+// bits (added pairwise; the second launch adds the chunks' in 64, 0.2 us of it).
 // The n_out greatest values of a group lie in the n_out segments with the greatest
 // maxima (ties: the lower beam, then the lower segment): a value in any other
 // segment has n_out segment maxima before it.  So the second launch, a workgroup per
 // group, chooses among the maxima and reads few segments again.
 //
-// Measured: 32 groups of 8 beams of 151936 bf16 logits, 16 of each 23.0 us: the first
+// Measured: 32 groups of 8 beams of 151936 bf16 logits, 16 of each 23.3 us: the first
 // launch 15.2 for 77.8 MB (5.1 TB/s; its VALU is busy for 10 of them, four tenths of
-// that with the exponentials), the second 8.8, a chain of some ten trips to memory and
-// barriers that a workgroup per group cannot hide.  One group of 4 beams 9.3: 2.8 + 6.5.
+// that with the exponentials), the second 8.6, a chain of some ten trips to memory and
+// barriers that a workgroup per group cannot hide.  One group of 4 beams 9.4: 2.8 + 6.7.
 #pragma once
 
 namespace kvc {
@@ -75,29 +76,35 @@ __global__ __launch_bounds__(256) void beam_max_kernel(BeamArgs a) {
     u32x4 w[STEPS];
 #pragma unroll
     for (int k = 0; k < STEPS; k++) w[k] = beam_load<BF16>(base, t0 + k * kSegLanes * E, a.vocab);
-    const auto logit = [&](int k, int i) { return beam_word<BF16>(w[k], i); };
-    float m = -INFINITY, s = 0.f;
+    const auto logit = [&](int k, int i) __attribute__((always_inline)) { return beam_word<BF16>(w[k], i); };
+    float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < STEPS; k++)
 #pragma unroll
         for (int i = 0; i < E; i++) m = fmaxf(m, logit(k, i));
     float me = m == -INFINITY ? 0.f : m;
+    // the lane's exponentials, added pairwise: log2 of their number roundings, not that
+    // many, and small ones beside a 1 are not lost one by one
+    const auto sum = [&](auto&& x) __attribute__((always_inline)) {
+        float e[STEPS * E];
 #pragma unroll
-    for (int k = 0; k < STEPS; k++)
+        for (int k = 0; k < STEPS * E; k++) e[k] = fast_exp2((x(k / E, k % E) - me) * kLog2e);
 #pragma unroll
-        for (int i = 0; i < E; i++) s += fast_exp2((logit(k, i) - me) * kLog2e);
+        for (int n = 1; n < STEPS * E; n *= 2)
+#pragma unroll
+            for (int k = 0; k < STEPS * E; k += 2 * n) e[k] += e[k + n];
+        return e[0];
+    };
+    float s = sum(logit);
     if (s != s) {  // a NaN counts as -inf; so does +inf here, whose sum nobody reads
+        const auto clean = [&](int k, int i) __attribute__((always_inline)) { return beam_clean(logit(k, i)); };
         m = -INFINITY;
-        s = 0.f;
 #pragma unroll
         for (int k = 0; k < STEPS; k++)
 #pragma unroll
-            for (int i = 0; i < E; i++) m = fmaxf(m, beam_clean(logit(k, i)));
+            for (int i = 0; i < E; i++) m = fmaxf(m, clean(k, i));
         me = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int k = 0; k < STEPS; k++)
-#pragma unroll
-            for (int i = 0; i < E; i++) s += fast_exp2((beam_clean(logit(k, i)) - me) * kLog2e);
+        s = sum(clean);
     }
     float seg = m;  // over the segment's lanes
     seg = fmaxf(seg, dpp<kDppXor1>(seg));
@@ -113,11 +120,48 @@ __global__ __launch_bounds__(256) void beam_max_kernel(BeamArgs a) {
     __syncthreads();
     if (threadIdx.x == 0) {
         const float M = fmaxf(fmaxf(red[0].x, red[1].x), fmaxf(red[2].x, red[3].x)), e = M == -INFINITY ? 0.f : M;
-        float t = 0.f;
+        float t[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) t += red[i].y * fast_exp2((red[i].x - e) * kLog2e);
-        *reinterpret_cast<float2*>(a.chunk_sum + (row * a.n_chunks + blockIdx.x) * 2) = make_float2(M, t);
+        for (int i = 0; i < 4; i++) t[i] = red[i].y * fast_exp2((red[i].x - e) * kLog2e);
+        *reinterpret_cast<float2*>(a.chunk_sum + (row * a.n_chunks + blockIdx.x) * 2) = make_float2(M, (t[0] + t[1]) + (t[2] + t[3]));
     }
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double x) {
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, 0xF, 0xF, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ double wave_sum64(double x) {
+    x += dpp64<kDppXor1>(x);
+    x += dpp64<kDppXor2>(x);
+    x += dpp64<kDppHalfMirror>(x);
+    x += dpp64<kDppRowRor8>(x);
+    uint32_t l = __double2loint(x), h = __double2hiint(x);
+    auto lo = __builtin_amdgcn_permlane16_swap(l, l, false, false), hi = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+    x = __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+    l = __double2loint(x), h = __double2hiint(x);
+    lo = __builtin_amdgcn_permlane32_swap(l, l, false, false), hi = __builtin_amdgcn_permlane32_swap(h, h, false, false);
+    return __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+}
+
+// e^(x - m), x <= m, as the hardware's exponential of the rounded argument and the
+// first order of what rounding took from it: off by that exponential's 2^-23.  0
+// for -inf (whose argument would leave NaN in the second part).
+__device__ __forceinline__ double beam_scale(float x, float m) {
+    const double y = fmax((double)x - (double)m, -300.0) * 1.4426950408889634;
+    const float p = (float)y, e = fast_exp2(p);
+    return (double)e + (double)(e * (float)(y - (double)p)) * 0.6931471805599453;
+}
+
+// log x of a finite x >= 1: the exponent's part and what rounding took from the
+// mantissa in 64 bits, the rounded mantissa's by the hardware, off by 2^-24 at most.
+__device__ __forceinline__ double beam_log(double x) {
+    const int hi = __double2hiint(x);
+    const double f = __hiloint2double((hi & 0xFFFFF) | 0x3FF00000, __double2loint(x));  // in [1, 2)
+    const float c = (float)f, d = (float)(f - (double)c);
+    return ((double)((hi >> 20) - 1023) + (double)__builtin_amdgcn_logf(c)) * 0.6931471805599453 +
+           (double)(d * __builtin_amdgcn_rcpf(c));
 }
 
 // Doubles as integers of the same order; 0 for -inf, which is never chosen.
@@ -128,14 +172,6 @@ __device__ __forceinline__ uint64_t beam_key(double v) {
 }
 __device__ __forceinline__ double beam_value(uint64_t k) {
     return __longlong_as_double((int64_t)(k >> 63 ? k & ~(1ull << 63) : ~k));
-}
-
-// log x of a finite x >= 1: the exponent's part in 64 bits, the mantissa's, below 1, off
-// by 2^-23 at most.
-__device__ __forceinline__ double beam_log(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const float f = __uint_as_float((u & 0x7FFFFFu) | 0x3F800000u);  // in [1, 2)
-    return ((double)((int)(u >> 23) - 127) + (double)__builtin_amdgcn_logf(f)) * 0.6931471805599453;
 }
 
 constexpr int kBeamThreads = 1024, kBeamWaves = kBeamThreads / 64;
@@ -333,12 +369,12 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamArgs a) {
         for (int c = lane + 128; c < a.n_chunks; c += 64) m = fmaxf(m, cs[c].x);
         m = wave_max(m);
         const bool fine = m > -INFINITY && m < INFINITY;
-        float s = 0.f;
+        double s = 0.0;
         if (fine) {
-            s = c0.y * fast_exp2((c0.x - m) * kLog2e) + c1.y * fast_exp2((c1.x - m) * kLog2e);
-            for (int c = lane + 128; c < a.n_chunks; c += 64) s += cs[c].y * fast_exp2((cs[c].x - m) * kLog2e);
+            s = (double)c0.y * beam_scale(c0.x, m) + (double)c1.y * beam_scale(c1.x, m);
+            for (int c = lane + 128; c < a.n_chunks; c += 64) s += (double)cs[c].y * beam_scale(cs[c].x, m);
         }
-        s = wave_sum(s);
+        s = wave_sum64(s);
         if (lane == 0) {
             sm.off[b] = fine && score > -INFINITY && score < INFINITY ? score - beam_log(s) : -INFINITY;
             sm.max[b] = fine ? m : 0.0;
