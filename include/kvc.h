@@ -458,13 +458,14 @@ int kvc_kv_checksum(kvc_ctx* ctx, int32_t layer, const int32_t* seqs,
  * order.  Within a beam the order is the logits' own.  Of equal sums (of two beams:
  * where scores and logits are the same) the lower beam comes first, then the lower
  * token.  A logit of -inf or NaN is never chosen; a beam whose score is not
- * finite, or whose greatest logit is not, gives nothing; where fewer than n_out values are left the
- * rest of a group's outputs is -inf, -1, -1.  logits: device, fp32 or bf16 by dtype,
- * rows of vocab tokens row_stride apart, at any address of their element.  scores:
- * device fp32 [n_groups][n_beams], NULL for zeros; it may be out_scores if n_out =
- * n_beams.  Otherwise no two arrays may overlap.  n_beams <= 64, n_out <= 128;
- * n_beams * vocab is bounded by the context's workspace (1 B per 64 tokens and a
- * little; KVC_ERR_RANGE).  It uses the context's split-K workspace and no
+ * finite, or whose greatest logit is not, gives nothing; where fewer than n_out
+ * values are left the rest of a group's outputs is -inf, -1, -1 (no index for
+ * kvc_seq_reorder: such a beam is its own parent).  logits: device, fp32 or bf16 by
+ * dtype, rows of vocab tokens row_stride apart, at any address of their element.
+ * scores: device fp32 [n_groups][n_beams], NULL for zeros; it may be out_scores if
+ * n_out = n_beams.  Otherwise no two arrays may overlap.  n_beams <= 64, n_out <=
+ * 128; n_beams * vocab is bounded by the context's workspace (1 B per 64 tokens and
+ * a little; KVC_ERR_RANGE).  It uses the context's split-K workspace and no
  * sequence; the context's device must be current.  The next step: kvc_seq_reorder
  * by the beams chosen. */
 int kvc_beam_select(kvc_ctx* ctx, const void* logits, int32_t dtype,
