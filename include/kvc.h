@@ -213,7 +213,10 @@ int kvc_seq_commit(kvc_ctx* ctx, const int32_t* seqs, int32_t n_seqs,
  * unless all other holders got their copies before or in the same call),
  * and a copy of the recurrent and conv state.  8-bit blocks are shared too, and
  * evicted tokens stay evicted.  A source may be released afterwards.  No source
- * may be a destination, and none may have tokens pending (KVC_ERR_STATE). */
+ * may be a destination, and none may have tokens pending (KVC_ERR_STATE).
+ * Sequences that share blocks belong on one stream, or their calls have to be
+ * ordered by the caller: a copy that one reserve makes reads the block that
+ * another sequence, its last holder, then writes to. */
 int kvc_seq_fork(kvc_ctx* ctx, const int32_t* src, const int32_t* dst, int32_t n,
                  void* stream);
 /* Beam search's step back to the parents, in place: seqs[i] becomes what

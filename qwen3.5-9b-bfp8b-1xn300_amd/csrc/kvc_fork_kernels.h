@@ -7,7 +7,7 @@ namespace kvc {
 // The first n_rows workgroups copy a block-table row each, the others pieces of
 // the states: a piece is read once and stored to every sequence that gets it.
 // Nothing is both read and written (a destination is nobody's source).  HBM-bound:
-// 52.7 MB read a source and written a copy; one state to four sequences 49 us (5.4
+// 52.7 MB read a source and written a copy; one state to four sequences 48 us (5.4
 // TB/s read + written), 13 copies of 5 163 us (5.8).  A thread moves one 16-B piece: 2,
 // 4 and 8 took 168, 169 and 193 us for the 163.  Loads and stores are nontemporal: the
 // states are larger than the caches, and the K/V in them stays (time the same without).

@@ -21,9 +21,10 @@
 // 4096 common tokens 14.5 (17.6): this launch 10.2, one trip after the other to the
 // arguments (0.8), the block ids and queries (1.1), the keys (3.9, at 5 TB/s: twice the
 // half blocks in flight took 15.0) and the fold of the waves (1.5); the second launch
-// 4.2.  64 on 8192, with tails of up to 1500 58 (194): this launch 54.8 for
-// 240 MB from HBM, the products 5 of them.  64 on 65536 141 (1228): bound by the
-// blocks' eight trips from L2 to LDS.  30 in a tree of prompts, fp32 output 22.5 (36).
+// 4.2.  64 on 8192, with tails of up to 1500 58 (194): this launch 54.6 for
+// 240 MB from HBM, most of them the tails', the products 5 of it.  64 on 65536 139 (1229):
+// bound by the blocks' eight trips from L2 to LDS.  30 in a tree of prompts, fp32 output
+// 22.5 (36).
 #pragma once
 
 namespace kvc {
@@ -303,8 +304,9 @@ __device__ __forceinline__ void shared_one(const SharedArgs& a, const SharedItem
     if (lane == 0) *reinterpret_cast<float2*>(a.stats + row * 2) = make_float2(m, l);
 }
 
+// (2 waves a SIMD: two workgroups on a CU, up to 256 registers a wave)
 template <int PARTS>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(SharedArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(SharedArgs a) {
     __shared__ __align__(1024) union {  // (the XORs with a fragment's number need it)
         SharedSmem tiles;
         SharedOneSmem one;

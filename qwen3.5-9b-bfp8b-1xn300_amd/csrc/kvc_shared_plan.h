@@ -175,10 +175,11 @@ inline bool shared_fits(const SharedPlan& p) { return p.path <= kSharedPath && p
 // Whether the plan beats kvc_decode_attn's launch, by the us that either takes: a
 // fixed part (here two launches, the first longer for more members), blocks from
 // memory, blocks that sequence by sequence come from the caches, and the tiles' LDS.
-// us per layer, kvc_decode_attn / shared: 4 sequences on 300 tokens 9.2 / 12.4, 4 on
-// 4096 13.4 / 13.1, 2 on 4096 11.5 / 12.7, 8 on 1000 9.5 / 13.0, 8 on 2000 12.4 / 13.4, 8
-// on 4096 17.6 / 14.5, 16 on 1000 12.2 / 14.0, 16 on 2000 17.0 / 13.0, 64 on 2000 47 /
-// 19.4, 64 with 96 tokens in common of 1031 47.7 / 53.6, 64 on 65536 1228 / 141.
+// us per layer, kvc_decode_attn / shared (profiles/shared_decode_rule.txt): 4 sequences on
+// 300 tokens 8.9 / 12.2, 2 on 4096 11.6 / 12.8, 4 on 4096 13.4 / 13.5, 8 on 1000 9.1 / 12.3,
+// 8 on 2000 11.3 / 12.3, 8 on 4096 17.9 / 13.7, 16 on 1000 11.5 / 12.5, 16 on 2000 16.5 /
+// 12.4, 64 on 2000 46.5 / 17.9, 64 with 96 tokens in common of 1031 45.5 / 47.2, 64 on
+// 65536 1229 / 139.
 // `always`: wherever blocks are shared.
 inline bool shared_pays(const SharedPlan& p, int32_t n, bool always) {
     if (!shared_fits(p) || p.blocks == p.blocks_apart) return false;

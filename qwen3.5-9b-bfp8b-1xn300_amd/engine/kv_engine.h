@@ -111,8 +111,9 @@ int generate_session(int session, const std::vector<int>& prompt_tokens, int max
 // session's sequence, decode together (kvc_decode_attn_shared), are chosen by
 // kvc_beam_select and follow their parents by kvc_seq_reorder; the session itself
 // stays at the prompt.  The logits are synthetic, N(0, 3) from the seed and the
-// tokens before them alone.  Returns the tokens per beam (max_tokens, or what the
-// context holds) with the beams best first, 0 on error.
+// tokens before them alone; no token ends a sequence, so all beams have one length.
+// Returns the tokens per beam (max_tokens, or what the context holds) with the beams
+// best first, 0 on error.
 struct Beam {
     std::vector<int> tokens;
     float score = 0.f;
